@@ -1,0 +1,523 @@
+// Attention of a decode or verify step over the paged cache.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2(e)
+//
+// The M = q_len * heads / kv_heads query rows that share a key head are the
+// columns of 16-wide MFMA tiles; each 32 keys of a wave cost 2 D/32 products
+// for K q^T and D/16 for V^T p^T and 4 D bytes of cache per key, so the stream
+// of the cache bounds the kernel and everything else has to stay out of its
+// way: K and V go straight into registers (no LDS, no barrier in the loop).
+//
+// S^T = K q^T comes out with a query row in every lane (column lane & 15) and
+// keys 4g + r of a 16-key tile in lane group g = lane >> 4.  That is a B
+// operand of the second product already: the contraction may run over the keys
+// in any order, so slots 0..3 of group g are given keys 4g..4g+3 of the first
+// tile and slots 4..7 those of the second, and p never crosses lanes.  V^T as
+// the A operand then wants, in lane (m, g), those eight keys at one element
+// d(m, t) per product t.  The lane loads VW = D / 16 consecutive elements
+// VW m.. of each of its keys (whole 16-byte pieces) and picks element t of all
+// eight with byte permutes: d(m, t) = VW m + t.  Column q of O^T stays in lane
+// q, so the running maximum and the rescaling are lane-local too.
+//
+// Work: the (sequence, key head) items' 128-key units in a row, cut into equal
+// shares for a fixed number of workgroups, so ragged lengths cost no balance
+// and the lengths are read on the device (a captured launch follows them).  An
+// item that lies in one share is finished there; the parts of the others go
+// through float32 partial rows (o, m, l) and k_paged_join.
+#include "attn.h"
+#include "attn_core.h"
+
+namespace dsk {
+namespace {
+
+constexpr int kPgThreads = 256;
+constexpr int kPgUnit = 128;        // keys of a unit: 32 for each wave
+
+struct PagedArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  const int32_t* lens;
+  CacheView c;
+  float* po;                        // partial rows [slot][M][D]
+  float* pml;                       // [slot][M][2]: maximum (of scores times c), sum
+  const float* pre_o;               // prefix partials [split][kv head][batch * M][D]
+  const float* pre_ml;
+  int64_t q_token, q_head, o_token, o_head;
+  float c2;                         // scale * log2(e)
+  int32_t batch, q_len, kv_heads, group, prefix, shares, splits;
+};
+
+// Keys of sequence b that the cache can hold; `bad` if lens[b] claims more.
+__device__ __forceinline__ int length_of(const PagedArgs& a, int b, bool& bad) {
+  const int n = a.lens[b], cap = a.c.max_pages << a.c.page_shift;
+  bad = n > cap;
+  return min(max(n, 0), cap);
+}
+__device__ __forceinline__ int units_of(const PagedArgs& a, int b) {
+  bool bad;
+  return (length_of(a, b, bad) + kPgUnit - 1) / kPgUnit;
+}
+
+// Sum of units over all sequences, and over those before `stop`, by the whole block.
+struct Totals { int64_t all, before; };
+__device__ Totals unit_totals(const PagedArgs& a, int stop, int64_t (&lds)[2 * kPgThreads / 64]) {
+  int64_t all = 0, before = 0;
+  for (int b = threadIdx.x; b < a.batch; b += kPgThreads) {
+    const int n = units_of(a, b);
+    all += n;
+    if (b < stop) before += n;
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) {
+    all += __shfl_xor(all, s, 64);
+    before += __shfl_xor(before, s, 64);
+  }
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) { lds[2 * wave] = all; lds[2 * wave + 1] = before; }
+  __syncthreads();
+  Totals t{0, 0};
+#pragma unroll
+  for (int w = 0; w < kPgThreads / 64; ++w) { t.all += lds[2 * w]; t.before += lds[2 * w + 1]; }
+  return t;
+}
+
+// The sequence that unit u of one key head lies in (u < the units of all), and
+// the units before it; every wave by itself.
+__device__ __forceinline__ int find_seq(const PagedArgs& a, int64_t u, int64_t& before) {
+  const int lane = threadIdx.x & 63;
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int n = b0 + lane < a.batch ? units_of(a, b0 + lane) : 0;
+    int64_t incl = n;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int64_t o = __shfl_up(incl, s, 64);
+      if (lane >= s) incl += o;
+    }
+    const uint64_t past = __ballot(base + incl > u);
+    if (past) {
+      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      before = base + __shfl(incl - n, l, 64);
+      return b0 + l;
+    }
+    base += __shfl(incl, 63, 64);
+  }
+  before = base;
+  return a.batch - 1;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)))) |
+         (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32);
+}
+
+template <int D>
+struct Step {                       // one wave's 32 keys
+  u32x4 k[2][D / 32];
+  uint32_t v[8][D / 32];            // VW = D / 16 elements of 8 keys
+};
+
+template <int VW>
+__device__ __forceinline__ void load_v(uint32_t (&v)[VW / 2], const uint16_t* p) {
+  if constexpr (VW == 8) {
+    const u32x4 r = ldg16(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r[i];
+  } else {
+    const u32x2 r = ldg<u32x2>(p);
+    v[0] = r[0];
+    v[1] = r[1];
+  }
+}
+
+template <int D, int RT>
+__global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const PagedArgs a) {
+  constexpr int VW = D / 16, KS = D / 32, kWaves = kPgThreads / 64;
+  constexpr int kLd = D + 4;
+  __shared__ float lds_o[kWaves][16][kLd];
+  __shared__ float lds_ml[kWaves][16 * RT][2];
+  __shared__ int64_t lds_t[2 * kWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n16 = lane & 15, g = lane >> 4;
+  const int M = a.q_len * a.group, r0 = 16 * RT * blockIdx.y;   // this block's rows: r0 ..
+  const int64_t total = unit_totals(a, 0, lds_t).all * a.kv_heads;
+  const int64_t quota = uniform64((total + a.shares - 1) / a.shares);
+  const int64_t u0 = blockIdx.x * quota, u1 = uniform64(min(u0 + quota, total));
+  if (u0 >= u1) return;
+  int64_t before;
+  int b = __builtin_amdgcn_readfirstlane(find_seq(a, u0 / a.kv_heads, before));
+  before = uniform64(before);
+  // find_seq counts units of one head; an item's first unit is kv_heads * before + h * units
+  for (int64_t u = u0; u < u1;) {
+    bool bad_len;
+    const int len = length_of(a, b, bad_len);
+    const int nb = (len + kPgUnit - 1) / kPgUnit;
+    const int64_t first = before * a.kv_heads;
+    if (nb == 0 || u >= first + static_cast<int64_t>(nb) * a.kv_heads) {
+      before += nb;
+      ++b;
+      continue;
+    }
+    const int h = static_cast<int>((u - first) / nb);
+    const int64_t item0 = first + static_cast<int64_t>(h) * nb;
+    const int k0 = static_cast<int>(u - item0);
+    const int k1 = static_cast<int>(min(static_cast<int64_t>(nb), u1 - item0));
+    const bool whole = k0 == 0 && k1 == nb;
+
+    // queries: column n16 of row tile rt is row 16 rt + n16 = token * group + head of the group
+    bf16x8 q[RT][KS];
+    int lim[RT];                    // last key that the lane's row sees
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = min(r0 + 16 * rt + n16, M - 1), tok = r / a.group, hd = h * a.group + r % a.group;
+      const uint16_t* p = a.q + (static_cast<int64_t>(b) * a.q_len + tok) * a.q_token + hd * a.q_head + 8 * g;
+      lim[rt] = len - a.q_len + tok;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) q[rt][ks] = as_bf16x8(ldg16(p + 32 * ks));
+    }
+    f32x4 o[RT][VW];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = kNegInf;
+      l[rt] = bad_len ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+      for (int t = 0; t < VW; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int32_t* trow = a.c.table + b * a.c.table_stride;
+    const int last_tile = (len - 1) >> 4, sub = a.c.page_shift - 4;
+    int ids = 0, ids0 = k0 - 32;    // lane 2 i + kt: the page of tile kt of step ids0 + i
+    bool bad = false;
+    auto page_ids = [&](int kk) {
+      ids0 = kk;
+      const int tile = min((kk + (lane >> 1)) * 8 + 2 * wave + (lane & 1), last_tile);
+      ids = ldg<int32_t>(trow + (tile >> sub));
+      const bool out_of = ids < 0 || ids >= a.c.n_pages;
+      bad = bad || (out_of && kk + (lane >> 1) < k1);
+      if (out_of) ids = 0;
+    };
+    auto load = [&](Step<D>& s, int kk) {
+      if (kk - ids0 >= 32) page_ids(kk);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int tile = min(kk * 8 + 2 * wave + kt, last_tile);
+        const int id = __builtin_amdgcn_readlane(ids, 2 * (kk - ids0) + kt);
+        const int last_row = len - 1 - tile * 16;     // rows past the length: the last one again
+        const int row0 = (tile * 16) & ((1 << a.c.page_shift) - 1);
+        const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + row0) * D;
+        const uint16_t* kp = a.c.k + base + min(n16, last_row) * D + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s.k[kt][ks] = ldg16(kp + 32 * ks);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          load_v<VW>(s.v[4 * kt + j], a.c.v + base + min(4 * g + j, last_row) * D + VW * n16);
+      }
+    };
+    // rarely: infinite and NaN values of step kk, to the rows that see them (the
+    // products then leave them out)
+    auto add_nonfinite = [&](int kk) {
+#pragma unroll 1
+      for (int key = kk * kPgUnit + 32 * wave, end = min(key + 32, len); key < end; ++key) {
+        int id = ldg<int32_t>(trow + (key >> a.c.page_shift));
+        if (id < 0 || id >= a.c.n_pages) id = 0;
+        const int in_page = key & ((1 << a.c.page_shift) - 1);
+        const uint16_t* vp = a.c.v + (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int t = 0; t < VW; ++t) {
+            const float x = nonfinite_only(ldg<uint16_t>(vp + VW * (4 * g + r) + t));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][t][r] += key <= lim[rt] ? x : 0.0f;
+          }
+      }
+    };
+    auto compute = [&](const Step<D>& s, int kk) {
+      const int key0 = kk * kPgUnit + 32 * wave;
+      const bool masked = key0 + 31 > len - a.q_len;
+      bf16x8 p[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 x[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) x[kt] = mfma16(as_bf16x8(s.k[kt][ks]), q[rt][ks], x[kt]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (key0 + 16 * kt + 4 * g + r > lim[rt]) x[kt][r] = kNegInf;
+        }
+        float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                          fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        top = max_across32(max_across16(top)) * a.c2;
+        if (__any(top > m[rt])) {
+          const float mn = fmaxf(m[rt], top);
+          const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
+          m[rt] = mn;
+          l[rt] *= f;
+#pragma unroll
+          for (int t = 0; t < VW; ++t) o[rt][t] *= f;
+        }
+        const float mu = m[rt] == kNegInf ? 0.0f : m[rt];
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
+          l[rt] += e[i];
+        }
+        // p to bf16: relative 2^-9 each, of random sign over the keys, next to the
+        // output's own rounding of 2^-9
+        p[rt] = as_bf16x8(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
+      }
+      // rows of several tokens see different keys here: are all the values finite?
+      bool finite = true;
+      if (masked && a.q_len > 1) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < VW / 2; ++i) bits |= nonfinite_bits(s.v[j][i]);
+        finite = !__any(bits != 0);
+      }
+      if (!finite) add_nonfinite(kk);
+#pragma unroll
+      for (int t = 0; t < VW; ++t) {
+        const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(s.v[2 * i + 1][t / 2], s.v[2 * i][t / 2], sel);
+        if (!finite)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), p[rt], o[rt][t]);
+      }
+    };
+
+    Step<D> s0, s1;
+    load(s0, k0);
+    int kk = k0;
+    for (; kk + 1 < k1; kk += 2) {
+      load(s1, kk + 1);
+      compute(s0, kk);
+      if (kk + 2 < k1) load(s0, kk + 2);
+      compute(s1, kk + 1);
+    }
+    if (kk < k1) compute(s0, kk);
+
+    // the four waves' parts
+    const bool any_bad = __any(bad);
+    __syncthreads();                 // the last item's reads of LDS are done
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] = sum_across32(sum_across16(l[rt]));
+      if (any_bad) l[rt] = __builtin_nanf("");
+      if (g == 0) {
+        lds_ml[wave][16 * rt + n16][0] = m[rt];
+        lds_ml[wave][16 * rt + n16][1] = l[rt];
+      }
+    }
+    __syncthreads();
+    const bool direct = whole && a.splits == 0;
+    const int64_t slot = direct ? 0
+                         : whole && a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h
+                         : u == u0 ? 2 * static_cast<int64_t>(blockIdx.x)
+                                   : 2 * static_cast<int64_t>(blockIdx.x) + 1;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (rt) __syncthreads();
+      float top = lds_ml[0][16 * rt + n16][0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_ml[w][16 * rt + n16][0]);
+      const float f = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < VW; t += 4)
+          *reinterpret_cast<f32x4*>(&lds_o[wave][n16][VW * (4 * g + r) + t]) =
+              f32x4{o[rt][t][r], o[rt][t + 1][r], o[rt][t + 2][r], o[rt][t + 3][r]} * f;
+      __syncthreads();
+      const int row = threadIdx.x / (D / 8), d0 = 8 * (threadIdx.x % (D / 8));
+      const int r = r0 + 16 * rt + row, rl = 16 * rt + row;
+      if (row < 16 && r < M) {
+        float mm = lds_ml[0][rl][0], ll = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, lds_ml[w][rl][0]);
+        const float mu = mm == kNegInf ? 0.0f : mm;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) ll += lds_ml[w][rl][1] * __builtin_amdgcn_exp2f(lds_ml[w][rl][0] - mu);
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = lds_o[0][row][d0 + i];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) y[i] += lds_o[w][row][d0 + i];
+        }
+        if (direct) {
+          const int tok = r / a.group, hd = h * a.group + r % a.group;
+          const float inv = len - a.q_len + tok >= 0 || ll != ll ? 1.0f / ll : 0.0f;
+          *reinterpret_cast<u32x4*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
+              u32x4{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv),
+                    pack_bf16(y[4] * inv, y[5] * inv), pack_bf16(y[6] * inv, y[7] * inv)};
+        } else {
+          float* po = a.po + (slot * M + r) * D + d0;
+          *reinterpret_cast<f32x4*>(po) = f32x4{y[0], y[1], y[2], y[3]};
+          *reinterpret_cast<f32x4*>(po + 4) = f32x4{y[4], y[5], y[6], y[7]};
+          if (d0 == 0) *reinterpret_cast<float2*>(a.pml + (slot * M + r) * 2) = float2{mm, ll};
+        }
+      }
+    }
+    u = item0 + k1;
+  }
+}
+
+// Joins a row's parts (shares of its own keys, splits of the prefix), one block
+// for a row: the parts' weights first, all at once, then 256 / (D / 4) groups of
+// threads add up the parts in a fixed order.  Also writes the rows of sequences
+// without keys.
+constexpr int kPgMostParts = 1024;   // of a row: shares and splits are at most 512 each
+
+template <int D>
+__global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
+  constexpr int kLanes = D / 4, kWays = kPgThreads / kLanes, kWaves = kPgThreads / 64;
+  __shared__ int64_t lds_t[2 * kWaves];
+  __shared__ float weight[kPgMostParts];
+  __shared__ float red[kWaves];
+  __shared__ f32x4 sum[kWays][kLanes];
+  const int M = a.q_len * a.group;
+  const int r = blockIdx.x % M, item = blockIdx.x / M, h = item % a.kv_heads, b = item / a.kv_heads;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Totals tt = unit_totals(a, b, lds_t);
+  const int64_t total = tt.all * a.kv_heads;
+  const int64_t quota = (total + a.shares - 1) / a.shares;
+  bool bad;
+  const int len = length_of(a, b, bad), nb = (len + kPgUnit - 1) / kPgUnit;
+  const int64_t item0 = tt.before * a.kv_heads + static_cast<int64_t>(h) * nb;
+  const int64_t s0 = nb ? item0 / quota : 0, s1 = nb ? (item0 + nb - 1) / quota : -1;
+  const bool whole = nb > 0 && s0 == s1;
+  if (whole && a.splits == 0) return;                 // finished where it was computed
+  const bool odd = nb && item0 % quota != 0;          // the first part is not its share's first
+  const int own = static_cast<int>(s1 - s0 + 1), parts = own + a.splits;
+  // row of part i among the partial rows; parts >= own are the prefix's
+  auto row_of = [&](int i) -> int64_t {
+    if (i >= own)
+      return (static_cast<int64_t>(i - own) * a.kv_heads + h) * (static_cast<int64_t>(a.batch) * M) + static_cast<int64_t>(b) * M + r;
+    const int64_t slot = whole ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h
+                               : 2 * (s0 + i) + (i == 0 && odd ? 1 : 0);
+    return slot * M + r;
+  };
+  auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };
+
+  float top = kNegInf;
+  for (int i = threadIdx.x; i < parts; i += kPgThreads) top = fmaxf(top, ml_of(i)[0]);
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = red[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red[w]);
+  const float mu = top == kNegInf ? 0.0f : top;
+  float ll = 0.0f;
+  for (int i = threadIdx.x; i < parts; i += kPgThreads) {
+    const f32x2 ml = ml_of(i);
+    const float f = __builtin_amdgcn_exp2f(ml[0] - mu);
+    weight[i] = f;
+    ll += ml[1] * f;
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) ll += __shfl_xor(ll, s, 64);
+  __syncthreads();                                    // everyone has read the maxima
+  if (lane == 0) red[wave] = ll;
+  __syncthreads();
+  ll = red[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) ll += red[w];
+
+  const int way = threadIdx.x / kLanes, d0 = 4 * (threadIdx.x % kLanes);
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = way; i < parts; i += kWays)
+    y += ldg<f32x4>((i < own ? a.po : a.pre_o) + row_of(i) * D + d0) * weight[i];
+  sum[way][threadIdx.x % kLanes] = y;
+  __syncthreads();
+  if (way) return;
+#pragma unroll
+  for (int w = 1; w < kWays; ++w) y += sum[w][threadIdx.x];
+  const int tok = r / a.group, hd = h * a.group + r % a.group;
+  const bool sees = a.prefix > 0 || len - a.q_len + tok >= 0 || ll != ll;   // else no key: zeros
+  const float inv = sees ? 1.0f / ll : 0.0f;
+  *reinterpret_cast<u32x2*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
+      u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
+}
+
+// Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's.
+struct PagedPlan {
+  int rt, shares, splits;
+  int64_t slots, rows, pre_rows;
+  size_t po, pml, pre_o, pre_ml, total;
+};
+
+PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
+  PagedPlan p{};
+  const int64_t M = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
+  p.rt = M <= 16 ? 1 : 2;
+  const int64_t items = static_cast<int64_t>(d.batch) * d.kv_heads;
+  const int64_t units = items * ((static_cast<int64_t>(c.max_pages) * c.page_size + kPgUnit - 1) / kPgUnit);
+  const int64_t most = p.rt == 1 ? 512 : 256;   // the workgroups that are resident at once
+  p.shares = static_cast<int>(units < most ? units : most);
+  p.slots = 2 * p.shares + (d.prefix_len > 0 ? items : 0);
+  p.rows = p.slots * M;
+  p.pre_rows = static_cast<int64_t>(d.batch) * M;
+  p.splits = d.prefix_len > 0 ? prefix_splits(p.pre_rows, d.kv_heads, d.prefix_len) : 0;
+  auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
+  const size_t pre = static_cast<size_t>(p.splits) * d.kv_heads * p.pre_rows;
+  p.po = 0;
+  p.pml = up(p.po + p.rows * d.head_dim * 4);
+  p.pre_o = up(p.pml + p.rows * 8);
+  p.pre_ml = up(p.pre_o + pre * d.head_dim * 4);
+  p.total = up(p.pre_ml + pre * 8);
+  return p;
+}
+
+template <int D>
+void launch_paged_d(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
+  const int M = a.q_len * a.group;
+  // more than 32 rows: every share twice, a half of the rows each (four row tiles
+  // spill registers); the halves run on one XCD, whose L2 holds what they both read
+  if (p.rt == 1) launch_kernel(k_paged<D, 1>, p.shares, kPgThreads, 0, s, a);
+  else launch_kernel(k_paged<D, 2>, dim3(p.shares, (M + 31) / 32), kPgThreads, 0, s, a);
+  launch_kernel(k_paged_join<D>, a.batch * a.kv_heads * M, kPgThreads, 0, s, a);
+}
+
+}  // namespace
+
+size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c) { return plan_of(d, c).total; }
+
+hipError_t launch_paged(const dsk_paged_desc& d, const void* q, const dsk_kv_cache& c, const int32_t* lens,
+                        const int32_t* prefix, void* out, void* ws, hipStream_t s) {
+  const PagedPlan p = plan_of(d, c);
+  char* w = static_cast<char*>(ws);
+  float* pre_o = reinterpret_cast<float*>(w + p.pre_o);
+  float* pre_ml = reinterpret_cast<float*>(w + p.pre_ml);
+  PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, cache_view(c),
+              reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml), pre_o, pre_ml,
+              d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
+              d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits};
+  if (d.prefix_len > 0) {
+    hipError_t e = launch_prefix(d, q, c, prefix, p.splits, pre_o, pre_ml, s);
+    if (e != hipSuccess) return e;
+  }
+  if (d.head_dim == 64) launch_paged_d<64>(p, a, s);
+  else launch_paged_d<128>(p, a, s);
+  return hipGetLastError();
+}
+
+}  // namespace dsk

@@ -1,0 +1,236 @@
+// Attention over packed prompts, and a batch's rows over the prefix they share.
+//
+// The rows of a tile are (token, head of the group) pairs of one key head,
+// token by token: the heads of a group share every key tile that is loaded, a
+// short prompt of a few tokens fills a tile with its heads, and the causal edge
+// crosses few keys of a tile.
+#include "attn_core.h"
+
+namespace dsk {
+namespace {
+
+constexpr int kFlWaves = 4;
+constexpr int kFlThreads = 64 * kFlWaves;
+constexpr int kFlRows = 32 * kFlWaves;
+
+// ------------------------------------------------------------------ prompts
+struct PromptArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* out;
+  const int32_t *cu_q, *cu_k;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
+  float c2;
+  int32_t tokens, kv_tokens, n_seqs, kv_heads, group, causal, tiles;
+};
+
+struct SeqRange { int q0, q1, k0, k1; };
+// The rows of sequence b, cut to the tensors; whatever cu holds, no row outside is touched.
+__device__ __forceinline__ SeqRange seq_range(const PromptArgs& a, int b) {
+  SeqRange r;
+  r.q0 = min(max(a.cu_q[b], 0), a.tokens);
+  r.q1 = min(max(a.cu_q[b + 1], r.q0), a.tokens);
+  r.k0 = min(max(a.cu_k[b], 0), a.kv_tokens);
+  r.k1 = min(max(a.cu_k[b + 1], r.k0), a.kv_tokens);
+  return r;
+}
+
+// Row tile `tile` counted over all sequences: its sequence (-1: none) and its place in it.
+__device__ __forceinline__ int find_tile(const PromptArgs& a, int tile, int& at) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+    int n = 0;
+    if (b0 + lane < a.n_seqs) {
+      const int q0 = min(max(a.cu_q[b0 + lane], 0), a.tokens);
+      const int q1 = min(max(a.cu_q[b0 + lane + 1], q0), a.tokens);
+      n = ((q1 - q0) * a.group + kFlRows - 1) / kFlRows;
+    }
+    int incl = n;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int o = __shfl_up(incl, s, 64);
+      if (lane >= s) incl += o;
+    }
+    const uint64_t past = __ballot(base + incl > tile);
+    if (past) {
+      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      at = tile - base - __shfl(incl - n, l, 64);
+      return b0 + l;
+    }
+    base += __shfl(incl, 63, 64);
+  }
+  return -1;
+}
+
+template <int D>
+__global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
+  __shared__ __align__(16) char lds[flash_lds<D>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hf = lane >> 5;
+  const int h = blockIdx.x % a.kv_heads;
+  int at;
+  const int b = __builtin_amdgcn_readfirstlane(find_tile(a, a.tiles - 1 - static_cast<int>(blockIdx.x / a.kv_heads), at));
+  if (b < 0) return;
+  const SeqRange sr = seq_range(a, b);
+  const int lq = sr.q1 - sr.q0, lk = sr.k1 - sr.k0, rows = lq * a.group;
+  // reversed within the sequence as over all: the tiles with most keys first
+  const int row0 = at * kFlRows, wr0 = row0 + 32 * wave;
+  const int r = min(wr0 + n, rows - 1), tok = r / a.group, hd = h * a.group + r % a.group;
+  const int shift = lk - lq;                        // query i sees the keys up to i + shift
+  const int lim = a.causal ? tok + shift : lk - 1;
+  const int w_first = min(wr0, rows - 1) / a.group, w_last = min(wr0 + 31, rows - 1) / a.group;
+  const int w_min = a.causal ? w_first + shift : lk - 1, w_max = a.causal ? w_last + shift : lk - 1;
+  const int b_min = a.causal ? row0 / a.group + shift : lk - 1;
+  const int b_last = min(row0 + kFlRows - 1, rows - 1) / a.group;
+  const int t1 = ((a.causal ? b_last + shift : lk - 1) + kFlKeys) / kFlKeys;   // <= 0 where no key is seen
+
+  bf16x8 q[D / 16];
+  const uint16_t* qp = a.q + (sr.q0 + static_cast<int64_t>(tok)) * a.q_token + hd * a.q_head + 8 * hf;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) q[ks] = as_bf16x8(ldg16(qp + 16 * ks));
+  FlashRows<D> st;
+  st.m = kNegInf;
+  st.l = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
+
+  const uint16_t* kb = a.k + sr.k0 * a.k_token + h * a.k_head;
+  const uint16_t* vb = a.v + sr.k0 * a.v_token + h * a.v_head;
+  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int64_t& ks, int64_t& vs, int& last) {
+    // rows past the sequence's end (another one's, or none): its last row again
+    const int key = min(t * kFlKeys + row, lk - 1);
+    kp = kb + key * a.k_token;
+    vp = vb + key * a.v_token;
+    ks = a.k_token;
+    vs = a.v_token;
+    last = lk - 1 - key;
+  };
+  flash<D, kFlWaves>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, src, st);
+
+  const float l = sum_across32(st.l);
+  const float inv = lim >= 0 ? 1.0f / l : 0.0f;     // a row that sees no key: zeros
+  uint16_t* op = a.out + (sr.q0 + static_cast<int64_t>(tok)) * a.o_token + hd * a.o_head;
+  const bool live = wr0 + n < rows;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      // a lane half has elements 8 a + 4 hf .. +4 of a = 2c, 2c + 1: swapped, half hf has all 8 of a = 2c + hf
+      uint32_t lo[2], hi[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        lo[i] = pack_bf16(st.o[dt][8 * c + 2 * i] * inv, st.o[dt][8 * c + 2 * i + 1] * inv);
+        hi[i] = pack_bf16(st.o[dt][8 * c + 4 + 2 * i] * inv, st.o[dt][8 * c + 4 + 2 * i + 1] * inv);
+      }
+      const auto s0 = __builtin_amdgcn_permlane32_swap(lo[0], hi[0], false, false);
+      const auto s1 = __builtin_amdgcn_permlane32_swap(lo[1], hi[1], false, false);
+      if (live) *reinterpret_cast<u32x4*>(op + 32 * dt + 16 * c + 8 * hf) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+    }
+}
+
+// ------------------------------------------------------------------ prefix
+struct PrefixArgs {
+  const uint16_t* q;
+  CacheView c;
+  const int32_t* pages;
+  float *po, *pml;
+  int64_t q_token, q_head, rows;     // rows: batch * q_len * group
+  float c2;
+  int32_t kv_heads, group, len, splits, row_tiles;
+};
+
+template <int D>
+__global__ __launch_bounds__(kFlThreads, 2) void k_prefix(const PrefixArgs a) {
+  __shared__ __align__(16) char lds[flash_lds<D>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hf = lane >> 5;
+  const int h = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
+  const int split = rest / a.row_tiles;
+  const int64_t wr0 = static_cast<int64_t>(rest % a.row_tiles) * kFlRows + 32 * wave;
+  const int tiles = (a.len + kFlKeys - 1) / kFlKeys;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  const int64_t r = min(wr0 + n, a.rows - 1), tok = r / a.group;
+  const int hd = h * a.group + static_cast<int>(r % a.group);
+
+  bf16x8 q[D / 16];
+  const uint16_t* qp = a.q + tok * a.q_token + hd * a.q_head + 8 * hf;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) q[ks] = as_bf16x8(ldg16(qp + 16 * ks));
+  FlashRows<D> st;
+  st.m = kNegInf;
+  st.l = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
+  bool bad = false;
+  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int64_t& ks, int64_t& vs, int& last) {
+    const int key = min(t * kFlKeys + row, a.len - 1);
+    int id = a.pages[key >> a.c.page_shift];
+    if (id < 0 || id >= a.c.n_pages) {
+      bad = true;
+      id = 0;
+    }
+    const int in_page = key & ((1 << a.c.page_shift) - 1);
+    const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
+    kp = a.c.k + base;
+    vp = a.c.v + base;
+    ks = D;
+    vs = D;
+    last = a.len - 1 - key;
+  };
+  const int w_max = wr0 < a.rows ? a.len - 1 : -1;    // a wave without rows only loads
+  flash<D, kFlWaves>(q, t0, t1, a.len - 1, a.len - 1, w_max, kNoMask, a.c2, lds, src, st);
+  // a page outside the cache: the waves load different rows, so all tell
+  const bool any_bad = __syncthreads_or(bad);
+  const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
+  if (wr0 + n < a.rows) {
+    const int64_t at = (static_cast<int64_t>(split) * a.kv_heads + h) * a.rows + r;
+    float* op = a.po + at * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<f32x4*>(op + 32 * dt + 8 * c + 4 * hf) =
+            f32x4{st.o[dt][4 * c], st.o[dt][4 * c + 1], st.o[dt][4 * c + 2], st.o[dt][4 * c + 3]};
+    if (hf == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = float2{st.m, l};
+  }
+}
+
+}  // namespace
+
+int prefix_splits(int64_t rows, int kv_heads, int prefix_len) {
+  const int64_t blocks = (rows + kFlRows - 1) / kFlRows * kv_heads;
+  const int64_t tiles = (prefix_len + kFlKeys - 1) / kFlKeys;
+  const int64_t want = (512 + blocks - 1) / blocks;     // two workgroups a CU
+  return static_cast<int>(want < tiles ? want : tiles);   // at most 512
+}
+
+hipError_t launch_prefix(const dsk_paged_desc& d, const void* q, const dsk_kv_cache& c, const int32_t* prefix,
+                         int splits, float* pre_o, float* pre_ml, hipStream_t s) {
+  const int group = d.heads / d.kv_heads;
+  const int64_t rows = static_cast<int64_t>(d.batch) * d.q_len * group;
+  const int row_tiles = static_cast<int>((rows + kFlRows - 1) / kFlRows);
+  const PrefixArgs a{static_cast<const uint16_t*>(q), cache_view(c), prefix, pre_o, pre_ml, d.q_token, d.q_head,
+                     rows, d.scale * kLog2e, d.kv_heads, group, d.prefix_len, splits, row_tiles};
+  const unsigned blocks = static_cast<unsigned>(row_tiles) * splits * d.kv_heads;
+  if (d.head_dim == 64) launch_kernel(k_prefix<64>, blocks, kFlThreads, 0, s, a);
+  else launch_kernel(k_prefix<128>, blocks, kFlThreads, 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k, const void* v, const int32_t* cu_q,
+                         const int32_t* cu_k, void* out, hipStream_t s) {
+  const int group = d.heads / d.kv_heads;
+  // every sequence's last tile may be partly filled
+  const int64_t tiles = static_cast<int64_t>(d.tokens) * group / kFlRows + d.n_seqs;
+  const PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                     static_cast<uint16_t*>(out), cu_q, cu_k, d.q_token, d.q_head, d.k_token, d.k_head, d.v_token,
+                     d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
+                     group, d.causal, static_cast<int32_t>(tiles)};
+  const unsigned blocks = static_cast<unsigned>(tiles * d.kv_heads);
+  if (d.head_dim == 64) launch_kernel(k_prompt<64>, blocks, kFlThreads, 0, s, a);
+  else launch_kernel(k_prompt<128>, blocks, kFlThreads, 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace dsk

@@ -59,7 +59,42 @@ class Residual(ctypes.Structure):
     _fields_ = [("h", _vp), ("d", _vp), ("gamma", _vp), ("eps", ctypes.c_float), ("h_out", _vp), ("x_out", _vp)]
 
 
+class KVCache(ctypes.Structure):
+    """Mirror of ``dsk_kv_cache``."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("table_stride", _i64), ("n_pages", _i32),
+                ("page_size", _i32), ("n_seqs", _i32), ("max_pages", _i32)]
+
+
+class QkDesc(ctypes.Structure):
+    """Mirror of ``dsk_qk_desc``."""
+
+    _fields_ = ([(n, _i32) for n in ("tokens", "heads", "kv_heads", "head_dim", "dtype", "norm", "rot_dim", "rot_first",
+                                     "interleaved", "prefix_len")]
+                + [("eps", ctypes.c_float), ("mscale", ctypes.c_float)]
+                + [(n, _i64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "qo_token",
+                                       "qo_head", "ko_token", "ko_head")])
+
+
+class PromptDesc(ctypes.Structure):
+    """Mirror of ``dsk_prompt_desc``."""
+
+    _fields_ = ([(n, _i32) for n in ("tokens", "kv_tokens", "n_seqs", "heads", "kv_heads", "head_dim", "causal")]
+                + [("scale", ctypes.c_float)]
+                + [(n, _i64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "o_token",
+                                       "o_head")])
+
+
+class PagedDesc(ctypes.Structure):
+    """Mirror of ``dsk_paged_desc``."""
+
+    _fields_ = ([(n, _i32) for n in ("batch", "q_len", "heads", "kv_heads", "head_dim", "prefix_len")]
+                + [("scale", ctypes.c_float)]
+                + [(n, _i64) for n in ("q_token", "q_head", "o_token", "o_head")])
+
+
 PDesc = ctypes.POINTER(Desc)
+PCache = ctypes.POINTER(KVCache)
 
 SIGNATURES = {
     "dsk_abi_version": (ctypes.c_int, []),
@@ -88,6 +123,12 @@ SIGNATURES = {
     "dsk_q3_dequant": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
     "dsk_q3_repack": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp]),
     "dsk_fp8_block_dequant": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "dsk_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "dsk_kv_append": (ctypes.c_int, [ctypes.POINTER(QkDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, PCache, _vp,
+                                     _vp, _vp]),
+    "dsk_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "dsk_paged_attention_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache, ctypes.POINTER(_sz)]),
+    "dsk_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedDesc), _vp, PCache, _vp, _vp, _vp, _vp, _sz, _vp]),
     "dsk_rmsnorm": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, ctypes.c_float, _i32, _vp, _vp, _vp]),
 }
 

@@ -1,0 +1,291 @@
+"""The attention half of a decoder layer: per-head norms and rotation, a paged
+key / value cache, attention over packed prompts and over the cache.
+
+Functions on torch tensors of one HIP device (any device, on its current
+stream); outputs are bf16 and are allocated unless given.  Queries, keys and
+values are [tokens, heads, head_dim] with any token and head strides that keep
+16-byte pieces (so views of one fused projection do); a head's elements are
+contiguous.  Outputs must not overlap inputs, except where said.
+
+    freq, mscale = rope_frequencies(128, base=10000.0, device="cuda")
+    q = kv_append(q, k, v, positions, seq, table, k_cache, v_cache, freq, q_gamma=gq, k_gamma=gk)
+    o = paged_attention(q, k_cache, v_cache, table, lens)
+
+``Attention`` is a whole sublayer (projections, norms, rotation, cache,
+attention, output projection) for ``MoEStack``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from . import _lib
+
+_F32, _BF16, _I32, _F64 = torch.float32, torch.bfloat16, torch.int32, torch.float64
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                     original_len: int = 4096, turns: tuple[float, float] = (1.0, 32.0),
+                     device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """(freq, mscale): radians per position of the rot_dim / 2 pairs (float64) and the
+    factor on the rotated elements.
+
+    ``scaling`` for contexts longer than the ``original_len`` that a model was trained on, by ``factor``:
+    "linear" turns every pair ``factor`` times slower; "base" raises the base so that the slowest pair does and
+    the quickest keeps its frequency; "ramp" keeps the pairs that make ``turns[1]`` turns or more over
+    ``original_len``, slows those that make ``turns[0]`` or less, blends between, and sets
+    mscale = 0.1 ln(factor) + 1."""
+    if rot_dim < 16 or rot_dim % 16:
+        raise ValueError(f"rot_dim must be a positive multiple of 16, got {rot_dim}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError(f"base must be positive and finite, got {base}")
+    if not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError(f"factor must be at least 1 and finite, got {factor}")
+    mscale = 1.0
+    if scaling == "base":
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freq = base ** (-torch.arange(0, rot_dim, 2, dtype=_F64) / rot_dim)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "ramp":
+        lo, hi = turns
+        if not 0 < lo < hi or original_len < 1:
+            raise ValueError("ramp scaling needs 0 < turns[0] < turns[1] and original_len >= 1")
+        keep = ((original_len * freq / (2.0 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
+        freq = freq * (keep + (1.0 - keep) / factor)
+        mscale = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "base"):
+        raise ValueError(f"scaling must be 'linear', 'base', 'ramp' or None, got {scaling!r}")
+    return freq.to(device), mscale
+
+
+# ------------------------------------------------------------------ checks
+def _rows(t: torch.Tensor, what: str, dtypes: tuple, dev: torch.device) -> None:
+    if t.device != dev:
+        raise ValueError(f"{what} is on {t.device}, not on {dev}")
+    if t.dim() != 3:
+        raise ValueError(f"{what} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
+    if t.stride(2) != 1:
+        raise ValueError(f"the elements of a head of {what} must be contiguous")
+
+
+def _vector(t: torch.Tensor, what: str, dtype: torch.dtype, n: int, dev: torch.device) -> None:
+    if t.device != dev or t.dtype != dtype or t.dim() != 1 or t.shape[0] < n or t.stride(0) != 1:
+        raise ValueError(f"{what} must be a contiguous {str(dtype)[6:]} vector of {n} elements on {dev}, "
+                         f"got {str(t.dtype)[6:]} {tuple(t.shape)} on {t.device}")
+
+
+def _exact(t: torch.Tensor, what: str, dtype: torch.dtype, n: int, dev: torch.device) -> None:
+    _vector(t, what, dtype, n, dev)
+    if t.shape[0] != n:
+        raise ValueError(f"{what} must have {n} elements, got {t.shape[0]}")
+
+
+def _hip(t: torch.Tensor) -> torch.device:
+    if not t.is_cuda:
+        raise ValueError(f"dsk_moe needs HIP device tensors, got a {t.device} tensor")
+    return t.device
+
+
+def _out(out: torch.Tensor | None, shape: tuple, dev: torch.device, what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=_BF16, device=dev)
+    _rows(out, what, (_BF16,), dev)
+    if tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(out.shape)}")
+    return out
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """The entry point on ``dev``'s current stream, with ``dev`` current."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, stream)
+
+
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, kv_heads: int, dim: int,
+           dev: torch.device) -> _lib.KVCache:
+    for t, what in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.device != dev or t.dtype != _BF16 or t.dim() != 4 or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous bf16 [pages, kv_heads, page_size, head_dim] on {dev}")
+    if k_cache.shape != v_cache.shape or k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim:
+        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} do not fit {kv_heads} key heads of {dim}")
+    if table.device != dev or table.dtype != _I32 or table.dim() != 2 or table.stride(1) != 1:
+        raise ValueError(f"table must be int32 [sequences, pages] on {dev} with contiguous rows")
+    return _lib.KVCache(k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), table.stride(0), k_cache.shape[0],
+                        k_cache.shape[2], table.shape[0], table.shape[1])
+
+
+# Descriptors hold sizes and strides alone, so calls of one shape share one.
+_qk_desc = functools.lru_cache(maxsize=256)(_lib.QkDesc)
+_prompt_desc = functools.lru_cache(maxsize=256)(_lib.PromptDesc)
+_paged_desc = functools.lru_cache(maxsize=256)(_lib.PagedDesc)
+
+
+# ------------------------------------------------------------------ norms, rotation, append
+def _qk(q, k, v, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gamma, norm, eps, q_out, k_out, want_k,
+        prefix_len):
+    """Checked arguments of the two entry points: device, descriptor, outputs."""
+    dev = _hip(k)
+    _rows(k, "k", (_BF16, _F32), dev)
+    tokens, kv_heads, dim = k.shape
+    if tokens < 1:
+        raise ValueError("k has no tokens")
+    heads, qs = 0, (0, 0, 0)
+    if q is not None:
+        _rows(q, "q", (k.dtype,), dev)
+        heads, qs = q.shape[1], q.stride()
+        if q.shape[0] != tokens or q.shape[2] != dim:
+            raise ValueError(f"q {tuple(q.shape)} does not fit k {tuple(k.shape)}")
+        q_out = _out(q_out, q.shape, dev, "q_out")
+    elif q_out is not None or q_gamma is not None:
+        raise ValueError("q_out and q_gamma need q")
+    _exact(positions, "positions", _I32, tokens, dev)
+    rot = 0
+    if freq is not None:
+        rot = 2 * freq.numel()
+        _exact(freq, "freq", _F64, rot // 2, dev)
+    for g, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        if g is not None:
+            _exact(g, what, _F32, dim, dev)
+    if want_k or k_out is not None:
+        k_out = _out(k_out, k.shape, dev, "k_out")
+    vs = (0, 0, 0)
+    if v is not None:
+        _rows(v, "v", (k.dtype,), dev)
+        if v.shape != k.shape:
+            raise ValueError(f"v {tuple(v.shape)} does not fit k {tuple(k.shape)}")
+        vs = v.stride()
+    ks = k.stride()
+    qo = q_out.stride() if q_out is not None else (0, 0, 0)
+    ko = k_out.stride() if k_out is not None else (0, 0, 0)
+    desc = _qk_desc(tokens, heads, kv_heads, dim, _lib.DTYPE_BF16 if k.dtype == _BF16 else _lib.DTYPE_F32,
+                    1 if norm else 0, rot, int(rot_first), 1 if interleaved else 0, int(prefix_len), float(eps),
+                    float(mscale), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qo[0], qo[1], ko[0], ko[1])
+    return dev, desc, q_out, k_out
+
+
+def _p(t: torch.Tensor | None):
+    return t.data_ptr() if t is not None else None
+
+
+def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor | None = None, *,
+                 interleaved: bool = False, rot_first: int = 0, mscale: float = 1.0,
+                 q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, norm: bool = True,
+                 eps: float = 1e-6, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor | None, torch.Tensor]:
+    """``dsk_qk_norm_rope``: RMS norm of every head of q and k (``norm``; gammas [head_dim] float32) and the rotation of
+    elements rot_first .. rot_first + 2 len(freq) by positions[t] * freq (``interleaved``: pairs (2i, 2i+1), otherwise (i,
+    i + len(freq))), in one pass.  q and k bf16 or float32; the results bf16.  Tokens at negative positions are left out
+    (their output rows are not written).  q_out / k_out may be q / k themselves."""
+    dev, desc, q_out, k_out = _qk(q, k, None, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gamma, norm, eps,
+                                  q_out, k_out, True, 0)
+    _call(dev, "dsk_qk_norm_rope", ctypes.byref(desc), _p(q), k.data_ptr(), positions.data_ptr(), _p(freq), _p(q_gamma),
+          _p(k_gamma), _p(q_out), k_out.data_ptr())
+    return q_out, k_out
+
+
+def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq: torch.Tensor,
+              table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, freq: torch.Tensor | None = None, *,
+              prefix_len: int = 0, interleaved: bool = False, rot_first: int = 0, mscale: float = 1.0,
+              q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, norm: bool = True,
+              eps: float = 1e-6, q_out: torch.Tensor | None = None,
+              k_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """``dsk_kv_append``: ``qk_norm_rope`` whose keys, with the values, go to the paged cache: token t to row
+    positions[t] - prefix_len of sequence seq[t] (int32), whose pages are table[seq[t]].  Returns q's result; the keys
+    are also written to ``k_out`` if given.  Tokens outside the table or with a page outside the cache are not kept; two
+    tokens of one call must not share a row."""
+    dev, desc, q_out, k_out = _qk(q, k, v, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gamma, norm, eps,
+                                  q_out, k_out, False, prefix_len)
+    _exact(seq, "seq", _I32, k.shape[0], dev)
+    cache = _cache(k_cache, v_cache, table, k.shape[1], k.shape[2], dev)
+    _call(dev, "dsk_kv_append", ctypes.byref(desc), _p(q), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
+          seq.data_ptr(), _p(freq), _p(q_gamma), _p(k_gamma), ctypes.byref(cache), _p(q_out), _p(k_out))
+    return q_out
+
+
+# ------------------------------------------------------------------ attention
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """``dsk_prompt_attention`` over packed sequences: queries cu_q[s] .. cu_q[s+1] with keys cu_k[s] .. cu_k[s+1] (int32;
+    cu_k: cu_q).  Causal: query i of Lq sees the keys j <= i + Lk - Lq; one that sees no key gives zeros.  scale:
+    head_dim ** -0.5.  Rows of ``out`` behind the last sequence are left as they were."""
+    dev = _hip(q)
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        _rows(t, what, (_BF16,), dev)
+    tokens, heads, dim = q.shape
+    if v.shape != k.shape or k.shape[2] != dim:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    n = cu_q.numel()
+    if cu_k is None:
+        cu_k = cu_q
+    _exact(cu_q, "cu_q", _I32, n, dev)
+    _exact(cu_k, "cu_k", _I32, n, dev)
+    out = _out(out, q.shape, dev, "out")
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    desc = _prompt_desc(tokens, k.shape[0], n - 1, heads, k.shape[1], dim, 1 if causal else 0,
+                        float(scale) if scale is not None else dim ** -0.5,
+                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
+    _call(dev, "dsk_prompt_attention", ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(),
+          cu_k.data_ptr(), out.data_ptr())
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
+                    lens: torch.Tensor, *, prefix: torch.Tensor | None = None, prefix_len: int = 0,
+                    scale: float | None = None, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``dsk_paged_attention``: q [batch, heads, head_dim] (one token of each sequence) or [batch, q_len, heads, head_dim]
+    over lens[s] (int32) keys of sequence s in the cache, the new tokens' among them.  ``prefix`` (int32 page ids) with
+    ``prefix_len`` keys that all sequences see first, read once for the batch.  The result has q's shape.  ``workspace``:
+    uint8, at least ``paged_workspace_size`` bytes; otherwise allocated (inside a graph capture, in the graph's pool)."""
+    dev = _hip(q)
+    batch = table.shape[0] if table.dim() == 2 else 0
+    if q.dim() == 4:
+        if q.shape[1] > 1 and q.shape[0] > 1 and q.stride(0) != q.shape[1] * q.stride(1):
+            raise ValueError("the tokens of q must be evenly spaced")
+        rows = q.flatten(0, 1)
+        if out is not None and (out.dim() != 4 or out.shape != q.shape):
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        if out is not None and out.shape[1] > 1 and out.shape[0] > 1 and out.stride(0) != out.shape[1] * out.stride(1):
+            raise ValueError("the tokens of out must be evenly spaced")
+        q_len = q.shape[1]
+    else:
+        rows, q_len = q, 1
+    _rows(rows, "q", (_BF16,), dev)
+    tokens, heads, dim = rows.shape
+    if batch < 1 or tokens != batch * q_len or q_len < 1:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a table of {batch} sequences")
+    cache = _cache(k_cache, v_cache, table, k_cache.shape[1] if k_cache.dim() == 4 else 0, dim, dev)
+    _exact(lens, "lens", _I32, batch, dev)
+    if prefix_len < 0 or (prefix_len > 0) != (prefix is not None):
+        raise ValueError("prefix and a positive prefix_len go together")
+    if prefix is not None:
+        _vector(prefix, "prefix", _I32, -(-prefix_len // k_cache.shape[2]), dev)
+    res = _out(out.flatten(0, 1) if out is not None and out.dim() == 4 else out, rows.shape, dev, "out")
+    qs, os = rows.stride(), res.stride()
+    desc = _paged_desc(batch, q_len, heads, k_cache.shape[1], dim, int(prefix_len),
+                       float(scale) if scale is not None else dim ** -0.5, qs[0], qs[1], os[0], os[1])
+    if workspace is None:
+        workspace = torch.empty(_workspace_bytes(desc, cache), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous uint8 on {dev}")
+    _call(dev, "dsk_paged_attention", ctypes.byref(desc), rows.data_ptr(), ctypes.byref(cache), lens.data_ptr(),
+          _p(prefix), res.data_ptr(), workspace.data_ptr(), workspace.numel())
+    return out if out is not None else res.view(q.shape)
+
+
+def _workspace_bytes(desc: _lib.PagedDesc, cache: _lib.KVCache) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(n))
+    return n.value

@@ -316,6 +316,113 @@ int dsk_q3_dequant(const uint8_t* packed, const uint16_t* scales,
 int dsk_rmsnorm(const void* x, const void* residual, const float* gamma, int64_t rows,
                 int32_t hidden, float eps, int32_t dtype, void* h_out, void* out, void* stream);
 
+/* ---------------------------------------------------------------- attention
+ * The attention half of a decoder layer between two MoE layers: queries, keys
+ * and values are bf16 rows of `head_dim` (64 or 128) elements, `heads` query
+ * heads share `kv_heads` key heads in groups of heads / kv_heads consecutive
+ * ones.  Scores, softmax statistics and sums are float32.  Strides count
+ * elements; rows are contiguous and 16-byte aligned (strides multiples of 16
+ * bytes).  The reference runs this half in MLX (src/deepseeker/mlx_runner.py:1465). */
+
+/* Paged KV cache.  k and v: [n_pages, kv_heads, page_size, head_dim] bf16;
+ * position p of sequence s is row p % page_size of page
+ * table[s * table_stride + p / page_size].  page_size: 16, 32, 64, 128 or 256. */
+typedef struct dsk_kv_cache {
+  void* k;
+  void* v;
+  const int32_t* table;   /* [n_seqs] rows of max_pages page ids */
+  int64_t table_stride;
+  int32_t n_pages;
+  int32_t page_size;
+  int32_t n_seqs;
+  int32_t max_pages;
+} dsk_kv_cache;
+
+typedef struct dsk_qk_desc {
+  int32_t tokens;         /* T, 1..2^23 */
+  int32_t heads;          /* 0..1024; 0: no queries */
+  int32_t kv_heads;       /* 1..1024 */
+  int32_t head_dim;       /* 64 or 128 */
+  int32_t dtype;          /* DSK_DTYPE_BF16 or _F32: q, k and v; the outputs are bf16 */
+  int32_t norm;           /* 1: every head of q and k is normalised, 0: it is not */
+  int32_t rot_dim;        /* rotated elements of a head: 0, or a multiple of 16 */
+  int32_t rot_first;      /* the first of them, a multiple of 8 */
+  int32_t interleaved;    /* pairs (2i, 2i+1) instead of (i, i + rot_dim / 2) */
+  int32_t prefix_len;     /* dsk_kv_append: a token at position p is row p - prefix_len of its sequence */
+  float eps;
+  float mscale;           /* multiplies the rotated elements (scaled frequencies; otherwise 1) */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;   /* strides of q, k, v */
+  int64_t qo_token, qo_head, ko_token, ko_head;                /* strides of q_out, k_out */
+} dsk_qk_desc;
+
+/* Norms of queries and keys for each head, then their rotation, in one pass.
+ * y = x / sqrt(mean(x^2) + eps) * gamma over one head (d->norm; gammas
+ * [head_dim] f32 or NULL: ones), then for pair i of the rotated elements
+ * (a, b) -> mscale (a cos t - b sin t, b cos t + a sin t), t = position * freq[i]
+ * (freq [rot_dim / 2] f64, radians per position; the angle is reduced in 64
+ * bits).  float32 throughout, one rounding to bf16.  A token at a negative
+ * position is left out: its output rows are not written.  q_out may be q (bf16)
+ * with the same strides, k_out may be k. */
+int dsk_qk_norm_rope(const dsk_qk_desc* d, const void* q, const void* k, const int32_t* positions,
+                     const double* freq, const float* q_gamma, const float* k_gamma, void* q_out,
+                     void* k_out, void* stream);
+
+/* dsk_qk_norm_rope that keeps the rotated keys and the values (rounded to bf16)
+ * in a paged cache: token t goes to row positions[t] - d->prefix_len of sequence
+ * seq[t].  A token whose sequence, row or page lies outside the table or the
+ * cache is not kept (its q_out and k_out are written).  q and q_out are NULL
+ * where d->heads is 0; k_out is optional (NULL: the keys go to the cache
+ * alone).  Two tokens of a call must not share a row. */
+int dsk_kv_append(const dsk_qk_desc* d, const void* q, const void* k, const void* v,
+                  const int32_t* positions, const int32_t* seq, const double* freq, const float* q_gamma,
+                  const float* k_gamma, const dsk_kv_cache* cache, void* q_out, void* k_out, void* stream);
+
+typedef struct dsk_prompt_desc {
+  int32_t tokens;         /* rows of q and out */
+  int32_t kv_tokens;      /* rows of k and v */
+  int32_t n_seqs;         /* 1..65535 */
+  int32_t heads;          /* a multiple of kv_heads, heads / kv_heads <= 64 */
+  int32_t kv_heads;
+  int32_t head_dim;       /* 64 or 128 */
+  int32_t causal;         /* 0: every key of its sequence is visible to a query */
+  float scale;            /* > 0: scores are scale * q.k */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;   /* strides */
+} dsk_prompt_desc;
+
+/* Attention over packed prompts.  Sequence s has the query rows cu_q[s] ..
+ * cu_q[s + 1] and the key rows cu_k[s] .. cu_k[s + 1] (cu_q, cu_k
+ * [n_seqs + 1] i32 ascending; cu_k may be cu_q).  Causal: query i of Lq sees the
+ * keys j <= i + Lk - Lq (its last key is the one at its own end); a query that
+ * sees no key gives zeros.  Rows of out that belong to no sequence are left as
+ * they were.  Bounds outside q or k are cut to them. */
+int dsk_prompt_attention(const dsk_prompt_desc* d, const void* q, const void* k, const void* v,
+                         const int32_t* cu_q, const int32_t* cu_k, void* out, void* stream);
+
+typedef struct dsk_paged_desc {
+  int32_t batch;          /* sequences, 1..65535 */
+  int32_t q_len;          /* query tokens of each, 1..16; q_len * heads / kv_heads <= 64 */
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;       /* 64 or 128 */
+  int32_t prefix_len;     /* keys that all sequences share, 0: none */
+  float scale;            /* > 0 */
+  int64_t q_token, q_head, o_token, o_head;   /* strides; sequence s has tokens s * q_len .. */
+} dsk_paged_desc;
+
+/* Attention of a decode or verify step over a paged cache.  Sequence s has
+ * lens[s] keys of its own (its table row; the new tokens' among them, appended
+ * before) after the prefix_len keys of the pages prefix[0 ..], which are read
+ * once for the whole batch.  Query i of q_len sees the prefix and its
+ * sequence's keys j <= lens[s] - q_len + i; a query that sees no key gives
+ * zeros (lens[s] <= 0 without a prefix: an unused slot).  Lengths beyond the
+ * table row and page ids outside the cache are never followed: the rows that
+ * would need them come out as NaN.  workspace: dsk_paged_attention_workspace_size
+ * bytes, 256-byte aligned, no initialisation; one call at a time. */
+int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, size_t* bytes);
+int dsk_paged_attention(const dsk_paged_desc* d, const void* q, const dsk_kv_cache* cache,
+                        const int32_t* lens, const int32_t* prefix, void* out, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,190 @@
+"""CPU checks of the attention entry points: what they refuse (before any
+launch, so no GPU is needed), the rotation's frequencies, and the float64
+restatement that the GPU tests compare with."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import dsk_moe
+from dsk_moe import _lib
+from dsk_moe import attention as A
+from oracle import attention as O
+
+P = ctypes.c_void_p(1 << 20)
+ODD = ctypes.c_void_p((1 << 20) + 8)
+
+
+def qk_desc(**kw):
+    base = dict(tokens=4, heads=8, kv_heads=2, head_dim=128, dtype=0, norm=1, rot_dim=64, rot_first=0, interleaved=0,
+                prefix_len=0, eps=1e-6, mscale=1.0, q_token=1024, q_head=128, k_token=256, k_head=128, v_token=256,
+                v_head=128, qo_token=1024, qo_head=128, ko_token=256, ko_head=128)
+    return _lib.QkDesc(**{**base, **kw})
+
+
+def cache(**kw):
+    base = dict(k=1 << 20, v=1 << 20, table=1 << 20, table_stride=8, n_pages=40, page_size=64, n_seqs=4, max_pages=8)
+    return _lib.KVCache(**{**base, **kw})
+
+
+def prompt_desc(**kw):
+    base = dict(tokens=10, kv_tokens=10, n_seqs=2, heads=8, kv_heads=2, head_dim=64, causal=1, scale=0.1, q_token=512,
+                q_head=64, k_token=128, k_head=64, v_token=128, v_head=64, o_token=512, o_head=64)
+    return _lib.PromptDesc(**{**base, **kw})
+
+
+def paged_desc(**kw):
+    base = dict(batch=4, q_len=1, heads=8, kv_heads=2, head_dim=128, prefix_len=0, scale=0.1, q_token=1024, q_head=128,
+                o_token=1024, o_head=128)
+    return _lib.PagedDesc(**{**base, **kw})
+
+
+def code(name, *args):
+    with pytest.raises(_lib.DskError) as e:
+        _lib.call(name, *args)
+    return e.value.code
+
+
+def rope_code(desc, q=P, k=P, pos=P, freq=P, gq=P, gk=P, qo=P, ko=P):
+    return code("dsk_qk_norm_rope", ctypes.byref(desc), q, k, pos, freq, gq, gk, qo, ko, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(tokens=0), -1), (dict(head_dim=96), -3), (dict(heads=-1), -1), (dict(heads=1025), -1), (dict(kv_heads=0), -1),
+    (dict(dtype=2), -1), (dict(rot_dim=24), -1), (dict(rot_dim=144), -1), (dict(rot_first=4), -1),
+    (dict(rot_first=72), -1), (dict(rot_dim=-16), -1), (dict(eps=-1.0), -1), (dict(eps=math.nan), -1),
+    (dict(mscale=math.inf), -1), (dict(norm=0), -1), (dict(q_token=1025), -2), (dict(k_head=-8), -1),
+    (dict(dtype=1, q_token=1026), -2), (dict(qo_head=64), -1), (dict(ko_token=0), -1), (dict(qo_token=1020), -1),
+    (dict(tokens=(1 << 23) + 1), -3)])
+def test_norm_rope_refuses(kw, want):
+    assert rope_code(qk_desc(**kw)) == want
+
+
+def test_norm_rope_refuses_pointers():
+    assert rope_code(qk_desc(), q=None) == -1 and rope_code(qk_desc(), ko=None) == -1
+    assert rope_code(qk_desc(), freq=None) == -1 and rope_code(qk_desc(heads=0)) == -1
+    assert rope_code(qk_desc(), q=ODD) == -2 and rope_code(qk_desc(), ko=ODD) == -2
+    assert rope_code(qk_desc(), pos=ctypes.c_void_p(5)) == -2
+    assert code("dsk_qk_norm_rope", None, P, P, P, P, P, P, P, P, None) == -1
+
+
+@pytest.mark.parametrize("kw,want", [(dict(k=None), -1), (dict(table=None), -1), (dict(page_size=48), -1),
+                                     (dict(page_size=512), -1), (dict(n_pages=0), -1), (dict(n_seqs=0), -1),
+                                     (dict(max_pages=0), -1), (dict(table_stride=7), -1), (dict(v=(1 << 20) + 8), -2),
+                                     (dict(max_pages=1 << 24, table_stride=1 << 24), -3)])
+def test_cache_refuses(kw, want):
+    c = cache(**kw)
+    args = [P] * 7
+    assert code("dsk_kv_append", ctypes.byref(qk_desc()), P, P, P, P, P, P, P, P, ctypes.byref(c), P, P, None) == want
+    size = ctypes.c_size_t()
+    assert code("dsk_paged_attention_workspace_size", ctypes.byref(paged_desc()), ctypes.byref(c), ctypes.byref(size)) == want
+
+
+def test_append_refuses():
+    call = lambda d, v=P, seq=P, c=cache(), ko=None: code(  # noqa: E731
+        "dsk_kv_append", ctypes.byref(d), P, P, v, P, seq, P, P, P, ctypes.byref(c) if c else None, P, ko, None)
+    assert call(qk_desc(), v=None) == -1 and call(qk_desc(), seq=None) == -1 and call(qk_desc(), c=None) == -1
+    assert call(qk_desc(prefix_len=-1)) == -1 and call(qk_desc(v_token=250)) == -2 and call(qk_desc(), v=ODD) == -2
+    assert call(qk_desc(ko_token=0), ko=P) == -1
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(tokens=0), -1), (dict(kv_tokens=0), -1), (dict(n_seqs=0), -1), (dict(n_seqs=65536), -1), (dict(head_dim=80), -3),
+    (dict(heads=9), -1), (dict(heads=0), -1), (dict(heads=130, kv_heads=2), -1), (dict(scale=0.0), -1),
+    (dict(scale=math.nan), -1), (dict(tokens=1 << 28), -3), (dict(kv_tokens=1 << 30), -3), (dict(k_token=130), -2),
+    (dict(o_token=256), -1), (dict(n_seqs=65535, heads=1024, kv_heads=1024), -3)])
+def test_prompt_refuses(kw, want):
+    assert code("dsk_prompt_attention", ctypes.byref(prompt_desc(**kw)), P, P, P, P, P, P, None) == want
+
+
+def test_prompt_refuses_pointers():
+    for i in range(6):
+        args = [P] * 6
+        args[i] = None
+        assert code("dsk_prompt_attention", ctypes.byref(prompt_desc()), *args, None) == -1
+        args[i] = ctypes.c_void_p((1 << 20) + 2)
+        assert code("dsk_prompt_attention", ctypes.byref(prompt_desc()), *args, None) == -2
+
+
+@pytest.mark.parametrize("kw,want", [(dict(batch=0), -1), (dict(batch=3), -1), (dict(q_len=0), -3), (dict(q_len=17), -3),
+                                     (dict(q_len=9, heads=16), -3), (dict(prefix_len=-1), -1), (dict(prefix_len=1 << 30), -1),
+                                     (dict(scale=-1.0), -1), (dict(q_head=60), -2), (dict(o_head=0), -1),
+                                     (dict(head_dim=256), -3)])
+def test_paged_refuses(kw, want):
+    size = ctypes.c_size_t()
+    assert code("dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache()),
+                ctypes.byref(size)) == want
+    assert code("dsk_paged_attention", ctypes.byref(paged_desc(**kw)), P, ctypes.byref(cache()), P, P, P, P, 1 << 40,
+                None) == want
+
+
+def test_paged_refuses_pointers_and_space():
+    call = lambda d, q=P, lens=P, prefix=None, out=P, ws=P, n=1 << 40: code(  # noqa: E731
+        "dsk_paged_attention", ctypes.byref(d), q, ctypes.byref(cache()), lens, prefix, out, ws, n, None)
+    assert call(paged_desc(), q=None) == -1 and call(paged_desc(), lens=None) == -1 and call(paged_desc(), ws=None) == -1
+    assert call(paged_desc(prefix_len=5)) == -1
+    assert call(paged_desc(), out=ODD) == -2 and call(paged_desc(), ws=ctypes.c_void_p((1 << 20) + 128)) == -2
+    assert call(paged_desc(), n=1024) == -5
+
+
+def test_paged_workspace_grows_with_the_batch():
+    size = lambda **kw: (lambda n: (_lib.call(  # noqa: E731
+        "dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache(n_seqs=kw.get("batch", 4))),
+        ctypes.byref(n)), n.value)[1])(ctypes.c_size_t())
+    assert 0 < size() < size(batch=8) and size() < size(prefix_len=1) and size() % 256 == 0
+
+
+def test_functions_refuse_cpu_tensors():
+    q = torch.zeros(4, 8, 128, dtype=torch.bfloat16)
+    i = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="HIP device"):
+        dsk_moe.qk_norm_rope(q, q, i)
+    with pytest.raises(ValueError, match="HIP device"):
+        dsk_moe.prompt_attention(q, q, q, i)
+    with pytest.raises(ValueError, match="HIP device"):
+        dsk_moe.paged_attention(q, q, q, i, i)
+
+
+def test_frequencies():
+    f, m = dsk_moe.rope_frequencies(64, 10000.0, device="cpu")
+    assert f.dtype == torch.float64 and f.shape == (32,) and m == 1.0
+    assert f[0] == 1.0 and math.isclose(float(f[31]), 10000.0 ** (-62 / 64), rel_tol=1e-14)
+    g, m = dsk_moe.rope_frequencies(64, scaling="linear", factor=4.0, device="cpu")
+    assert m == 1.0 and torch.allclose(g, f / 4, rtol=1e-14)
+    g, _ = dsk_moe.rope_frequencies(64, scaling="base", factor=4.0, device="cpu")
+    assert g[0] == 1.0 and math.isclose(float(g[31]), float(f[31]) / 4, rel_tol=1e-12)
+    g, m = dsk_moe.rope_frequencies(64, scaling="ramp", factor=4.0, original_len=4096, device="cpu")
+    turns = 4096 * f / (2 * math.pi)
+    assert math.isclose(m, 0.1 * math.log(4.0) + 1.0)
+    assert torch.equal(g[turns >= 32], f[turns >= 32]) and torch.allclose(g[turns <= 1], f[turns <= 1] / 4, rtol=1e-14)
+    mid = (turns > 1) & (turns < 32)
+    assert mid.any() and bool(((g < f) & (g > f / 4))[mid].all())
+    for kw in (dict(rot_dim=24), dict(rot_dim=0), dict(rot_dim=32, base=-1.0), dict(rot_dim=32, scaling="other"),
+               dict(rot_dim=32, scaling="linear", factor=0.5), dict(rot_dim=32, scaling="ramp", factor=2.0, turns=(4.0, 4.0))):
+        with pytest.raises(ValueError):
+            dsk_moe.rope_frequencies(**{"device": "cpu", **kw})
+
+
+# ------------------------------------------------------------------ the restatement itself
+def test_oracle_rotation_is_a_complex_turn():
+    x = torch.randn(3, 2, 32, dtype=torch.float64)
+    pos, f = torch.tensor([0, 5, 1 << 20]), torch.tensor([1.0, 0.1, 0.01, 0.001] * 2, dtype=torch.float64)
+    y, _ = O.norm_rope(x, pos, f, interleaved=True, rot_first=8, norm=False)
+    z = torch.view_as_complex(x[..., 8:24].reshape(3, 2, 8, 2).contiguous())
+    z = z * torch.polar(torch.ones(8, dtype=torch.float64), pos.double()[:, None] * f)[:, None]
+    assert torch.allclose(torch.view_as_real(z).flatten(-2), y[..., 8:24], atol=1e-12)
+    assert torch.equal(y[..., :8], x[..., :8]) and torch.equal(y[..., 24:], x[..., 24:])
+
+
+def test_oracle_attention_against_torch():
+    q, k, v = (torch.randn(n, 4, 16, dtype=torch.float64) for n in (5, 9, 9))
+    o, _ = O.attention(q, k, v, torch.arange(5) + 4, 0.25)
+    mask = torch.arange(9)[None] <= torch.arange(5)[:, None] + 4
+    want = torch.nn.functional.scaled_dot_product_attention(*(t.transpose(0, 1) for t in (q, k, v)), attn_mask=mask, scale=0.25)
+    assert torch.allclose(o, want.transpose(0, 1), atol=1e-12)
+    o, _ = O.attention(q, k, v, torch.tensor([-2, -1, 0, 1, 2]), 0.25)
+    assert not o[:2].any() and torch.allclose(o[2], v[0])

@@ -1,0 +1,604 @@
+"""GPU parity of the attention kernels with the float64 restatement, value by
+value within the rounding errors that it derives (``oracle/attention.py``):
+norm and rotation, the append to a paged cache, prompts and decode steps, with
+and without a shared prefix; then a run of them as a server would make it,
+captured and eager."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import dsk_moe
+from dsk_moe import _lib
+from oracle import attention as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+NAN, INF = math.nan, math.inf
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, *shape, dtype=BF16):
+    return torch.randn(shape, generator=g).to(dtype)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=I32, device=DEV)
+
+
+def assert_within(got, want, tol, what=""):
+    got = got.detach().cpu().double()
+    assert not got.isnan().any(), f"{what}: NaN"
+    over = ((got - want).abs() / tol).max() if got.numel() else 0.0
+    assert over <= 1.0, f"{what}: off by {float(over):.3f} of what the roundings allow"
+
+
+# ------------------------------------------------------------------ norm and rotation
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,rot,first,inter", [(128, 128, 0, False), (128, 128, 0, True), (128, 64, 64, False),
+                                                 (128, 32, 8, True), (64, 64, 0, False), (64, 16, 48, False),
+                                                 (64, 48, 16, True), (128, 0, 0, False)])
+@pytest.mark.parametrize("tokens,heads,kv", [(1, 32, 8), (5, 3, 1), (600, 9, 4)])
+def test_norm_rope(dtype, dim, rot, first, inter, tokens, heads, kv):
+    print(f"norm_rope {dtype} {dim} {rot}+{first} inter={inter} {tokens}x{heads},{kv}", flush=True)
+    g = gen(dim + rot + first + tokens)
+    q, k = normal(g, tokens, heads, dim, dtype=dtype) * 3, normal(g, tokens, kv, dim, dtype=dtype)
+    pos = torch.randint(0, 5000, (tokens,), generator=g, dtype=I32)
+    gq, gk = torch.rand(dim, generator=g) + 0.5, torch.randn(dim, generator=g)
+    freq = dsk_moe.rope_frequencies(rot, device="cpu")[0] if rot else None
+    kw = dict(interleaved=inter, rot_first=first, mscale=1.25)
+    got_q, got_k = dsk_moe.qk_norm_rope(q.to(DEV), k.to(DEV), pos.to(DEV), freq.to(DEV) if rot else None, q_gamma=gq.to(DEV),
+                                        k_gamma=gk.to(DEV), **kw)
+    assert got_q.dtype == got_k.dtype == BF16
+    assert_within(got_q, *O.norm_rope(q, pos, freq, gamma=gq, **kw), "q")
+    assert_within(got_k, *O.norm_rope(k, pos, freq, gamma=gk, **kw), "k")
+
+
+def test_far_positions_and_padding():
+    """Angles of positions up to 2^31 - 1; tokens at negative positions keep their output rows."""
+    g = gen(3)
+    pos = torch.tensor([(1 << 31) - 1, 123456789, -1, 0, -(1 << 31), 1 << 20], dtype=I32)
+    q, k = normal(g, 6, 4, 128), normal(g, 6, 2, 128)
+    freq, mscale = dsk_moe.rope_frequencies(128, 1e6, scaling="ramp", factor=8.0, device="cpu")
+    qo, ko = torch.full((6, 4, 128), 7.0, dtype=BF16, device=DEV), torch.full((6, 2, 128), 8.0, dtype=BF16, device=DEV)
+    dsk_moe.qk_norm_rope(q.to(DEV), k.to(DEV), pos.to(DEV), freq.to(DEV), mscale=mscale, q_out=qo, k_out=ko)
+    live = pos >= 0
+    for x, o, fill in ((q, qo, 7.0), (k, ko, 8.0)):
+        y, tol = O.norm_rope(x, pos, freq, mscale=mscale)
+        # positions * freq / (2 pi) in float64 at 2^31: 2^-21 of a turn
+        tol = tol + 2 * math.pi * 2.0 ** -21 * 2.0 ** -1 * x.double().abs().amax(-1, keepdim=True) * 4
+        assert_within(o.cpu()[live], y[live], tol[live])
+        assert (o.cpu()[~live] == fill).all()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_norm_rope_views_and_in_place(inter):
+    """Views of one projection's rows, heads-first layouts, and the results written over the inputs."""
+    g = gen(4)
+    qkv = normal(g, 33, (6 + 2 + 2) * 64).to(DEV)
+    q, k, _ = (p.unflatten(1, (-1, 64)) for p in qkv.split([384, 128, 128], 1))
+    pos, freq = torch.arange(33, dtype=I32, device=DEV), dsk_moe.rope_frequencies(64)[0]
+    want = dsk_moe.qk_norm_rope(q.contiguous(), k.contiguous(), pos, freq, interleaved=inter)
+    for a, b in zip(dsk_moe.qk_norm_rope(q, k, pos, freq, interleaved=inter), want):
+        assert torch.equal(a, b)
+    qt = q.transpose(0, 1).contiguous().transpose(0, 1)         # [heads][tokens] in memory
+    out = torch.empty_like(qt)
+    assert out.stride() == qt.stride()
+    got, _ = dsk_moe.qk_norm_rope(qt, k, pos, freq, interleaved=inter, q_out=out)
+    assert torch.equal(got, want[0])
+    before = qkv.clone()
+    dsk_moe.qk_norm_rope(q, k, pos, freq, interleaved=inter, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(qkv[:, 512:], before[:, 512:])
+
+
+def test_no_norm_is_the_rotation_alone():
+    g = gen(5)
+    k = normal(g, 9, 2, 64, dtype=F32) * 100
+    pos = torch.arange(9, dtype=I32)
+    freq = dsk_moe.rope_frequencies(32, device="cpu")[0]
+    _, got = dsk_moe.qk_norm_rope(None, k.to(DEV), pos.to(DEV), freq.to(DEV), norm=False)
+    assert_within(got, *O.norm_rope(k, pos, freq, norm=False))
+    _, got = dsk_moe.qk_norm_rope(None, k.to(DEV), pos.to(DEV), norm=False)
+    assert torch.equal(got.cpu(), k.to(BF16))
+
+
+# ------------------------------------------------------------------ append
+def paged_setup(g, used, width, spare, kv, page, dim, fill=None):
+    """(table [len(used), width] with used[b] shuffled pages, k_cache, v_cache)."""
+    n = sum(used) + spare
+    ids = torch.randperm(n, generator=g)[:sum(used)].to(I32)
+    table = torch.zeros((len(used), width), dtype=I32)
+    at = 0
+    for b, u in enumerate(used):
+        table[b, :u] = ids[at:at + u]
+        at += u
+    make = (lambda: normal(g, n, kv, page, dim)) if fill is None else (lambda: torch.full((n, kv, page, dim), fill, dtype=BF16))
+    return table, make(), make()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,page,prefix,inter", [(128, 64, 0, False), (64, 16, 0, True), (128, 256, 37, False), (64, 32, 5, False)])
+def test_append(dtype, dim, page, prefix, inter):
+    g = gen(dim + page)
+    kv, heads = 3, 6
+    lens, starts = [70, 1, 33, 2], [0, 500, 15, 255]
+    used = [(a + n - 1) // page + 1 for a, n in zip(starts, lens)]
+    table, kc, vc = paged_setup(g, used, max(used) + 2, 2, kv, page, dim)
+    t = sum(lens)
+    q, k, v = normal(g, t, heads, dim, dtype=dtype), normal(g, t, kv, dim, dtype=dtype), normal(g, t, kv, dim, dtype=dtype)
+    row = torch.tensor([a + i for a, n in zip(starts, lens) for i in range(n)], dtype=I32)
+    seq = torch.tensor([b for b, n in enumerate(lens) for _ in range(n)], dtype=I32)
+    order = torch.randperm(t, generator=g)                       # tokens in any order
+    row, seq, pos = row[order], seq[order], row[order] + prefix
+    freq = dsk_moe.rope_frequencies(dim // 2, device="cpu")[0]
+    gamma = torch.rand(dim, generator=g) + 0.5
+    kd, vd = kc.to(DEV), vc.to(DEV)
+    ko = torch.empty((t, kv, dim), dtype=BF16, device=DEV)
+    got = dsk_moe.kv_append(q.to(DEV), k.to(DEV), v.to(DEV), pos.to(DEV), seq.to(DEV), table.to(DEV), kd, vd, freq.to(DEV),
+                            prefix_len=prefix, interleaved=inter, k_gamma=gamma.to(DEV), k_out=ko)
+    assert_within(got, *O.norm_rope(q, pos, freq, interleaved=inter), "q")
+    assert_within(ko, *O.norm_rope(k, pos, freq, interleaved=inter, gamma=gamma), "k")
+    at, r = table[seq.long(), row.long() // page].long(), row.long() % page
+    kc[at, :, r] = ko.cpu()
+    vc[at, :, r] = v.to(BF16)
+    assert torch.equal(kd.cpu(), kc) and torch.equal(vd.cpu(), vc)
+
+
+def test_append_leaves_out_what_has_no_place():
+    """Negative positions, rows before the prefix's end or behind the table, unknown sequences and pages outside the
+    cache: nothing of the cache changes; q is still written (not at negative positions)."""
+    g = gen(8)
+    kc, vc = normal(g, 4, 2, 16, 64), normal(g, 4, 2, 16, 64)
+    table = torch.tensor([[0, 4, -1], [1, 2, 1 << 30]], dtype=I32)
+    pos = torch.tensor([-1, 2, 10 + 16, 10 + 32, 10 + 48, 10 + 32, 10 + 3, 10 + 3, 10 + 17], dtype=I32)
+    seq = torch.tensor([0, 0, 0, 0, 0, 1, 2, -1, 1], dtype=I32)
+    q, k, v = normal(g, 9, 2, 64), normal(g, 9, 2, 64), normal(g, 9, 2, 64)
+    kd, vd = kc.to(DEV), vc.to(DEV)
+    qo = torch.full((9, 2, 64), 9.0, dtype=BF16, device=DEV)
+    dsk_moe.kv_append(q.to(DEV), k.to(DEV), v.to(DEV), pos.to(DEV), seq.to(DEV), table.to(DEV), kd, vd, prefix_len=10,
+                      norm=False, q_out=qo)
+    kc[2, :, 1], vc[2, :, 1] = k[8], v[8]                         # the last token alone has a place
+    assert torch.equal(kd.cpu(), kc) and torch.equal(vd.cpu(), vc)
+    assert torch.equal(qo.cpu()[1:], q[1:]) and (qo.cpu()[0] == 9.0).all()
+
+
+def test_append_without_queries():
+    g = gen(9)
+    kd, vd = (torch.zeros(2, 1, 32, 128, dtype=BF16, device=DEV) for _ in range(2))
+    k, v = normal(g, 3, 1, 128), normal(g, 3, 1, 128)
+    assert dsk_moe.kv_append(None, k.to(DEV), v.to(DEV), ints([31, 32, 0]), ints([0, 0, 0]), ints([[1, 0]]), kd, vd, norm=False) is None
+    assert torch.equal(kd[1, 0, 31].cpu(), k[0, 0]) and torch.equal(vd[0, 0, 0].cpu(), v[1, 0]) and torch.equal(kd[1, 0, 0].cpu(), k[2, 0])
+    assert int((kd != 0).any(-1).sum()) == 3
+
+
+# ------------------------------------------------------------------ prompts
+def cumulative(lens):
+    return [sum(lens[:i]) for i in range(len(lens) + 1)]
+
+
+def run_prompt(q, k, v, lens, lens_k=None, **kw):
+    cu, ck = cumulative(lens), cumulative(lens_k or lens)
+    got = dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), ints(cu), ints(ck) if lens_k else None, **kw)
+    return got, O.prompt(q, k, v, cu, ck, **{x: kw[x] for x in ("causal", "scale") if x in kw})
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (8, 2, 128), (10, 2, 64), (8, 1, 128), (3, 1, 128)])
+@pytest.mark.parametrize("lens", [[1], [17], [64], [65, 1, 0, 127, 3], [0, 0, 5], [200], [128, 129]])
+def test_prompt(heads, kv, dim, lens):
+    print(f"prompt {heads},{kv},{dim} {lens}", flush=True)
+    g = gen(sum(lens) + heads)
+    t = sum(lens)
+    q, k, v = normal(g, t, heads, dim), normal(g, t, kv, dim), normal(g, t, kv, dim)
+    got, (want, tol) = run_prompt(q, k, v, lens)
+    assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,lens,lens_k", [(128, [3, 40, 1, 20], [70, 40, 130, 300]), (64, [30, 5, 7], [10, 0, 1]), (128, [64], [1])])
+def test_prompt_with_other_keys(causal, dim, lens, lens_k):
+    """Keys of earlier tokens before the prompt's, or fewer keys than queries (rows without a key are zero)."""
+    g = gen(7 * sum(lens))
+    q, k, v = normal(g, sum(lens), 4, dim), normal(g, sum(lens_k), 2, dim), normal(g, sum(lens_k), 2, dim)
+    got, (want, tol) = run_prompt(q, k, v, lens, lens_k, causal=causal, scale=0.2)
+    assert_within(got, want, tol)
+    if min(lens_k) == 0:
+        assert not got[30:35].any()
+
+
+def test_prompt_views_and_padding_rows():
+    """Views of a fused projection, heads-first outputs; rows behind the last sequence stay as they were."""
+    g = gen(21)
+    lens, t = [50, 31], 90
+    qkv = normal(g, t, (6 + 2 + 2) * 64)
+    q, k, v = (p.unflatten(1, (-1, 64)) for p in qkv.split([384, 128, 128], 1))
+    out = torch.full((6, t, 64), 5.0, dtype=BF16, device=DEV).transpose(0, 1)
+    qd, kd, vd = (p.unflatten(1, (-1, 64)) for p in qkv.to(DEV).split([384, 128, 128], 1))
+    got = dsk_moe.prompt_attention(qd, kd, vd, ints(cumulative(lens)), out=out)
+    want, tol = O.prompt(q[:81], k[:81], v[:81], cumulative(lens), cumulative(lens))
+    assert got is out
+    assert_within(out[:81], want, tol)
+    assert (out[81:] == 5.0).all()
+
+
+@pytest.mark.parametrize("poison", [NAN, INF, -INF])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_unseen_values_stay_unseen(dim, poison):
+    """NaN and infinities in keys and values of later tokens, other sequences and padding reach no row that does not
+    see them; rows that do see them show it."""
+    g = gen(22)
+    lens = [70, 90, 20]
+    cu = cumulative(lens)
+    q, k, v = normal(g, 200, 4, dim), normal(g, 200, 2, dim), normal(g, 200, 2, dim)
+    want, tol = O.prompt(q[:180], k[:180], v[:180], cu, cu)
+    seen = torch.ones(180, dtype=torch.bool)
+    for bad in ([0], [75, 135], [180]):                          # tokens: of sequence 0, of sequence 1, of padding
+        for b in bad:
+            if b < 180:
+                end = next(c for c in cu if c > b)
+                seen[b:end] = False                              # its own row and its sequence's later ones
+            v[b, 1, 3] = poison
+            k[b, 0, 5] = poison if b >= 180 else k[b, 0, 5]
+    got = dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), ints(cu)).cpu()[:180].double()
+    # heads 0, 1 read key head 0, whose values are finite
+    clean = torch.ones(180, 4, dim, dtype=torch.bool)
+    clean[~seen, 2:, 3] = False
+    assert not torch.isfinite(got[~clean]).any()
+    assert ((got - want).abs() <= tol)[clean].all()
+
+
+def test_prompt_poisoned_later_keys():
+    g = gen(23)
+    q, k, v = normal(g, 100, 2, 128), normal(g, 100, 1, 128), normal(g, 100, 1, 128)
+    want, tol = O.prompt(q, k, v, [0, 100], [0, 100])
+    k[60] = NAN
+    got = dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), ints([0, 100]))
+    assert_within(got[:60], want[:60], tol[:60])
+    assert got[60:].isnan().all()
+
+
+def test_prompt_bounds_outside_are_cut():
+    """Sequence bounds that are not ascending or leave the tensors touch no row outside."""
+    g = gen(24)
+    q, k, v = normal(g, 40, 2, 64), normal(g, 40, 1, 64), normal(g, 40, 1, 64)
+    out = torch.full((40, 2, 64), 3.0, dtype=BF16, device=DEV)
+    dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), ints([-5, 10, 7, 30, 1 << 30]), out=out)
+    want, tol = O.prompt(q, k, v, [0, 10], [0, 10])
+    assert_within(out[:7], want[:7], tol[:7])
+    assert torch.isfinite(out).all()
+
+
+def test_prompt_long_rows():
+    """2000 tokens: every row of a few heads against float64 on the device (tolerances as the oracle's)."""
+    g = torch.Generator(device=DEV).manual_seed(25)
+    q, k, v = (torch.randn((2000, h, 128), generator=g, device=DEV).to(BF16) for h in (8, 2, 2))
+    got = dsk_moe.prompt_attention(q, k, v, ints([0, 2000])).double()
+    hidden = torch.ones((2000, 2000), dtype=torch.bool, device=DEV).triu(1)
+    for h in range(8):
+        qh, kh, vh = q[:, h].double(), k[:, h // 4].double(), v[:, h // 4].double()
+        w = torch.softmax((qh @ kh.T / 128 ** 0.5).masked_fill(hidden, -INF), -1)
+        size = float((qh.abs() @ kh.abs().T).max()) / 128 ** 0.5
+        slack = 4 * (2000 + 128 * size + 16) * 2.0 ** -24
+        want = w @ vh
+        tol = (w @ vh.abs()) * (2.0 ** -8 + slack) + want.abs() * 2.0 ** -8 * (1 + 2.0 ** -6)
+        assert ((got[:, h] - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------ decode
+@pytest.mark.parametrize("heads,kv,dim,page,q_len", [(8, 2, 128, 64, 1), (4, 4, 64, 16, 1), (8, 1, 64, 32, 3), (16, 1, 128, 16, 4),
+                                                     (10, 2, 128, 128, 2), (64, 1, 64, 256, 1), (3, 3, 128, 16, 16), (20, 1, 128, 32, 2)])
+@pytest.mark.parametrize("prefix", [0, 1, 130])
+def test_paged(heads, kv, dim, page, q_len, prefix):
+    print(f"paged {heads},{kv},{dim} page {page} q_len {q_len} prefix {prefix}", flush=True)
+    g = gen(heads * dim + page + prefix)
+    lens = [0, 1, 15, 16, 17, 127, 128, 129, 300]
+    used = [-(-n // page) for n in lens]
+    shared = -(-prefix // page)
+    table, kc, vc = paged_setup(g, used + [shared], max(max(used) + 1, shared), 2, kv, page, dim)
+    pre, table = table[-1, :shared], table[:-1]
+    # what no sequence holds is NaN: rows behind the lengths, and pages of nobody
+    held = torch.zeros(kc.shape[0], page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for j in range(n):
+            held[table[b, j // page], j % page] = True
+    for j in range(prefix):
+        held[pre[j // page], j % page] = True
+    for c in (kc, vc):
+        c.transpose(1, 2)[~held] = NAN
+    q = normal(g, len(lens), q_len, heads, dim)
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints(lens),
+                                  prefix=pre.to(DEV) if prefix else None, prefix_len=prefix, scale=0.15)
+    want, tol = O.paged(q, kc, vc, table, lens, pre, prefix, scale=0.15)
+    assert got.shape == q.shape
+    assert_within(got, want, tol)
+    if not prefix:
+        assert not got[0].any()
+
+
+@pytest.mark.parametrize("batch,longest", [(1, 5000), (3, 2500), (150, 300)])
+def test_paged_long_and_many(batch, longest):
+    """Items over many shares, many items in a share."""
+    g = gen(batch)
+    lens = [int(x) for x in torch.randint(0, longest, (batch,), generator=g)]
+    lens[batch // 2] = longest
+    used = [-(-n // 64) for n in lens]
+    table, kc, vc = paged_setup(g, used, max(used), 1, 2, 64, 128)
+    q = normal(g, batch, 4, 128)
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints(lens))
+    want, tol = O.paged(q[:, None], kc, vc, table, lens)
+    assert_within(got, want[:, 0], tol[:, 0])
+
+
+def test_paged_long_prefix():
+    g = gen(31)
+    table, kc, vc = paged_setup(g, [3, 1, 60], 60, 1, 1, 64, 128)
+    pre, table = table[2], table[:2]
+    q = normal(g, 2, 40, 128)
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints([150, 0]), prefix=pre.to(DEV), prefix_len=3801)
+    want, tol = O.paged(q[:, None], kc, vc, table, [150, 0], pre, 3801)
+    assert_within(got, want[:, 0], tol[:, 0])
+
+
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_paged_bad_pages_and_lengths_show(prefix):
+    """A page outside the cache or a length beyond the table: NaN rows of that sequence alone; no read outside."""
+    g = gen(32)
+    table, kc, vc = paged_setup(g, [4, 4, 4, 4, 3], 4, 0, 2, 16, 64)
+    pre, table = table[4, :3], table[:4]
+    bad = table.clone()
+    bad[1, 2], bad[2, 0] = 1 << 30, -7
+    lens = [50, 50, 64, 1 << 30]
+    q = normal(g, 4, 4, 64)
+    kw = dict(prefix=pre.to(DEV), prefix_len=prefix) if prefix else {}
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bad.to(DEV), ints(lens), **kw)
+    want, tol = O.paged(q[:, None], kc, vc, table, [50, 50, 64, 64], pre, prefix)
+    assert_within(got[0], want[0, 0], tol[0, 0])
+    assert got[1:].isnan().all()
+    # the bad page lies behind the length: nobody asks for it
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bad.to(DEV), ints([50, 32, 0, 64]), **kw)
+    want, tol = O.paged(q[:, None], kc, vc, table, [50, 32, 0, 64], pre, prefix)
+    assert_within(got, want[:, 0], tol[:, 0])
+    if prefix:
+        pre[1] = 1 << 20
+        got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints([50] * 4), prefix=pre.to(DEV), prefix_len=prefix)
+        assert got.isnan().all()
+
+
+@pytest.mark.parametrize("dim,heads,q_len", [(64, 4, 3), (128, 2, 4), (128, 32, 2)])
+@pytest.mark.parametrize("poison", [NAN, INF])
+def test_paged_unseen_values_stay_unseen(dim, heads, q_len, poison):
+    """In a verify step the last token's value must not reach the tokens before it."""
+    g = gen(33)
+    for n in (q_len, 32, 33, 130):
+        table, kc, vc = paged_setup(g, [9], 9, 0, 1, 16, dim)
+        q = normal(g, 1, q_len, heads, dim)
+        want, tol = O.paged(q, kc, vc, table, [n])
+        j = n - 1
+        vc[table[0, j // 16], 0, j % 16, 9] = poison
+        got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints([n])).cpu().double()
+        assert ((got - want).abs() <= tol)[:, :-1].all()
+        assert not torch.isfinite(got[0, -1, :, 9]).any()
+        keep = torch.arange(dim) != 9
+        assert ((got - want).abs() <= tol)[..., keep].all()
+
+
+def test_paged_far_pages():
+    """Pages beyond 2^31 elements and 2^32 bytes of the cache."""
+    pages = (1 << 31) // (8 * 256 * 128) + 40
+    kc, vc = (torch.empty((pages, 8, 256, 128), dtype=BF16, device=DEV) for _ in range(2))
+    g = gen(34)
+    ids = [pages - 1, pages // 2 + 1, 5]
+    ks, vs = normal(g, 3, 8, 256, 128), normal(g, 3, 8, 256, 128)
+    kc[ids], vc[ids] = ks.to(DEV), vs.to(DEV)
+    k1, v1 = normal(g, 1, 8, 128), normal(g, 1, 8, 128)
+    table = ints([[ids[1], ids[0]]])
+    dsk_moe.kv_append(None, k1.to(DEV), v1.to(DEV), ints([300]), ints([0]), table, kc, vc, norm=False)
+    ks[0, :, 44], vs[0, :, 44] = k1[0], v1[0]
+    q = normal(g, 1, 8, 128)
+    got = dsk_moe.paged_attention(q.to(DEV), kc, vc, table, ints([301]), prefix=ints([ids[2]]), prefix_len=200)
+    want, tol = O.paged(q[:, None], ks, vs, torch.tensor([[1, 0]]), [301], torch.tensor([2]), 200)
+    assert_within(got, want[:, 0], tol[:, 0])
+
+
+def test_paged_views_and_scratch():
+    """Strided queries and outputs; a workspace of the caller's, full of NaN, twice."""
+    g = gen(35)
+    table, kc, vc = paged_setup(g, [3, 7], 8, 0, 2, 16, 64)
+    dev = [x.to(DEV) for x in (kc, vc, table)]
+    q = normal(g, 2, 2, 4, 64)
+    qkv = torch.cat([q.flatten(2), normal(g, 2, 2, 256)], -1).to(DEV)
+    view = qkv[..., :256].unflatten(2, (4, 64))
+    out = torch.zeros((2, 2, 4, 128), dtype=BF16, device=DEV)[..., 64:]
+    ws = torch.full((64 << 20,), 255, dtype=torch.uint8, device=DEV)
+    want, tol = O.paged(q, kc, vc, table, [40, 111])
+    for _ in range(2):
+        got = dsk_moe.paged_attention(view, *dev, ints([40, 111]), out=out, workspace=ws)
+        assert got is out
+        assert_within(out, want, tol)
+    with pytest.raises(_lib.DskError, match="DSK_ESPACE"):
+        dsk_moe.paged_attention(view, *dev, ints([40, 111]), workspace=ws[:256])
+
+
+def test_same_call_same_bits():
+    g = gen(36)
+    table, kc, vc = paged_setup(g, [20, 3, 40, 9], 40, 0, 2, 16, 128)
+    q = normal(g, 4, 8, 128).to(DEV)
+    args = [x.to(DEV) for x in (kc, vc, table)] + [ints([320, 33, 640, 140])]
+    want = dsk_moe.paged_attention(q, *args, prefix=args[2][2], prefix_len=600)
+    for _ in range(5):
+        assert torch.equal(dsk_moe.paged_attention(q, *args, prefix=args[2][2], prefix_len=600), want)
+
+
+def test_refusals_on_the_device():
+    g = gen(37)
+    q, k = normal(g, 4, 8, 128).to(DEV), normal(g, 4, 2, 128).to(DEV)
+    pos, cu = ints([0, 1, 2, 3]), ints([0, 4])
+    kc, table, lens = torch.zeros(4, 2, 16, 128, dtype=BF16, device=DEV), ints([[0], [1], [2], [3]]), ints([1, 1, 1, 1])
+    bad = [lambda: dsk_moe.qk_norm_rope(q, k, pos.long()), lambda: dsk_moe.qk_norm_rope(q, k.float(), pos),
+           lambda: dsk_moe.qk_norm_rope(q, k, pos[:3]), lambda: dsk_moe.qk_norm_rope(q[..., ::2], k, pos),
+           lambda: dsk_moe.qk_norm_rope(q, k, pos, torch.ones(64, device=DEV)), lambda: dsk_moe.qk_norm_rope(q.half(), k.half(), pos),
+           lambda: dsk_moe.qk_norm_rope(q, k, pos, q_gamma=torch.ones(64, device=DEV)),
+           lambda: dsk_moe.qk_norm_rope(q[:3], k, pos), lambda: dsk_moe.qk_norm_rope(q, k, pos.cpu()),
+           lambda: dsk_moe.qk_norm_rope(q, k, pos, q_out=torch.empty_like(k)),
+           lambda: dsk_moe.kv_append(q, k, k[:, :1], pos, pos, table, kc, kc), lambda: dsk_moe.kv_append(q, k, k, pos, pos, table, kc, kc[:, :1]),
+           lambda: dsk_moe.kv_append(q, k, k, pos, pos, table.long(), kc, kc),
+           lambda: dsk_moe.prompt_attention(q, k, k[:3], cu), lambda: dsk_moe.prompt_attention(q.float(), k, k, cu),
+           lambda: dsk_moe.prompt_attention(q, k, k, cu, ints([0, 2, 4])), lambda: dsk_moe.prompt_attention(q, k, k, cu.long()),
+           lambda: dsk_moe.paged_attention(q[:3], kc, kc, table, lens), lambda: dsk_moe.paged_attention(q, kc, kc, table, lens[:3]),
+           lambda: dsk_moe.paged_attention(q, kc, kc, table, lens, prefix_len=3), lambda: dsk_moe.paged_attention(q, kc, kc, table, lens, prefix=lens),
+           lambda: dsk_moe.paged_attention(q, kc, kc, table, lens, prefix=lens, prefix_len=65),
+           lambda: dsk_moe.paged_attention(q, kc[..., :64], kc[..., :64], table, lens),
+           lambda: dsk_moe.paged_attention(q, kc, kc, table, lens, workspace=torch.empty(9, device=DEV))]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            print("accepted", i)
+    for f in (lambda: dsk_moe.prompt_attention(q[:, :7], k, k, cu), lambda: dsk_moe.prompt_attention(q, k, k, cu[:1]),
+              lambda: dsk_moe.prompt_attention(q, k, k, cu, scale=-1.0),
+              lambda: dsk_moe.paged_attention(q[:, None].expand(4, 17, 8, 128).contiguous(), kc, kc, table, lens)):
+        with pytest.raises(_lib.DskError):
+            f()
+
+
+# ------------------------------------------------------------------ as a server runs them
+class Server:
+    """Four conversations behind a shared prefix: prompts, then steps of two tokens, on one cache."""
+
+    def __init__(self, seed, dim=64, heads=8, kv=2, page=16, prefix=37):
+        self.g = gen(seed)
+        self.dim, self.heads, self.kv, self.page, self.prefix = dim, heads, kv, page, prefix
+        self.freq = dsk_moe.rope_frequencies(dim // 2, device="cpu")[0]
+        self.gq, self.gk = torch.rand(dim, generator=self.g) + 0.5, torch.rand(dim, generator=self.g) + 0.5
+        self.shared = -(-prefix // page)
+        self.table, kc, vc = paged_setup(self.g, [12, 12, 12, 12, self.shared], 12, 0, kv, page, dim, fill=NAN)
+        self.pre = self.table[4, :self.shared]
+        self.table = self.table[:4].contiguous()
+        self.kc, self.vc = kc.to(DEV), vc.to(DEV)
+        self.k = [torch.zeros(0, kv, dim, dtype=BF16) for _ in range(4)]     # as appended
+        self.v = [torch.zeros(0, kv, dim, dtype=BF16) for _ in range(4)]
+
+    def rows(self, t):
+        return normal(self.g, t, (self.heads + 2 * self.kv) * self.dim)
+
+    def split(self, qkv):
+        return (p.unflatten(1, (-1, self.dim)) for p in qkv.split([self.heads * self.dim] + [self.kv * self.dim] * 2, 1))
+
+    def append(self, qkv, pos, seq, table, prefix_len, k_out=None):
+        q, k, v = self.split(qkv)
+        return dsk_moe.kv_append(q, k, v, pos, seq, table, self.kc, self.vc, self.freq.to(DEV), prefix_len=prefix_len,
+                                 q_gamma=self.gq.to(DEV), k_gamma=self.gk.to(DEV), k_out=k_out)
+
+
+def test_prompts_then_decode_steps():
+    """Shared prefix, packed prompts behind it, then two-token steps: the cache's reader sees what the appends wrote.
+    Every output against attention in float64 over the rotated rows (rounded to bf16 as the cache holds them)."""
+    s = Server(40)
+    # the prefix as a prompt of its own
+    qkv = s.rows(s.prefix)
+    ar = torch.arange(s.prefix, dtype=I32, device=DEV)
+    kp = torch.empty((s.prefix, s.kv, s.dim), dtype=BF16, device=DEV)
+    q = s.append(qkv.to(DEV), ar, torch.zeros_like(ar), s.pre[None].to(DEV), 0, kp)
+    vp = list(s.split(qkv))[2]
+    got = dsk_moe.prompt_attention(q, kp, vp.to(DEV), ints([0, s.prefix]))
+    want, tol = O.prompt(q.cpu(), kp.cpu(), vp, [0, s.prefix], [0, s.prefix])
+    assert_within(got, want, tol, "prefix")
+    # the prompts: keys and values of the prefix before their own
+    lens = [5, 33, 1, 16]
+    t, cu = sum(lens), cumulative(lens)
+    qkv = s.rows(t)
+    row = [i for n in lens for i in range(n)]
+    seq = [b for b, n in enumerate(lens) for _ in range(n)]
+    ko = torch.empty((t, s.kv, s.dim), dtype=BF16, device=DEV)
+    q = s.append(qkv.to(DEV), ints([r + s.prefix for r in row]), ints(seq), s.table.to(DEV), s.prefix, ko)
+    y, tol = O.norm_rope(list(s.split(qkv))[1], torch.tensor(row) + s.prefix, s.freq, gamma=s.gk)
+    assert_within(ko, y, tol, "prompt keys")
+    vo = list(s.split(qkv))[2]
+    for b in range(4):
+        s.k[b], s.v[b] = ko.cpu()[cu[b]:cu[b + 1]], vo[cu[b]:cu[b + 1]]
+    kk = torch.cat([x for b in range(4) for x in (kp.cpu(), s.k[b])])
+    vv = torch.cat([x for b in range(4) for x in (vp, s.v[b])])
+    ck = cumulative([n + s.prefix for n in lens])
+    got = dsk_moe.prompt_attention(q, kk.to(DEV), vv.to(DEV), ints(cu), ints(ck))
+    want, tol = O.prompt(q.cpu(), kk, vv, cu, ck)
+    assert_within(got, want, tol, "prompts")
+    # steps of two tokens
+    for step in range(3):
+        at = [len(k) for k in s.k]
+        qkv = s.rows(8)
+        pos = ints([a + i + s.prefix for a in at for i in range(2)])
+        ko = torch.empty((8, s.kv, s.dim), dtype=BF16, device=DEV)
+        q = s.append(qkv.to(DEV), pos, ints([0, 0, 1, 1, 2, 2, 3, 3]), s.table.to(DEV), s.prefix, ko).view(4, 2, s.heads, s.dim)
+        vo = list(s.split(qkv))[2]
+        for b in range(4):
+            s.k[b], s.v[b] = torch.cat([s.k[b], ko.cpu()[2 * b:2 * b + 2]]), torch.cat([s.v[b], vo[2 * b:2 * b + 2]])
+        lens = [len(k) for k in s.k]
+        got = dsk_moe.paged_attention(q, s.kc, s.vc, s.table.to(DEV), ints(lens), prefix=s.pre.to(DEV), prefix_len=s.prefix)
+        for b in range(4):
+            want, tol = O.attention(q[b].cpu(), torch.cat([kp.cpu(), s.k[b]]), torch.cat([vp, s.v[b]]),
+                                    torch.tensor([s.prefix + lens[b] - 2, s.prefix + lens[b] - 1]), s.dim ** -0.5)
+            assert_within(got[b], want, tol, f"step {step} sequence {b}")
+
+
+@pytest.mark.parametrize("prefix", [0, 37])
+def test_captured_steps_follow_the_lengths(prefix):
+    """A decode step (append and attention) captured once and replayed while the sequences grow; a second graph of
+    another batch between the replays, and eager work that must not disturb them."""
+    def build(seed):
+        s = Server(seed, prefix=prefix or 1)
+        for c in (s.kc, s.vc):
+            c.copy_(normal(s.g, *c.shape))
+        st = dict(qkv=s.rows(4).to(DEV), pos=ints([0, 60, 15, 130]) + prefix, lens=ints([1, 61, 16, 131]), seq=ints([0, 1, 2, 3]),
+                  table=s.table.to(DEV), pre=s.pre.to(DEV), freq=s.freq.to(DEV), gq=s.gq.to(DEV))
+
+        def step():
+            q, k, v = s.split(st["qkv"])
+            q = dsk_moe.kv_append(q, k, v, st["pos"], st["seq"], st["table"], s.kc, s.vc, st["freq"], prefix_len=prefix, q_gamma=st["gq"])
+            return dsk_moe.paged_attention(q, s.kc, s.vc, st["table"], st["lens"], prefix=st["pre"] if prefix else None, prefix_len=prefix)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        return s, st, step, graph, out
+
+    one, two = build(41), build(42)
+    for i in range(4):
+        for s, st, step, graph, out in (one, two):
+            st["qkv"].copy_(s.rows(4))
+            st["pos"] += 1
+            st["lens"] += 1
+        for s, st, step, graph, out in (one, two):
+            graph.replay()
+        torch.cuda.synchronize()
+        for s, st, step, graph, out in (one, two):
+            held = out.clone()
+            assert torch.equal(step(), held), i                  # the eager step writes the same rows again
+
+
+def test_calls_on_two_streams():
+    """Concurrent calls on two streams, each with its own scratch memory."""
+    g = gen(50)
+    table, kc, vc = paged_setup(g, [30] * 8, 30, 0, 2, 16, 128)
+    kc, vc, table, lens = kc.to(DEV), vc.to(DEV), table.to(DEV), ints([480, 3, 100, 250, 7, 480, 64, 128])
+    q = [normal(g, 8, 8, 128).to(DEV) for _ in range(2)]
+    want = [dsk_moe.paged_attention(x, kc, vc, table, lens) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(dsk_moe.paged_attention(q[i], kc, vc, table, lens))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
