@@ -42,7 +42,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kNoMask = 0x7fffffff;   // every row sees every key of its tiles
 
 // Two floats as bf16, rounded to nearest even (one instruction on gfx950).
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {

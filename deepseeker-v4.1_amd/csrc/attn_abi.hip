@@ -147,6 +147,8 @@ int dsk_prompt_attention(const dsk_prompt_desc* d, const void* q, const void* k,
   if (!rc) rc = check_strides(fn, "k", d->k_token, d->k_head, 8);
   if (!rc) rc = check_strides(fn, "v", d->v_token, d->v_head, 8);
   if (!rc) rc = check_out(fn, "out", d->o_token, d->o_head, d->heads, d->head_dim);
+  if (!rc && (d->k_token >= (1 << 26) || d->v_token >= (1 << 26)))
+    rc = fail(DSK_EUNSUPPORTED, "%s: token strides of k and v must stay below 2^26", fn);
   if (rc) return rc;
   return hip_check(launch_prompt(*d, q, k, v, cu_q, cu_k, out, static_cast<hipStream_t>(stream)), fn);
 }

@@ -31,9 +31,28 @@ __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void dma16(const void* g, void* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// 16 bytes a lane from base + off (bytes) to LDS at `lds` + 16 lane (both uniform).  Written
+// out, since the compiler makes every later transposing read wait for all loads in
+// flight when it knows that they go to LDS; the loops wait by themselves
+// (wait_all_barrier), and the load has no result register.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 is reserved, and is clobbered
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) const void*)(p))));
+}
+template <typename T>
+__device__ __forceinline__ const T* uniform_ptr(const T* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  // readfirstlane gives an int: through 32 bits without a sign
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(v))));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(v >> 32))));
+  return reinterpret_cast<const T*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // Every load of this wave has landed and its LDS reads are complete, then the workgroup barrier.
@@ -65,57 +84,66 @@ constexpr int flash_lds() { return 2 * 2 * kFlKeys * D * 2; }
 
 // Tiles [t0, t1) of 64 keys; q[ks]: the lane's row, elements 16 ks + 8 (lane >> 5) .. +8;
 // lim: the last key that the lane's row sees, w_min / w_max: least and largest lim of
-// the wave's rows (wave-uniform); b_min: least lim of the workgroup's rows.  rows(tile, wave's first row in it, &k, &v, &ks, &vs, &last): pointers
-// to that row of K and V, their strides, and the last row after it that may be read.
+// the wave's rows (wave-uniform); b_min: least lim of the workgroup's rows.  rows(tile,
+// wave's first row in it, &k, &v, &last): that row of K and V (the last of all where it
+// lies behind) and how many rows after it may be read; kstride, vstride: elements from row to row,
+// below 2^26.
 template <int D, int NW, class Rows>
 __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1, int lim, int w_min, int w_max,
-                                      int b_min, float c2, char* lds, Rows rows, FlashRows<D>& st) {
+                                      int b_min, float c2, char* lds, int64_t kstride,
+                                      int64_t vstride, Rows rows, FlashRows<D>& st) {
+  // wave-uniform by their meaning: in scalar registers
+  t0 = __builtin_amdgcn_readfirstlane(t0);
+  t1 = __builtin_amdgcn_readfirstlane(t1);
+  w_min = __builtin_amdgcn_readfirstlane(w_min);
+  w_max = __builtin_amdgcn_readfirstlane(w_max);
+  b_min = __builtin_amdgcn_readfirstlane(b_min);
   constexpr int CH = D / 8, RPI = 64 / CH, WR = kFlKeys / NW, NI = WR / RPI, KS = D / 16;
   constexpr int kTile = kFlKeys * D * 2;
-  static_assert(NI >= 1, "every wave loads whole instructions");
+  static_assert(NI >= 1 && RPI % 4 == 0, "every wave loads whole instructions");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
 
-  auto issue = [&](int t, int buf) {
+  // LDS: K of even and odd tiles, then V of even and odd tiles
+  const uint32_t ldsw = lds_address(lds) + wave * WR * D * 2;
+  // K (V) of tile t; rows past the last one: the last one again
+  auto issue_k = [&](int t) {
     const uint16_t *kp, *vp;
-    int64_t ks, vs;
     int last;
-    rows(t, wave * WR, kp, vp, ks, vs, last);
-    char* kd = lds + buf * 2 * kTile + wave * WR * D * 2;
+    rows(t, wave * WR, kp, vp, last);
+    kp = uniform_ptr(kp);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = i * RPI + lane / CH, rr = min(r, last);
-      const int row = wave * WR + r;
-      dma16(kp + rr * ks + 8 * ((lane % CH) ^ swz_k<D>(row)), kd + i * RPI * D * 2);
+      const int r = i * RPI + lane / CH;
+      const uint32_t rr = min(r, last);
+      dma16(kp, 2 * (rr * static_cast<uint32_t>(kstride) + 8 * ((lane % CH) ^ swz_k<D>(wave * WR + r))),
+            ldsw + (t & 1) * kTile + i * RPI * D * 2);
     }
+  };
+  auto issue_v = [&](int t) {
+    const uint16_t *kp, *vp;
+    int last;
+    rows(t, wave * WR, kp, vp, last);
+    vp = uniform_ptr(vp);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = i * RPI + lane / CH, rr = min(r, last);
-      const int row = wave * WR + r;
-      dma16(vp + rr * vs + 8 * ((lane % CH) ^ swz_v<D>(row)), kd + kTile + i * RPI * D * 2);
+      const int r = i * RPI + lane / CH;
+      const uint32_t rr = min(r, last);
+      dma16(vp, 2 * (rr * static_cast<uint32_t>(vstride) + 8 * ((lane % CH) ^ swz_v<D>(wave * WR + r))),
+            ldsw + (2 + (t & 1)) * kTile + i * RPI * D * 2);
     }
   };
 
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    wait_all_barrier();
-    if (t + 1 < t1) issue(t + 1, buf ^ 1);
-    const char* kl = lds + buf * 2 * kTile;
-    const char* vl = kl + kTile;
-    // some rows see a part of the tile only: are all of its values finite?
-    bool finite = true;
-    if (t * kFlKeys + kFlKeys - 1 > b_min) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int i = threadIdx.x; i < kTile / 16; i += 64 * NW) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(vl + 16 * i);
-        bits |= nonfinite_bits(x[0]) | nonfinite_bits(x[1]) | nonfinite_bits(x[2]) | nonfinite_bits(x[3]);
-      }
-      finite = !__syncthreads_or(bits);
-    }
-    if (t * kFlKeys > w_max) continue;               // keys that none of the wave's rows sees
-    f32x16 s[2];
+  const int l16 = lane & 15;
+  // A operand of the second product: keys 16 s4 .. +16, elements 32 dt .. +32
+  auto value_frag = [&](const char* vl, int s4, int dt) {
+    const int r0 = 16 * s4 + 4 * hf + (l16 >> 2);
+    const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    const u32x2 lo = read_tr(vl + r0 * D * 2 + 16 * (c ^ swz_v<D>(r0)) + 8 * (l16 & 1));
+    const u32x2 hi = read_tr(vl + (r0 + 8) * D * 2 + 16 * (c ^ swz_v<D>(r0 + 8)) + 8 * (l16 & 1));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto scores = [&](const char* kl, f32x16 (&s)[2]) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       s[kt] = f32x16{};
@@ -125,18 +153,18 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       for (int ks = 0; ks < KS; ++ks)
         s[kt] = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(kr + 16 * ((2 * ks + hf) ^ swz_k<D>(row)))), q[ks], s[kt]);
     }
-    if (t * kFlKeys + kFlKeys - 1 > w_min) {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t * kFlKeys + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[kt][i] = kNegInf;
-    }
+  };
+  // the largest score of the lane's row, times c2
+  auto top_of = [&](const f32x16 (&s)[2]) {
     float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
-    top = max_across32(top) * c2;
-    if (__any(top > st.m)) {
+    return max_across32(top) * c2;
+  };
+  // the reference point follows the maximum once it lags by more than 2^8: p stays
+  // below 2^8, and most tiles leave o as it is
+  auto follow = [&](float top) {
+    if (__any(top > st.m + 8.0f)) {
       const float mn = fmaxf(st.m, top);
       const float f = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
       st.m = mn;
@@ -144,8 +172,9 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= f;
     }
+  };
+  auto weights = [&](const f32x16 (&s)[2], bf16x8 (&p)[4]) {
     const float mu = st.m == kNegInf ? 0.0f : st.m;
-    bf16x8 p[4];
 #pragma unroll
     for (int s4 = 0; s4 < 4; ++s4) {
       float e[8];
@@ -154,42 +183,137 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
         e[i] = __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + i] * c2 - mu);
         st.l += e[i];
       }
-      // p to bf16: relative 2^-9 each, of random sign over the keys, next to the
-      // output's own rounding of 2^-9
+      // p to bf16: at most 2^-8 of each, of random sign over the keys, next to the
+      // output's own rounding of 2^-8
       p[s4] = as_bf16x8(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
     }
-    const int l16 = lane & 15;
-    if (!finite) {
+  };
+  auto values = [&](const char* vl, const bf16x8 (&p)[4]) {
+#pragma unroll
+    for (int s4 = 0; s4 < 4; ++s4)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = mfma32(as_bf16x8(value_frag(vl, s4, dt)), p[s4], st.o[dt]);
+  };
+
+  if (t0 >= t1) return;
+  wait_vm_all();                     // q is here: nothing in the loops waits for it
+  // Tile t's scores are made while tile t - 1's weights are: the matrix pipe and the
+  // vector pipe have work of one wave at the same time.  Between two barriers, tile
+  // t + 1's K and tile t's V are read; tile t + 2's K and tile t + 1's V arrive.
+  issue_k(t0);
+  issue_v(t0);
+  if (t0 + 1 < t1) issue_k(t0 + 1);
+  wait_all_barrier();
+  f32x16 s[2];
+  scores(lds + (t0 & 1) * kTile, s);
+  float top = top_of(s);
+  int t = t0;
+  {
+    // tiles up to two before the last that all rows of the workgroup see in full: the
+    // lanes' offsets from a tile's first row stay the same.  K's chunks are placed by
+    // the row in the tile, V's by its last bits, which are the same in every load
+    uint32_t koff[NI], voff;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = i * RPI + lane / CH;
+      koff[i] = 2 * (r * static_cast<uint32_t>(kstride) + 8 * ((lane % CH) ^ swz_k<D>(wave * WR + r)));
+    }
+    voff = 2 * (lane / CH * static_cast<uint32_t>(vstride) + 8 * ((lane % CH) ^ swz_v<D>(lane / CH)));
+    const int full = min(t1, (b_min + 1) / kFlKeys) - 2;      // tile full + 1 is the last full one
+    auto step = [&](const f32x16 (&s)[2], f32x16 (&next)[2]) {
+      wait_all_barrier();
+      const uint16_t *kp, *vp, *unused;
+      int last;
+      rows(t + 2, wave * WR, kp, unused, last);
+      rows(t + 1, wave * WR, unused, vp, last);
+      kp = uniform_ptr(kp);
+      vp = uniform_ptr(vp);
+      const uint32_t kd = ldsw + (t & 1) * kTile, vd = ldsw + (3 - (t & 1)) * kTile;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        dma16(kp, koff[i], kd + i * RPI * D * 2);
+        dma16(vp + i * RPI * vstride, voff, vd + i * RPI * D * 2);
+      }
+      follow(top);
+      bf16x8 p[4];
+      scores(lds + ((t & 1) ^ 1) * kTile, next);
+      weights(s, p);
+      values(lds + (2 + (t & 1)) * kTile, p);
+      top = top_of(next);
+      ++t;
+    };
+    // two at a time: the scores change places without moves
+    f32x16 other[2];
+    for (; t + 1 < full;) {
+      step(s, other);
+      step(other, s);
+    }
+    if (t < full) {
+      step(s, other);
+      s[0] = other[0];
+      s[1] = other[1];
+    }
+  }
+  // the last of them, and tiles that some rows see a part of, or nothing
+  for (;; ++t) {
+    wait_all_barrier();
+    if (t + 2 < t1) issue_k(t + 2);
+    if (t + 1 < t1) issue_v(t + 1);
+    const char* vl = lds + (2 + (t & 1)) * kTile;
+    bool finite = true;
+    if (t * kFlKeys + kFlKeys - 1 > b_min) {
+      uint32_t bits = 0;
+      for (int i = threadIdx.x; i < kTile / 16; i += 64 * NW) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(vl + 16 * i);
+        bits |= nonfinite_bits(x[0]) | nonfinite_bits(x[1]) | nonfinite_bits(x[2]) | nonfinite_bits(x[3]);
+      }
+      finite = !__syncthreads_or(bits);
+    }
+    if (t * kFlKeys + kFlKeys - 1 > w_min) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t * kFlKeys + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[kt][i] = kNegInf;
+    }
+    bf16x8 p[4];
+    if (t * kFlKeys <= w_max) {
+      follow(top_of(s));
+      weights(s, p);
+    }
+    if (t * kFlKeys > w_max) {
+      // keys that none of the wave's rows sees
+    } else if (finite) {
+      values(vl, p);
+    } else {
       // rarely: the product of the finite values, and the others to the rows that see them
+#pragma unroll
+      for (int s4 = 0; s4 < 4; ++s4)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          u32x4 w = value_frag(vl, s4, dt);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
+          st.o[dt] = mfma32(as_bf16x8(w), p[s4], st.o[dt]);
+        }
 #pragma unroll 1
       for (int key = 0; key < kFlKeys; ++key) {
-        const bool sees = t * kFlKeys + key <= lim;
+        int row = key;
+        asm volatile("" : "+v"(row));                // keeps the addresses out of registers
+        const bool sees = t * kFlKeys + row <= lim;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = 32 * dt + 8 * (i >> 2) + 4 * hf + (i & 3);
-            const float x = nonfinite_only(*reinterpret_cast<const uint16_t*>(
-                vl + key * D * 2 + 16 * ((d >> 3) ^ swz_v<D>(key)) + 2 * (d & 7)));
-            st.o[dt][i] += sees ? x : 0.0f;
+          for (int g = 0; g < 4; ++g) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(vl + row * D * 2 + 16 * ((4 * dt + g) ^ swz_v<D>(row)) + 8 * hf);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              st.o[dt][4 * g + i] += sees ? nonfinite_only(static_cast<uint16_t>(x[i >> 1] >> (16 * (i & 1)))) : 0.0f;
           }
       }
     }
-#pragma unroll
-    for (int s4 = 0; s4 < 4; ++s4) {
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        const int r0 = 16 * s4 + 4 * hf + (l16 >> 2);
-        const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-        const u32x2 lo = read_tr(vl + r0 * D * 2 + 16 * (c ^ swz_v<D>(r0)) + 8 * (l16 & 1));
-        const u32x2 hi = read_tr(vl + (r0 + 8) * D * 2 + 16 * (c ^ swz_v<D>(r0 + 8)) + 8 * (l16 & 1));
-        u32x4 w{lo[0], lo[1], hi[0], hi[1]};
-        if (!finite)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
-        st.o[dt] = mfma32(as_bf16x8(w), p[s4], st.o[dt]);
-      }
-    }
+    if (t + 1 >= t1) break;
+    if ((t + 1) * kFlKeys <= w_max) scores(lds + ((t & 1) ^ 1) * kTile, s);
   }
 }
 

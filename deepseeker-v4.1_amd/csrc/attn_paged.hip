@@ -257,7 +257,8 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
         float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                           fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
         top = max_across32(max_across16(top)) * a.c2;
-        if (__any(top > m[rt])) {
+        // the reference point follows the maximum once it lags by more than 2^8
+        if (__any(top > m[rt] + 8.0f)) {
           const float mn = fmaxf(m[rt], top);
           const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
           m[rt] = mn;

@@ -64,13 +64,14 @@ __device__ __forceinline__ int find_tile(const PromptArgs& a, int tile, int& at)
 
 template <int D>
 __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
-  __shared__ __align__(16) char lds[flash_lds<D>()];
+  extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % a.kv_heads;
   int at;
   const int b = __builtin_amdgcn_readfirstlane(find_tile(a, a.tiles - 1 - static_cast<int>(blockIdx.x / a.kv_heads), at));
   if (b < 0) return;
+  at = __builtin_amdgcn_readfirstlane(at);
   const SeqRange sr = seq_range(a, b);
   const int lq = sr.q1 - sr.q0, lk = sr.k1 - sr.k0, rows = lq * a.group;
   // reversed within the sequence as over all: the tiles with most keys first
@@ -96,16 +97,14 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
 
   const uint16_t* kb = a.k + sr.k0 * a.k_token + h * a.k_head;
   const uint16_t* vb = a.v + sr.k0 * a.v_token + h * a.v_head;
-  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int64_t& ks, int64_t& vs, int& last) {
+  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
     // rows past the sequence's end (another one's, or none): its last row again
     const int key = min(t * kFlKeys + row, lk - 1);
     kp = kb + key * a.k_token;
     vp = vb + key * a.v_token;
-    ks = a.k_token;
-    vs = a.v_token;
     last = lk - 1 - key;
   };
-  flash<D, kFlWaves>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, src, st);
+  flash<D, kFlWaves>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
 
   const float l = sum_across32(st.l);
   const float inv = lim >= 0 ? 1.0f / l : 0.0f;     // a row that sees no key: zeros
@@ -141,7 +140,7 @@ struct PrefixArgs {
 
 template <int D>
 __global__ __launch_bounds__(kFlThreads, 2) void k_prefix(const PrefixArgs a) {
-  __shared__ __align__(16) char lds[flash_lds<D>()];
+  extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
@@ -163,7 +162,7 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prefix(const PrefixArgs a) {
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
   bool bad = false;
-  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int64_t& ks, int64_t& vs, int& last) {
+  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
     const int key = min(t * kFlKeys + row, a.len - 1);
     int id = a.pages[key >> a.c.page_shift];
     if (id < 0 || id >= a.c.n_pages) {
@@ -174,12 +173,10 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prefix(const PrefixArgs a) {
     const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
     kp = a.c.k + base;
     vp = a.c.v + base;
-    ks = D;
-    vs = D;
     last = a.len - 1 - key;
   };
   const int w_max = wr0 < a.rows ? a.len - 1 : -1;    // a wave without rows only loads
-  flash<D, kFlWaves>(q, t0, t1, a.len - 1, a.len - 1, w_max, kNoMask, a.c2, lds, src, st);
+  flash<D, kFlWaves>(q, t0, t1, a.len - 1, a.len - 1, w_max, a.len - 1, a.c2, lds, D, D, src, st);
   // a page outside the cache: the waves load different rows, so all tell
   const bool any_bad = __syncthreads_or(bad);
   const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
@@ -213,8 +210,8 @@ hipError_t launch_prefix(const dsk_paged_desc& d, const void* q, const dsk_kv_ca
   const PrefixArgs a{static_cast<const uint16_t*>(q), cache_view(c), prefix, pre_o, pre_ml, d.q_token, d.q_head,
                      rows, d.scale * kLog2e, d.kv_heads, group, d.prefix_len, splits, row_tiles};
   const unsigned blocks = static_cast<unsigned>(row_tiles) * splits * d.kv_heads;
-  if (d.head_dim == 64) launch_kernel(k_prefix<64>, blocks, kFlThreads, 0, s, a);
-  else launch_kernel(k_prefix<128>, blocks, kFlThreads, 0, s, a);
+  if (d.head_dim == 64) launch_kernel(k_prefix<64>, blocks, kFlThreads, flash_lds<64>(), s, a);
+  else launch_kernel(k_prefix<128>, blocks, kFlThreads, flash_lds<128>(), s, a);
   return hipGetLastError();
 }
 
@@ -228,8 +225,8 @@ hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
                      group, d.causal, static_cast<int32_t>(tiles)};
   const unsigned blocks = static_cast<unsigned>(tiles * d.kv_heads);
-  if (d.head_dim == 64) launch_kernel(k_prompt<64>, blocks, kFlThreads, 0, s, a);
-  else launch_kernel(k_prompt<128>, blocks, kFlThreads, 0, s, a);
+  if (d.head_dim == 64) launch_kernel(k_prompt<64>, blocks, kFlThreads, flash_lds<64>(), s, a);
+  else launch_kernel(k_prompt<128>, blocks, kFlThreads, flash_lds<128>(), s, a);
   return hipGetLastError();
 }
 

@@ -18,7 +18,6 @@ attention, output projection) for ``MoEStack``.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 
 import torch
@@ -93,18 +92,19 @@ def _hip(t: torch.Tensor) -> torch.device:
     return t.device
 
 
-def _out(out: torch.Tensor | None, shape: tuple, dev: torch.device, what: str) -> torch.Tensor:
+def _out_strides(out: torch.Tensor | None, shape: tuple, dev: torch.device, what: str) -> tuple[int, int]:
+    """Token and head stride of a checked output, or of the one that will be allocated."""
     if out is None:
-        return torch.empty(shape, dtype=_BF16, device=dev)
+        return shape[1] * shape[2], shape[2]
     _rows(out, what, (_BF16,), dev)
     if tuple(out.shape) != tuple(shape):
         raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(out.shape)}")
-    return out
+    return out.stride()[:2]
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
     """The entry point on ``dev``'s current stream, with ``dev`` current."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if torch.cuda.current_device() == dev.index:
         _lib.call(name, *args, stream)
     else:
@@ -112,8 +112,28 @@ def _call(dev: torch.device, name: str, *args) -> None:
             _lib.call(name, *args, stream)
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, kv_heads: int, dim: int,
-           dev: torch.device) -> _lib.KVCache:
+# A call's checks depend on its tensors' sizes, strides, types and devices and on its numbers alone, so what they
+# found (the descriptor and the outputs' shapes; no tensor, no address) serves later calls of the same kind: a decode
+# step's host work is a third of that of checking each time (decode_1: 18.3 us a call, without).
+_plans: dict[tuple, tuple] = {}
+_MOST_PLANS = 4096
+
+
+def _sig(t: torch.Tensor | None):
+    return (t.shape, t.stride(), t.dtype, t.get_device()) if t is not None else None
+
+
+def _planned(key: tuple, make, *args, **kwargs) -> tuple:
+    plan = _plans.get(key)
+    if plan is None:
+        plan = make(*args, **kwargs)
+        if len(_plans) >= _MOST_PLANS:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
+
+
+def _check_cache(k_cache, v_cache, table, kv_heads: int, dim: int, dev: torch.device) -> None:
     for t, what in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         if t.device != dev or t.dtype != _BF16 or t.dim() != 4 or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous bf16 [pages, kv_heads, page_size, head_dim] on {dev}")
@@ -121,20 +141,23 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, kv
         raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} do not fit {kv_heads} key heads of {dim}")
     if table.device != dev or table.dtype != _I32 or table.dim() != 2 or table.stride(1) != 1:
         raise ValueError(f"table must be int32 [sequences, pages] on {dev} with contiguous rows")
-    return _lib.KVCache(k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), table.stride(0), k_cache.shape[0],
-                        k_cache.shape[2], table.shape[0], table.shape[1])
 
 
-# Descriptors hold sizes and strides alone, so calls of one shape share one.
-_qk_desc = functools.lru_cache(maxsize=256)(_lib.QkDesc)
-_prompt_desc = functools.lru_cache(maxsize=256)(_lib.PromptDesc)
-_paged_desc = functools.lru_cache(maxsize=256)(_lib.PagedDesc)
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor) -> _lib.KVCache:
+    n_pages, _, page_size, _ = k_cache.shape
+    n_seqs, max_pages = table.shape
+    return _lib.KVCache(k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), table.stride(0), n_pages, page_size,
+                        n_seqs, max_pages)
+
+
+def _p(t: torch.Tensor | None):
+    return t.data_ptr() if t is not None else None
 
 
 # ------------------------------------------------------------------ norms, rotation, append
-def _qk(q, k, v, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gamma, norm, eps, q_out, k_out, want_k,
-        prefix_len):
-    """Checked arguments of the two entry points: device, descriptor, outputs."""
+def _qk_plan(q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache, interleaved,
+             rot_first, mscale, norm, eps, prefix_len):
+    """(device, descriptor) of a checked call; the outputs have q's and k's shapes."""
     dev = _hip(k)
     _rows(k, "k", (_BF16, _F32), dev)
     tokens, kv_heads, dim = k.shape
@@ -146,7 +169,6 @@ def _qk(q, k, v, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gam
         heads, qs = q.shape[1], q.stride()
         if q.shape[0] != tokens or q.shape[2] != dim:
             raise ValueError(f"q {tuple(q.shape)} does not fit k {tuple(k.shape)}")
-        q_out = _out(q_out, q.shape, dev, "q_out")
     elif q_out is not None or q_gamma is not None:
         raise ValueError("q_out and q_gamma need q")
     _exact(positions, "positions", _I32, tokens, dev)
@@ -157,25 +179,21 @@ def _qk(q, k, v, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gam
     for g, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
         if g is not None:
             _exact(g, what, _F32, dim, dev)
-    if want_k or k_out is not None:
-        k_out = _out(k_out, k.shape, dev, "k_out")
     vs = (0, 0, 0)
     if v is not None:
         _rows(v, "v", (k.dtype,), dev)
         if v.shape != k.shape:
             raise ValueError(f"v {tuple(v.shape)} does not fit k {tuple(k.shape)}")
         vs = v.stride()
+        _exact(seq, "seq", _I32, tokens, dev)
+        _check_cache(k_cache, v_cache, table, kv_heads, dim, dev)
+    qo, ko = ((0, 0), (0, 0)) if q is None else (_out_strides(q_out, q.shape, dev, "q_out"), (0, 0))
+    if k_out is not None or v is None:
+        ko = _out_strides(k_out, k.shape, dev, "k_out")
     ks = k.stride()
-    qo = q_out.stride() if q_out is not None else (0, 0, 0)
-    ko = k_out.stride() if k_out is not None else (0, 0, 0)
-    desc = _qk_desc(tokens, heads, kv_heads, dim, _lib.DTYPE_BF16 if k.dtype == _BF16 else _lib.DTYPE_F32,
-                    1 if norm else 0, rot, int(rot_first), 1 if interleaved else 0, int(prefix_len), float(eps),
-                    float(mscale), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qo[0], qo[1], ko[0], ko[1])
-    return dev, desc, q_out, k_out
-
-
-def _p(t: torch.Tensor | None):
-    return t.data_ptr() if t is not None else None
+    return dev, _lib.QkDesc(tokens, heads, kv_heads, dim, _lib.DTYPE_BF16 if k.dtype == _BF16 else _lib.DTYPE_F32,
+                            1 if norm else 0, rot, int(rot_first), 1 if interleaved else 0, int(prefix_len), float(eps),
+                            float(mscale), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], *qo, *ko)
 
 
 def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor | None = None, *,
@@ -187,8 +205,14 @@ def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tenso
     elements rot_first .. rot_first + 2 len(freq) by positions[t] * freq (``interleaved``: pairs (2i, 2i+1), otherwise (i,
     i + len(freq))), in one pass.  q and k bf16 or float32; the results bf16.  Tokens at negative positions are left out
     (their output rows are not written).  q_out / k_out may be q / k themselves."""
-    dev, desc, q_out, k_out = _qk(q, k, None, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gamma, norm, eps,
-                                  q_out, k_out, True, 0)
+    tensors = (q, k, None, positions, freq, q_gamma, k_gamma, q_out, k_out, None, None, None, None)
+    numbers = (interleaved, rot_first, mscale, norm, eps, 0)
+    key = ("qk", _sig(q), _sig(k), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out), numbers)
+    dev, desc = _planned(key, _qk_plan, *tensors, *numbers)
+    if q_out is None and q is not None:
+        q_out = torch.empty(q.shape, dtype=_BF16, device=dev)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=_BF16, device=dev)
     _call(dev, "dsk_qk_norm_rope", ctypes.byref(desc), _p(q), k.data_ptr(), positions.data_ptr(), _p(freq), _p(q_gamma),
           _p(k_gamma), _p(q_out), k_out.data_ptr())
     return q_out, k_out
@@ -204,22 +228,20 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, position
     positions[t] - prefix_len of sequence seq[t] (int32), whose pages are table[seq[t]].  Returns q's result; the keys
     are also written to ``k_out`` if given.  Tokens outside the table or with a page outside the cache are not kept; two
     tokens of one call must not share a row."""
-    dev, desc, q_out, k_out = _qk(q, k, v, positions, freq, interleaved, rot_first, mscale, q_gamma, k_gamma, norm, eps,
-                                  q_out, k_out, False, prefix_len)
-    _exact(seq, "seq", _I32, k.shape[0], dev)
-    cache = _cache(k_cache, v_cache, table, k.shape[1], k.shape[2], dev)
+    tensors = (q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache)
+    numbers = (interleaved, rot_first, mscale, norm, eps, prefix_len)
+    key = ("append", *map(_sig, tensors), numbers)
+    dev, desc = _planned(key, _qk_plan, *tensors, *numbers)
+    if q_out is None and q is not None:
+        q_out = torch.empty(q.shape, dtype=_BF16, device=dev)
     _call(dev, "dsk_kv_append", ctypes.byref(desc), _p(q), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
-          seq.data_ptr(), _p(freq), _p(q_gamma), _p(k_gamma), ctypes.byref(cache), _p(q_out), _p(k_out))
+          seq.data_ptr(), _p(freq), _p(q_gamma), _p(k_gamma), ctypes.byref(_cache(k_cache, v_cache, table)), _p(q_out),
+          _p(k_out))
     return q_out
 
 
 # ------------------------------------------------------------------ attention
-def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
-                     cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
-    """``dsk_prompt_attention`` over packed sequences: queries cu_q[s] .. cu_q[s+1] with keys cu_k[s] .. cu_k[s+1] (int32;
-    cu_k: cu_q).  Causal: query i of Lq sees the keys j <= i + Lk - Lq; one that sees no key gives zeros.  scale:
-    head_dim ** -0.5.  Rows of ``out`` behind the last sequence are left as they were."""
+def _prompt_plan(q, k, v, cu_q, cu_k, out, causal, scale):
     dev = _hip(q)
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         _rows(t, what, (_BF16,), dev)
@@ -227,18 +249,67 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     if v.shape != k.shape or k.shape[2] != dim:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
     n = cu_q.numel()
-    if cu_k is None:
-        cu_k = cu_q
     _exact(cu_q, "cu_q", _I32, n, dev)
     _exact(cu_k, "cu_k", _I32, n, dev)
-    out = _out(out, q.shape, dev, "out")
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    desc = _prompt_desc(tokens, k.shape[0], n - 1, heads, k.shape[1], dim, 1 if causal else 0,
-                        float(scale) if scale is not None else dim ** -0.5,
-                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
+    return dev, _lib.PromptDesc(tokens, k.shape[0], n - 1, heads, k.shape[1], dim, 1 if causal else 0,
+                                float(scale) if scale is not None else dim ** -0.5,
+                                *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_out_strides(out, q.shape, dev, "out"))
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """``dsk_prompt_attention`` over packed sequences: queries cu_q[s] .. cu_q[s+1] with keys cu_k[s] .. cu_k[s+1] (int32;
+    cu_k: cu_q).  Causal: query i of Lq sees the keys j <= i + Lk - Lq; one that sees no key gives zeros.  scale:
+    head_dim ** -0.5.  Rows of ``out`` behind the last sequence are left as they were."""
+    if cu_k is None:
+        cu_k = cu_q
+    key = ("prompt", _sig(q), _sig(k), _sig(v), _sig(cu_q), _sig(cu_k), _sig(out), causal, scale)
+    dev, desc = _planned(key, _prompt_plan, q, k, v, cu_q, cu_k, out, causal, scale)
+    if out is None:
+        out = torch.empty(q.shape, dtype=_BF16, device=dev)
     _call(dev, "dsk_prompt_attention", ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(),
           cu_k.data_ptr(), out.data_ptr())
     return out
+
+
+def _token_rows(t: torch.Tensor, q_len: int, what: str) -> torch.Tensor:
+    """[batch, q_len, heads, dim] as [batch * q_len, heads, dim], a view."""
+    if t.dim() != 4 or t.shape[1] != q_len:
+        raise ValueError(f"{what} must be [batch, {q_len}, heads, head_dim], got {tuple(t.shape)}")
+    if q_len > 1 and t.shape[0] > 1 and t.stride(0) != q_len * t.stride(1):
+        raise ValueError(f"the tokens of {what} must be evenly spaced")
+    return t.flatten(0, 1)
+
+
+def _paged_plan(q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale):
+    """(device, descriptor, bytes of workspace)."""
+    dev = _hip(q)
+    q_len = q.shape[1] if q.dim() == 4 else 1
+    if q_len < 1:
+        raise ValueError("q has no tokens")
+    rows = _token_rows(q, q_len, "q") if q.dim() == 4 else q
+    _rows(rows, "q", (_BF16,), dev)
+    tokens, heads, dim = rows.shape
+    kv_heads = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    _check_cache(k_cache, v_cache, table, kv_heads, dim, dev)
+    batch = table.shape[0]
+    if batch < 1 or tokens != batch * q_len:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a table of {batch} sequences")
+    _exact(lens, "lens", _I32, batch, dev)
+    if prefix_len < 0 or (prefix_len > 0) != (prefix is not None):
+        raise ValueError("prefix and a positive prefix_len go together")
+    if prefix is not None:
+        _vector(prefix, "prefix", _I32, -(-prefix_len // k_cache.shape[2]), dev)
+    if out is not None and q.dim() == 4:
+        out = _token_rows(out, q_len, "out")
+    desc = _lib.PagedDesc(batch, q_len, heads, kv_heads, dim, int(prefix_len),
+                          float(scale) if scale is not None else dim ** -0.5, *rows.stride()[:2],
+                          *_out_strides(out, rows.shape, dev, "out"))
+    n = ctypes.c_size_t(0)
+    _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(desc), ctypes.byref(_cache(k_cache, v_cache, table)),
+              ctypes.byref(n))
+    return dev, desc, n.value
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
@@ -248,44 +319,18 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """``dsk_paged_attention``: q [batch, heads, head_dim] (one token of each sequence) or [batch, q_len, heads, head_dim]
     over lens[s] (int32) keys of sequence s in the cache, the new tokens' among them.  ``prefix`` (int32 page ids) with
     ``prefix_len`` keys that all sequences see first, read once for the batch.  The result has q's shape.  ``workspace``:
-    uint8, at least ``paged_workspace_size`` bytes; otherwise allocated (inside a graph capture, in the graph's pool)."""
-    dev = _hip(q)
-    batch = table.shape[0] if table.dim() == 2 else 0
-    if q.dim() == 4:
-        if q.shape[1] > 1 and q.shape[0] > 1 and q.stride(0) != q.shape[1] * q.stride(1):
-            raise ValueError("the tokens of q must be evenly spaced")
-        rows = q.flatten(0, 1)
-        if out is not None and (out.dim() != 4 or out.shape != q.shape):
-            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-        if out is not None and out.shape[1] > 1 and out.shape[0] > 1 and out.stride(0) != out.shape[1] * out.stride(1):
-            raise ValueError("the tokens of out must be evenly spaced")
-        q_len = q.shape[1]
-    else:
-        rows, q_len = q, 1
-    _rows(rows, "q", (_BF16,), dev)
-    tokens, heads, dim = rows.shape
-    if batch < 1 or tokens != batch * q_len or q_len < 1:
-        raise ValueError(f"q {tuple(q.shape)} does not fit a table of {batch} sequences")
-    cache = _cache(k_cache, v_cache, table, k_cache.shape[1] if k_cache.dim() == 4 else 0, dim, dev)
-    _exact(lens, "lens", _I32, batch, dev)
-    if prefix_len < 0 or (prefix_len > 0) != (prefix is not None):
-        raise ValueError("prefix and a positive prefix_len go together")
-    if prefix is not None:
-        _vector(prefix, "prefix", _I32, -(-prefix_len // k_cache.shape[2]), dev)
-    res = _out(out.flatten(0, 1) if out is not None and out.dim() == 4 else out, rows.shape, dev, "out")
-    qs, os = rows.stride(), res.stride()
-    desc = _paged_desc(batch, q_len, heads, k_cache.shape[1], dim, int(prefix_len),
-                       float(scale) if scale is not None else dim ** -0.5, qs[0], qs[1], os[0], os[1])
+    uint8, 256-byte aligned, as large as ``dsk_paged_attention_workspace_size`` says, for one call at a time; otherwise
+    allocated (inside a graph capture, in the graph's pool)."""
+    key = ("paged", _sig(q), _sig(k_cache), _sig(v_cache), _sig(table), _sig(lens), _sig(prefix), _sig(out), prefix_len, scale)
+    dev, desc, nbytes = _planned(key, _paged_plan, q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale)
+    if out is None:
+        out = torch.empty(q.shape, dtype=_BF16, device=dev)
     if workspace is None:
-        workspace = torch.empty(_workspace_bytes(desc, cache), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous uint8 on {dev}")
-    _call(dev, "dsk_paged_attention", ctypes.byref(desc), rows.data_ptr(), ctypes.byref(cache), lens.data_ptr(),
-          _p(prefix), res.data_ptr(), workspace.data_ptr(), workspace.numel())
-    return out if out is not None else res.view(q.shape)
-
-
-def _workspace_bytes(desc: _lib.PagedDesc, cache: _lib.KVCache) -> int:
-    n = ctypes.c_size_t(0)
-    _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(n))
-    return n.value
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    else:
+        nbytes = workspace.numel()
+        if workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous uint8 on {dev}")
+    _call(dev, "dsk_paged_attention", ctypes.byref(desc), q.data_ptr(), ctypes.byref(_cache(k_cache, v_cache, table)),
+          lens.data_ptr(), _p(prefix), out.data_ptr(), workspace.data_ptr(), nbytes)
+    return out

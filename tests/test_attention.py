@@ -96,7 +96,7 @@ def test_append_refuses():
     (dict(tokens=0), -1), (dict(kv_tokens=0), -1), (dict(n_seqs=0), -1), (dict(n_seqs=65536), -1), (dict(head_dim=80), -3),
     (dict(heads=9), -1), (dict(heads=0), -1), (dict(heads=130, kv_heads=2), -1), (dict(scale=0.0), -1),
     (dict(scale=math.nan), -1), (dict(tokens=1 << 28), -3), (dict(kv_tokens=1 << 30), -3), (dict(k_token=130), -2),
-    (dict(o_token=256), -1), (dict(n_seqs=65535, heads=1024, kv_heads=1024), -3)])
+    (dict(o_token=256), -1), (dict(v_token=1 << 26), -3), (dict(n_seqs=65535, heads=1024, kv_heads=1024), -3)])
 def test_prompt_refuses(kw, want):
     assert code("dsk_prompt_attention", ctypes.byref(prompt_desc(**kw)), P, P, P, P, P, P, None) == want
 
