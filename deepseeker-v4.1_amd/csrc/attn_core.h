@@ -1,9 +1,9 @@
 // Query rows against a run of keys with both products on 32x32x16 MFMAs, the
 // building block of prompt attention and of a shared prefix.
 //
-// A workgroup of NW waves holds 32 NW query rows, 32 a wave; every 64 keys and
-// values are brought to LDS once for all of them (global_load_lds: no registers
-// in between), two buffers deep.  As in the paged kernel, S^T = K q^T leaves a
+// NW waves hold 32 NW query rows, 32 a wave; every 64 keys and values are brought
+// to LDS once for all of them (global_load_lds: no registers in between), two
+// buffers deep.  As in the paged kernel, S^T = K q^T leaves a
 // query row in every lane (column lane & 31) and its keys 8 a + 4 h + b in the
 // registers 4 a + b of lane half h = lane >> 5, which is the B operand of
 // O^T = V^T p^T for the key order {16 s + 4 h + 0..3, 16 s + 8 + 4 h + 0..3}: p stays in its lane,
@@ -80,7 +80,7 @@ struct FlashRows {
 };
 
 template <int D>
-constexpr int flash_lds() { return 2 * 2 * kFlKeys * D * 2; }
+constexpr int flash_lds() { return 2 * 2 * kFlKeys * D * 2; }   // two tiles of K and of V
 
 // Tiles [t0, t1) of 64 keys; q[ks]: the lane's row, elements 16 ks + 8 (lane >> 5) .. +8;
 // lim: the last key that the lane's row sees, w_min / w_max: least and largest lim of
@@ -103,6 +103,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   static_assert(NI >= 1 && RPI % 4 == 0, "every wave loads whole instructions");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
+  if (t0 >= t1) return;
 
   // LDS: K of even and odd tiles, then V of even and odd tiles
   const uint32_t ldsw = lds_address(lds) + wave * WR * D * 2;
@@ -143,16 +144,17 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
     const u32x2 hi = read_tr(vl + (r0 + 8) * D * 2 + 16 * (c ^ swz_v<D>(r0 + 8)) + 8 * (l16 & 1));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
+  auto scores32 = [&](const char* kl, int kt, f32x16& s) {
+    s = f32x16{};
+    const int row = 32 * kt + n;
+    const char* kr = kl + row * D * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      s = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(kr + 16 * ((2 * ks + hf) ^ swz_k<D>(row)))), q[ks], s);
+  };
   auto scores = [&](const char* kl, f32x16 (&s)[2]) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      s[kt] = f32x16{};
-      const int row = 32 * kt + n;
-      const char* kr = kl + row * D * 2;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s[kt] = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(kr + 16 * ((2 * ks + hf) ^ swz_k<D>(row)))), q[ks], s[kt]);
-    }
+    scores32(kl, 0, s[0]);
+    scores32(kl, 1, s[1]);
   };
   // the largest score of the lane's row, times c2
   auto top_of = [&](const f32x16 (&s)[2]) {
@@ -195,10 +197,8 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = mfma32(as_bf16x8(value_frag(vl, s4, dt)), p[s4], st.o[dt]);
   };
 
-  if (t0 >= t1) return;
-  wait_vm_all();                     // q is here: nothing in the loops waits for it
-  // Tile t's scores are made while tile t - 1's weights are: the matrix pipe and the
-  // vector pipe have work of one wave at the same time.  Between two barriers, tile
+  // A tile's scores are made while the weights of the tile before are: the matrix pipe
+  // and the vector pipe have work of one wave at the same time.  Between two barriers, tile
   // t + 1's K and tile t's V are read; tile t + 2's K and tile t + 1's V arrive.
   issue_k(t0);
   issue_v(t0);
@@ -229,16 +229,34 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       kp = uniform_ptr(kp);
       vp = uniform_ptr(vp);
       const uint32_t kd = ldsw + (t & 1) * kTile, vd = ldsw + (3 - (t & 1)) * kTile;
+      const char* kl = lds + ((t & 1) ^ 1) * kTile;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        dma16(kp, koff[i], kd + i * RPI * D * 2);
-        dma16(vp + i * RPI * vstride, voff, vd + i * RPI * D * 2);
-      }
+      for (int i = 0; i < NI; ++i) dma16(vp + i * RPI * vstride, voff, vd + i * RPI * D * 2);
       follow(top);
       bf16x8 p[4];
-      scores(lds + ((t & 1) ^ 1) * kTile, next);
+      scores32(kl, 0, next[0]);
+      scores32(kl, 1, next[1]);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma16(kp, koff[i], kd + i * RPI * D * 2);
       weights(s, p);
       values(lds + (2 + (t & 1)) * kTile, p);
+      // The order of issue: four fragments of K ahead, then behind every product the next
+      // fragment and the vector work that its time covers (8192 tokens, 32 heads of 128: 492 us as the
+      // compiler orders it, 484 with the products' order, 476 with the loads of K
+      // behind the first products)
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, 384 / D, 0);
+      }
       top = top_of(next);
       ++t;
     };
@@ -276,31 +294,15 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
         for (int i = 0; i < 16; ++i)
           if (t * kFlKeys + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[kt][i] = kNegInf;
     }
-    bf16x8 p[4];
-    if (t * kFlKeys <= w_max) {
-      follow(top_of(s));
-      weights(s, p);
-    }
-    if (t * kFlKeys > w_max) {
-      // keys that none of the wave's rows sees
-    } else if (finite) {
-      values(vl, p);
-    } else {
-      // rarely: the product of the finite values, and the others to the rows that see them
-#pragma unroll
-      for (int s4 = 0; s4 < 4; ++s4)
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
-          u32x4 w = value_frag(vl, s4, dt);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
-          st.o[dt] = mfma32(as_bf16x8(w), p[s4], st.o[dt]);
-        }
+    const bool sees = t * kFlKeys <= w_max;   // else: keys that none of the wave's rows sees
+    if (sees) follow(top_of(s));
+    if (!finite) {
+      // rarely: infinite and NaN values to the rows that see them, then out of the tile
 #pragma unroll 1
       for (int key = 0; key < kFlKeys; ++key) {
         int row = key;
         asm volatile("" : "+v"(row));                // keeps the addresses out of registers
-        const bool sees = t * kFlKeys + row <= lim;
+        const bool seen = t * kFlKeys + row <= lim;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -308,9 +310,21 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
             const u32x2 x = *reinterpret_cast<const u32x2*>(vl + row * D * 2 + 16 * ((4 * dt + g) ^ swz_v<D>(row)) + 8 * hf);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              st.o[dt][4 * g + i] += sees ? nonfinite_only(static_cast<uint16_t>(x[i >> 1] >> (16 * (i & 1)))) : 0.0f;
+              st.o[dt][4 * g + i] += seen ? nonfinite_only(static_cast<uint16_t>(x[i >> 1] >> (16 * (i & 1)))) : 0.0f;
           }
       }
+      wait_all_barrier();
+#pragma unroll 1
+      for (int i = threadIdx.x; i < kTile / 4; i += 64 * NW) {
+        uint32_t* x = reinterpret_cast<uint32_t*>(const_cast<char*>(vl) + 4 * i);
+        *x = finite_only(*x);
+      }
+      wait_all_barrier();
+    }
+    if (sees) {
+      bf16x8 p[4];
+      weights(s, p);
+      values(vl, p);
     }
     if (t + 1 >= t1) break;
     if ((t + 1) * kFlKeys <= w_max) scores(lds + ((t & 1) ^ 1) * kTile, s);

@@ -23,28 +23,19 @@ struct PromptArgs {
   int32_t tokens, kv_tokens, n_seqs, kv_heads, group, causal, tiles;
 };
 
-struct SeqRange { int q0, q1, k0, k1; };
-// The rows of sequence b, cut to the tensors; whatever cu holds, no row outside is touched.
-__device__ __forceinline__ SeqRange seq_range(const PromptArgs& a, int b) {
-  SeqRange r;
-  r.q0 = min(max(a.cu_q[b], 0), a.tokens);
-  r.q1 = min(max(a.cu_q[b + 1], r.q0), a.tokens);
-  r.k0 = min(max(a.cu_k[b], 0), a.kv_tokens);
-  r.k1 = min(max(a.cu_k[b + 1], r.k0), a.kv_tokens);
-  return r;
-}
+// A sequence's rows, cut to the tensors (whatever cu holds, no row outside is
+// touched), and a row tile's place in it.
+struct TilePlace { int q0, q1, k0, k1, at; };
 
-// Row tile `tile` counted over all sequences: its sequence (-1: none) and its place in it.
-__device__ __forceinline__ int find_tile(const PromptArgs& a, int tile, int& at) {
+// Row tile `tile` counted over all sequences; false: there are fewer.
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePlace& p) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    int n = 0;
-    if (b0 + lane < a.n_seqs) {
-      const int q0 = min(max(a.cu_q[b0 + lane], 0), a.tokens);
-      const int q1 = min(max(a.cu_q[b0 + lane + 1], q0), a.tokens);
-      n = ((q1 - q0) * a.group + kFlRows - 1) / kFlRows;
-    }
+    const int b = min(b0 + lane, a.n_seqs - 1);
+    const int q0 = min(max(a.cu_q[b], 0), a.tokens), q1 = min(max(a.cu_q[b + 1], q0), a.tokens);
+    const int k0 = min(max(a.cu_k[b], 0), a.kv_tokens), k1 = min(max(a.cu_k[b + 1], k0), a.kv_tokens);
+    const int n = b0 + lane < a.n_seqs ? ((q1 - q0) * a.group + kFlRows - 1) / kFlRows : 0;
     int incl = n;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -54,12 +45,16 @@ __device__ __forceinline__ int find_tile(const PromptArgs& a, int tile, int& at)
     const uint64_t past = __ballot(base + incl > tile);
     if (past) {
       const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      at = tile - base - __shfl(incl - n, l, 64);
-      return b0 + l;
+      p.q0 = __builtin_amdgcn_readlane(q0, l);
+      p.q1 = __builtin_amdgcn_readlane(q1, l);
+      p.k0 = __builtin_amdgcn_readlane(k0, l);
+      p.k1 = __builtin_amdgcn_readlane(k1, l);
+      p.at = tile - base - __builtin_amdgcn_readlane(incl - n, l);
+      return true;
     }
-    base += __shfl(incl, 63, 64);
+    base += __builtin_amdgcn_readlane(incl, 63);
   }
-  return -1;
+  return false;
 }
 
 template <int D>
@@ -68,14 +63,11 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % a.kv_heads;
-  int at;
-  const int b = __builtin_amdgcn_readfirstlane(find_tile(a, a.tiles - 1 - static_cast<int>(blockIdx.x / a.kv_heads), at));
-  if (b < 0) return;
-  at = __builtin_amdgcn_readfirstlane(at);
-  const SeqRange sr = seq_range(a, b);
+  TilePlace sr;
+  if (!find_tile(a, a.tiles - 1 - static_cast<int>(blockIdx.x / a.kv_heads), sr)) return;
   const int lq = sr.q1 - sr.q0, lk = sr.k1 - sr.k0, rows = lq * a.group;
   // reversed within the sequence as over all: the tiles with most keys first
-  const int row0 = at * kFlRows, wr0 = row0 + 32 * wave;
+  const int row0 = sr.at * kFlRows, wr0 = row0 + 32 * wave;
   const int r = min(wr0 + n, rows - 1), tok = r / a.group, hd = h * a.group + r % a.group;
   const int shift = lk - lq;                        // query i sees the keys up to i + shift
   const int lim = a.causal ? tok + shift : lk - 1;
@@ -193,6 +185,11 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prefix(const PrefixArgs a) {
   }
 }
 
+template <int D, class Args>
+void launch_flash(void (*kernel)(Args), const Args& a, unsigned blocks, hipStream_t s) {
+  launch_kernel(kernel, blocks, kFlThreads, flash_lds<D>(), s, a);
+}
+
 }  // namespace
 
 int prefix_splits(int64_t rows, int kv_heads, int prefix_len) {
@@ -210,8 +207,8 @@ hipError_t launch_prefix(const dsk_paged_desc& d, const void* q, const dsk_kv_ca
   const PrefixArgs a{static_cast<const uint16_t*>(q), cache_view(c), prefix, pre_o, pre_ml, d.q_token, d.q_head,
                      rows, d.scale * kLog2e, d.kv_heads, group, d.prefix_len, splits, row_tiles};
   const unsigned blocks = static_cast<unsigned>(row_tiles) * splits * d.kv_heads;
-  if (d.head_dim == 64) launch_kernel(k_prefix<64>, blocks, kFlThreads, flash_lds<64>(), s, a);
-  else launch_kernel(k_prefix<128>, blocks, kFlThreads, flash_lds<128>(), s, a);
+  if (d.head_dim == 64) launch_flash<64>(k_prefix<64>, a, blocks, s);
+  else launch_flash<128>(k_prefix<128>, a, blocks, s);
   return hipGetLastError();
 }
 
@@ -225,8 +222,8 @@ hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
                      group, d.causal, static_cast<int32_t>(tiles)};
   const unsigned blocks = static_cast<unsigned>(tiles * d.kv_heads);
-  if (d.head_dim == 64) launch_kernel(k_prompt<64>, blocks, kFlThreads, flash_lds<64>(), s, a);
-  else launch_kernel(k_prompt<128>, blocks, kFlThreads, flash_lds<128>(), s, a);
+  if (d.head_dim == 64) launch_flash<64>(k_prompt<64>, a, blocks, s);
+  else launch_flash<128>(k_prompt<128>, a, blocks, s);
   return hipGetLastError();
 }
 
