@@ -331,9 +331,4 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   }
 }
 
-// Splits of a shared prefix over workgroups, and its pass over all of the batch's rows.
-int prefix_splits(int64_t rows, int kv_heads, int prefix_len);
-hipError_t launch_prefix(const dsk_paged_desc& d, const void* q, const dsk_kv_cache& c, const int32_t* prefix,
-                         int splits, float* pre_o, float* pre_ml, hipStream_t s);
-
 }  // namespace dsk

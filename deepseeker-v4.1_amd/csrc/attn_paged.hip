@@ -23,15 +23,21 @@
 // shares for a fixed number of workgroups, so ragged lengths cost no balance
 // and the lengths are read on the device (a captured launch follows them).  An
 // item that lies in one share is finished there; the parts of the others go
-// through float32 partial rows (o, m, l) and k_paged_join.
-#include "attn.h"
+// through float32 partial rows (o, m, l) and k_paged_join.  Tables of at most
+// kPgShort keys need neither: a workgroup of eight waves takes a whole item.
+//
+// A prefix that the batch shares is a pass of its own over all of the batch's rows
+// (flash, attn_core.h), split along its keys; its workgroups come first in the
+// launch of the shares, so that its products run beside their loads.
 #include "attn_core.h"
 
 namespace dsk {
 namespace {
 
 constexpr int kPgThreads = 256;
-constexpr int kPgUnit = 128;        // keys of a unit: 32 for each wave
+constexpr int kPgUnit = 128;        // keys of a unit: 32 for each of four waves
+constexpr int kPgShort = 1024;      // keys of a table row that one workgroup takes alone
+constexpr int kPgShortWaves = 8;
 
 struct PagedArgs {
   const uint16_t* q;
@@ -40,11 +46,13 @@ struct PagedArgs {
   CacheView c;
   float* po;                        // partial rows [slot][M][D]
   float* pml;                       // [slot][M][2]: maximum (of scores times c), sum
-  const float* pre_o;               // prefix partials [split][kv head][batch * M][D]
-  const float* pre_ml;
+  float* pre_o;                     // prefix partials [split][kv head][batch * M][D]
+  float* pre_ml;
+  const int32_t* pages;             // of the prefix
   int64_t q_token, q_head, o_token, o_head;
   float c2;                         // scale * log2(e)
   int32_t batch, q_len, kv_heads, group, prefix, shares, splits;
+  int32_t row_tiles, prefix_blocks; // of the prefix: tiles of all rows, workgroups
 };
 
 // Keys of sequence b that the cache can hold; `bad` if lens[b] claims more.
@@ -58,28 +66,28 @@ __device__ __forceinline__ int units_of(const PagedArgs& a, int b) {
   return (length_of(a, b, bad) + kPgUnit - 1) / kPgUnit;
 }
 
-// Sum of units over all sequences, and over those before `stop`, by the whole block.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)))) |
+         (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32);
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
+  return uniform64(v);
+}
+
+// Units of one key head over all sequences, and over those before `stop`; every
+// wave by itself.
 struct Totals { int64_t all, before; };
-__device__ Totals unit_totals(const PagedArgs& a, int stop, int64_t (&lds)[2 * kPgThreads / 64]) {
+__device__ __forceinline__ Totals unit_totals(const PagedArgs& a, int stop) {
   int64_t all = 0, before = 0;
-  for (int b = threadIdx.x; b < a.batch; b += kPgThreads) {
+  for (int b = threadIdx.x & 63; b < a.batch; b += 64) {
     const int n = units_of(a, b);
     all += n;
     if (b < stop) before += n;
   }
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) {
-    all += __shfl_xor(all, s, 64);
-    before += __shfl_xor(before, s, 64);
-  }
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) { lds[2 * wave] = all; lds[2 * wave + 1] = before; }
-  __syncthreads();
-  Totals t{0, 0};
-#pragma unroll
-  for (int w = 0; w < kPgThreads / 64; ++w) { t.all += lds[2 * w]; t.before += lds[2 * w + 1]; }
-  return t;
+  return Totals{wave_sum(all), wave_sum(before)};
 }
 
 // The sequence that unit u of one key head lies in (u < the units of all), and
@@ -98,18 +106,13 @@ __device__ __forceinline__ int find_seq(const PagedArgs& a, int64_t u, int64_t& 
     const uint64_t past = __ballot(base + incl > u);
     if (past) {
       const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      before = base + __shfl(incl - n, l, 64);
+      before = uniform64(base + __shfl(incl - n, l, 64));
       return b0 + l;
     }
-    base += __shfl(incl, 63, 64);
+    base += uniform64(__shfl(incl, 63, 64));
   }
   before = base;
   return a.batch - 1;
-}
-
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  return static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)))) |
-         (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32);
 }
 
 template <int D>
@@ -131,40 +134,22 @@ __device__ __forceinline__ void load_v(uint32_t (&v)[VW / 2], const uint16_t* p)
   }
 }
 
-template <int D, int RT>
-__global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const PagedArgs a) {
-  constexpr int VW = D / 16, KS = D / 32, kWaves = kPgThreads / 64;
-  constexpr int kLd = D + 4;
-  __shared__ float lds_o[kWaves][16][kLd];
-  __shared__ float lds_ml[kWaves][16 * RT][2];
-  __shared__ int64_t lds_t[2 * kWaves];
+// LDS of a segment of W waves: their rows, then maxima and sums.
+template <int D, int RT, int W>
+struct SegLds {
+  float o[W][16][D + 4];
+  float ml[W][16 * RT][2];
+};
+
+// Units [k0, k1) of the keys of item (b, h), in units of 32 W keys, for the rows from
+// r0 on: to `out` (slot < 0: they are all of the item's) or to the partial rows of `slot`.
+template <int D, int RT, int W>
+__device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int len, bool bad_len, int r0, int k0, int k1,
+                                        int64_t slot, SegLds<D, RT, W>& lds) {
+  constexpr int VW = D / 16, KS = D / 32, kUnit = 32 * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
-  const int M = a.q_len * a.group, r0 = 16 * RT * blockIdx.y;   // this block's rows: r0 ..
-  const int64_t total = unit_totals(a, 0, lds_t).all * a.kv_heads;
-  const int64_t quota = uniform64((total + a.shares - 1) / a.shares);
-  const int64_t u0 = blockIdx.x * quota, u1 = uniform64(min(u0 + quota, total));
-  if (u0 >= u1) return;
-  int64_t before;
-  int b = __builtin_amdgcn_readfirstlane(find_seq(a, u0 / a.kv_heads, before));
-  before = uniform64(before);
-  // find_seq counts units of one head; an item's first unit is kv_heads * before + h * units
-  for (int64_t u = u0; u < u1;) {
-    bool bad_len;
-    const int len = length_of(a, b, bad_len);
-    const int nb = (len + kPgUnit - 1) / kPgUnit;
-    const int64_t first = before * a.kv_heads;
-    if (nb == 0 || u >= first + static_cast<int64_t>(nb) * a.kv_heads) {
-      before += nb;
-      ++b;
-      continue;
-    }
-    const int h = static_cast<int>((u - first) / nb);
-    const int64_t item0 = first + static_cast<int64_t>(h) * nb;
-    const int k0 = static_cast<int>(u - item0);
-    const int k1 = static_cast<int>(min(static_cast<int64_t>(nb), u1 - item0));
-    const bool whole = k0 == 0 && k1 == nb;
-
+  const int M = a.q_len * a.group;
     // queries: column n16 of row tile rt is row 16 rt + n16 = token * group + head of the group
     bf16x8 q[RT][KS];
     int lim[RT];                    // last key that the lane's row sees
@@ -192,7 +177,7 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
     bool bad = false;
     auto page_ids = [&](int kk) {
       ids0 = kk;
-      const int tile = min((kk + (lane >> 1)) * 8 + 2 * wave + (lane & 1), last_tile);
+      const int tile = min((kk + (lane >> 1)) * (2 * W) + 2 * wave + (lane & 1), last_tile);
       ids = ldg<int32_t>(trow + (tile >> sub));
       const bool out_of = ids < 0 || ids >= a.c.n_pages;
       bad = bad || (out_of && kk + (lane >> 1) < k1);
@@ -202,7 +187,7 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
       if (kk - ids0 >= 32) page_ids(kk);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const int tile = min(kk * 8 + 2 * wave + kt, last_tile);
+        const int tile = min(kk * (2 * W) + 2 * wave + kt, last_tile);
         const int id = __builtin_amdgcn_readlane(ids, 2 * (kk - ids0) + kt);
         const int last_row = len - 1 - tile * 16;     // rows past the length: the last one again
         const int row0 = (tile * 16) & ((1 << a.c.page_shift) - 1);
@@ -219,7 +204,7 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
     // products then leave them out)
     auto add_nonfinite = [&](int kk) {
 #pragma unroll 1
-      for (int key = kk * kPgUnit + 32 * wave, end = min(key + 32, len); key < end; ++key) {
+      for (int key = kk * kUnit + 32 * wave, end = min(key + 32, len); key < end; ++key) {
         int id = ldg<int32_t>(trow + (key >> a.c.page_shift));
         if (id < 0 || id >= a.c.n_pages) id = 0;
         const int in_page = key & ((1 << a.c.page_shift) - 1);
@@ -235,7 +220,7 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
       }
     };
     auto compute = [&](const Step<D>& s, int kk) {
-      const int key0 = kk * kPgUnit + 32 * wave;
+      const int key0 = kk * kUnit + 32 * wave;
       const bool masked = key0 + 31 > len - a.q_len;
       bf16x8 p[RT];
 #pragma unroll
@@ -313,57 +298,52 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
     }
     if (kk < k1) compute(s0, kk);
 
-    // the four waves' parts
+    // the waves' parts
     const bool any_bad = __any(bad);
-    __syncthreads();                 // the last item's reads of LDS are done
+    __syncthreads();                 // the last segment's reads of LDS are done
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       l[rt] = sum_across32(sum_across16(l[rt]));
       if (any_bad) l[rt] = __builtin_nanf("");
       if (g == 0) {
-        lds_ml[wave][16 * rt + n16][0] = m[rt];
-        lds_ml[wave][16 * rt + n16][1] = l[rt];
+        lds.ml[wave][16 * rt + n16][0] = m[rt];
+        lds.ml[wave][16 * rt + n16][1] = l[rt];
       }
     }
     __syncthreads();
-    const bool direct = whole && a.splits == 0;
-    const int64_t slot = direct ? 0
-                         : whole && a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h
-                         : u == u0 ? 2 * static_cast<int64_t>(blockIdx.x)
-                                   : 2 * static_cast<int64_t>(blockIdx.x) + 1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (rt) __syncthreads();
-      float top = lds_ml[0][16 * rt + n16][0];
+      float top = lds.ml[0][16 * rt + n16][0];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_ml[w][16 * rt + n16][0]);
+      for (int w = 1; w < W; ++w) top = fmaxf(top, lds.ml[w][16 * rt + n16][0]);
       const float f = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int t = 0; t < VW; t += 4)
-          *reinterpret_cast<f32x4*>(&lds_o[wave][n16][VW * (4 * g + r) + t]) =
+          *reinterpret_cast<f32x4*>(&lds.o[wave][n16][VW * (4 * g + r) + t]) =
               f32x4{o[rt][t][r], o[rt][t + 1][r], o[rt][t + 2][r], o[rt][t + 3][r]} * f;
       __syncthreads();
       const int row = threadIdx.x / (D / 8), d0 = 8 * (threadIdx.x % (D / 8));
       const int r = r0 + 16 * rt + row, rl = 16 * rt + row;
       if (row < 16 && r < M) {
-        float mm = lds_ml[0][rl][0], ll = 0.0f;
+        float mm = lds.ml[0][rl][0], ll = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, lds_ml[w][rl][0]);
+        for (int w = 1; w < W; ++w) mm = fmaxf(mm, lds.ml[w][rl][0]);
         const float mu = mm == kNegInf ? 0.0f : mm;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) ll += lds_ml[w][rl][1] * __builtin_amdgcn_exp2f(lds_ml[w][rl][0] - mu);
+        for (int w = 0; w < W; ++w) ll += lds.ml[w][rl][1] * __builtin_amdgcn_exp2f(lds.ml[w][rl][0] - mu);
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          y[i] = lds_o[0][row][d0 + i];
+          y[i] = lds.o[0][row][d0 + i];
 #pragma unroll
-          for (int w = 1; w < kWaves; ++w) y[i] += lds_o[w][row][d0 + i];
+          for (int w = 1; w < W; ++w) y[i] += lds.o[w][row][d0 + i];
         }
-        if (direct) {
+        if (slot < 0) {
           const int tok = r / a.group, hd = h * a.group + r % a.group;
-          const float inv = len - a.q_len + tok >= 0 || ll != ll ? 1.0f / ll : 0.0f;
+          const float inv = len - a.q_len + tok >= 0 || ll != ll ? 1.0f / ll : 0.0f;   // no key: zeros
           *reinterpret_cast<u32x4*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
               u32x4{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv),
                     pack_bf16(y[4] * inv, y[5] * inv), pack_bf16(y[6] * inv, y[7] * inv)};
@@ -375,7 +355,138 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
         }
       }
     }
+}
+
+// Workgroup `share` of a.shares takes its share of all units.
+template <int D, int RT>
+__device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, SegLds<D, RT, 4>& lds) {
+  const int64_t total = unit_totals(a, 0).all * a.kv_heads;
+  const int64_t quota = (total + a.shares - 1) / a.shares;
+  const int64_t u0 = share * quota, u1 = min(u0 + quota, total);
+  if (u0 >= u1) return;
+  int64_t before;                    // units of one key head in the sequences before b
+  int b = find_seq(a, u0 / a.kv_heads, before);
+  for (int64_t u = u0; u < u1;) {
+    bool bad_len;
+    const int len = length_of(a, b, bad_len), nb = (len + kPgUnit - 1) / kPgUnit;
+    const int64_t first = before * a.kv_heads;
+    if (nb == 0 || u >= first + static_cast<int64_t>(nb) * a.kv_heads) {
+      before += nb;
+      ++b;
+      continue;
+    }
+    // an item's first unit is kv_heads * before + h * its units
+    const int h = static_cast<int>((u - first) / nb);
+    const int64_t item0 = first + static_cast<int64_t>(h) * nb;
+    const int k0 = static_cast<int>(u - item0);
+    const int k1 = static_cast<int>(min(static_cast<int64_t>(nb), u1 - item0));
+    const bool whole = k0 == 0 && k1 == nb;
+    const int64_t slot = whole ? (a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h : -1)
+                               : 2 * static_cast<int64_t>(share) + (u == u0 ? 0 : 1);
+    segment<D, RT, 4>(a, b, h, len, bad_len, r0, k0, k1, slot, lds);
     u = item0 + k1;
+  }
+}
+
+// All rows of the batch against a part of the prefix: tile `row_tile` of 128 rows of
+// head h, split `split` of the keys.
+constexpr int kPreWaves = 4;
+constexpr int kPreRows = 32 * kPreWaves;
+#ifndef PREB
+#define PREB 256
+#endif
+constexpr int kPreBlocks = PREB;     // workgroups of the prefix, about
+
+template <int D>
+__device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char* lds) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hf = lane >> 5;
+  const int h = block % a.kv_heads, rest = block / a.kv_heads, split = rest / a.row_tiles;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.group;
+  const int64_t wr0 = static_cast<int64_t>(rest % a.row_tiles) * kPreRows + 32 * wave;
+  const int tiles = (a.prefix + kFlKeys - 1) / kFlKeys;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  const int64_t r = min(wr0 + n, rows - 1), tok = r / a.group;
+  const int hd = h * a.group + static_cast<int>(r % a.group);
+
+  // lane l: the page of the wave's 16 rows of tile ids0 + l
+  int ids = 0, ids0 = t0 - 64;
+  bool bad = false;
+  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
+    if (t - ids0 >= 64) {              // first asked for K, a tile ahead of V
+      ids0 = max(t - 1, t0);
+      ids = ldg<int32_t>(a.pages + (min((ids0 + lane) * kFlKeys + row, a.prefix - 1) >> a.c.page_shift));
+      const bool out_of = ids < 0 || ids >= a.c.n_pages;
+      bad = bad || (out_of && ids0 + lane < t1);
+      if (out_of) ids = 0;
+    }
+    const int key = min(t * kFlKeys + row, a.prefix - 1);
+    const int id = __builtin_amdgcn_readlane(ids, t - ids0);
+    const int in_page = key & ((1 << a.c.page_shift) - 1);
+    const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
+    kp = a.c.k + base;
+    vp = a.c.v + base;
+    last = a.prefix - 1 - key;
+  };
+  bf16x8 q[D / 16];
+  const uint16_t* qp = a.q + tok * a.q_token + hd * a.q_head + 8 * hf;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) q[ks] = as_bf16x8(ldg16(qp + 16 * ks));
+  FlashRows<D> st;
+  st.m = kNegInf;
+  st.l = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
+  const int w_max = wr0 < rows ? a.prefix - 1 : -1;   // a wave without rows only loads
+  flash<D, kPreWaves>(q, t0, t1, a.prefix - 1, a.prefix - 1, w_max, a.prefix - 1, a.c2, lds, D, D, src, st);
+  // a page outside the cache: the waves load different rows, so all tell
+  const bool any_bad = __syncthreads_or(bad);
+  const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
+  if (wr0 + n < rows) {
+    const int64_t at = (static_cast<int64_t>(split) * a.kv_heads + h) * rows + r;
+    float* op = a.pre_o + at * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<f32x4*>(op + 32 * dt + 8 * c + 4 * hf) =
+            f32x4{st.o[dt][4 * c], st.o[dt][4 * c + 1], st.o[dt][4 * c + 2], st.o[dt][4 * c + 3]};
+    if (hf == 0) *reinterpret_cast<float2*>(a.pre_ml + at * 2) = float2{st.m, l};
+  }
+}
+
+template <int D, int RT>
+__global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const PagedArgs a) {
+  __shared__ SegLds<D, RT, 4> lds;
+  shares<D, RT>(a, blockIdx.x, 16 * RT * blockIdx.y, lds);
+}
+
+// The prefix's workgroups, then the shares (more than 32 rows: a half of the rows each).
+template <int D, int RT>
+__global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged_prefix(const PagedArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  const int block = blockIdx.x - a.prefix_blocks;
+  if (block < 0) prefix_part<D>(a, blockIdx.x, lds);
+  else shares<D, RT>(a, block % a.shares, 16 * RT * (block / a.shares), *reinterpret_cast<SegLds<D, RT, 4>*>(lds));
+}
+
+// A workgroup for 16 rows of an item; nothing is left to join.
+template <int D>
+__global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const PagedArgs a) {
+  __shared__ SegLds<D, 1, kPgShortWaves> lds;
+  constexpr int kUnit = 32 * kPgShortWaves;
+  const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, M = a.q_len * a.group, r0 = 16 * blockIdx.y;
+  bool bad_len;
+  const int len = length_of(a, b, bad_len);
+  if (len > 0) {
+    segment<D, 1, kPgShortWaves>(a, b, h, len, bad_len, r0, 0, (len + kUnit - 1) / kUnit, -1, lds);
+    return;
+  }
+  for (int i = threadIdx.x; i < (min(M, r0 + 16) - r0) * (D / 8); i += 64 * kPgShortWaves) {
+    const int r = r0 + i / (D / 8), tok = r / a.group, hd = h * a.group + r % a.group;
+    *reinterpret_cast<u32x4*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + 8 * (i % (D / 8))) =
+        u32x4{0u, 0u, 0u, 0u};
   }
 }
 
@@ -383,19 +494,18 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const Pag
 // for a row: the parts' weights first, all at once, then 256 / (D / 4) groups of
 // threads add up the parts in a fixed order.  Also writes the rows of sequences
 // without keys.
-constexpr int kPgMostParts = 1024;   // of a row: shares and splits are at most 512 each
+constexpr int kPgMostParts = 1024;   // of a row: shares are at most 512, splits at most kPreBlocks
 
 template <int D>
 __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   constexpr int kLanes = D / 4, kWays = kPgThreads / kLanes, kWaves = kPgThreads / 64;
-  __shared__ int64_t lds_t[2 * kWaves];
   __shared__ float weight[kPgMostParts];
   __shared__ float red[kWaves];
   __shared__ f32x4 sum[kWays][kLanes];
   const int M = a.q_len * a.group;
   const int r = blockIdx.x % M, item = blockIdx.x / M, h = item % a.kv_heads, b = item / a.kv_heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Totals tt = unit_totals(a, b, lds_t);
+  const Totals tt = unit_totals(a, b);
   const int64_t total = tt.all * a.kv_heads;
   const int64_t quota = (total + a.shares - 1) / a.shares;
   bool bad;
@@ -461,40 +571,56 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
 
 // Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's.
 struct PagedPlan {
-  int rt, shares, splits;
-  int64_t slots, rows, pre_rows;
+  int rt, shares, splits, row_tiles;
+  bool alone;                        // k_paged_short
   size_t po, pml, pre_o, pre_ml, total;
 };
 
 PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
   PagedPlan p{};
+  auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
   const int64_t M = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
   p.rt = M <= 16 ? 1 : 2;
-  const int64_t items = static_cast<int64_t>(d.batch) * d.kv_heads;
-  const int64_t units = items * ((static_cast<int64_t>(c.max_pages) * c.page_size + kPgUnit - 1) / kPgUnit);
+  const int64_t items = static_cast<int64_t>(d.batch) * d.kv_heads, keys = static_cast<int64_t>(c.max_pages) * c.page_size;
+  p.alone = d.prefix_len == 0 && keys <= kPgShort;
+  p.total = 256;
+  if (p.alone) return p;
+  const int64_t units = items * ((keys + kPgUnit - 1) / kPgUnit);
   const int64_t most = p.rt == 1 ? 512 : 256;   // the workgroups that are resident at once
   p.shares = static_cast<int>(units < most ? units : most);
-  p.slots = 2 * p.shares + (d.prefix_len > 0 ? items : 0);
-  p.rows = p.slots * M;
-  p.pre_rows = static_cast<int64_t>(d.batch) * M;
-  p.splits = d.prefix_len > 0 ? prefix_splits(p.pre_rows, d.kv_heads, d.prefix_len) : 0;
-  auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
-  const size_t pre = static_cast<size_t>(p.splits) * d.kv_heads * p.pre_rows;
+  const int64_t rows = static_cast<int64_t>(d.batch) * M;
+  if (d.prefix_len > 0) {
+    p.row_tiles = static_cast<int>((rows + kPreRows - 1) / kPreRows);
+    const int64_t blocks = static_cast<int64_t>(p.row_tiles) * d.kv_heads, tiles = (d.prefix_len + kFlKeys - 1) / kFlKeys;
+    const int64_t want = (kPreBlocks + blocks - 1) / blocks;
+    p.splits = static_cast<int>(want < tiles ? want : tiles);
+  }
+  const size_t own = (2 * static_cast<size_t>(p.shares) + (p.splits ? items : 0)) * M;
+  const size_t pre = static_cast<size_t>(p.splits) * d.kv_heads * rows;
   p.po = 0;
-  p.pml = up(p.po + p.rows * d.head_dim * 4);
-  p.pre_o = up(p.pml + p.rows * 8);
+  p.pml = up(p.po + own * d.head_dim * 4);
+  p.pre_o = up(p.pml + own * 8);
   p.pre_ml = up(p.pre_o + pre * d.head_dim * 4);
   p.total = up(p.pre_ml + pre * 8);
   return p;
 }
 
-template <int D>
-void launch_paged_d(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
+template <int D, int RT>
+void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
   const int M = a.q_len * a.group;
-  // more than 32 rows: every share twice, a half of the rows each (four row tiles
-  // spill registers); the halves run on one XCD, whose L2 holds what they both read
-  if (p.rt == 1) launch_kernel(k_paged<D, 1>, p.shares, kPgThreads, 0, s, a);
-  else launch_kernel(k_paged<D, 2>, dim3(p.shares, (M + 31) / 32), kPgThreads, 0, s, a);
+  // more than 32 rows: every share (item) twice, a half of the rows each (four row tiles
+  // spill registers)
+  const int halves = (M + 16 * RT - 1) / (16 * RT);
+  if (p.alone) {
+    launch_kernel(k_paged_short<D>, dim3(a.batch * a.kv_heads, (M + 15) / 16), 64 * kPgShortWaves, 0, s, a);
+    return;
+  }
+  if (p.splits) {
+    constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D>();
+    launch_kernel(k_paged_prefix<D, RT>, a.prefix_blocks + p.shares * halves, kPgThreads, lds, s, a);
+  } else {
+    launch_kernel(k_paged<D, RT>, dim3(p.shares, halves), kPgThreads, 0, s, a);
+  }
   launch_kernel(k_paged_join<D>, a.batch * a.kv_heads * M, kPgThreads, 0, s, a);
 }
 
@@ -506,18 +632,19 @@ hipError_t launch_paged(const dsk_paged_desc& d, const void* q, const dsk_kv_cac
                         const int32_t* prefix, void* out, void* ws, hipStream_t s) {
   const PagedPlan p = plan_of(d, c);
   char* w = static_cast<char*>(ws);
-  float* pre_o = reinterpret_cast<float*>(w + p.pre_o);
-  float* pre_ml = reinterpret_cast<float*>(w + p.pre_ml);
-  PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, cache_view(c),
-              reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml), pre_o, pre_ml,
-              d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
-              d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits};
-  if (d.prefix_len > 0) {
-    hipError_t e = launch_prefix(d, q, c, prefix, p.splits, pre_o, pre_ml, s);
-    if (e != hipSuccess) return e;
+  const PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, cache_view(c),
+                    reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml),
+                    reinterpret_cast<float*>(w + p.pre_o), reinterpret_cast<float*>(w + p.pre_ml), prefix,
+                    d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
+                    d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits, p.row_tiles,
+                    p.row_tiles * p.splits * d.kv_heads};
+  if (d.head_dim == 64) {
+    if (p.rt == 1) launch_paged_rt<64, 1>(p, a, s);
+    else launch_paged_rt<64, 2>(p, a, s);
+  } else {
+    if (p.rt == 1) launch_paged_rt<128, 1>(p, a, s);
+    else launch_paged_rt<128, 2>(p, a, s);
   }
-  if (d.head_dim == 64) launch_paged_d<64>(p, a, s);
-  else launch_paged_d<128>(p, a, s);
   return hipGetLastError();
 }
 

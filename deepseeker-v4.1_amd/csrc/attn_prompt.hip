@@ -1,4 +1,4 @@
-// Attention over packed prompts, and a batch's rows over the prefix they share.
+// Attention over packed prompts.
 //
 // The rows of a tile are (token, head of the group) pairs of one key head,
 // token by token: the heads of a group share every key tile that is loaded, a
@@ -13,7 +13,6 @@ constexpr int kFlWaves = 4;
 constexpr int kFlThreads = 64 * kFlWaves;
 constexpr int kFlRows = 32 * kFlWaves;
 
-// ------------------------------------------------------------------ prompts
 struct PromptArgs {
   const uint16_t *q, *k, *v;
   uint16_t* out;
@@ -119,98 +118,12 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
     }
 }
 
-// ------------------------------------------------------------------ prefix
-struct PrefixArgs {
-  const uint16_t* q;
-  CacheView c;
-  const int32_t* pages;
-  float *po, *pml;
-  int64_t q_token, q_head, rows;     // rows: batch * q_len * group
-  float c2;
-  int32_t kv_heads, group, len, splits, row_tiles;
-};
-
-template <int D>
-__global__ __launch_bounds__(kFlThreads, 2) void k_prefix(const PrefixArgs a) {
-  extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 31, hf = lane >> 5;
-  const int h = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const int split = rest / a.row_tiles;
-  const int64_t wr0 = static_cast<int64_t>(rest % a.row_tiles) * kFlRows + 32 * wave;
-  const int tiles = (a.len + kFlKeys - 1) / kFlKeys;
-  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-  const int64_t r = min(wr0 + n, a.rows - 1), tok = r / a.group;
-  const int hd = h * a.group + static_cast<int>(r % a.group);
-
-  bf16x8 q[D / 16];
-  const uint16_t* qp = a.q + tok * a.q_token + hd * a.q_head + 8 * hf;
-#pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) q[ks] = as_bf16x8(ldg16(qp + 16 * ks));
-  FlashRows<D> st;
-  st.m = kNegInf;
-  st.l = 0.0f;
-#pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
-  bool bad = false;
-  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
-    const int key = min(t * kFlKeys + row, a.len - 1);
-    int id = a.pages[key >> a.c.page_shift];
-    if (id < 0 || id >= a.c.n_pages) {
-      bad = true;
-      id = 0;
-    }
-    const int in_page = key & ((1 << a.c.page_shift) - 1);
-    const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
-    kp = a.c.k + base;
-    vp = a.c.v + base;
-    last = a.len - 1 - key;
-  };
-  const int w_max = wr0 < a.rows ? a.len - 1 : -1;    // a wave without rows only loads
-  flash<D, kFlWaves>(q, t0, t1, a.len - 1, a.len - 1, w_max, a.len - 1, a.c2, lds, D, D, src, st);
-  // a page outside the cache: the waves load different rows, so all tell
-  const bool any_bad = __syncthreads_or(bad);
-  const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
-  if (wr0 + n < a.rows) {
-    const int64_t at = (static_cast<int64_t>(split) * a.kv_heads + h) * a.rows + r;
-    float* op = a.po + at * D;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<f32x4*>(op + 32 * dt + 8 * c + 4 * hf) =
-            f32x4{st.o[dt][4 * c], st.o[dt][4 * c + 1], st.o[dt][4 * c + 2], st.o[dt][4 * c + 3]};
-    if (hf == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = float2{st.m, l};
-  }
-}
-
 template <int D, class Args>
 void launch_flash(void (*kernel)(Args), const Args& a, unsigned blocks, hipStream_t s) {
   launch_kernel(kernel, blocks, kFlThreads, flash_lds<D>(), s, a);
 }
 
 }  // namespace
-
-int prefix_splits(int64_t rows, int kv_heads, int prefix_len) {
-  const int64_t blocks = (rows + kFlRows - 1) / kFlRows * kv_heads;
-  const int64_t tiles = (prefix_len + kFlKeys - 1) / kFlKeys;
-  const int64_t want = (512 + blocks - 1) / blocks;     // two workgroups a CU
-  return static_cast<int>(want < tiles ? want : tiles);   // at most 512
-}
-
-hipError_t launch_prefix(const dsk_paged_desc& d, const void* q, const dsk_kv_cache& c, const int32_t* prefix,
-                         int splits, float* pre_o, float* pre_ml, hipStream_t s) {
-  const int group = d.heads / d.kv_heads;
-  const int64_t rows = static_cast<int64_t>(d.batch) * d.q_len * group;
-  const int row_tiles = static_cast<int>((rows + kFlRows - 1) / kFlRows);
-  const PrefixArgs a{static_cast<const uint16_t*>(q), cache_view(c), prefix, pre_o, pre_ml, d.q_token, d.q_head,
-                     rows, d.scale * kLog2e, d.kv_heads, group, d.prefix_len, splits, row_tiles};
-  const unsigned blocks = static_cast<unsigned>(row_tiles) * splits * d.kv_heads;
-  if (d.head_dim == 64) launch_flash<64>(k_prefix<64>, a, blocks, s);
-  else launch_flash<128>(k_prefix<128>, a, blocks, s);
-  return hipGetLastError();
-}
 
 hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k, const void* v, const int32_t* cu_q,
                          const int32_t* cu_k, void* out, hipStream_t s) {

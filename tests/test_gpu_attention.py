@@ -293,14 +293,15 @@ def test_prompt_long_rows():
 # ------------------------------------------------------------------ decode
 @pytest.mark.parametrize("heads,kv,dim,page,q_len", [(8, 2, 128, 64, 1), (4, 4, 64, 16, 1), (8, 1, 64, 32, 3), (16, 1, 128, 16, 4),
                                                      (10, 2, 128, 128, 2), (64, 1, 64, 256, 1), (3, 3, 128, 16, 16), (20, 1, 128, 32, 2)])
-@pytest.mark.parametrize("prefix", [0, 1, 130])
-def test_paged(heads, kv, dim, page, q_len, prefix):
+@pytest.mark.parametrize("prefix,spare", [(0, 1), (0, 70), (1, 1), (130, 1)])
+def test_paged(heads, kv, dim, page, q_len, prefix, spare):
     print(f"paged {heads},{kv},{dim} page {page} q_len {q_len} prefix {prefix}", flush=True)
     g = gen(heads * dim + page + prefix)
     lens = [0, 1, 15, 16, 17, 127, 128, 129, 300]
     used = [-(-n // page) for n in lens]
     shared = -(-prefix // page)
-    table, kc, vc = paged_setup(g, used + [shared], max(max(used) + 1, shared), 2, kv, page, dim)
+    # wide tables: the work is shared out; short ones: a workgroup for an item
+    table, kc, vc = paged_setup(g, used + [shared], max(max(used) + spare, shared), 2, kv, page, dim)
     pre, table = table[-1, :shared], table[:-1]
     # what no sequence holds is NaN: rows behind the lengths, and pages of nobody
     held = torch.zeros(kc.shape[0], page, dtype=torch.bool)
@@ -406,10 +407,12 @@ def test_paged_far_pages():
     assert_within(got, want[:, 0], tol[:, 0])
 
 
-def test_paged_views_and_scratch():
-    """Strided queries and outputs; a workspace of the caller's, full of NaN, twice."""
+@pytest.mark.parametrize("width", [8, 80])
+def test_paged_views_and_scratch(width):
+    """Strided queries and outputs; a workspace of the caller's, full of NaN, twice; a table row that one workgroup takes
+    alone, and one that needs the workspace."""
     g = gen(35)
-    table, kc, vc = paged_setup(g, [3, 7], 8, 0, 2, 16, 64)
+    table, kc, vc = paged_setup(g, [3, 7], width, 0, 2, 16, 64)
     dev = [x.to(DEV) for x in (kc, vc, table)]
     q = normal(g, 2, 2, 4, 64)
     qkv = torch.cat([q.flatten(2), normal(g, 2, 2, 256)], -1).to(DEV)
@@ -422,7 +425,7 @@ def test_paged_views_and_scratch():
         assert got is out
         assert_within(out, want, tol)
     with pytest.raises(_lib.DskError, match="DSK_ESPACE"):
-        dsk_moe.paged_attention(view, *dev, ints([40, 111]), workspace=ws[:256])
+        dsk_moe.paged_attention(view, *dev, ints([40, 111]), workspace=ws[:128 if width == 8 else 1024])
 
 
 def test_same_call_same_bits():
