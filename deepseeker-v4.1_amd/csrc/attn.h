@@ -33,8 +33,8 @@ struct CacheView {
 
 inline int page_shift_of(int page_size) { return __builtin_ctz(static_cast<unsigned>(page_size)); }
 
-inline CacheView cache_view(const dsk_kv_cache& c) {
-  return CacheView{static_cast<uint16_t*>(c.k), static_cast<uint16_t*>(c.v), c.table, c.table_stride,
+inline CacheView cache_view(const dsk_kv_cache& c, void* k, void* v, const int32_t* table) {
+  return CacheView{static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), table, c.table_stride,
                    c.n_pages, page_shift_of(c.page_size), c.n_seqs, c.max_pages};
 }
 
@@ -69,12 +69,12 @@ __device__ __forceinline__ float sum_across16(float x) {
 
 hipError_t launch_qk(const dsk_qk_desc& d, const void* q, const void* k, const void* v, const int32_t* positions,
                      const int32_t* seq, const double* freq, const float* q_gamma, const float* k_gamma,
-                     const dsk_kv_cache* cache, void* q_out, void* k_out, hipStream_t s);
+                     const CacheView* cache, void* q_out, void* k_out, hipStream_t s);   // cache: null, no append
 
 // Workspace of dsk_paged_attention, in bytes.
 size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c);
-hipError_t launch_paged(const dsk_paged_desc& d, const void* q, const dsk_kv_cache& c, const int32_t* lens,
-                        const int32_t* prefix, void* out, void* ws, hipStream_t s);
+hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const void* q, const CacheView& view,
+                        const int32_t* lens, const int32_t* prefix, void* out, void* ws, hipStream_t s);
 hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k, const void* v, const int32_t* cu_q,
                          const int32_t* cu_k, void* out, hipStream_t s);
 

@@ -44,9 +44,7 @@ int check_out(const char* fn, const char* what, int64_t token, int64_t head, int
 }
 
 int check_cache(const char* fn, const dsk_kv_cache* c) {
-  if (!c || !c->k || !c->v || !c->table) return fail(DSK_EINVAL, "%s: NULL cache, k, v or table", fn);
-  if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(DSK_EALIGN, "%s: the cache must be 16-byte aligned", fn);
-  if (!aligned(c->table, 4)) return fail(DSK_EALIGN, "%s: the page table must be 4-byte aligned", fn);
+  if (!c) return fail(DSK_EINVAL, "%s: cache is NULL", fn);
   const int p = c->page_size;
   if (p != 16 && p != 32 && p != 64 && p != 128 && p != 256)
     return fail(DSK_EINVAL, "%s: page_size=%d must be 16, 32, 64, 128 or 256", fn, p);
@@ -56,6 +54,13 @@ int check_cache(const char* fn, const dsk_kv_cache* c) {
     return fail(DSK_EUNSUPPORTED, "%s: a sequence of %lld positions exceeds 2^30", fn, static_cast<long long>(c->max_pages) * p);
   if (c->table_stride < c->max_pages && c->n_seqs > 1)
     return fail(DSK_EINVAL, "%s: table_stride=%lld is less than max_pages=%d", fn, static_cast<long long>(c->table_stride), c->max_pages);
+  return DSK_OK;
+}
+
+int check_cache_pointers(const char* fn, const void* k, const void* v, const int32_t* table) {
+  if (!k || !v || !table) return fail(DSK_EINVAL, "%s: k_cache, v_cache or table is NULL", fn);
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(DSK_EALIGN, "%s: the cache must be 16-byte aligned", fn);
+  if (!aligned(table, 4)) return fail(DSK_EALIGN, "%s: the page table must be 4-byte aligned", fn);
   return DSK_OK;
 }
 
@@ -108,9 +113,10 @@ int dsk_qk_norm_rope(const dsk_qk_desc* d, const void* q, const void* k, const i
                              static_cast<hipStream_t>(stream)), fn);
 }
 
-int dsk_kv_append(const dsk_qk_desc* d, const void* q, const void* k, const void* v, const int32_t* positions,
-                  const int32_t* seq, const double* freq, const float* q_gamma, const float* k_gamma,
-                  const dsk_kv_cache* cache, void* q_out, void* k_out, void* stream) {
+int dsk_kv_append(const dsk_qk_desc* d, const dsk_kv_cache* cache, const void* q, const void* k, const void* v,
+                  const int32_t* positions, const int32_t* seq, const double* freq, const float* q_gamma,
+                  const float* k_gamma, void* k_cache, void* v_cache, const int32_t* table, void* q_out, void* k_out,
+                  void* stream) {
   const char* fn = "dsk_kv_append";
   int rc = check_qk(fn, d, q, k, positions, freq, q_gamma, k_gamma, q_out);
   if (rc) return rc;
@@ -119,10 +125,12 @@ int dsk_kv_append(const dsk_qk_desc* d, const void* q, const void* k, const void
   if (!aligned(seq, 4)) return fail(DSK_EALIGN, "%s: seq must be 4-byte aligned", fn);
   if (d->prefix_len < 0) return fail(DSK_EINVAL, "%s: prefix_len=%d must be >= 0", fn, d->prefix_len);
   rc = check_cache(fn, cache);
+  if (!rc) rc = check_cache_pointers(fn, k_cache, v_cache, table);
   if (!rc) rc = check_strides(fn, "v", d->v_token, d->v_head, d->dtype == DSK_DTYPE_BF16 ? 8 : 4);
   if (!rc && k_out) rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->kv_heads, d->head_dim);
   if (rc) return rc;
-  return hip_check(launch_qk(*d, q, k, v, positions, seq, freq, q_gamma, k_gamma, cache, q_out, k_out,
+  const CacheView view = cache_view(*cache, k_cache, v_cache, table);
+  return hip_check(launch_qk(*d, q, k, v, positions, seq, freq, q_gamma, k_gamma, &view, q_out, k_out,
                              static_cast<hipStream_t>(stream)), fn);
 }
 
@@ -181,10 +189,13 @@ int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cac
   return DSK_OK;
 }
 
-int dsk_paged_attention(const dsk_paged_desc* d, const void* q, const dsk_kv_cache* cache, const int32_t* lens,
-                        const int32_t* prefix, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, const void* q, const void* k_cache,
+                        const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix,
+                        void* out, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "dsk_paged_attention";
   int rc = check_paged(fn, d, cache);
+  if (rc) return rc;
+  rc = check_cache_pointers(fn, k_cache, v_cache, table);
   if (rc) return rc;
   if (!q || !lens || !out || !workspace || (d->prefix_len > 0 && !prefix))
     return fail(DSK_EINVAL, "%s: NULL pointer argument", fn);
@@ -193,7 +204,8 @@ int dsk_paged_attention(const dsk_paged_desc* d, const void* q, const dsk_kv_cac
   if (!aligned(lens, 4) || !aligned(prefix, 4)) return fail(DSK_EALIGN, "%s: lens and prefix must be 4-byte aligned", fn);
   if (workspace_bytes < paged_workspace(*d, *cache))
     return fail(DSK_ESPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, paged_workspace(*d, *cache));
-  return hip_check(launch_paged(*d, q, *cache, lens, prefix, out, workspace, static_cast<hipStream_t>(stream)), fn);
+  const CacheView view = cache_view(*cache, const_cast<void*>(k_cache), const_cast<void*>(v_cache), table);
+  return hip_check(launch_paged(*d, *cache, q, view, lens, prefix, out, workspace, static_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

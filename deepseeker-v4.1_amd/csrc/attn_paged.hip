@@ -392,10 +392,8 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
 // head h, split `split` of the keys.
 constexpr int kPreWaves = 4;
 constexpr int kPreRows = 32 * kPreWaves;
-#ifndef PREB
-#define PREB 256
-#endif
-constexpr int kPreBlocks = PREB;     // workgroups of the prefix, about
+constexpr int kPreBlocks = 256;      // workgroups of the prefix, about: one a CU
+constexpr int kPreStages = 2;
 
 template <int D>
 __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char* lds) {
@@ -439,7 +437,7 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
   const int w_max = wr0 < rows ? a.prefix - 1 : -1;   // a wave without rows only loads
-  flash<D, kPreWaves>(q, t0, t1, a.prefix - 1, a.prefix - 1, w_max, a.prefix - 1, a.c2, lds, D, D, src, st);
+  flash<D, kPreWaves, kPreStages>(q, t0, t1, a.prefix - 1, a.prefix - 1, w_max, a.prefix - 1, a.c2, lds, D, D, src, st);
   // a page outside the cache: the waves load different rows, so all tell
   const bool any_bad = __syncthreads_or(bad);
   const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
@@ -616,7 +614,7 @@ void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
     return;
   }
   if (p.splits) {
-    constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D>();
+    constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D, kPreStages>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D, kPreStages>();
     launch_kernel(k_paged_prefix<D, RT>, a.prefix_blocks + p.shares * halves, kPgThreads, lds, s, a);
   } else {
     launch_kernel(k_paged<D, RT>, dim3(p.shares, halves), kPgThreads, 0, s, a);
@@ -628,11 +626,11 @@ void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
 
 size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c) { return plan_of(d, c).total; }
 
-hipError_t launch_paged(const dsk_paged_desc& d, const void* q, const dsk_kv_cache& c, const int32_t* lens,
-                        const int32_t* prefix, void* out, void* ws, hipStream_t s) {
+hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const void* q, const CacheView& view,
+                        const int32_t* lens, const int32_t* prefix, void* out, void* ws, hipStream_t s) {
   const PagedPlan p = plan_of(d, c);
   char* w = static_cast<char*>(ws);
-  const PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, cache_view(c),
+  const PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, view,
                     reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml),
                     reinterpret_cast<float*>(w + p.pre_o), reinterpret_cast<float*>(w + p.pre_ml), prefix,
                     d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,

@@ -218,11 +218,11 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& a, hipStream_t s) {
 
 hipError_t launch_qk(const dsk_qk_desc& d, const void* q, const void* k, const void* v, const int32_t* positions,
                      const int32_t* seq, const double* freq, const float* q_gamma, const float* k_gamma,
-                     const dsk_kv_cache* cache, void* q_out, void* k_out, hipStream_t s) {
+                     const CacheView* cache, void* q_out, void* k_out, hipStream_t s) {
   QkArgs a{q, k, v, positions, seq, freq, q_gamma, k_gamma, static_cast<uint16_t*>(q_out),
            static_cast<uint16_t*>(k_out), d.q_token, d.q_head, d.k_token, d.k_head, d.v_token, d.v_head,
            d.qo_token, d.qo_head, d.ko_token, d.ko_head, d.tokens, d.heads, d.kv_heads, d.rot_dim, d.rot_first,
-           d.prefix_len, d.norm, d.eps, d.mscale, cache ? cache_view(*cache) : CacheView{}, cache != nullptr};
+           d.prefix_len, d.norm, d.eps, d.mscale, cache ? *cache : CacheView{}, cache != nullptr};
   if (d.head_dim == 64) launch_qk_d<64>(d, a, s);
   else launch_qk_d<128>(d, a, s);
   return hipGetLastError();

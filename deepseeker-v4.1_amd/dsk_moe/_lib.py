@@ -62,8 +62,7 @@ class Residual(ctypes.Structure):
 class KVCache(ctypes.Structure):
     """Mirror of ``dsk_kv_cache``."""
 
-    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("table_stride", _i64), ("n_pages", _i32),
-                ("page_size", _i32), ("n_seqs", _i32), ("max_pages", _i32)]
+    _fields_ = [("table_stride", _i64)] + [(n, _i32) for n in ("n_pages", "page_size", "n_seqs", "max_pages")]
 
 
 class QkDesc(ctypes.Structure):
@@ -124,11 +123,10 @@ SIGNATURES = {
     "dsk_q3_repack": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp]),
     "dsk_fp8_block_dequant": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
     "dsk_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "dsk_kv_append": (ctypes.c_int, [ctypes.POINTER(QkDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, PCache, _vp,
-                                     _vp, _vp]),
+    "dsk_kv_append": (ctypes.c_int, [ctypes.POINTER(QkDesc), PCache] + [_vp] * 14),
     "dsk_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "dsk_paged_attention_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache, ctypes.POINTER(_sz)]),
-    "dsk_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedDesc), _vp, PCache, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dsk_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache] + [_vp] * 8 + [_sz, _vp]),
     "dsk_rmsnorm": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, ctypes.c_float, _i32, _vp, _vp, _vp]),
 }
 
@@ -164,10 +162,12 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def check(name: str, rc: int) -> None:
+    """Raise DskError if an entry point returned a negative status."""
+    if rc != DSK_OK:
+        raise DskError(name, rc, load().dsk_last_error().decode(errors="replace"))
+
+
 def call(name: str, *args) -> None:
     """Call an entry point and raise DskError on a negative status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
-    if rc != DSK_OK:
-        msg = lib.dsk_last_error().decode(errors="replace")
-        raise DskError(name, rc, msg)
+    check(name, getattr(load(), name)(*args))

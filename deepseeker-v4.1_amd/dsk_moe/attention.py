@@ -102,35 +102,40 @@ def _out_strides(out: torch.Tensor | None, shape: tuple, dev: torch.device, what
     return out.stride()[:2]
 
 
-def _call(dev: torch.device, name: str, *args) -> None:
-    """The entry point on ``dev``'s current stream, with ``dev`` current."""
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args, stream)
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, stream)
-
-
 # A call's checks depend on its tensors' sizes, strides, types and devices and on its numbers alone, so what they
-# found (the descriptor and the outputs' shapes; no tensor, no address) serves later calls of the same kind: a decode
-# step's host work is a third of that of checking each time (decode_1: 18.3 us a call, without).
-_plans: dict[tuple, tuple] = {}
-_MOST_PLANS = 4096
+# found -- a plan: the device, the entry point and its descriptors; no tensor, no address -- serves later calls of the
+# same kind.  A decode step's host work is then a third of that of checking each time (18 us a call).
+_plans: dict[str, dict[tuple, tuple]] = {"qk": {}, "append": {}, "prompt": {}, "paged": {}}
+_MOST_PLANS = 1024
+_CONTIGUOUS = torch.contiguous_format
 
 
 def _sig(t: torch.Tensor | None):
     return (t.shape, t.stride(), t.dtype, t.get_device()) if t is not None else None
 
 
-def _planned(key: tuple, make, *args, **kwargs) -> tuple:
-    plan = _plans.get(key)
-    if plan is None:
-        plan = make(*args, **kwargs)
-        if len(_plans) >= _MOST_PLANS:
-            _plans.clear()
-        _plans[key] = plan
+def _plan(kind: str, key: tuple, make, *args) -> tuple:
+    plan = make(*args)
+    if len(_plans[kind]) >= _MOST_PLANS:
+        _plans[kind].clear()
+    _plans[kind][key] = plan
     return plan
+
+
+def _call(name: str, fn, dev: torch.device, *args) -> None:
+    """The entry point on ``dev``'s current stream, with ``dev`` current."""
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(name, rc)
+
+
+def _p(t: torch.Tensor | None):
+    return t.data_ptr() if t is not None else None
 
 
 def _check_cache(k_cache, v_cache, table, kv_heads: int, dim: int, dev: torch.device) -> None:
@@ -143,21 +148,14 @@ def _check_cache(k_cache, v_cache, table, kv_heads: int, dim: int, dev: torch.de
         raise ValueError(f"table must be int32 [sequences, pages] on {dev} with contiguous rows")
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor) -> _lib.KVCache:
-    n_pages, _, page_size, _ = k_cache.shape
-    n_seqs, max_pages = table.shape
-    return _lib.KVCache(k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), table.stride(0), n_pages, page_size,
-                        n_seqs, max_pages)
-
-
-def _p(t: torch.Tensor | None):
-    return t.data_ptr() if t is not None else None
+def _cache(k_cache: torch.Tensor, table: torch.Tensor) -> _lib.KVCache:
+    return _lib.KVCache(table.stride(0), k_cache.shape[0], k_cache.shape[2], table.shape[0], table.shape[1])
 
 
 # ------------------------------------------------------------------ norms, rotation, append
 def _qk_plan(q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache, interleaved,
              rot_first, mscale, norm, eps, prefix_len):
-    """(device, descriptor) of a checked call; the outputs have q's and k's shapes."""
+    """(entry point, device, descriptor, cache) of a checked call; the outputs have q's and k's shapes."""
     dev = _hip(k)
     _rows(k, "k", (_BF16, _F32), dev)
     tokens, kv_heads, dim = k.shape
@@ -191,9 +189,13 @@ def _qk_plan(q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, tabl
     if k_out is not None or v is None:
         ko = _out_strides(k_out, k.shape, dev, "k_out")
     ks = k.stride()
-    return dev, _lib.QkDesc(tokens, heads, kv_heads, dim, _lib.DTYPE_BF16 if k.dtype == _BF16 else _lib.DTYPE_F32,
+    desc = _lib.QkDesc(tokens, heads, kv_heads, dim, _lib.DTYPE_BF16 if k.dtype == _BF16 else _lib.DTYPE_F32,
                             1 if norm else 0, rot, int(rot_first), 1 if interleaved else 0, int(prefix_len), float(eps),
                             float(mscale), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], *qo, *ko)
+    lib = _lib.load()
+    if v is None:
+        return lib.dsk_qk_norm_rope, dev, ctypes.byref(desc), None
+    return lib.dsk_kv_append, dev, ctypes.byref(desc), ctypes.byref(_cache(k_cache, table))
 
 
 def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor | None = None, *,
@@ -205,15 +207,18 @@ def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tenso
     elements rot_first .. rot_first + 2 len(freq) by positions[t] * freq (``interleaved``: pairs (2i, 2i+1), otherwise (i,
     i + len(freq))), in one pass.  q and k bf16 or float32; the results bf16.  Tokens at negative positions are left out
     (their output rows are not written).  q_out / k_out may be q / k themselves."""
-    tensors = (q, k, None, positions, freq, q_gamma, k_gamma, q_out, k_out, None, None, None, None)
-    numbers = (interleaved, rot_first, mscale, norm, eps, 0)
-    key = ("qk", _sig(q), _sig(k), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out), numbers)
-    dev, desc = _planned(key, _qk_plan, *tensors, *numbers)
+    key = (_sig(q), _sig(k), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out),
+           interleaved, rot_first, mscale, norm, eps)
+    plan = _plans["qk"].get(key)
+    if plan is None:
+        plan = _plan("qk", key, _qk_plan, q, k, None, positions, freq, q_gamma, k_gamma, q_out, k_out, None, None, None, None,
+                     interleaved, rot_first, mscale, norm, eps, 0)
+    fn, dev, desc, _ = plan
     if q_out is None and q is not None:
-        q_out = torch.empty(q.shape, dtype=_BF16, device=dev)
+        q_out = torch.empty_like(q, dtype=_BF16, memory_format=_CONTIGUOUS)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=_BF16, device=dev)
-    _call(dev, "dsk_qk_norm_rope", ctypes.byref(desc), _p(q), k.data_ptr(), positions.data_ptr(), _p(freq), _p(q_gamma),
+        k_out = torch.empty_like(k, dtype=_BF16, memory_format=_CONTIGUOUS)
+    _call("dsk_qk_norm_rope", fn, dev, desc, _p(q), k.data_ptr(), positions.data_ptr(), _p(freq), _p(q_gamma),
           _p(k_gamma), _p(q_out), k_out.data_ptr())
     return q_out, k_out
 
@@ -228,15 +233,17 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, position
     positions[t] - prefix_len of sequence seq[t] (int32), whose pages are table[seq[t]].  Returns q's result; the keys
     are also written to ``k_out`` if given.  Tokens outside the table or with a page outside the cache are not kept; two
     tokens of one call must not share a row."""
-    tensors = (q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache)
-    numbers = (interleaved, rot_first, mscale, norm, eps, prefix_len)
-    key = ("append", *map(_sig, tensors), numbers)
-    dev, desc = _planned(key, _qk_plan, *tensors, *numbers)
+    key = (_sig(q), _sig(k), _sig(v), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out),
+           _sig(seq), _sig(table), _sig(k_cache), _sig(v_cache), interleaved, rot_first, mscale, norm, eps, prefix_len)
+    plan = _plans["append"].get(key)
+    if plan is None:
+        plan = _plan("append", key, _qk_plan, q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache,
+                     interleaved, rot_first, mscale, norm, eps, prefix_len)
+    fn, dev, desc, cache = plan
     if q_out is None and q is not None:
-        q_out = torch.empty(q.shape, dtype=_BF16, device=dev)
-    _call(dev, "dsk_kv_append", ctypes.byref(desc), _p(q), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
-          seq.data_ptr(), _p(freq), _p(q_gamma), _p(k_gamma), ctypes.byref(_cache(k_cache, v_cache, table)), _p(q_out),
-          _p(k_out))
+        q_out = torch.empty_like(q, dtype=_BF16, memory_format=_CONTIGUOUS)
+    _call("dsk_kv_append", fn, dev, desc, cache, _p(q), k.data_ptr(), v.data_ptr(), positions.data_ptr(), seq.data_ptr(),
+          _p(freq), _p(q_gamma), _p(k_gamma), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), _p(q_out), _p(k_out))
     return q_out
 
 
@@ -251,9 +258,10 @@ def _prompt_plan(q, k, v, cu_q, cu_k, out, causal, scale):
     n = cu_q.numel()
     _exact(cu_q, "cu_q", _I32, n, dev)
     _exact(cu_k, "cu_k", _I32, n, dev)
-    return dev, _lib.PromptDesc(tokens, k.shape[0], n - 1, heads, k.shape[1], dim, 1 if causal else 0,
-                                float(scale) if scale is not None else dim ** -0.5,
-                                *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_out_strides(out, q.shape, dev, "out"))
+    desc = _lib.PromptDesc(tokens, k.shape[0], n - 1, heads, k.shape[1], dim, 1 if causal else 0,
+                           float(scale) if scale is not None else dim ** -0.5,
+                           *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_out_strides(out, q.shape, dev, "out"))
+    return _lib.load().dsk_prompt_attention, dev, ctypes.byref(desc)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -264,12 +272,15 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     head_dim ** -0.5.  Rows of ``out`` behind the last sequence are left as they were."""
     if cu_k is None:
         cu_k = cu_q
-    key = ("prompt", _sig(q), _sig(k), _sig(v), _sig(cu_q), _sig(cu_k), _sig(out), causal, scale)
-    dev, desc = _planned(key, _prompt_plan, q, k, v, cu_q, cu_k, out, causal, scale)
+    key = (_sig(q), _sig(k), _sig(v), _sig(cu_q), _sig(cu_k), _sig(out), causal, scale)
+    plan = _plans["prompt"].get(key)
+    if plan is None:
+        plan = _plan("prompt", key, _prompt_plan, q, k, v, cu_q, cu_k, out, causal, scale)
+    fn, dev, desc = plan
     if out is None:
-        out = torch.empty(q.shape, dtype=_BF16, device=dev)
-    _call(dev, "dsk_prompt_attention", ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(),
-          cu_k.data_ptr(), out.data_ptr())
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    _call("dsk_prompt_attention", fn, dev, desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+          out.data_ptr())
     return out
 
 
@@ -283,7 +294,7 @@ def _token_rows(t: torch.Tensor, q_len: int, what: str) -> torch.Tensor:
 
 
 def _paged_plan(q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale):
-    """(device, descriptor, bytes of workspace)."""
+    """(entry point, device, descriptor, cache, bytes of workspace)."""
     dev = _hip(q)
     q_len = q.shape[1] if q.dim() == 4 else 1
     if q_len < 1:
@@ -306,10 +317,10 @@ def _paged_plan(q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale
     desc = _lib.PagedDesc(batch, q_len, heads, kv_heads, dim, int(prefix_len),
                           float(scale) if scale is not None else dim ** -0.5, *rows.stride()[:2],
                           *_out_strides(out, rows.shape, dev, "out"))
+    cache = ctypes.byref(_cache(k_cache, table))
     n = ctypes.c_size_t(0)
-    _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(desc), ctypes.byref(_cache(k_cache, v_cache, table)),
-              ctypes.byref(n))
-    return dev, desc, n.value
+    _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(desc), cache, ctypes.byref(n))
+    return _lib.load().dsk_paged_attention, dev, ctypes.byref(desc), cache, n.value
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
@@ -321,16 +332,19 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``prefix_len`` keys that all sequences see first, read once for the batch.  The result has q's shape.  ``workspace``:
     uint8, 256-byte aligned, as large as ``dsk_paged_attention_workspace_size`` says, for one call at a time; otherwise
     allocated (inside a graph capture, in the graph's pool)."""
-    key = ("paged", _sig(q), _sig(k_cache), _sig(v_cache), _sig(table), _sig(lens), _sig(prefix), _sig(out), prefix_len, scale)
-    dev, desc, nbytes = _planned(key, _paged_plan, q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale)
+    key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(table), _sig(lens), _sig(prefix), _sig(out), prefix_len, scale)
+    plan = _plans["paged"].get(key)
+    if plan is None:
+        plan = _plan("paged", key, _paged_plan, q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale)
+    fn, dev, desc, cache, nbytes = plan
     if out is None:
-        out = torch.empty(q.shape, dtype=_BF16, device=dev)
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     else:
         nbytes = workspace.numel()
         if workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
             raise ValueError(f"workspace must be contiguous uint8 on {dev}")
-    _call(dev, "dsk_paged_attention", ctypes.byref(desc), q.data_ptr(), ctypes.byref(_cache(k_cache, v_cache, table)),
-          lens.data_ptr(), _p(prefix), out.data_ptr(), workspace.data_ptr(), nbytes)
+    _call("dsk_paged_attention", fn, dev, desc, cache, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+          table.data_ptr(), lens.data_ptr(), _p(prefix), out.data_ptr(), workspace.data_ptr(), nbytes)
     return out

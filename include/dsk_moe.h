@@ -324,13 +324,11 @@ int dsk_rmsnorm(const void* x, const void* residual, const float* gamma, int64_t
  * elements; rows are contiguous and 16-byte aligned (strides multiples of 16
  * bytes).  The reference runs this half in MLX (src/deepseeker/mlx_runner.py:1465). */
 
-/* Paged KV cache.  k and v: [n_pages, kv_heads, page_size, head_dim] bf16;
- * position p of sequence s is row p % page_size of page
+/* Geometry of a paged KV cache: k_cache and v_cache [n_pages, kv_heads, page_size,
+ * head_dim] bf16 and a table of page ids, [n_seqs] rows of max_pages; position p
+ * of sequence s is row p % page_size of page
  * table[s * table_stride + p / page_size].  page_size: 16, 32, 64, 128 or 256. */
 typedef struct dsk_kv_cache {
-  void* k;
-  void* v;
-  const int32_t* table;   /* [n_seqs] rows of max_pages page ids */
   int64_t table_stride;
   int32_t n_pages;
   int32_t page_size;
@@ -373,9 +371,10 @@ int dsk_qk_norm_rope(const dsk_qk_desc* d, const void* q, const void* k, const i
  * cache is not kept (its q_out and k_out are written).  q and q_out are NULL
  * where d->heads is 0; k_out is optional (NULL: the keys go to the cache
  * alone).  Two tokens of a call must not share a row. */
-int dsk_kv_append(const dsk_qk_desc* d, const void* q, const void* k, const void* v,
+int dsk_kv_append(const dsk_qk_desc* d, const dsk_kv_cache* cache, const void* q, const void* k, const void* v,
                   const int32_t* positions, const int32_t* seq, const double* freq, const float* q_gamma,
-                  const float* k_gamma, const dsk_kv_cache* cache, void* q_out, void* k_out, void* stream);
+                  const float* k_gamma, void* k_cache, void* v_cache, const int32_t* table, void* q_out,
+                  void* k_out, void* stream);
 
 typedef struct dsk_prompt_desc {
   int32_t tokens;         /* rows of q and out */
@@ -419,9 +418,9 @@ typedef struct dsk_paged_desc {
  * would need them come out as NaN.  workspace: dsk_paged_attention_workspace_size
  * bytes, 256-byte aligned, no initialisation; one call at a time. */
 int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, size_t* bytes);
-int dsk_paged_attention(const dsk_paged_desc* d, const void* q, const dsk_kv_cache* cache,
-                        const int32_t* lens, const int32_t* prefix, void* out, void* workspace,
-                        size_t workspace_bytes, void* stream);
+int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, const void* q, const void* k_cache,
+                        const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix,
+                        void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

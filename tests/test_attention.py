@@ -27,7 +27,7 @@ def qk_desc(**kw):
 
 
 def cache(**kw):
-    base = dict(k=1 << 20, v=1 << 20, table=1 << 20, table_stride=8, n_pages=40, page_size=64, n_seqs=4, max_pages=8)
+    base = dict(table_stride=8, n_pages=40, page_size=64, n_seqs=4, max_pages=8)
     return _lib.KVCache(**{**base, **kw})
 
 
@@ -72,21 +72,22 @@ def test_norm_rope_refuses_pointers():
     assert code("dsk_qk_norm_rope", None, P, P, P, P, P, P, P, P, None) == -1
 
 
-@pytest.mark.parametrize("kw,want", [(dict(k=None), -1), (dict(table=None), -1), (dict(page_size=48), -1),
+@pytest.mark.parametrize("kw,want", [(dict(page_size=48), -1),
                                      (dict(page_size=512), -1), (dict(n_pages=0), -1), (dict(n_seqs=0), -1),
-                                     (dict(max_pages=0), -1), (dict(table_stride=7), -1), (dict(v=(1 << 20) + 8), -2),
+                                     (dict(max_pages=0), -1), (dict(table_stride=7), -1),
                                      (dict(max_pages=1 << 24, table_stride=1 << 24), -3)])
 def test_cache_refuses(kw, want):
     c = cache(**kw)
-    args = [P] * 7
-    assert code("dsk_kv_append", ctypes.byref(qk_desc()), P, P, P, P, P, P, P, P, ctypes.byref(c), P, P, None) == want
+    assert code("dsk_kv_append", ctypes.byref(qk_desc()), ctypes.byref(c), *[P] * 13, None) == want
     size = ctypes.c_size_t()
     assert code("dsk_paged_attention_workspace_size", ctypes.byref(paged_desc()), ctypes.byref(c), ctypes.byref(size)) == want
 
 
 def test_append_refuses():
-    call = lambda d, v=P, seq=P, c=cache(), ko=None: code(  # noqa: E731
-        "dsk_kv_append", ctypes.byref(d), P, P, v, P, seq, P, P, P, ctypes.byref(c) if c else None, P, ko, None)
+    call = lambda d, v=P, seq=P, c=cache(), ko=None, kc=P, vc=P, table=P: code(  # noqa: E731
+        "dsk_kv_append", ctypes.byref(d), ctypes.byref(c) if c else None, P, P, v, P, seq, P, P, P, kc, vc, table, P, ko, None)
+    assert call(qk_desc(), kc=None) == -1 and call(qk_desc(), vc=None) == -1 and call(qk_desc(), table=None) == -1
+    assert call(qk_desc(), kc=ODD) == -2 and call(qk_desc(), vc=ODD) == -2
     assert call(qk_desc(), v=None) == -1 and call(qk_desc(), seq=None) == -1 and call(qk_desc(), c=None) == -1
     assert call(qk_desc(prefix_len=-1)) == -1 and call(qk_desc(v_token=250)) == -2 and call(qk_desc(), v=ODD) == -2
     assert call(qk_desc(ko_token=0), ko=P) == -1
@@ -118,22 +119,22 @@ def test_paged_refuses(kw, want):
     size = ctypes.c_size_t()
     assert code("dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache()),
                 ctypes.byref(size)) == want
-    assert code("dsk_paged_attention", ctypes.byref(paged_desc(**kw)), P, ctypes.byref(cache()), P, P, P, P, 1 << 40,
-                None) == want
+    assert code("dsk_paged_attention", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache()), *[P] * 8, 1 << 40, None) == want
 
 
 def test_paged_refuses_pointers_and_space():
-    call = lambda d, q=P, lens=P, prefix=None, out=P, ws=P, n=1 << 40: code(  # noqa: E731
-        "dsk_paged_attention", ctypes.byref(d), q, ctypes.byref(cache()), lens, prefix, out, ws, n, None)
+    call = lambda d, q=P, lens=P, prefix=None, out=P, ws=P, n=1 << 40, kc=P, table=P: code(  # noqa: E731
+        "dsk_paged_attention", ctypes.byref(d), ctypes.byref(cache()), q, kc, P, table, lens, prefix, out, ws, n, None)
+    assert call(paged_desc(), kc=None) == -1 and call(paged_desc(), table=None) == -1 and call(paged_desc(), kc=ODD) == -2
     assert call(paged_desc(), q=None) == -1 and call(paged_desc(), lens=None) == -1 and call(paged_desc(), ws=None) == -1
     assert call(paged_desc(prefix_len=5)) == -1
     assert call(paged_desc(), out=ODD) == -2 and call(paged_desc(), ws=ctypes.c_void_p((1 << 20) + 128)) == -2
-    assert call(paged_desc(), n=1024) == -5
+    assert call(paged_desc(), n=128) == -5
 
 
 def test_paged_workspace_grows_with_the_batch():
     size = lambda **kw: (lambda n: (_lib.call(  # noqa: E731
-        "dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache(n_seqs=kw.get("batch", 4))),
+        "dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache(n_seqs=kw.get("batch", 4), max_pages=32, table_stride=32)),
         ctypes.byref(n)), n.value)[1])(ctypes.c_size_t())
     assert 0 < size() < size(batch=8) and size() < size(prefix_len=1) and size() % 256 == 0
 
