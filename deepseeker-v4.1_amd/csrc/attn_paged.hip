@@ -141,11 +141,22 @@ struct SegLds {
   float ml[W][16 * RT][2];
 };
 
+// Lane 2 i + kt: the page of the wave's 16-key tile kt in step kk + i (the table row's
+// last one behind its end; the sequence's length need not be known yet).
+template <int W>
+__device__ __forceinline__ int page_ids(const PagedArgs& a, int b, int kk) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t tile = (static_cast<int64_t>(kk) + (lane >> 1)) * (2 * W) + 2 * wave + (lane & 1);
+  const int page = static_cast<int>(min(tile >> (a.c.page_shift - 4), static_cast<int64_t>(a.c.max_pages - 1)));
+  return ldg<int32_t>(a.c.table + b * a.c.table_stride + page);
+}
+
 // Units [k0, k1) of the keys of item (b, h), in units of 32 W keys, for the rows from
 // r0 on: to `out` (slot < 0: they are all of the item's) or to the partial rows of `slot`.
+// first_ids: page_ids of k0.
 template <int D, int RT, int W>
 __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int len, bool bad_len, int r0, int k0, int k1,
-                                        int64_t slot, SegLds<D, RT, W>& lds) {
+                                        int64_t slot, int first_ids, SegLds<D, RT, W>& lds) {
   constexpr int VW = D / 16, KS = D / 32, kUnit = 32 * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
@@ -172,23 +183,28 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     }
 
     const int32_t* trow = a.c.table + b * a.c.table_stride;
-    const int last_tile = (len - 1) >> 4, sub = a.c.page_shift - 4;
-    int ids = 0, ids0 = k0 - 32;    // lane 2 i + kt: the page of tile kt of step ids0 + i
+    const int last_tile = (len - 1) >> 4;
+    int ids = first_ids, ids0 = k0;   // lane 2 i + kt: the page of tile kt of step ids0 + i
     bool bad = false;
-    auto page_ids = [&](int kk) {
-      ids0 = kk;
-      const int tile = min((kk + (lane >> 1)) * (2 * W) + 2 * wave + (lane & 1), last_tile);
-      ids = ldg<int32_t>(trow + (tile >> sub));
+    auto check_ids = [&]() {
+      const int step = ids0 + (lane >> 1);
       const bool out_of = ids < 0 || ids >= a.c.n_pages;
-      bad = bad || (out_of && kk + (lane >> 1) < k1);
+      bad = bad || (out_of && step < k1 && step * (2 * W) + 2 * wave + (lane & 1) <= last_tile);
       if (out_of) ids = 0;
     };
+    check_ids();
     auto load = [&](Step<D>& s, int kk) {
-      if (kk - ids0 >= 32) page_ids(kk);
+      if (kk - ids0 >= 32) {
+        ids0 = kk;
+        ids = page_ids<W>(a, b, kk);
+        check_ids();
+      }
+      const int tile0 = kk * (2 * W) + 2 * wave;
+      if (tile0 > last_tile) return;                  // none of the wave's keys in this step
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const int tile = min(kk * (2 * W) + 2 * wave + kt, last_tile);
-        const int id = __builtin_amdgcn_readlane(ids, 2 * (kk - ids0) + kt);
+        const int tile = min(tile0 + kt, last_tile);
+        const int id = __builtin_amdgcn_readlane(ids, 2 * (kk - ids0) + tile - tile0);
         const int last_row = len - 1 - tile * 16;     // rows past the length: the last one again
         const int row0 = (tile * 16) & ((1 << a.c.page_shift) - 1);
         const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + row0) * D;
@@ -221,6 +237,7 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     };
     auto compute = [&](const Step<D>& s, int kk) {
       const int key0 = kk * kUnit + 32 * wave;
+      if (key0 >= len) return;
       const bool masked = key0 + 31 > len - a.q_len;
       bf16x8 p[RT];
 #pragma unroll
@@ -383,7 +400,7 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
     const bool whole = k0 == 0 && k1 == nb;
     const int64_t slot = whole ? (a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h : -1)
                                : 2 * static_cast<int64_t>(share) + (u == u0 ? 0 : 1);
-    segment<D, RT, 4>(a, b, h, len, bad_len, r0, k0, k1, slot, lds);
+    segment<D, RT, 4>(a, b, h, len, bad_len, r0, k0, k1, slot, page_ids<4>(a, b, k0), lds);
     u = item0 + k1;
   }
 }
@@ -475,10 +492,11 @@ __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const Pag
   __shared__ SegLds<D, 1, kPgShortWaves> lds;
   constexpr int kUnit = 32 * kPgShortWaves;
   const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, M = a.q_len * a.group, r0 = 16 * blockIdx.y;
+  const int ids = page_ids<kPgShortWaves>(a, b, 0);   // on its way beside the length
   bool bad_len;
   const int len = length_of(a, b, bad_len);
   if (len > 0) {
-    segment<D, 1, kPgShortWaves>(a, b, h, len, bad_len, r0, 0, (len + kUnit - 1) / kUnit, -1, lds);
+    segment<D, 1, kPgShortWaves>(a, b, h, len, bad_len, r0, 0, (len + kUnit - 1) / kUnit, -1, ids, lds);
     return;
   }
   for (int i = threadIdx.x; i < (min(M, r0 + 16) - r0) * (D / 8); i += 64 * kPgShortWaves) {
@@ -524,6 +542,11 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   };
   auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };
 
+  // the first row of every group of threads, on its way beside the maxima and sums
+  const int way = threadIdx.x / kLanes, d0 = 4 * (threadIdx.x % kLanes);
+  auto part_of = [&](int i) { return ldg<f32x4>((i < own ? a.po : a.pre_o) + row_of(i) * D + d0); };
+  f32x4 y = way < parts ? part_of(way) : f32x4{0.f, 0.f, 0.f, 0.f};
+
   float top = kNegInf;
   for (int i = threadIdx.x; i < parts; i += kPgThreads) top = fmaxf(top, ml_of(i)[0]);
 #pragma unroll
@@ -550,11 +573,9 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) ll += red[w];
 
-  const int way = threadIdx.x / kLanes, d0 = 4 * (threadIdx.x % kLanes);
-  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  if (way < parts) y *= weight[way];
 #pragma unroll 4
-  for (int i = way; i < parts; i += kWays)
-    y += ldg<f32x4>((i < own ? a.po : a.pre_o) + row_of(i) * D + d0) * weight[i];
+  for (int i = way + kWays; i < parts; i += kWays) y += part_of(i) * weight[i];
   sum[way][threadIdx.x % kLanes] = y;
   __syncthreads();
   if (way) return;
