@@ -11,15 +11,24 @@
 // Angles: position * freq[i] turns by millions of radians at far positions,
 // where float32 has no digit of the fraction left.  The product is formed in
 // float64, its whole turns are taken off there, and the remaining fraction of a
-// turn (error below 2^-50 position) goes to float32.  A block handles one token
-// (or a part of its heads), so each pair's sine and cosine are computed once
-// per token and shared through LDS.
+// turn (error below 2^-50 position) goes to float32.
+//
+// One wave a token, its heads in turn, so that what belongs to the token is made
+// once: each lane computes a pair's sine and cosine (exchanged through LDS) and
+// keeps its 8 elements' factors, gamma cos and +-gamma' sin, in registers.  A
+// head then takes two multiply-adds an element, and the traffic bounds the
+// kernel: 8192 tokens of 32 + 8 + 8 heads of 128 into a cache take 36 us (5.6
+// TB/s), 4095 of 32 + 8 20.5 us (4.1 TB/s); a block for four tokens with the factors
+// from LDS for every head took 53 and 28 us.  Few tokens: a token's heads over
+// several waves, queries apart from keys and values, for the latency.
 #include "attn.h"
 
 namespace dsk {
 namespace {
 
-constexpr int kQkThreads = 256;
+constexpr int kQkWaves = 4;            // of a workgroup, a token each
+constexpr int kQkAhead = 4;            // heads of a group of lanes whose loads are in flight together
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));   // gammas may start anywhere
 
 struct QkArgs {
   const void *q, *k, *v;
@@ -29,6 +38,7 @@ struct QkArgs {
   uint16_t *q_out, *k_out;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head, ko_token, ko_head;
   int32_t tokens, heads, kv_heads, rot_dim, rot_first, prefix_len, norm;
+  int32_t q_parts, kv_parts;         // waves of a token for queries, and for keys and values; 0: one for all
   float eps, mscale;
   CacheView cache;
   bool append;
@@ -53,165 +63,177 @@ struct Raw8 {
   }
 };
 
-__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
-  return u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-}
-
-// TB tokens a block; its rows are each token's query heads, its key heads, and
-// with a cache its value heads.  A group of lanes takes one head of all TB tokens
-// at a time, their loads together.
-template <int D, bool kBF16, bool kInter, int TB>
-__global__ __launch_bounds__(kQkThreads) void k_qk(const QkArgs a) {
-  constexpr int kLanes = D / 8;                       // lanes of one head row
-  constexpr int kRows = kQkThreads / kLanes;          // heads of one pass of the block
-  __shared__ float2 turn[TB][D / 2];
-  __shared__ __align__(16) float gam[2][D];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TB;
-  const int rows = a.heads + (a.append ? 2 : 1) * a.kv_heads;
-  const int lane = threadIdx.x % kLanes, e = 8 * lane;
+// A lane's part of a head row: elements e .. e + 7 of 8 lanes (D 64) or 16 (D 128).
+template <int D, bool kBF16, bool kInter>
+__global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a head row, rows of a wave
+  __shared__ float2 turns[kQkWaves][D / 2];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wl = threadIdx.x & 63;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kQkWaves + wave;
+  if (t >= a.tokens) return;
+  const int lane = wl % kLanes, e = 8 * lane;
   const int half = a.rot_dim / 2, er = e - a.rot_first;       // this lane's first element among the rotated
-  const bool rotated = er >= 0 && er < a.rot_dim;
+  const bool rotated = er >= 0 && er < a.rot_dim, low = er < half;
   // half pairs: the elements that pair with the lane's own
-  const int ep = kInter || !rotated ? e : (er < half ? e + half : e - half);
+  const int ep = kInter || !rotated ? e : (low ? e + half : e - half);
+  // this lane's heads: row0, row0 + step, ..
+  const bool all = a.q_parts == 0, is_q = all || static_cast<int>(blockIdx.y) < a.q_parts;
+  const int part = is_q ? blockIdx.y : blockIdx.y - a.q_parts;
+  const int row0 = part * kRows + wl / kLanes, step = (all ? 1 : is_q ? a.q_parts : a.kv_parts) * kRows;
 
-  int pos[TB];                                        // negative: padding
-  int64_t slot[TB];                                   // the token's page, or -1
+  // heads row, row + step, .. of one tensor: kQkAhead of them
+  struct Heads { Raw8<kBF16> x[kQkAhead], y[kQkAhead]; };
+  auto load = [&](Heads& r, const void* p, int64_t token, int64_t head, int row, int rows, bool pairs) {
 #pragma unroll
-  for (int i = 0; i < TB; ++i) {
-    pos[i] = t0 + i < a.tokens ? a.positions[t0 + i] : -1;
-    slot[i] = -1;
-    if (a.append && pos[i] >= 0) {
-      const int s = a.seq[t0 + i];
-      const int64_t at = static_cast<int64_t>(pos[i]) - a.prefix_len, page = at >> a.cache.page_shift;
-      if (s >= 0 && s < a.cache.n_seqs && at >= 0 && page < a.cache.max_pages) {
-        const int id = a.cache.table[s * a.cache.table_stride + page];
-        if (id >= 0 && id < a.cache.n_pages) slot[i] = id;
-      }
+    for (int i = 0; i < kQkAhead; ++i) {
+      const int64_t at = t * token + min(row + i * step, rows - 1) * head;
+      r.x[i].load(p, at + e);
+      if (!kInter && pairs) r.y[i].load(p, at + ep);
     }
+  };
+  // the first heads, in flight beside the angles
+  Heads r, v;
+  if (is_q && row0 < a.heads) load(r, a.q, a.q_token, a.q_head, row0, a.heads, true);
+  if (!is_q && row0 < a.kv_heads) {
+    load(r, a.k, a.k_token, a.k_head, row0, a.kv_heads, true);
+    if (a.append) load(v, a.v, a.v_token, a.v_head, row0, a.kv_heads, false);
   }
-  auto source = [&](int row, int& kind, int& h, const void*& p, int64_t& token, int64_t& at) {
-    kind = row < a.heads ? 0 : row < a.heads + a.kv_heads ? 1 : 2;
-    h = kind == 0 ? row : kind == 1 ? row - a.heads : row - a.heads - a.kv_heads;
-    p = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    token = kind == 0 ? a.q_token : kind == 1 ? a.k_token : a.v_token;
-    at = t0 * token + h * (kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head);
-  };
-  Raw8<kBF16> x[TB], y[TB];
-  auto load = [&](int row) {
-    int kind, h;
-    const void* p;
-    int64_t token, at;
-    source(row, kind, h, p, token, at);
-#pragma unroll
-    for (int i = 0; i < TB; ++i)
-      if (pos[i] >= 0) {
-        x[i].load(p, at + i * token + e);
-        if (!kInter && kind != 2) y[i].load(p, at + i * token + ep);
-      }
-  };
-  int row = blockIdx.y * kRows + threadIdx.x / kLanes;
-  if (row < rows) load(row);                          // in flight while the angles are computed
-  for (int i = threadIdx.x; i < TB * half; i += kQkThreads) {
-    const int ti = i / half, pair = i - ti * half;
-    const int p = t0 + ti < a.tokens ? a.positions[t0 + ti] : 0;
-    double r = static_cast<double>(p) * (a.freq[pair] * 0.15915494309189533577);   // turns: / (2 pi)
-    r -= rint(r);
+
+  const int pos = a.positions[t];
+  if (pos < 0) return;                                // a token of padding
+  float2* turn = turns[wave];
+  if (wl < half) {
+    double c = static_cast<double>(pos) * (a.freq[wl] * 0.15915494309189533577);   // turns: / (2 pi)
+    c -= rint(c);
     float sn, cs;
-    sincospif(2.0f * static_cast<float>(r), &sn, &cs);
-    turn[ti][pair] = float2{cs * a.mscale, sn * a.mscale};
+    sincospif(2.0f * static_cast<float>(c), &sn, &cs);
+    turn[wl] = float2{cs * a.mscale, sn * a.mscale};
   }
-  for (int i = threadIdx.x; i < D; i += kQkThreads) {
-    gam[0][i] = a.q_gamma ? a.q_gamma[i] : 1.0f;
-    gam[1][i] = a.k_gamma ? a.k_gamma[i] : 1.0f;
-  }
-  __syncthreads();
-  while (row < rows) {
-    int kind, h;
-    const void* p;
-    int64_t token, at;
-    source(row, kind, h, p, token, at);
-    u32x4 out[TB];
-#pragma unroll
-    for (int i = 0; i < TB; ++i) {
-      float z[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] = x[i][j];
-      if (kind != 2) {
-        float rstd = 1.0f;
-        if (a.norm) {
-          float ss = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ss += z[j] * z[j];
-#pragma unroll
-          for (int m = kLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
-          rstd = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-        }
-        const float* g = gam[kind];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = z[j] * rstd * g[e + j];
-        if (rotated) {
-          if constexpr (kInter) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 cs = turn[i][er / 2 + j];
-              const float u = z[2 * j], v = z[2 * j + 1];
-              z[2 * j] = u * cs.x - v * cs.y;
-              z[2 * j + 1] = v * cs.x + u * cs.y;
-            }
-          } else {
-            const float sign = er < half ? -rstd : rstd;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float2 cs = turn[i][(er < half ? er : er - half) + j];
-              z[j] = z[j] * cs.x + (y[i][j] * sign * g[ep + j]) * cs.y;
-            }
-          }
-        }
-      }
-      out[i] = pack8(z);
+  // the token's row of the cache, or none
+  int64_t slot = -1;
+  if (a.append) {
+    const int sq = a.seq[t];
+    const int64_t at = static_cast<int64_t>(pos) - a.prefix_len, page = at >> a.cache.page_shift;
+    if (sq >= 0 && sq < a.cache.n_seqs && at >= 0 && page < a.cache.max_pages) {
+      const int id = a.cache.table[sq * a.cache.table_stride + page];
+      if (id >= 0 && id < a.cache.n_pages)
+        slot = ((static_cast<int64_t>(id) * a.kv_heads) << a.cache.page_shift) + (at & ((1 << a.cache.page_shift) - 1));
     }
-    const int next = row + gridDim.y * kRows;
-    // the next head's loads before this one's stores; results over the inputs stay
-    // possible, since a head is read whole before its own stores
-    if (next < rows) load(next);
+  }
+
+  // own[j] x[j] + pair[j] y[j] is element j, before the norm's factor: gamma alone where
+  // nothing turns, gamma cos and -+gamma' sin (interleaved: of the lane's other element) where it does
+  auto factors = [&](const float* gamma, float (&own)[8], float (&pair)[8]) {
+    float g[8], gp[8];
 #pragma unroll
-    for (int i = 0; i < TB; ++i) {
-      if (pos[i] < 0) continue;
-      const int64_t t = t0 + i;
-      if (kind == 0) {
-        *reinterpret_cast<u32x4*>(a.q_out + t * a.qo_token + h * a.qo_head + e) = out[i];
-      } else {
-        if (kind == 1 && a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + e) = out[i];
-        if (slot[i] >= 0) {
-          const int in_page = static_cast<int>((pos[i] - a.prefix_len) & ((1 << a.cache.page_shift) - 1));
-          const int64_t to = (((slot[i] * a.kv_heads + h) << a.cache.page_shift) + in_page) * D + e;
-          *reinterpret_cast<u32x4*>((kind == 1 ? a.cache.k : a.cache.v) + to) = out[i];
-        }
+    for (int j = 0; j < 8; ++j) g[j] = gp[j] = 1.0f;
+    if (gamma) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const f32x4 u = *reinterpret_cast<const f32x4_a4*>(gamma + e + j), v = *reinterpret_cast<const f32x4_a4*>(gamma + ep + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { g[j + i] = u[i]; gp[j + i] = v[i]; }
       }
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int pr = kInter ? er / 2 + j / 2 : (low ? er : er - half) + j;
+      const float2 cs = rotated ? turn[pr] : float2{1.0f, 0.0f};
+      own[j] = g[j] * cs.x;
+      if constexpr (kInter) pair[j] = j & 1 ? g[j - 1] * cs.y : -(g[j + 1] * cs.y);
+      else pair[j] = (low ? -cs.y : cs.y) * gp[j];
+    }
+  };
+  auto normed = [&](const Raw8<kBF16>& x, const Raw8<kBF16>& y, const float (&own)[8], const float (&pair)[8]) {
+    float rstd = 1.0f, z[8];
+    if (a.norm) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+#pragma unroll
+      for (int m = kLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
+      rstd = rsqrtf(ss * (1.0f / D) + a.eps);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // the other one's product only where something turns: it may be infinite
+      const float other = kInter ? x[j ^ 1] : y[j];
+      z[j] = x[j] * own[j];
+      if (rotated) z[j] += other * pair[j];
+      z[j] *= rstd;
+    }
+    return u32x4{pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]), pack_bf16(z[4], z[5]), pack_bf16(z[6], z[7])};
+  };
+
+  // each wave reads its own angles alone: its LDS writes are done before
+  __builtin_amdgcn_wave_barrier();
+  float own[8], pair[8];
+  if (is_q && a.heads > 0) {
+    factors(a.q_gamma, own, pair);
+    for (int row = row0; row < a.heads;) {
+      u32x4 out[kQkAhead];
+#pragma unroll
+      for (int i = 0; i < kQkAhead; ++i) out[i] = normed(r.x[i], r.y[i], own, pair);
+      const int next = row + kQkAhead * step;
+      // the next heads' loads before these stores; q_out may be q, since a head is read
+      // whole before it is written
+      if (next < a.heads) load(r, a.q, a.q_token, a.q_head, next, a.heads, true);
+#pragma unroll
+      for (int i = 0; i < kQkAhead; ++i)
+        if (row + i * step < a.heads)
+          *reinterpret_cast<u32x4*>(a.q_out + t * a.qo_token + (row + i * step) * a.qo_head + e) = out[i];
+      row = next;
+    }
+  }
+  if (row0 >= a.kv_heads || (is_q && !all)) return;
+  if (all) {
+    load(r, a.k, a.k_token, a.k_head, row0, a.kv_heads, true);
+    if (slot >= 0) load(v, a.v, a.v_token, a.v_head, row0, a.kv_heads, false);
+  }
+  factors(a.k_gamma, own, pair);
+  for (int row = row0; row < a.kv_heads;) {
+    u32x4 out[kQkAhead];
+#pragma unroll
+    for (int i = 0; i < kQkAhead; ++i) out[i] = normed(r.x[i], r.y[i], own, pair);
+    const int next = row + kQkAhead * step;
+    if (next < a.kv_heads) load(r, a.k, a.k_token, a.k_head, next, a.kv_heads, true);
+#pragma unroll
+    for (int i = 0; i < kQkAhead; ++i) {
+      const int h = row + i * step;
+      if (h >= a.kv_heads) break;
+      if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + e) = out[i];
+      if (slot >= 0) {
+        const int64_t to = (slot + (static_cast<int64_t>(h) << a.cache.page_shift)) * D + e;
+        *reinterpret_cast<u32x4*>(a.cache.k + to) = out[i];
+        const Raw8<kBF16>& x = v.x[i];
+        *reinterpret_cast<u32x4*>(a.cache.v + to) =
+            u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+      }
+    }
+    if (next < a.kv_heads && slot >= 0) load(v, a.v, a.v_token, a.v_head, next, a.kv_heads, false);
     row = next;
   }
 }
 
-template <int D, int TB>
-void launch_qk_t(const dsk_qk_desc& d, const QkArgs& a, dim3 grid, hipStream_t s) {
-  if (d.dtype == DSK_DTYPE_BF16) {
-    if (d.interleaved) launch_kernel(k_qk<D, true, true, TB>, grid, kQkThreads, 0, s, a);
-    else launch_kernel(k_qk<D, true, false, TB>, grid, kQkThreads, 0, s, a);
-  } else {
-    if (d.interleaved) launch_kernel(k_qk<D, false, true, TB>, grid, kQkThreads, 0, s, a);
-    else launch_kernel(k_qk<D, false, false, TB>, grid, kQkThreads, 0, s, a);
-  }
-}
-
 template <int D>
-void launch_qk_d(const dsk_qk_desc& d, const QkArgs& a, hipStream_t s) {
-  constexpr int kRows = kQkThreads / (D / 8);
-  const int rows = d.heads + (a.append ? 2 : 1) * d.kv_heads;
-  const int passes = (rows + kRows - 1) / kRows;
-  // few tokens: one a block, its heads over several blocks, so that one pass covers them
-  if (d.tokens < 1024) launch_qk_t<D, 1>(d, a, dim3(d.tokens, passes), s);
-  else launch_qk_t<D, 4>(d, a, dim3((d.tokens + 3) / 4, 1), s);
+void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
+  constexpr int kRows = 64 / (D / 8);
+  // few tokens: a token's heads over several waves, kQkAhead heads to a group of lanes;
+  // from 4096 waves of whole tokens on the chip is full
+  const int per = kRows * kQkAhead;
+  const bool split = d.tokens < 2048 && d.heads > 0;
+  const int q_parts = split ? (d.heads + per - 1) / per : 0, kv_parts = split ? (d.kv_heads + per - 1) / per : 0;
+  QkArgs a = args;
+  a.q_parts = q_parts;
+  a.kv_parts = kv_parts;
+  const dim3 grid((d.tokens + kQkWaves - 1) / kQkWaves, split ? q_parts + kv_parts : 1);
+  if (d.dtype == DSK_DTYPE_BF16) {
+    if (d.interleaved) launch_kernel(k_qk<D, true, true>, grid, 64 * kQkWaves, 0, s, a);
+    else launch_kernel(k_qk<D, true, false>, grid, 64 * kQkWaves, 0, s, a);
+  } else {
+    if (d.interleaved) launch_kernel(k_qk<D, false, true>, grid, 64 * kQkWaves, 0, s, a);
+    else launch_kernel(k_qk<D, false, false>, grid, 64 * kQkWaves, 0, s, a);
+  }
 }
 
 }  // namespace
@@ -222,7 +244,7 @@ hipError_t launch_qk(const dsk_qk_desc& d, const void* q, const void* k, const v
   QkArgs a{q, k, v, positions, seq, freq, q_gamma, k_gamma, static_cast<uint16_t*>(q_out),
            static_cast<uint16_t*>(k_out), d.q_token, d.q_head, d.k_token, d.k_head, d.v_token, d.v_head,
            d.qo_token, d.qo_head, d.ko_token, d.ko_head, d.tokens, d.heads, d.kv_heads, d.rot_dim, d.rot_first,
-           d.prefix_len, d.norm, d.eps, d.mscale, cache ? *cache : CacheView{}, cache != nullptr};
+           d.prefix_len, d.norm, 0, 0, d.eps, d.mscale, cache ? *cache : CacheView{}, cache != nullptr};
   if (d.head_dim == 64) launch_qk_d<64>(d, a, s);
   else launch_qk_d<128>(d, a, s);
   return hipGetLastError();
