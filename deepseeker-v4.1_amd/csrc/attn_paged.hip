@@ -360,10 +360,12 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
         }
         if (slot < 0) {
           const int tok = r / a.group, hd = h * a.group + r % a.group;
-          const float inv = len - a.q_len + tok >= 0 || ll != ll ? 1.0f / ll : 0.0f;   // no key: zeros
+          const bool sees = len - a.q_len + tok >= 0 || ll != ll;   // else no key: zeros
+          const float inv = 1.0f / ll;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = sees ? y[i] * inv : 0.0f;
           *reinterpret_cast<u32x4*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
-              u32x4{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv),
-                    pack_bf16(y[4] * inv, y[5] * inv), pack_bf16(y[6] * inv, y[7] * inv)};
+              u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])};
         } else {
           float* po = a.po + (slot * M + r) * D + d0;
           *reinterpret_cast<f32x4*>(po) = f32x4{y[0], y[1], y[2], y[3]};
@@ -582,10 +584,11 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
 #pragma unroll
   for (int w = 1; w < kWays; ++w) y += sum[w][threadIdx.x];
   const int tok = r / a.group, hd = h * a.group + r % a.group;
-  const bool sees = a.prefix > 0 || len - a.q_len + tok >= 0 || ll != ll;   // else no key: zeros
-  const float inv = sees ? 1.0f / ll : 0.0f;
+  // no key, or an unused slot (its q may hold anything): zeros
+  const bool sees = a.lens[b] >= 0 && (a.prefix > 0 || len - a.q_len + tok >= 0 || ll != ll);
+  y = sees ? y * (1.0f / ll) : f32x4{0.f, 0.f, 0.f, 0.f};
   *reinterpret_cast<u32x2*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
-      u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
+      u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
 }
 
 // Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's.

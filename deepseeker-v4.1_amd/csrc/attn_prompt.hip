@@ -98,7 +98,8 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
   flash<D, kFlWaves, 2>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
 
   const float l = sum_across32(st.l);
-  const float inv = lim >= 0 ? 1.0f / l : 0.0f;     // a row that sees no key: zeros
+  const bool sees = lim >= 0;                       // else no key: zeros
+  const float inv = 1.0f / l;
   uint16_t* op = a.out + (sr.q0 + static_cast<int64_t>(tok)) * a.o_token + hd * a.o_head;
   const bool live = wr0 + n < rows;
 #pragma unroll
@@ -106,11 +107,14 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       // a lane half has elements 8 a + 4 hf .. +4 of a = 2c, 2c + 1: swapped, half hf has all 8 of a = 2c + hf
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = sees ? st.o[dt][8 * c + i] * inv : 0.0f;
       uint32_t lo[2], hi[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        lo[i] = pack_bf16(st.o[dt][8 * c + 2 * i] * inv, st.o[dt][8 * c + 2 * i + 1] * inv);
-        hi[i] = pack_bf16(st.o[dt][8 * c + 4 + 2 * i] * inv, st.o[dt][8 * c + 4 + 2 * i + 1] * inv);
+        lo[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+        hi[i] = pack_bf16(y[4 + 2 * i], y[4 + 2 * i + 1]);
       }
       const auto s0 = __builtin_amdgcn_permlane32_swap(lo[0], hi[0], false, false);
       const auto s1 = __builtin_amdgcn_permlane32_swap(lo[1], hi[1], false, false);

@@ -11,7 +11,8 @@ ctypes on the current HIP stream.
 """
 
 from ._lib import DskError, load as load_library
-from .attention import kv_append, paged_attention, prompt_attention, qk_norm_rope, rope_frequencies
+from .attention import (Attention, DecodeStep, PromptStep, kv_append, paged_attention, prompt_attention, qk_norm_rope,
+                        rope_frequencies)
 from .bank import ResidentBank, SharedExpert
 from .checkpoint import Checkpoint, build_manifest, fp8_block_dequant
 from .layer import MoELayer, moe_layer
@@ -23,4 +24,4 @@ from .ops import (align_block_size, dispatch, fp4_dequant, fp4_quantize, q3_dequ
 
 __all__ = ["Checkpoint", "DskError", "MoELayer", "MoEStack", "ResidentBank", "SharedExpert", "TraceSink", "align_block_size",
            "build_manifest", "dispatch", "expert_rows", "gather_pinned_contributions", "fp4_dequant", "fp8_block_dequant", "fp4_quantize", "load_library", "moe_layer",
-           "q3_dequant", "q3_quantize", "q3_repack", "rmsnorm", "route", "kv_append", "paged_attention", "prompt_attention", "qk_norm_rope", "rope_frequencies", "workspace_size", "Geometry", "Trace"]
+           "q3_dequant", "q3_quantize", "q3_repack", "rmsnorm", "route", "Attention", "DecodeStep", "PromptStep", "kv_append", "paged_attention", "prompt_attention", "qk_norm_rope", "rope_frequencies", "workspace_size", "Geometry", "Trace"]

@@ -12,13 +12,15 @@ contiguous.  Outputs must not overlap inputs, except where said.
     o = paged_attention(q, k_cache, v_cache, table, lens)
 
 ``Attention`` is a whole sublayer (projections, norms, rotation, cache,
-attention, output projection) for ``MoEStack``.
+attention, output projection); ``MoEStack(layers, attention=[...])`` runs one
+before every MoE layer, on a ``PromptStep`` or a ``DecodeStep``.
 """
 
 from __future__ import annotations
 
 import ctypes
 import math
+from dataclasses import dataclass
 
 import torch
 
@@ -328,7 +330,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     scale: float | None = None, out: torch.Tensor | None = None,
                     workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``dsk_paged_attention``: q [batch, heads, head_dim] (one token of each sequence) or [batch, q_len, heads, head_dim]
-    over lens[s] (int32) keys of sequence s in the cache, the new tokens' among them.  ``prefix`` (int32 page ids) with
+    over lens[s] (int32) keys of sequence s in the cache, the new tokens' among them (negative: an unused slot, zeros).  ``prefix`` (int32 page ids) with
     ``prefix_len`` keys that all sequences see first, read once for the batch.  The result has q's shape.  ``workspace``:
     uint8, 256-byte aligned, as large as ``dsk_paged_attention_workspace_size`` says, for one call at a time; otherwise
     allocated (inside a graph capture, in the graph's pool)."""
@@ -348,3 +350,82 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _call("dsk_paged_attention", fn, dev, desc, cache, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
           table.data_ptr(), lens.data_ptr(), _p(prefix), out.data_ptr(), workspace.data_ptr(), nbytes)
     return out
+
+
+# ------------------------------------------------------------------ a sublayer
+@dataclass
+class PromptStep:
+    """Whole prompts, packed: token t is at positions[t] of sequence seq[t], whose pages are table[seq[t]]; sequence s has
+    the rows cu[s] .. cu[s+1] (all int32 on the device).  Rows behind the last sequence have position -1."""
+
+    positions: torch.Tensor
+    seq: torch.Tensor
+    table: torch.Tensor
+    cu: torch.Tensor
+
+
+@dataclass
+class DecodeStep:
+    """``q_len`` new tokens of every sequence, token t of sequence seq[t] = t // q_len at positions[t]; lens[s] keys of its
+    own with them, behind ``prefix_len`` keys of the pages ``prefix`` that all sequences share.  An unused slot: positions
+    and length -1."""
+
+    positions: torch.Tensor
+    seq: torch.Tensor
+    table: torch.Tensor
+    lens: torch.Tensor
+    q_len: int = 1
+    prefix: torch.Tensor | None = None
+    prefix_len: int = 0
+
+
+class Attention:
+    """One attention sublayer over bf16 rows y [T, hidden]: y w_qkv^T, norms and rotation, the cache, attention, and the
+    output projection w_o.
+
+    w_qkv [(heads + 2 kv_heads) head_dim, hidden]: queries, keys, values; w_o [hidden, heads head_dim] (bf16).  The
+    layer owns its cache: ``k_cache`` and ``v_cache`` [pages, kv_heads, page_size, head_dim], which ``new_cache``
+    allocates; the steps' tables hold its page ids."""
+
+    def __init__(self, w_qkv: torch.Tensor, w_o: torch.Tensor, heads: int, kv_heads: int, *,
+                 freq: torch.Tensor | None = None, mscale: float = 1.0, interleaved: bool = False, rot_first: int = 0,
+                 q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, norm: bool = True,
+                 eps: float = 1e-6, scale: float | None = None):
+        if w_qkv.dim() != 2 or w_o.dim() != 2 or w_qkv.dtype != _BF16 or w_o.dtype != _BF16:
+            raise ValueError("w_qkv and w_o must be 2-D bfloat16")
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"heads={heads} must be a multiple of kv_heads={kv_heads}")
+        dim, rest = divmod(w_qkv.shape[0], heads + 2 * kv_heads)
+        if rest or w_o.shape != (w_qkv.shape[1], heads * dim):
+            raise ValueError(f"w_qkv {tuple(w_qkv.shape)} and w_o {tuple(w_o.shape)} do not fit {heads} + 2 x {kv_heads} heads")
+        self.w_qkv, self.w_o, self.heads, self.kv_heads, self.head_dim = w_qkv, w_o, heads, kv_heads, dim
+        self.scale = scale
+        self._rotate = dict(freq=freq, mscale=mscale, interleaved=interleaved, rot_first=rot_first, q_gamma=q_gamma,
+                            k_gamma=k_gamma, norm=norm, eps=eps)
+        self.k_cache = self.v_cache = None
+
+    def new_cache(self, n_pages: int, page_size: int = 64) -> None:
+        """Allocate the layer's pages (zeros)."""
+        shape = (n_pages, self.kv_heads, page_size, self.head_dim)
+        self.k_cache, self.v_cache = (torch.zeros(shape, dtype=_BF16, device=self.w_qkv.device) for _ in range(2))
+
+    def __call__(self, y: torch.Tensor, step: PromptStep | DecodeStep, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The sublayer's output [T, hidden] for y [T, hidden]; its new keys and values are in the cache afterwards.  Rows
+        of a ``PromptStep`` behind the last sequence come out as zeros."""
+        if self.k_cache is None:
+            raise RuntimeError("new_cache() the attention layer first")
+        if y.dim() != 2 or y.dtype != _BF16 or y.shape[1] != self.w_qkv.shape[1]:
+            raise ValueError(f"y must be bfloat16 [tokens, {self.w_qkv.shape[1]}], got {str(y.dtype)[6:]} {tuple(y.shape)}")
+        t, h, kv, d = y.shape[0], self.heads, self.kv_heads, self.head_dim
+        qkv = torch.mm(y, self.w_qkv.t())
+        q, k, v = (p.view(t, -1, d) for p in qkv.split([h * d, kv * d, kv * d], 1))
+        if isinstance(step, PromptStep):
+            kr = torch.empty((t, kv, d), dtype=_BF16, device=y.device)
+            q = kv_append(q, k, v, step.positions, step.seq, step.table, self.k_cache, self.v_cache, k_out=kr, **self._rotate)
+            o = prompt_attention(q, kr, v, step.cu, scale=self.scale, out=torch.zeros_like(q))
+        else:
+            q = kv_append(q, k, v, step.positions, step.seq, step.table, self.k_cache, self.v_cache,
+                          prefix_len=step.prefix_len, **self._rotate)
+            o = paged_attention(q.view(-1, step.q_len, h, d), self.k_cache, self.v_cache, step.table, step.lens,
+                                prefix=step.prefix, prefix_len=step.prefix_len, scale=self.scale)
+        return torch.mm(o.view(t, h * d), self.w_o.t(), out=out) if out is not None else torch.mm(o.view(t, h * d), self.w_o.t())

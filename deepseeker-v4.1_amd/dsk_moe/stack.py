@@ -16,6 +16,13 @@ blocks all read the stream before one of them writes the update) -- and a
 final residual add.  ``capture(tokens)`` records the whole stack as one HIP
 graph (after an eager warm-up, so the workspace and buffers exist outside the
 graph) and ``replay(x)`` runs it.
+
+With ``attention`` sublayers it is a decoder: every layer is
+
+    h = h + attention_l(rmsnorm(h));  h = h + layer_l(rmsnorm(h))
+
+on the tokens of a ``PromptStep`` or ``DecodeStep``.  A captured decode step reads
+its positions, lengths and page table from the step's tensors at every replay.
 """
 
 from __future__ import annotations
@@ -23,6 +30,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .attention import Attention, DecodeStep, PromptStep
 from .layer import MoELayer
 from .ops import new_workspace, ptr, require_device, stream_of
 
@@ -52,11 +60,17 @@ def rmsnorm(x: torch.Tensor, eps: float = 1e-6, gamma: torch.Tensor | None = Non
 
 
 class MoEStack:
-    """``len(layers)`` MoE layers on an RMSNorm residual stream (eps, gamma per layer or none)."""
+    """``len(layers)`` MoE layers on an RMSNorm residual stream (eps, gamma per layer or none), each after an attention
+    sublayer of its own if ``attention`` (one for each layer; ``attention_gammas`` likewise) is given."""
 
-    def __init__(self, layers: list[MoELayer], eps: float = 1e-6, gammas: list[torch.Tensor] | None = None):
+    def __init__(self, layers: list[MoELayer], eps: float = 1e-6, gammas: list[torch.Tensor] | None = None,
+                 attention: list[Attention] | None = None, attention_gammas: list[torch.Tensor] | None = None):
         if not layers:
             raise ValueError("a stack needs at least one layer")
+        if attention is not None and len(attention) != len(layers):
+            raise ValueError(f"{len(attention)} attention sublayers for {len(layers)} layers")
+        self.attention = list(attention) if attention is not None else None
+        self.attention_gammas = attention_gammas if attention_gammas is not None else [None] * len(layers)
         self.layers, self.eps = list(layers), float(eps)
         self.gammas = gammas if gammas is not None else [None] * len(layers)
         self._graph = None
@@ -65,11 +79,15 @@ class MoEStack:
         return tuple(torch.empty_like(x) for _ in range(4))   # h (two, alternating), y, d
 
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, bufs=None,
-                record: list | None = None, trace=None, ws: torch.Tensor | None = None) -> torch.Tensor:
+                record: list | None = None, trace=None, ws: torch.Tensor | None = None,
+                step: PromptStep | DecodeStep | None = None) -> torch.Tensor:
         """h_L for input rows x [T, H].  ``record`` (optional list) receives, per
         layer, copies of (h_l, rmsnorm(h_l), idx_l, layer output); ``trace``
         (optional, e.g. a ``TraceSink``) receives every layer's routing as
-        ``trace(layer, idx, weights)`` on the host."""
+        ``trace(layer, idx, weights)`` on the host.  ``step``: the tokens' places,
+        with attention sublayers."""
+        if (step is not None) != (self.attention is not None):
+            raise ValueError("a step and attention sublayers go together")
         h0, h1, y, d = bufs if bufs is not None else self._buffers(x)
         if out is None:
             out = torch.empty_like(x)
@@ -78,7 +96,13 @@ class MoEStack:
         for l, layer in enumerate(self.layers):
             if record is not None:
                 idx = torch.empty((x.shape[0], layer.top_k), dtype=torch.int32, device=x.device)
-            if l == 0:
+            if self.attention is not None:
+                if l == 0:
+                    rmsnorm(x, self.eps, self.attention_gammas[0], out=y)
+                else:
+                    rmsnorm(prev, self.eps, self.attention_gammas[l], residual=d, h_out=prev, out=y)
+                self.attention[l](y, step, out=d)
+            if l == 0 and self.attention is None:
                 rmsnorm(x, self.eps, self.gammas[0], out=y)
                 layer(y, out=d, idx=idx, trace=trace, layer_id=l, ws=ws)
             else:
@@ -93,10 +117,13 @@ class MoEStack:
 
     __call__ = forward
 
-    def capture(self, tokens: int, dtype: torch.dtype = torch.bfloat16, warmup: int = 2) -> None:
+    def capture(self, tokens: int, dtype: torch.dtype = torch.bfloat16, warmup: int = 2,
+                step: DecodeStep | None = None) -> None:
         """Record the stack for ``tokens`` rows as one HIP graph (static input / output
         buffers).  The graph owns its workspace (sized for the largest layer), so
-        later eager calls of any size, or other captures, cannot move it."""
+        later eager calls of any size, or other captures, cannot move it.  With
+        attention sublayers: on ``step``'s tensors, which must stay where they are
+        (the warm-up writes cache rows at the positions that they hold)."""
         dev = self.layers[0].gate_w.device
         hidden = self.layers[0].gate_w.shape[1]
         self._x = torch.zeros((tokens, hidden), dtype=dtype, device=dev)
@@ -107,12 +134,13 @@ class MoEStack:
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
             for _ in range(warmup):
-                self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws)
+                self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=step)
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
+        self._step = step                # the graph reads its tensors
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph):
-            self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws)
+            self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=step)
         torch.cuda.synchronize(dev)
 
     def replay(self, x: torch.Tensor | None = None) -> torch.Tensor:

@@ -413,7 +413,7 @@ typedef struct dsk_paged_desc {
  * before) after the prefix_len keys of the pages prefix[0 ..], which are read
  * once for the whole batch.  Query i of q_len sees the prefix and its
  * sequence's keys j <= lens[s] - q_len + i; a query that sees no key gives
- * zeros (lens[s] <= 0 without a prefix: an unused slot).  Lengths beyond the
+ * zeros.  lens[s] < 0: an unused slot, zeros whatever its q holds.  Lengths beyond the
  * table row and page ids outside the cache are never followed: the rows that
  * would need them come out as NaN.  workspace: dsk_paged_attention_workspace_size
  * bytes, 256-byte aligned, no initialisation; one call at a time. */

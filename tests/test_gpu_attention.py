@@ -297,8 +297,8 @@ def test_prompt_long_rows():
 def test_paged(heads, kv, dim, page, q_len, prefix, spare):
     print(f"paged {heads},{kv},{dim} page {page} q_len {q_len} prefix {prefix}", flush=True)
     g = gen(heads * dim + page + prefix)
-    lens = [0, 1, 15, 16, 17, 127, 128, 129, 300]
-    used = [-(-n // page) for n in lens]
+    lens = [0, 1, 15, 16, 17, 127, 128, 129, 300, -1]
+    used = [-(-max(n, 0) // page) for n in lens]
     shared = -(-prefix // page)
     # wide tables: the work is shared out; short ones: a workgroup for an item
     table, kc, vc = paged_setup(g, used + [shared], max(max(used) + spare, shared), 2, kv, page, dim)
@@ -313,11 +313,13 @@ def test_paged(heads, kv, dim, page, q_len, prefix, spare):
     for c in (kc, vc):
         c.transpose(1, 2)[~held] = NAN
     q = normal(g, len(lens), q_len, heads, dim)
+    q[-1, :, 1] = NAN                                            # an unused slot's q may hold anything
     got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints(lens),
                                   prefix=pre.to(DEV) if prefix else None, prefix_len=prefix, scale=0.15)
-    want, tol = O.paged(q, kc, vc, table, lens, pre, prefix, scale=0.15)
+    want, tol = O.paged(q[:-1], kc, vc, table, lens[:-1], pre, prefix, scale=0.15)
     assert got.shape == q.shape
-    assert_within(got, want, tol)
+    assert_within(got[:-1], want, tol)
+    assert (got[-1] == 0).all()
     if not prefix:
         assert not got[0].any()
 
@@ -605,3 +607,146 @@ def test_calls_on_two_streams():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+# ------------------------------------------------------------------ the stack
+def make_decoder(seed, n=2, heads=8, kv=2, dim=64, pages=80, page=16):
+    """A small MoE stack with attention sublayers (hidden 1024), and the same sublayers one by one."""
+    from dsk_moe import synth as gsynth
+    g = gen(seed)
+    layers = [gsynth.make_layer(hidden=1024, n_experts=64, top_k=6, inter=512, inter_shared=512, seed=seed + l, device=DEV)
+              for l in range(n)]
+    freq, mscale = dsk_moe.rope_frequencies(dim, scaling="ramp", factor=2.0)
+    att = []
+    for _ in range(n):
+        a = dsk_moe.Attention((normal(g, (heads + 2 * kv) * dim, 1024, dtype=F32) / 32).to(BF16).to(DEV),
+                              (normal(g, 1024, heads * dim, dtype=F32) / 32).to(BF16).to(DEV), heads, kv, freq=freq,
+                              mscale=mscale, q_gamma=(torch.rand(dim, generator=g) + 0.5).to(DEV),
+                              k_gamma=(torch.rand(dim, generator=g) + 0.5).to(DEV))
+        a.new_cache(pages, page)
+        att.append(a)
+    gam = [(torch.rand(1024, generator=g) + 0.5).to(DEV) for _ in range(2 * n)]
+    return g, dsk_moe.MoEStack(layers, gammas=gam[:n], attention=att, attention_gammas=gam[n:])
+
+
+def decoder_by_hand(stack, x, step):
+    """The stack's composition from its public pieces, with the attention sublayer's own pieces apart."""
+    h = x
+    for l, layer in enumerate(stack.layers):
+        a = stack.attention[l]
+        y = dsk_moe.rmsnorm(h, stack.eps, stack.attention_gammas[l])
+        qkv = torch.mm(y, a.w_qkv.t())
+        q, k, v = (p.unflatten(1, (-1, a.head_dim)) for p in qkv.split([a.heads * a.head_dim] + [a.kv_heads * a.head_dim] * 2, 1))
+        if isinstance(step, dsk_moe.PromptStep):
+            kr = torch.empty_like(k, memory_format=torch.contiguous_format)
+            q = dsk_moe.kv_append(q, k, v, step.positions, step.seq, step.table, a.k_cache, a.v_cache, k_out=kr, **a._rotate)
+            o = dsk_moe.prompt_attention(q, kr, v, step.cu, out=torch.zeros_like(q))
+        else:
+            q = dsk_moe.kv_append(q, k, v, step.positions, step.seq, step.table, a.k_cache, a.v_cache,
+                                  prefix_len=step.prefix_len, **a._rotate)
+            o = dsk_moe.paged_attention(q.unflatten(0, (-1, step.q_len)), a.k_cache, a.v_cache, step.table, step.lens,
+                                        prefix=step.prefix, prefix_len=step.prefix_len)
+        d = torch.mm(o.reshape(x.shape[0], -1), a.w_o.t())
+        h2, y = torch.empty_like(h), torch.empty_like(h)
+        d = layer.forward_residual(h, d, h2, y, torch.empty_like(h), gamma=stack.gammas[l], eps=stack.eps)
+        h = torch.empty_like(h)
+        dsk_moe.rmsnorm(h2, stack.eps, residual=d, h_out=h, out=False)
+    return h
+
+
+def test_decoder_stack_prompts_and_steps():
+    """Prompts, then steps of one and two tokens: the stack against its pieces, bit for bit."""
+    g, stack = make_decoder(60)
+    table = torch.randperm(60, generator=g)[:36].view(3, 12).to(I32).to(DEV)
+    lens = [20, 1, 33]
+    pos = ints([i for n in lens for i in range(n)] + [-1, -1])
+    seq = ints([b for b, n in enumerate(lens) for _ in range(n)] + [0, 0])
+    step = dsk_moe.PromptStep(pos, seq, table, ints(cumulative(lens)))
+    x = normal(g, 56, 1024).to(DEV)
+    got = stack(x, step=step).clone()
+    assert torch.equal(got, decoder_by_hand(stack, x, step)) and torch.isfinite(got.float()).all()
+    for q_len in (1, 2, 1):
+        pos = ints([n + i for n in lens for i in range(q_len)])
+        lens = [n + q_len for n in lens]
+        step = dsk_moe.DecodeStep(pos, ints([b for b in range(3) for _ in range(q_len)]), table, ints(lens), q_len)
+        x = normal(g, 3 * q_len, 1024).to(DEV)
+        got = stack(x, step=step).clone()
+        assert torch.equal(got, decoder_by_hand(stack, x, step)) and torch.isfinite(got.float()).all()
+
+
+def test_decoder_steps_agree_with_the_prompt():
+    """A prompt in one piece, and its last tokens in decode steps: the same attention over the same cache rows.  One
+    layer without experts' routing in between: its attention output, within the roundings of both."""
+    g, stack = make_decoder(61, n=1)
+    a = stack.attention[0]
+    table = torch.arange(12, dtype=I32, device=DEV)[None]
+    y = normal(g, 40, 1024).to(DEV)
+    ar = torch.arange(40, dtype=I32, device=DEV)
+    zero = torch.zeros_like(ar)
+    qkv = torch.mm(y, a.w_qkv.t())
+    q, k, v = (p.unflatten(1, (-1, 64)) for p in qkv.split([512, 128, 128], 1))
+    kr = torch.empty((40, 2, 64), dtype=BF16, device=DEV)
+    q = dsk_moe.kv_append(q, k, v, ar, zero, table, a.k_cache, a.v_cache, k_out=kr, **a._rotate)
+    want, tol = O.prompt(q.cpu(), kr.cpu(), v.cpu(), [0, 40], [0, 40])
+    assert_within(dsk_moe.prompt_attention(q, kr, v, ints([0, 40])), want, tol, "prompt")
+    for i in range(30, 40):
+        got = dsk_moe.paged_attention(q[i:i + 1], a.k_cache, a.v_cache, table, ints([i + 1]))
+        assert_within(got, want[i:i + 1], tol[i:i + 1], f"token {i}")
+
+
+@pytest.mark.parametrize("prefix", [0, 25])
+def test_captured_decoder(prefix):
+    """A decode step of the stack as a graph: replays follow the step's positions and lengths, against the eager stack,
+    with eager prompts between them; an unused slot stays out of it."""
+    g, stack = make_decoder(62)
+    for a in stack.attention:
+        for c in (a.k_cache, a.v_cache):
+            c.copy_(normal(g, *c.shape))
+    table = torch.randperm(70, generator=g)[:48].view(4, 12).to(I32).to(DEV)
+    pre = torch.arange(70, 72, dtype=I32, device=DEV)
+    other = torch.randperm(70, generator=g)[:12].view(1, 12).to(I32).to(DEV)
+    pos, lens = ints([3, 100, -1, 17]), ints([4, 101, -1, 18])
+    pos[pos >= 0] += prefix
+    step = dsk_moe.DecodeStep(pos, ints([0, 1, 2, 3]), table, lens, 1, pre if prefix else None, prefix)
+    stack.capture(4, step=step)
+    for rep in range(4):
+        live = lens >= 0
+        pos[live] += 1
+        lens[live] += 1
+        x = normal(g, 4, 1024).to(DEV)
+        x[2] = 0
+        held = [(a.k_cache.clone(), a.v_cache.clone()) for a in stack.attention]
+        got = stack.replay(x).clone()
+        torch.cuda.synchronize()
+        after = [(a.k_cache.clone(), a.v_cache.clone()) for a in stack.attention]
+        for a, (k, v) in zip(stack.attention, held):
+            a.k_cache.copy_(k)
+            a.v_cache.copy_(v)
+        want = stack(x, step=step)
+        assert torch.equal(got, want), rep
+        assert torch.isfinite(got.float()).all()
+        for a, (k, v) in zip(stack.attention, after):
+            assert torch.equal(a.k_cache, k) and torch.equal(a.v_cache, v)
+        # an eager prompt of another size, on pages of its own kind, in between
+        ar = torch.arange(9, dtype=I32, device=DEV)
+        stack(normal(g, 9, 1024).to(DEV), step=dsk_moe.PromptStep(ar, torch.zeros_like(ar), other, ints([0, 9])))
+
+
+def test_decoder_refuses():
+    g, stack = make_decoder(63, n=1)
+    x = normal(g, 1, 1024).to(DEV)
+    with pytest.raises(ValueError, match="go together"):
+        stack(x)
+    with pytest.raises(ValueError, match="go together"):
+        dsk_moe.MoEStack(stack.layers)(x, step=dsk_moe.DecodeStep(None, None, None, None))
+    with pytest.raises(ValueError, match="sublayers for"):
+        dsk_moe.MoEStack(stack.layers, attention=[])
+    a = stack.attention[0]
+    with pytest.raises(ValueError, match="bfloat16"):
+        a(x.float(), None)
+    b = dsk_moe.Attention(a.w_qkv, a.w_o, 8, 2)
+    with pytest.raises(RuntimeError, match="new_cache"):
+        b(x, None)
+    for heads, kv in ((8, 3), (7, 7), (0, 0)):
+        with pytest.raises(ValueError):
+            dsk_moe.Attention(a.w_qkv, a.w_o, heads, kv)
