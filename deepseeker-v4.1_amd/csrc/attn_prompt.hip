@@ -19,39 +19,38 @@ struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
   float c2;
-  int32_t tokens, kv_tokens, n_seqs, kv_heads, group, causal, tiles;
+  int32_t tokens, kv_tokens, n_seqs, kv_heads, group, causal;
 };
 
 // A sequence's rows, cut to the tensors (whatever cu holds, no row outside is
 // touched), and a row tile's place in it.
 struct TilePlace { int q0, q1, k0, k1, at; };
 
-// Row tile `tile` counted over all sequences; false: there are fewer.
+// Row tile `tile` of all (false: there are fewer): sequences with more keys first (64
+// at a time), of each its last tile first, so that the longest rows start first.
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePlace& p) {
   const int lane = threadIdx.x & 63;
-  int base = 0;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    const int b = min(b0 + lane, a.n_seqs - 1);
+    const int b = min(b0 + lane, a.n_seqs - 1), here = min(a.n_seqs - b0, 64);
     const int q0 = min(max(a.cu_q[b], 0), a.tokens), q1 = min(max(a.cu_q[b + 1], q0), a.tokens);
     const int k0 = min(max(a.cu_k[b], 0), a.kv_tokens), k1 = min(max(a.cu_k[b + 1], k0), a.kv_tokens);
-    const int n = b0 + lane < a.n_seqs ? ((q1 - q0) * a.group + kFlRows - 1) / kFlRows : 0;
-    int incl = n;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int o = __shfl_up(incl, s, 64);
-      if (lane >= s) incl += o;
+    const int n = lane < here ? ((q1 - q0) * a.group + kFlRows - 1) / kFlRows : 0, len = k1 - k0;
+    int before = 0, all = 0;                         // tiles of the sequences before this lane's in that order
+    for (int j = 0; j < here; ++j) {
+      const int nj = __builtin_amdgcn_readlane(n, j), lj = __builtin_amdgcn_readlane(len, j);
+      before += lj > len || (lj == len && j < lane) ? nj : 0;
+      all += nj;
     }
-    const uint64_t past = __ballot(base + incl > tile);
-    if (past) {
-      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+    if (tile < all) {
+      const int l = __ffsll(static_cast<unsigned long long>(__ballot(tile >= before && tile < before + n))) - 1;
       p.q0 = __builtin_amdgcn_readlane(q0, l);
       p.q1 = __builtin_amdgcn_readlane(q1, l);
       p.k0 = __builtin_amdgcn_readlane(k0, l);
       p.k1 = __builtin_amdgcn_readlane(k1, l);
-      p.at = tile - base - __builtin_amdgcn_readlane(incl - n, l);
+      p.at = __builtin_amdgcn_readlane(before + n - 1, l) - tile;
       return true;
     }
-    base += __builtin_amdgcn_readlane(incl, 63);
+    tile -= all;
   }
   return false;
 }
@@ -63,9 +62,8 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % a.kv_heads;
   TilePlace sr;
-  if (!find_tile(a, a.tiles - 1 - static_cast<int>(blockIdx.x / a.kv_heads), sr)) return;
+  if (!find_tile(a, static_cast<int>(blockIdx.x / a.kv_heads), sr)) return;
   const int lq = sr.q1 - sr.q0, lk = sr.k1 - sr.k0, rows = lq * a.group;
-  // reversed within the sequence as over all: the tiles with most keys first
   const int row0 = sr.at * kFlRows, wr0 = row0 + 32 * wave;
   const int r = min(wr0 + n, rows - 1), tok = r / a.group, hd = h * a.group + r % a.group;
   const int shift = lk - lq;                        // query i sees the keys up to i + shift
@@ -137,7 +135,7 @@ hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k,
   const PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                      static_cast<uint16_t*>(out), cu_q, cu_k, d.q_token, d.q_head, d.k_token, d.k_head, d.v_token,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
-                     group, d.causal, static_cast<int32_t>(tiles)};
+                     group, d.causal};
   const unsigned blocks = static_cast<unsigned>(tiles * d.kv_heads);
   if (d.head_dim == 64) launch_flash<64>(k_prompt<64>, a, blocks, s);
   else launch_flash<128>(k_prompt<128>, a, blocks, s);
