@@ -2,7 +2,7 @@
 // building block of prompt attention and of a shared prefix.
 //
 // NW waves hold 32 NW query rows, 32 a wave; every 64 keys and values are brought
-// to LDS once for all of them (global_load_lds: no registers in between), NS
+// to LDS once for all of them (global_load_lds: no registers in between), two
 // buffers deep.  As in the paged kernel, S^T = K q^T leaves a
 // query row in every lane (column lane & 31) and its keys 8 a + 4 h + b in the
 // registers 4 a + b of lane half h = lane >> 5, which is the B operand of
@@ -55,25 +55,9 @@ __device__ __forceinline__ const T* uniform_ptr(const T* p) {
   return reinterpret_cast<const T*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// Every load of this wave but the newest N has landed and its LDS reads are
-// complete, then the workgroup barrier.
-template <int N>
-__device__ __forceinline__ void wait_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-// ... but the newest n (0..6, wave-uniform) times NI.
-template <int NI>
-__device__ __forceinline__ void wait_barrier_n(int n) {
-  switch (n) {
-    case 0: wait_barrier<0>(); break;
-    case 1: wait_barrier<NI>(); break;
-    case 2: wait_barrier<2 * NI>(); break;
-    case 3: wait_barrier<3 * NI>(); break;
-    case 4: wait_barrier<4 * NI>(); break;
-    case 5: wait_barrier<5 * NI>(); break;
-    default: wait_barrier<6 * NI>(); break;
-  }
-}
+// Every load of this wave has landed and its LDS reads are complete, then the
+// workgroup barrier.
+__device__ __forceinline__ void wait_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int D>
 __device__ __forceinline__ int swz_k(int r) { return r & (D / 8 - 1); }
@@ -94,8 +78,10 @@ struct FlashRows {
   float m, l;
 };
 
-template <int D, int NS>
-constexpr int flash_lds() { return 2 * NS * kFlKeys * D * 2; }   // NS tiles of K and of V
+constexpr int kFlBuffers = 2;        // tiles of K and of V in LDS
+
+template <int D>
+constexpr int flash_lds() { return 2 * kFlBuffers * kFlKeys * D * 2; }
 
 // Tiles [t0, t1) of 64 keys; q[ks]: the lane's row, elements 16 ks + 8 (lane >> 5) .. +8;
 // lim: the last key that the lane's row sees, w_min / w_max: least and largest lim of
@@ -103,7 +89,7 @@ constexpr int flash_lds() { return 2 * NS * kFlKeys * D * 2; }   // NS tiles of 
 // wave's first row in it, &k, &v, &last): that row of K and V (the last of all where it
 // lies behind) and how many rows after it may be read; kstride, vstride: elements from row to row,
 // below 2^26.
-template <int D, int NW, int NS, class Rows>
+template <int D, int NW, class Rows>
 __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1, int lim, int w_min, int w_max,
                                       int b_min, float c2, char* lds, int64_t kstride,
                                       int64_t vstride, Rows rows, FlashRows<D>& st) {
@@ -114,13 +100,14 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   w_max = __builtin_amdgcn_readfirstlane(w_max);
   b_min = __builtin_amdgcn_readfirstlane(b_min);
   constexpr int CH = D / 8, RPI = 64 / CH, WR = kFlKeys / NW, NI = WR / RPI, KS = D / 16;
-  constexpr int kTile = kFlKeys * D * 2;
+  constexpr int kTile = kFlKeys * D * 2, NS = kFlBuffers;
   static_assert(NI >= 1 && RPI % 4 == 0, "every wave loads whole instructions");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   if (t0 >= t1) return;
 
-  // LDS: K of tiles t, t + 1, .. at t mod NS, then V
+  // LDS: K of tile t0 + j at j mod NS, then V likewise (from the first tile, so that an
+  // unrolled loop knows its addresses)
   const uint32_t ldsw = lds_address(lds) + wave * WR * D * 2;
   // K (V) of tile t; rows past the last one: the last one again
   auto issue_k = [&](int t) {
@@ -133,7 +120,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       const int r = i * RPI + lane / CH;
       const uint32_t rr = min(r, last);
       dma16(kp, 2 * (rr * static_cast<uint32_t>(kstride) + 8 * ((lane % CH) ^ swz_k<D>(wave * WR + r))),
-            ldsw + (t % NS) * kTile + i * RPI * D * 2);
+            ldsw + ((t - t0) % NS) * kTile + i * RPI * D * 2);
     }
   };
   auto issue_v = [&](int t) {
@@ -146,7 +133,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       const int r = i * RPI + lane / CH;
       const uint32_t rr = min(r, last);
       dma16(vp, 2 * (rr * static_cast<uint32_t>(vstride) + 8 * ((lane % CH) ^ swz_v<D>(wave * WR + r))),
-            ldsw + (NS + t % NS) * kTile + i * RPI * D * 2);
+            ldsw + (NS + (t - t0) % NS) * kTile + i * RPI * D * 2);
     }
   };
 
@@ -214,35 +201,16 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
 
   // A tile's scores are made while the weights of the tile before are: the matrix pipe
   // and the vector pipe have work of one wave at the same time.  Between two barriers, tile
-  // t + 1's K and tile t's V are read; tile t + NS's K and tile t + NS - 1's V are asked for,
-  // and what is wanted after the next barrier has been for NS - 1 tiles.
-  static_assert(NS == 2 || NS == 4, "wait_tile counts the loads of later tiles");
-  const int count = t1 - t0;
+  // t + 1's K and tile t's V are read; tile t + 2's K and tile t + 1's V are asked for, to be
+  // there at the next (four buffers and loads two tiles earlier took the same time).
   issue_k(t0);
   issue_v(t0);
-  int ahead = 1;                                     // loads (of NI) after tile t0's K
-#pragma unroll
-  for (int i = 1; i < NS; ++i)
-    if (i < count) {
-      issue_k(t0 + i);
-      if (i < NS - 1) issue_v(t0 + i);
-      ahead += i < NS - 1 ? 2 : 1;
-    }
-  wait_barrier_n<NI>(NS == 2 ? 0 : ahead);
-  // tile t's V and tile t + 1's K have landed: after them come, as far as there are such
-  // tiles, for NS 4 the loads of (V t + 1, K t + 2) and (V t + 2, K t + 3)
-  auto wait_tile = [&](int t) {
-    if (NS == 2) {
-      wait_barrier<0>();
-    } else {
-      const int r = t1 - t;
-      wait_barrier_n<NI>(r > 3 ? 4 : r == 3 ? 3 : r == 2 ? 1 : 0);
-    }
-  };
+  if (t0 + 1 < t1) issue_k(t0 + 1);
+  wait_barrier();
   f32x16 s[2];
-  scores(lds + (t0 % NS) * kTile, s);
+  scores(lds, s);
   float top = top_of(s);
-  int t = t0;
+  int j = 0;                                         // tile t0 + j
   {
     // tiles up to NS before the last that all rows of the workgroup see in full: the
     // lanes' offsets from a tile's first row stay the same.  K's chunks are placed by
@@ -254,18 +222,17 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       koff[i] = 2 * (r * static_cast<uint32_t>(kstride) + 8 * ((lane % CH) ^ swz_k<D>(wave * WR + r)));
     }
     voff = 2 * (lane / CH * static_cast<uint32_t>(vstride) + 8 * ((lane % CH) ^ swz_v<D>(lane / CH)));
-    const int full = min(t1, (b_min + 1) / kFlKeys) - NS;     // tile full + NS - 1 is the last full one
+    const int full = min(t1, (b_min + 1) / kFlKeys) - NS - t0;   // tile t0 + full + NS - 1 is the last full one
     auto step = [&](const f32x16 (&s)[2], f32x16 (&next)[2]) {
-      if constexpr (NS == 2) wait_barrier<0>();
-      else wait_barrier<4 * NI>();
+      wait_barrier();
       const uint16_t *kp, *vp, *unused;
       int last;
-      rows(t + NS, wave * WR, kp, unused, last);
-      rows(t + NS - 1, wave * WR, unused, vp, last);
+      rows(t0 + j + NS, wave * WR, kp, unused, last);
+      rows(t0 + j + NS - 1, wave * WR, unused, vp, last);
       kp = uniform_ptr(kp);
       vp = uniform_ptr(vp);
-      const uint32_t kd = ldsw + (t % NS) * kTile, vd = ldsw + (NS + (t + NS - 1) % NS) * kTile;
-      const char* kl = lds + ((t + 1) % NS) * kTile;
+      const uint32_t kd = ldsw + (j % NS) * kTile, vd = ldsw + (NS + (j + NS - 1) % NS) * kTile;
+      const char* kl = lds + ((j + 1) % NS) * kTile;
 #pragma unroll
       for (int i = 0; i < NI; ++i) dma16(vp + i * RPI * vstride, voff, vd + i * RPI * D * 2);
       follow(top);
@@ -275,7 +242,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
 #pragma unroll
       for (int i = 0; i < NI; ++i) dma16(kp, koff[i], kd + i * RPI * D * 2);
       weights(s, p);
-      values(lds + (NS + t % NS) * kTile, p);
+      values(lds + (NS + j % NS) * kTile, p);
       // The order of issue: four fragments of K ahead, then behind every product the next
       // fragment and the vector work that its time covers (8192 tokens, 32 heads of 128: 492 us as the
       // compiler orders it, 484 with the products' order, 476 with the loads of K
@@ -294,26 +261,27 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
         __builtin_amdgcn_sched_group_barrier(0x402, 384 / D, 0);
       }
       top = top_of(next);
-      ++t;
+      ++j;
     };
     // two at a time: the scores change places without moves
     f32x16 other[2];
-    for (; t + 1 < full;) {
+    for (; j + 1 < full;) {
       step(s, other);
       step(other, s);
     }
-    if (t < full) {
+    if (j < full) {
       step(s, other);
       s[0] = other[0];
       s[1] = other[1];
     }
   }
   // the last of them, and tiles that some rows see a part of, or nothing
-  for (;; ++t) {
-    wait_tile(t);
+  for (;; ++j) {
+    const int t = t0 + j;
+    wait_barrier();
     if (t + NS - 1 < t1) issue_v(t + NS - 1);
     if (t + NS < t1) issue_k(t + NS);
-    const char* vl = lds + (NS + t % NS) * kTile;
+    const char* vl = lds + (NS + j % NS) * kTile;
     bool finite = true;
     if (t * kFlKeys + kFlKeys - 1 > b_min) {
       uint32_t bits = 0;
@@ -349,13 +317,13 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
               st.o[dt][4 * g + i] += seen ? nonfinite_only(static_cast<uint16_t>(x[i >> 1] >> (16 * (i & 1)))) : 0.0f;
           }
       }
-      wait_barrier<0>();
+      wait_barrier();
 #pragma unroll 1
       for (int i = threadIdx.x; i < kTile / 4; i += 64 * NW) {
         uint32_t* x = reinterpret_cast<uint32_t*>(const_cast<char*>(vl) + 4 * i);
         *x = finite_only(*x);
       }
-      wait_barrier<0>();
+      wait_barrier();
     }
     if (sees) {
       bf16x8 p[4];
@@ -363,7 +331,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       values(vl, p);
     }
     if (t + 1 >= t1) break;
-    if ((t + 1) * kFlKeys <= w_max) scores(lds + ((t + 1) % NS) * kTile, s);
+    if ((t + 1) * kFlKeys <= w_max) scores(lds + ((j + 1) % NS) * kTile, s);
   }
 }
 

@@ -115,6 +115,13 @@ __device__ __forceinline__ int find_seq(const PagedArgs& a, int64_t u, int64_t& 
   return a.batch - 1;
 }
 
+// LDS writes of a wave's lanes before the reads of others of its lanes.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int D>
 struct Step {                       // one wave's 32 keys
   u32x4 k[2][D / 32];
@@ -412,41 +419,20 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
 constexpr int kPreWaves = 4;
 constexpr int kPreRows = 32 * kPreWaves;
 constexpr int kPreBlocks = 256;      // workgroups of the prefix, about: one a CU
-constexpr int kPreStages = 2;
+constexpr int kPreChunk = 64;        // tiles whose places in the cache a wave holds at once
 
 template <int D>
 __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   const int h = block % a.kv_heads, rest = block / a.kv_heads, split = rest / a.row_tiles;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.group;
-  const int64_t wr0 = static_cast<int64_t>(rest % a.row_tiles) * kPreRows + 32 * wave;
+  const int rows = a.batch * a.q_len * a.group;      // at most 2^23
+  const int wr0 = rest % a.row_tiles * kPreRows + 32 * wave;
   const int tiles = (a.prefix + kFlKeys - 1) / kFlKeys;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-  const int64_t r = min(wr0 + n, rows - 1), tok = r / a.group;
-  const int hd = h * a.group + static_cast<int>(r % a.group);
-
-  // lane l: the page of the wave's 16 rows of tile ids0 + l
-  int ids = 0, ids0 = t0 - 64;
-  bool bad = false;
-  auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
-    if (t - ids0 >= 64) {              // first asked for K, a tile ahead of V
-      ids0 = max(t - 1, t0);
-      ids = ldg<int32_t>(a.pages + (min((ids0 + lane) * kFlKeys + row, a.prefix - 1) >> a.c.page_shift));
-      const bool out_of = ids < 0 || ids >= a.c.n_pages;
-      bad = bad || (out_of && ids0 + lane < t1);
-      if (out_of) ids = 0;
-    }
-    const int key = min(t * kFlKeys + row, a.prefix - 1);
-    const int id = __builtin_amdgcn_readlane(ids, t - ids0);
-    const int in_page = key & ((1 << a.c.page_shift) - 1);
-    const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
-    kp = a.c.k + base;
-    vp = a.c.v + base;
-    last = a.prefix - 1 - key;
-  };
   bf16x8 q[D / 16];
+  const int rq = min(wr0 + n, rows - 1), tok = rq / a.group, hd = h * a.group + rq % a.group;
   const uint16_t* qp = a.q + tok * a.q_token + hd * a.q_head + 8 * hf;
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) q[ks] = as_bf16x8(ldg16(qp + 16 * ks));
@@ -456,21 +442,53 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
   const int w_max = wr0 < rows ? a.prefix - 1 : -1;   // a wave without rows only loads
-  flash<D, kPreWaves, kPreStages>(q, t0, t1, a.prefix - 1, a.prefix - 1, w_max, a.prefix - 1, a.c2, lds, D, D, src, st);
-  // a page outside the cache: the waves load different rows, so all tell
-  const bool any_bad = __syncthreads_or(bad);
-  const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
-  if (wr0 + n < rows) {
-    const int64_t at = (static_cast<int64_t>(split) * a.kv_heads + h) * rows + r;
-    float* op = a.pre_o + at * D;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<f32x4*>(op + 32 * dt + 8 * c + 4 * hf) =
-            f32x4{st.o[dt][4 * c], st.o[dt][4 * c + 1], st.o[dt][4 * c + 2], st.o[dt][4 * c + 3]};
-    if (hf == 0) *reinterpret_cast<float2*>(a.pre_ml + at * 2) = float2{st.m, l};
+  uint64_t bad = 0;
+  // where the wave's rows of kPreChunk tiles lie in the cache, a tile a lane: flash's loop
+  // has neither a branch nor a multiplication for them
+  for (int c0 = t0; c0 < t1; c0 += kPreChunk) {
+    const int c1 = min(c0 + kPreChunk, t1), row = wave * (kFlKeys / kPreWaves);
+    const int key = min((c0 + lane) * kFlKeys + row, a.prefix - 1);
+    int id = ldg<int32_t>(a.pages + (key >> a.c.page_shift));
+    const bool out_of = id < 0 || id >= a.c.n_pages;
+    bad |= __ballot(out_of && c0 + lane < c1);
+    if (out_of) id = 0;
+    const int64_t at = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))) * D;
+    const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
+    auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
+      const uint32_t lo = __builtin_amdgcn_readlane(at_lo, t - c0), hi = __builtin_amdgcn_readlane(at_hi, t - c0);
+      const int64_t base = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+      kp = a.c.k + base;
+      vp = a.c.v + base;
+      last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
+    };
+    if (c0 > t0) __syncthreads();      // the last chunk's reads of LDS are done
+    flash<D, kPreWaves>(q, c0, c1, a.prefix - 1, a.prefix - 1, w_max, a.prefix - 1, a.c2, lds, D, D, src, st);
   }
+  // a page outside the cache: the waves load different rows, so all tell
+  const bool any_bad = __syncthreads_or(bad != 0);
+  const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
+  // the rows' partial sums by way of LDS (32 rows a wave, 16-byte chunk c of row n at c ^ n), so that a
+  // store writes whole lines (16.8 MB of them: 0.8 us less than from the registers, 32 bytes
+  // of a row at a time)
+  constexpr int kChunks = D / 4;
+  static_assert(kPreWaves * 32 * D * 4 <= flash_lds<D>(), "the rows fit the tiles' LDS");
+  char* wl = lds + wave * 32 * D * 4;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<f32x4*>(wl + n * D * 4 + 16 * ((8 * dt + 2 * c + hf) ^ (n & (kChunks - 1)))) =
+          f32x4{st.o[dt][4 * c], st.o[dt][4 * c + 1], st.o[dt][4 * c + 2], st.o[dt][4 * c + 3]};
+  wave_fence();
+  const int64_t at0 = (static_cast<int64_t>(split) * a.kv_heads + h) * rows + wr0;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    const int row = i * (64 / kChunks) + lane / kChunks, c = lane % kChunks;
+    if (wr0 + row < rows)
+      *reinterpret_cast<f32x4*>(a.pre_o + (at0 + row) * D + 4 * c) =
+          *reinterpret_cast<const f32x4*>(wl + row * D * 4 + 16 * (c ^ (row & (kChunks - 1))));
+  }
+  if (hf == 0 && wr0 + n < rows) *reinterpret_cast<float2*>(a.pre_ml + (at0 + n) * 2) = float2{st.m, l};
 }
 
 template <int D, int RT>
@@ -508,21 +526,23 @@ __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const Pag
   }
 }
 
-// Joins a row's parts (shares of its own keys, splits of the prefix), one block
-// for a row: the parts' weights first, all at once, then 256 / (D / 4) groups of
-// threads add up the parts in a fixed order.  Also writes the rows of sequences
-// without keys.
-constexpr int kPgMostParts = 1024;   // of a row: shares are at most 512, splits at most kPreBlocks
+// Joins a row's parts (shares of its own keys, splits of the prefix), WPR waves a
+// row: their maxima and sums first, a part a lane, then groups of D / 4 lanes add up the
+// parts in a fixed order.  Also writes the rows of sequences without keys.
+// From kPgWaveRows rows on a wave each, since a workgroup then has little to do a row: 2048 rows of
+// 18 and of 2 parts of 128 take 7.7 and 5.7 us so, 10.6 and 8.1 with four waves; below, four
+// waves: 256 rows of 17 parts of 64 take 5.9 us, with one 7.8.
+constexpr int kPgWaveRows = 1024;
 
-template <int D>
+template <int D, int WPR>
 __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
-  constexpr int kLanes = D / 4, kWays = kPgThreads / kLanes, kWaves = kPgThreads / 64;
-  __shared__ float weight[kPgMostParts];
-  __shared__ float red[kWaves];
-  __shared__ f32x4 sum[kWays][kLanes];
-  const int M = a.q_len * a.group;
-  const int r = blockIdx.x % M, item = blockIdx.x / M, h = item % a.kv_heads, b = item / a.kv_heads;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kLanes = D / 4, kThreads = 64 * WPR, kWays = kThreads / kLanes, kRows = kPgThreads / kThreads;
+  __shared__ float red[kRows][WPR];
+  __shared__ f32x4 sums[kRows][kWays][kLanes];
+  const int M = a.q_len * a.group, tid = threadIdx.x % kThreads, lane = threadIdx.x & 63, wave = tid >> 6;
+  const int mine = threadIdx.x / kThreads, row = blockIdx.x * kRows + mine;
+  const bool live = row < a.batch * a.kv_heads * M;
+  const int r = row % M, item = row / M, h = item % a.kv_heads, b = live ? item / a.kv_heads : 0;
   const Totals tt = unit_totals(a, b);
   const int64_t total = tt.all * a.kv_heads;
   const int64_t quota = (total + a.shares - 1) / a.shares;
@@ -531,9 +551,10 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   const int64_t item0 = tt.before * a.kv_heads + static_cast<int64_t>(h) * nb;
   const int64_t s0 = nb ? item0 / quota : 0, s1 = nb ? (item0 + nb - 1) / quota : -1;
   const bool whole = nb > 0 && s0 == s1;
-  if (whole && a.splits == 0) return;                 // finished where it was computed
+  if (WPR > 1 && whole && a.splits == 0) return;      // finished where it was computed
   const bool odd = nb && item0 % quota != 0;          // the first part is not its share's first
-  const int own = static_cast<int>(s1 - s0 + 1), parts = own + a.splits;
+  const int own = static_cast<int>(s1 - s0 + 1);
+  const int parts = !live || (whole && a.splits == 0) ? 0 : own + a.splits;
   // row of part i among the partial rows; parts >= own are the prefix's
   auto row_of = [&](int i) -> int64_t {
     if (i >= own)
@@ -543,46 +564,57 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
     return slot * M + r;
   };
   auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };
-
-  // the first row of every group of threads, on its way beside the maxima and sums
-  const int way = threadIdx.x / kLanes, d0 = 4 * (threadIdx.x % kLanes);
+  // the first parts of every group of lanes, on their way beside the maxima and sums
+  const int way = tid / kLanes, d0 = 4 * (tid % kLanes);
   auto part_of = [&](int i) { return ldg<f32x4>((i < own ? a.po : a.pre_o) + row_of(i) * D + d0); };
-  f32x4 y = way < parts ? part_of(way) : f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kAhead = 8 / WPR;
+  f32x4 first[kAhead];
+  float first_m[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const bool is = way + i * kWays < parts;
+    first[i] = is ? part_of(way + i * kWays) : f32x4{0.f, 0.f, 0.f, 0.f};
+    first_m[i] = is ? ml_of(way + i * kWays)[0] : kNegInf;
+  }
 
-  float top = kNegInf;
-  for (int i = threadIdx.x; i < parts; i += kPgThreads) top = fmaxf(top, ml_of(i)[0]);
+  float top = kNegInf, ll = 0.0f;
+  for (int i = tid; i < parts; i += kThreads) top = fmaxf(top, ml_of(i)[0]);
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-  top = red[0];
+  if constexpr (WPR > 1) {
+    if (lane == 0) red[mine][wave] = top;
+    __syncthreads();
+    top = red[mine][0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red[w]);
+    for (int w = 1; w < WPR; ++w) top = fmaxf(top, red[mine][w]);
+    __syncthreads();                                  // everyone has read the maxima
+  }
   const float mu = top == kNegInf ? 0.0f : top;
-  float ll = 0.0f;
-  for (int i = threadIdx.x; i < parts; i += kPgThreads) {
+  for (int i = tid; i < parts; i += kThreads) {
     const f32x2 ml = ml_of(i);
-    const float f = __builtin_amdgcn_exp2f(ml[0] - mu);
-    weight[i] = f;
-    ll += ml[1] * f;
+    ll += ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
   }
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) ll += __shfl_xor(ll, s, 64);
-  __syncthreads();                                    // everyone has read the maxima
-  if (lane == 0) red[wave] = ll;
-  __syncthreads();
-  ll = red[0];
+  if constexpr (WPR > 1) {
+    if (lane == 0) red[mine][wave] = ll;
+    __syncthreads();
+    ll = red[mine][0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) ll += red[w];
-
-  if (way < parts) y *= weight[way];
+    for (int w = 1; w < WPR; ++w) ll += red[mine][w];
+  }
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (way + i * kWays < parts) y += first[i] * __builtin_amdgcn_exp2f(first_m[i] - mu);
 #pragma unroll 4
-  for (int i = way + kWays; i < parts; i += kWays) y += part_of(i) * weight[i];
-  sum[way][threadIdx.x % kLanes] = y;
-  __syncthreads();
-  if (way) return;
+  for (int i = way + kAhead * kWays; i < parts; i += kWays) y += part_of(i) * __builtin_amdgcn_exp2f(ml_of(i)[0] - mu);
+  sums[mine][way][tid % kLanes] = y;
+  if constexpr (WPR > 1) __syncthreads();
+  else wave_fence();
+  if (way || !live || (whole && a.splits == 0)) return;
 #pragma unroll
-  for (int w = 1; w < kWays; ++w) y += sum[w][threadIdx.x];
+  for (int w = 1; w < kWays; ++w) y += sums[mine][w][tid % kLanes];
   const int tok = r / a.group, hd = h * a.group + r % a.group;
   // no key, or an unused slot (its q may hold anything): zeros
   const bool sees = a.lens[b] >= 0 && (a.prefix > 0 || len - a.q_len + tok >= 0 || ll != ll);
@@ -638,12 +670,14 @@ void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
     return;
   }
   if (p.splits) {
-    constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D, kPreStages>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D, kPreStages>();
+    constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D>();
     launch_kernel(k_paged_prefix<D, RT>, a.prefix_blocks + p.shares * halves, kPgThreads, lds, s, a);
   } else {
     launch_kernel(k_paged<D, RT>, dim3(p.shares, halves), kPgThreads, 0, s, a);
   }
-  launch_kernel(k_paged_join<D>, a.batch * a.kv_heads * M, kPgThreads, 0, s, a);
+  const int rows = a.batch * a.kv_heads * M;
+  if (rows >= kPgWaveRows) launch_kernel(k_paged_join<D, 1>, (rows + 3) / 4, kPgThreads, 0, s, a);
+  else launch_kernel(k_paged_join<D, 4>, rows, kPgThreads, 0, s, a);
 }
 
 }  // namespace

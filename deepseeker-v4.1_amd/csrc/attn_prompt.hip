@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
     vp = vb + key * a.v_token;
     last = lk - 1 - key;
   };
-  flash<D, kFlWaves, 2>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
+  flash<D, kFlWaves>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
 
   const float l = sum_across32(st.l);
   const bool sees = lim >= 0;                       // else no key: zeros
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
 
 template <int D, class Args>
 void launch_flash(void (*kernel)(Args), const Args& a, unsigned blocks, hipStream_t s) {
-  launch_kernel(kernel, blocks, kFlThreads, flash_lds<D, 2>(), s, a);
+  launch_kernel(kernel, blocks, kFlThreads, flash_lds<D>(), s, a);
 }
 
 }  // namespace

@@ -348,6 +348,24 @@ def test_paged_long_prefix():
     assert_within(got, want[:, 0], tol[:, 0])
 
 
+def test_paged_prefix_in_one_piece():
+    """So many rows that a part of the prefix is longer than the 64 tiles whose places a wave holds at once."""
+    heads, kv, dim, page, batch, q_len, prefix = 64, 8, 64, 64, 130, 4, 4230
+    g = gen(23)
+    n_pages = -(-prefix // page) + 3
+    kc, vc = normal(g, n_pages, kv, page, dim), normal(g, n_pages, kv, page, dim)
+    q = normal(g, batch, q_len, heads, dim)
+    ids = torch.randperm(n_pages, generator=g)
+    pre, own = ids[:-2].to(I32), ids[-1:].to(I32)
+    lens = torch.zeros(batch, dtype=I32)
+    lens[7] = 9
+    table = own.repeat(batch, 1)
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), lens.to(DEV), prefix=pre.to(DEV), prefix_len=prefix)
+    rows = [0, 7, 64, 129]
+    want, tol = O.paged(q[rows], kc, vc, table[rows], lens[rows].tolist(), pre, prefix)
+    assert_within(got[rows], want, tol)
+
+
 @pytest.mark.parametrize("prefix", [0, 40])
 def test_paged_bad_pages_and_lengths_show(prefix):
     """A page outside the cache or a length beyond the table: NaN rows of that sequence alone; no read outside."""
