@@ -59,6 +59,8 @@ __device__ __forceinline__ const T* uniform_ptr(const T* p) {
 // workgroup barrier.
 __device__ __forceinline__ void wait_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <int D>
 __device__ __forceinline__ int swz_k(int r) { return r & (D / 8 - 1); }
 template <int D>
@@ -81,23 +83,21 @@ struct FlashRows {
 constexpr int kFlBuffers = 2;        // tiles of K and of V in LDS
 
 template <int D>
-constexpr int flash_lds() { return 2 * kFlBuffers * kFlKeys * D * 2; }
+constexpr int flash_lds() { return 2 * kFlBuffers * kFlKeys * D * 2 + 16; }   // and two flags
 
 // Tiles [t0, t1) of 64 keys; q[ks]: the lane's row, elements 16 ks + 8 (lane >> 5) .. +8;
-// lim: the last key that the lane's row sees, w_min / w_max: least and largest lim of
+// lim: the last key that the lane's row sees, w_min: least lim of
 // the wave's rows (wave-uniform); b_min: least lim of the workgroup's rows.  rows(tile,
 // wave's first row in it, &k, &v, &last): that row of K and V (the last of all where it
 // lies behind) and how many rows after it may be read; kstride, vstride: elements from row to row,
 // below 2^26.
 template <int D, int NW, class Rows>
-__device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1, int lim, int w_min, int w_max,
-                                      int b_min, float c2, char* lds, int64_t kstride,
-                                      int64_t vstride, Rows rows, FlashRows<D>& st) {
+__device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1, int lim, int w_min, int b_min,
+                                      float c2, char* lds, int64_t kstride, int64_t vstride, Rows rows, FlashRows<D>& st) {
   // wave-uniform by their meaning: in scalar registers
   t0 = __builtin_amdgcn_readfirstlane(t0);
   t1 = __builtin_amdgcn_readfirstlane(t1);
   w_min = __builtin_amdgcn_readfirstlane(w_min);
-  w_max = __builtin_amdgcn_readfirstlane(w_max);
   b_min = __builtin_amdgcn_readfirstlane(b_min);
   constexpr int CH = D / 8, RPI = 64 / CH, WR = kFlKeys / NW, NI = WR / RPI, KS = D / 16;
   constexpr int kTile = kFlKeys * D * 2, NS = kFlBuffers;
@@ -203,10 +203,31 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   // and the vector pipe have work of one wave at the same time.  Between two barriers, tile
   // t + 1's K and tile t's V are read; tile t + 2's K and tile t + 1's V are asked for, to be
   // there at the next (four buffers and loads two tiles earlier took the same time).
+  int* flags = reinterpret_cast<int*>(lds + 2 * NS * kTile);   // of tiles j, by j mod 2
+  if (threadIdx.x == 0) flags[0] = flags[1] = 0;
   issue_k(t0);
   issue_v(t0);
   if (t0 + 1 < t1) issue_k(t0 + 1);
   wait_barrier();
+  // The order of issue: four fragments of K ahead, then behind every product the next
+  // fragment and the vector work that its time covers (8192 tokens, 32 heads of 128: 492 us as the
+  // compiler orders it, 484 with the products' order, 476 with the loads of K
+  // behind the first products)
+  auto order = [&]() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * KS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 384 / D, 0);
+    }
+  };
   f32x16 s[2];
   scores(lds, s);
   float top = top_of(s);
@@ -243,23 +264,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       for (int i = 0; i < NI; ++i) dma16(kp, koff[i], kd + i * RPI * D * 2);
       weights(s, p);
       values(lds + (NS + j % NS) * kTile, p);
-      // The order of issue: four fragments of K ahead, then behind every product the next
-      // fragment and the vector work that its time covers (8192 tokens, 32 heads of 128: 492 us as the
-      // compiler orders it, 484 with the products' order, 476 with the loads of K
-      // behind the first products)
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-      for (int i = 0; i < 2 * KS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, 384 / D, 0);
-      }
+      order();
       top = top_of(next);
       ++j;
     };
@@ -275,33 +280,41 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       s[1] = other[1];
     }
   }
-  // the last of them, and tiles that some rows see a part of, or nothing
-  for (;; ++j) {
-    const int t = t0 + j;
+  // The last of them, and tiles that some rows see a part of, or nothing: there an
+  // infinite or NaN value must not reach the rows that do not see it.
+  auto ready = [&](int t) {                          // all of tile t's values are finite
+    const bool edge = t * kFlKeys + kFlKeys - 1 > b_min;
+    if (edge) {
+      // what the wave itself has loaded, before the barrier that tells the others; the
+      // flag of the tile after next is set behind the next barrier, when this one has been read
+      wait_loads();
+      uint32_t bits = 0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(lds + (NS + j % NS) * kTile + wave * WR * D * 2 + i * 1024 + 16 * lane);
+        bits |= nonfinite_bits(x[0]) | nonfinite_bits(x[1]) | nonfinite_bits(x[2]) | nonfinite_bits(x[3]);
+      }
+      if (bits) flags[j & 1] = 1;
+    }
     wait_barrier();
     if (t + NS - 1 < t1) issue_v(t + NS - 1);
     if (t + NS < t1) issue_k(t + NS);
-    const char* vl = lds + (NS + j % NS) * kTile;
-    bool finite = true;
-    if (t * kFlKeys + kFlKeys - 1 > b_min) {
-      uint32_t bits = 0;
-      for (int i = threadIdx.x; i < kTile / 16; i += 64 * NW) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(vl + 16 * i);
-        bits |= nonfinite_bits(x[0]) | nonfinite_bits(x[1]) | nonfinite_bits(x[2]) | nonfinite_bits(x[3]);
-      }
-      finite = !__syncthreads_or(bits);
-    }
+    return !edge || __builtin_amdgcn_readfirstlane(flags[j & 1]) == 0;
+  };
+  auto prepare = [&](int t, f32x16 (&s)[2]) {
+    const bool finite = ready(t);
     if (t * kFlKeys + kFlKeys - 1 > w_min) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (t * kFlKeys + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[kt][i] = kNegInf;
+      top = top_of(s);
     }
-    const bool sees = t * kFlKeys <= w_max;   // else: keys that none of the wave's rows sees
-    if (sees) follow(top_of(s));
+    follow(top);
     if (!finite) {
       // rarely: infinite and NaN values to the rows that see them, then out of the tile
+      char* vl = lds + (NS + j % NS) * kTile;
 #pragma unroll 1
       for (int key = 0; key < kFlKeys; ++key) {
         int row = key;
@@ -320,19 +333,28 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       wait_barrier();
 #pragma unroll 1
       for (int i = threadIdx.x; i < kTile / 4; i += 64 * NW) {
-        uint32_t* x = reinterpret_cast<uint32_t*>(const_cast<char*>(vl) + 4 * i);
+        uint32_t* x = reinterpret_cast<uint32_t*>(vl + 4 * i);
         *x = finite_only(*x);
       }
       wait_barrier();
     }
-    if (sees) {
-      bf16x8 p[4];
-      weights(s, p);
-      values(vl, p);
-    }
-    if (t + 1 >= t1) break;
-    if ((t + 1) * kFlKeys <= w_max) scores(lds + ((j + 1) % NS) * kTile, s);
+  };
+  for (; t0 + j + 1 < t1; ++j) {
+    prepare(t0 + j, s);
+    f32x16 next[2];
+    bf16x8 p[4];
+    scores(lds + ((j + 1) % NS) * kTile, next);
+    weights(s, p);
+    values(lds + (NS + j % NS) * kTile, p);
+    order();
+    top = top_of(next);
+    s[0] = next[0];
+    s[1] = next[1];
   }
+  prepare(t0 + j, s);
+  bf16x8 p[4];
+  weights(s, p);
+  values(lds + (NS + j % NS) * kTile, p);
 }
 
 }  // namespace dsk

@@ -441,7 +441,6 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
   st.l = 0.0f;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
-  const int w_max = wr0 < rows ? a.prefix - 1 : -1;   // a wave without rows only loads
   uint64_t bad = 0;
   // where the wave's rows of kPreChunk tiles lie in the cache, a tile a lane: flash's loop
   // has neither a branch nor a multiplication for them
@@ -462,7 +461,7 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
       last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
     };
     if (c0 > t0) __syncthreads();      // the last chunk's reads of LDS are done
-    flash<D, kPreWaves>(q, c0, c1, a.prefix - 1, a.prefix - 1, w_max, a.prefix - 1, a.c2, lds, D, D, src, st);
+    flash<D, kPreWaves>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
   }
   // a page outside the cache: the waves load different rows, so all tell
   const bool any_bad = __syncthreads_or(bad != 0);

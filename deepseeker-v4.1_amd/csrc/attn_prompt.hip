@@ -12,6 +12,8 @@ namespace {
 constexpr int kFlWaves = 4;
 constexpr int kFlThreads = 64 * kFlWaves;
 constexpr int kFlRows = 32 * kFlWaves;
+constexpr int kCus = 256;
+constexpr int kMostRank = 1 << 23;   // of a sequence's first tile; tiles are at most 2^23
 
 struct PromptArgs {
   const uint16_t *q, *k, *v;
@@ -20,37 +22,59 @@ struct PromptArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
   float c2;
   int32_t tokens, kv_tokens, n_seqs, kv_heads, group, causal;
+  int32_t first;                    // tiles whose workgroups (one a key head) come to a CU each
 };
 
 // A sequence's rows, cut to the tensors (whatever cu holds, no row outside is
 // touched), and a row tile's place in it.
 struct TilePlace { int q0, q1, k0, k1, at; };
 
-// Row tile `tile` of all (false: there are fewer): sequences with more keys first (64
-// at a time), of each its last tile first, so that the longest rows start first.
+// Row tile `tile` of all (false: there are fewer), the most keys first, 64 sequences at a
+// time: tile i of a sequence has rank lo + i, lo for the keys before its first query, and
+// those of a high rank come first.  The rank is searched for by 64 lanes at once.
+// Workgroups are dealt out to the CUs in turn, two to each; where all of them
+// are there at once, the second of a CU is taken from the other end.
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePlace& p) {
   const int lane = threadIdx.x & 63;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
     const int b = min(b0 + lane, a.n_seqs - 1), here = min(a.n_seqs - b0, 64);
     const int q0 = min(max(a.cu_q[b], 0), a.tokens), q1 = min(max(a.cu_q[b + 1], q0), a.tokens);
     const int k0 = min(max(a.cu_k[b], 0), a.kv_tokens), k1 = min(max(a.cu_k[b + 1], k0), a.kv_tokens);
-    const int n = lane < here ? ((q1 - q0) * a.group + kFlRows - 1) / kFlRows : 0, len = k1 - k0;
-    int before = 0, all = 0;                         // tiles of the sequences before this lane's in that order
-    for (int j = 0; j < here; ++j) {
-      const int nj = __builtin_amdgcn_readlane(n, j), lj = __builtin_amdgcn_readlane(len, j);
-      before += lj > len || (lj == len && j < lane) ? nj : 0;
-      all += nj;
+    const int n = lane < here ? ((q1 - q0) * a.group + kFlRows - 1) / kFlRows : 0;
+    const int before = a.causal ? max(k1 - k0 - (q1 - q0), 0) : k1 - k0;
+    const int lo = min(before / kFlRows, kMostRank / a.group) * a.group, hi = lo + n;
+    auto from = [&](int rank) {                      // tiles of at least that rank
+      int c = 0;
+      for (int j = 0; j < here; ++j)
+        c += min(max(__builtin_amdgcn_readlane(hi, j) - rank, 0), __builtin_amdgcn_readlane(n, j));
+      return c;
+    };
+    int step = !__any(hi > 64) ? 1 : !__any(hi > 4096) ? 64 : !__any(hi > 262144) ? 4096 : 262144;
+    int count = from(lane * step), rank = 0, above = 0;   // above: tiles of a higher rank
+    const int all = __builtin_amdgcn_readfirstlane(count);
+    if (tile >= all) {
+      tile -= all;
+      continue;
     }
-    if (tile < all) {
-      const int l = __ffsll(static_cast<unsigned long long>(__ballot(tile >= before && tile < before + n))) - 1;
-      p.q0 = __builtin_amdgcn_readlane(q0, l);
-      p.q1 = __builtin_amdgcn_readlane(q1, l);
-      p.k0 = __builtin_amdgcn_readlane(k0, l);
-      p.k1 = __builtin_amdgcn_readlane(k1, l);
-      p.at = __builtin_amdgcn_readlane(before + n - 1, l) - tile;
-      return true;
+    if (a.n_seqs <= 64 && all <= 2 * a.first && tile >= a.first) tile = all - 1 - (tile - a.first);
+    for (;;) {
+      const int l = 63 - __clzll(__ballot(count > tile));  // lane 0 always
+      rank += l * step;
+      if (l < 63) above = __builtin_amdgcn_readlane(count, l + 1);
+      if (step == 1) break;
+      step /= 64;
+      count = from(rank + lane * step);
     }
-    tile -= all;
+    // the sequences that have such a tile, in their order
+    uint64_t have = __ballot(rank >= lo && rank < hi);
+    for (int i = tile - above; i > 0; --i) have &= have - 1;
+    const int l = __ffsll(static_cast<unsigned long long>(have)) - 1;
+    p.q0 = __builtin_amdgcn_readlane(q0, l);
+    p.q1 = __builtin_amdgcn_readlane(q1, l);
+    p.k0 = __builtin_amdgcn_readlane(k0, l);
+    p.k1 = __builtin_amdgcn_readlane(k1, l);
+    p.at = rank - __builtin_amdgcn_readlane(lo, l);
+    return true;
   }
   return false;
 }
@@ -68,8 +92,7 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
   const int r = min(wr0 + n, rows - 1), tok = r / a.group, hd = h * a.group + r % a.group;
   const int shift = lk - lq;                        // query i sees the keys up to i + shift
   const int lim = a.causal ? tok + shift : lk - 1;
-  const int w_first = min(wr0, rows - 1) / a.group, w_last = min(wr0 + 31, rows - 1) / a.group;
-  const int w_min = a.causal ? w_first + shift : lk - 1, w_max = a.causal ? w_last + shift : lk - 1;
+  const int w_min = a.causal ? min(wr0, rows - 1) / a.group + shift : lk - 1;
   const int b_min = a.causal ? row0 / a.group + shift : lk - 1;
   const int b_last = min(row0 + kFlRows - 1, rows - 1) / a.group;
   const int t1 = ((a.causal ? b_last + shift : lk - 1) + kFlKeys) / kFlKeys;   // <= 0 where no key is seen
@@ -93,7 +116,7 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
     vp = vb + key * a.v_token;
     last = lk - 1 - key;
   };
-  flash<D, kFlWaves>(q, 0, t1, lim, w_min, w_max, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
+  flash<D, kFlWaves>(q, 0, t1, lim, w_min, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
 
   const float l = sum_across32(st.l);
   const bool sees = lim >= 0;                       // else no key: zeros
@@ -135,7 +158,7 @@ hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k,
   const PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                      static_cast<uint16_t*>(out), cu_q, cu_k, d.q_token, d.q_head, d.k_token, d.k_head, d.v_token,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
-                     group, d.causal};
+                     group, d.causal, kCus / d.kv_heads};
   const unsigned blocks = static_cast<unsigned>(tiles * d.kv_heads);
   if (d.head_dim == 64) launch_flash<64>(k_prompt<64>, a, blocks, s);
   else launch_flash<128>(k_prompt<128>, a, blocks, s);
