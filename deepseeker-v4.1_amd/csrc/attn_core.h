@@ -91,7 +91,10 @@ constexpr int flash_lds() { return 2 * kFlBuffers * kFlKeys * D * 2 + 16; }   //
 // wave's first row in it, &k, &v, &last): that row of K and V (the last of all where it
 // lies behind) and how many rows after it may be read; kstride, vstride: elements from row to row,
 // below 2^26.
-template <int D, int NW, class Rows>
+//
+// KH 2: two waves for 32 rows, with the lower and the upper 32 keys of every tile
+// (half = wave / (NW / 2); add_halves joins them).
+template <int D, int NW, int KH, class Rows>
 __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1, int lim, int w_min, int b_min,
                                       float c2, char* lds, int64_t kstride, int64_t vstride, Rows rows, FlashRows<D>& st) {
   // wave-uniform by their meaning: in scalar registers
@@ -100,10 +103,11 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   w_min = __builtin_amdgcn_readfirstlane(w_min);
   b_min = __builtin_amdgcn_readfirstlane(b_min);
   constexpr int CH = D / 8, RPI = 64 / CH, WR = kFlKeys / NW, NI = WR / RPI, KS = D / 16;
-  constexpr int kTile = kFlKeys * D * 2, NS = kFlBuffers;
+  constexpr int kTile = kFlKeys * D * 2, NS = kFlBuffers, KT = 2 / KH;   // KT: a wave's 32-key parts of a tile
   static_assert(NI >= 1 && RPI % 4 == 0, "every wave loads whole instructions");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
+  const int key0 = KH == 2 ? 32 * (wave / (NW / 2)) : 0;   // the wave's first key in a tile
   if (t0 >= t1) return;
 
   // LDS: K of tile t0 + j at j mod NS, then V likewise (from the first tile, so that an
@@ -138,9 +142,9 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   };
 
   const int l16 = lane & 15;
-  // A operand of the second product: keys 16 s4 .. +16, elements 32 dt .. +32
+  // A operand of the second product: the wave's keys 16 s4 .. +16, elements 32 dt .. +32
   auto value_frag = [&](const char* vl, int s4, int dt) {
-    const int r0 = 16 * s4 + 4 * hf + (l16 >> 2);
+    const int r0 = key0 + 16 * s4 + 4 * hf + (l16 >> 2);
     const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
     const u32x2 lo = read_tr(vl + r0 * D * 2 + 16 * (c ^ swz_v<D>(r0)) + 8 * (l16 & 1));
     const u32x2 hi = read_tr(vl + (r0 + 8) * D * 2 + 16 * (c ^ swz_v<D>(r0 + 8)) + 8 * (l16 & 1));
@@ -148,21 +152,21 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   };
   auto scores32 = [&](const char* kl, int kt, f32x16& s) {
     s = f32x16{};
-    const int row = 32 * kt + n;
+    const int row = key0 + 32 * kt + n;
     const char* kr = kl + row * D * 2;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       s = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(kr + 16 * ((2 * ks + hf) ^ swz_k<D>(row)))), q[ks], s);
   };
-  auto scores = [&](const char* kl, f32x16 (&s)[2]) {
-    scores32(kl, 0, s[0]);
-    scores32(kl, 1, s[1]);
+  auto scores = [&](const char* kl, f32x16 (&s)[KT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) scores32(kl, kt, s[kt]);
   };
   // the largest score of the lane's row, times c2
-  auto top_of = [&](const f32x16 (&s)[2]) {
-    float top = fmaxf(s[0][0], s[1][0]);
+  auto top_of = [&](const f32x16 (&s)[KT]) {
+    float top = fmaxf(s[0][0], s[KT - 1][0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+    for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[KT - 1][i]);
     return max_across32(top) * c2;
   };
   // the reference point follows the maximum once it lags by more than 2^8: p stays
@@ -177,10 +181,10 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= f;
     }
   };
-  auto weights = [&](const f32x16 (&s)[2], bf16x8 (&p)[4]) {
+  auto weights = [&](const f32x16 (&s)[KT], bf16x8 (&p)[2 * KT]) {
     const float mu = st.m == kNegInf ? 0.0f : st.m;
 #pragma unroll
-    for (int s4 = 0; s4 < 4; ++s4) {
+    for (int s4 = 0; s4 < 2 * KT; ++s4) {
       float e[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -192,9 +196,9 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       p[s4] = as_bf16x8(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
     }
   };
-  auto values = [&](const char* vl, const bf16x8 (&p)[4]) {
+  auto values = [&](const char* vl, const bf16x8 (&p)[2 * KT]) {
 #pragma unroll
-    for (int s4 = 0; s4 < 4; ++s4)
+    for (int s4 = 0; s4 < 2 * KT; ++s4)
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = mfma32(as_bf16x8(value_frag(vl, s4, dt)), p[s4], st.o[dt]);
   };
@@ -216,19 +220,19 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   auto order = [&]() {
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int i = 0; i < 2 * KS; ++i) {
+    for (int i = 0; i < KT * KS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
     }
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
+    for (int i = 0; i < KT * D / 16; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       __builtin_amdgcn_sched_group_barrier(0x402, 384 / D, 0);
     }
   };
-  f32x16 s[2];
+  f32x16 s[KT];
   scores(lds, s);
   float top = top_of(s);
   int j = 0;                                         // tile t0 + j
@@ -244,7 +248,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
     }
     voff = 2 * (lane / CH * static_cast<uint32_t>(vstride) + 8 * ((lane % CH) ^ swz_v<D>(lane / CH)));
     const int full = min(t1, (b_min + 1) / kFlKeys) - NS - t0;   // tile t0 + full + NS - 1 is the last full one
-    auto step = [&](const f32x16 (&s)[2], f32x16 (&next)[2]) {
+    auto step = [&](const f32x16 (&s)[KT], f32x16 (&next)[KT]) {
       wait_barrier();
       const uint16_t *kp, *vp, *unused;
       int last;
@@ -257,9 +261,8 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
 #pragma unroll
       for (int i = 0; i < NI; ++i) dma16(vp + i * RPI * vstride, voff, vd + i * RPI * D * 2);
       follow(top);
-      bf16x8 p[4];
-      scores32(kl, 0, next[0]);
-      scores32(kl, 1, next[1]);
+      bf16x8 p[2 * KT];
+      scores(kl, next);
 #pragma unroll
       for (int i = 0; i < NI; ++i) dma16(kp, koff[i], kd + i * RPI * D * 2);
       weights(s, p);
@@ -269,15 +272,15 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       ++j;
     };
     // two at a time: the scores change places without moves
-    f32x16 other[2];
+    f32x16 other[KT];
     for (; j + 1 < full;) {
       step(s, other);
       step(other, s);
     }
     if (j < full) {
       step(s, other);
-      s[0] = other[0];
-      s[1] = other[1];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) s[kt] = other[kt];
     }
   }
   // The last of them, and tiles that some rows see a part of, or nothing: there an
@@ -301,14 +304,14 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
     if (t + NS < t1) issue_k(t + NS);
     return !edge || __builtin_amdgcn_readfirstlane(flags[j & 1]) == 0;
   };
-  auto prepare = [&](int t, f32x16 (&s)[2]) {
+  auto prepare = [&](int t, f32x16 (&s)[KT]) {
     const bool finite = ready(t);
     if (t * kFlKeys + kFlKeys - 1 > w_min) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (t * kFlKeys + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[kt][i] = kNegInf;
+          if (t * kFlKeys + key0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[kt][i] = kNegInf;
       top = top_of(s);
     }
     follow(top);
@@ -316,7 +319,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       // rarely: infinite and NaN values to the rows that see them, then out of the tile
       char* vl = lds + (NS + j % NS) * kTile;
 #pragma unroll 1
-      for (int key = 0; key < kFlKeys; ++key) {
+      for (int key = key0; key < key0 + 32 * KT; ++key) {
         int row = key;
         asm volatile("" : "+v"(row));                // keeps the addresses out of registers
         const bool seen = t * kFlKeys + row <= lim;
@@ -341,20 +344,56 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   };
   for (; t0 + j + 1 < t1; ++j) {
     prepare(t0 + j, s);
-    f32x16 next[2];
-    bf16x8 p[4];
+    f32x16 next[KT];
+    bf16x8 p[2 * KT];
     scores(lds + ((j + 1) % NS) * kTile, next);
     weights(s, p);
     values(lds + (NS + j % NS) * kTile, p);
     order();
     top = top_of(next);
-    s[0] = next[0];
-    s[1] = next[1];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) s[kt] = next[kt];
   }
   prepare(t0 + j, s);
-  bf16x8 p[4];
+  bf16x8 p[2 * KT];
   weights(s, p);
   values(lds + (NS + j % NS) * kTile, p);
+}
+
+// The two waves of 32 rows (KH 2) put their keys together: afterwards both have the
+// rows' maximum and their parts of the sums; of o, in registers o[0 .. D / 64), the wave of half 0 has
+// elements 0 .. D / 2 and that of half 1 the others.  For all NW waves.
+template <int D, int NW>
+__device__ __forceinline__ void add_halves(FlashRows<D>& st, char* lds) {
+  constexpr int DT = D / 64, kWave = 64 * (16 * DT + 2) * 4;
+  static_assert(NW * kWave <= flash_lds<D>(), "in the tiles' LDS");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool up = wave >= NW / 2;
+  char *mine = lds + wave * kWave + 16 * lane, *other = lds + (wave ^ (NW / 2)) * kWave + 16 * lane;
+  __syncthreads();                                   // the last tile's reads are done
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const f32x16 give = up ? st.o[dt] : st.o[DT + dt];
+    if (up) st.o[dt] = st.o[DT + dt];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<f32x4*>(mine + (4 * dt + c) * 1024) = f32x4{give[4 * c], give[4 * c + 1], give[4 * c + 2], give[4 * c + 3]};
+  }
+  *reinterpret_cast<float2*>(mine + DT * 4096 - 8 * lane) = float2{st.m, st.l};
+  __syncthreads();
+  const float2 ml = *reinterpret_cast<const float2*>(other + DT * 4096 - 8 * lane);
+  const float top = fmaxf(st.m, ml.x), mu = top == kNegInf ? 0.0f : top;
+  const float f = __builtin_amdgcn_exp2f(st.m - mu), fo = __builtin_amdgcn_exp2f(ml.x - mu);
+  st.m = top;
+  st.l = st.l * f + ml.y * fo;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(other + (4 * dt + c) * 1024);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st.o[dt][4 * c + i] = st.o[dt][4 * c + i] * f + x[i] * fo;
+    }
 }
 
 }  // namespace dsk

@@ -461,7 +461,7 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
       last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
     };
     if (c0 > t0) __syncthreads();      // the last chunk's reads of LDS are done
-    flash<D, kPreWaves>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
+    flash<D, kPreWaves, 1>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
   }
   // a page outside the cache: the waves load different rows, so all tell
   const bool any_bad = __syncthreads_or(bad != 0);

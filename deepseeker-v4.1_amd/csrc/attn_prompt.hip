@@ -13,6 +13,7 @@ constexpr int kFlWaves = 4;
 constexpr int kFlThreads = 64 * kFlWaves;
 constexpr int kFlRows = 32 * kFlWaves;
 constexpr int kCus = 256;
+constexpr int64_t kFewElements = 1 << 22;   // of K and of V: 8 MB each
 constexpr int kMostRank = 1 << 23;   // of a sequence's first tile; tiles are at most 2^23
 
 struct PromptArgs {
@@ -34,15 +35,16 @@ struct TilePlace { int q0, q1, k0, k1, at; };
 // those of a high rank come first.  The rank is searched for by 64 lanes at once.
 // Workgroups are dealt out to the CUs in turn, two to each; where all of them
 // are there at once, the second of a CU is taken from the other end.
+template <int ROWS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePlace& p) {
   const int lane = threadIdx.x & 63;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
     const int b = min(b0 + lane, a.n_seqs - 1), here = min(a.n_seqs - b0, 64);
     const int q0 = min(max(a.cu_q[b], 0), a.tokens), q1 = min(max(a.cu_q[b + 1], q0), a.tokens);
     const int k0 = min(max(a.cu_k[b], 0), a.kv_tokens), k1 = min(max(a.cu_k[b + 1], k0), a.kv_tokens);
-    const int n = lane < here ? ((q1 - q0) * a.group + kFlRows - 1) / kFlRows : 0;
+    const int n = lane < here ? ((q1 - q0) * a.group + ROWS - 1) / ROWS : 0;
     const int before = a.causal ? max(k1 - k0 - (q1 - q0), 0) : k1 - k0;
-    const int lo = min(before / kFlRows, kMostRank / a.group) * a.group, hi = lo + n;
+    const int lo = min(before / ROWS, kMostRank / a.group) * a.group, hi = lo + n;
     auto from = [&](int rank) {                      // tiles of at least that rank
       int c = 0;
       for (int j = 0; j < here; ++j)
@@ -79,22 +81,24 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePla
   return false;
 }
 
-template <int D>
+// KH waves for every 32 rows.
+template <int D, int KH>
 __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
   extern __shared__ __align__(16) char lds[];
+  constexpr int ROWS = kFlRows / KH, RW = kFlWaves / KH;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % a.kv_heads;
   TilePlace sr;
-  if (!find_tile(a, static_cast<int>(blockIdx.x / a.kv_heads), sr)) return;
+  if (!find_tile<ROWS>(a, static_cast<int>(blockIdx.x / a.kv_heads), sr)) return;
   const int lq = sr.q1 - sr.q0, lk = sr.k1 - sr.k0, rows = lq * a.group;
-  const int row0 = sr.at * kFlRows, wr0 = row0 + 32 * wave;
+  const int row0 = sr.at * ROWS, wr0 = row0 + 32 * (wave % RW);
   const int r = min(wr0 + n, rows - 1), tok = r / a.group, hd = h * a.group + r % a.group;
   const int shift = lk - lq;                        // query i sees the keys up to i + shift
   const int lim = a.causal ? tok + shift : lk - 1;
   const int w_min = a.causal ? min(wr0, rows - 1) / a.group + shift : lk - 1;
   const int b_min = a.causal ? row0 / a.group + shift : lk - 1;
-  const int b_last = min(row0 + kFlRows - 1, rows - 1) / a.group;
+  const int b_last = min(row0 + ROWS - 1, rows - 1) / a.group;
   const int t1 = ((a.causal ? b_last + shift : lk - 1) + kFlKeys) / kFlKeys;   // <= 0 where no key is seen
 
   bf16x8 q[D / 16];
@@ -116,15 +120,17 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
     vp = vb + key * a.v_token;
     last = lk - 1 - key;
   };
-  flash<D, kFlWaves>(q, 0, t1, lim, w_min, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
+  flash<D, kFlWaves, KH>(q, 0, t1, lim, w_min, b_min, a.c2, lds, a.k_token, a.v_token, src, st);
 
+  constexpr int DT = D / 32 / KH;                   // 32-element parts of a row that a wave ends up with
+  if constexpr (KH == 2) add_halves<D, kFlWaves>(st, lds);
   const float l = sum_across32(st.l);
   const bool sees = lim >= 0;                       // else no key: zeros
   const float inv = 1.0f / l;
-  uint16_t* op = a.out + (sr.q0 + static_cast<int64_t>(tok)) * a.o_token + hd * a.o_head;
+  uint16_t* op = a.out + (sr.q0 + static_cast<int64_t>(tok)) * a.o_token + hd * a.o_head + wave / RW * (D / 2);
   const bool live = wr0 + n < rows;
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       // a lane half has elements 8 a + 4 hf .. +4 of a = 2c, 2c + 1: swapped, half hf has all 8 of a = 2c + hf
@@ -143,25 +149,33 @@ __global__ __launch_bounds__(kFlThreads, 2) void k_prompt(const PromptArgs a) {
     }
 }
 
-template <int D, class Args>
-void launch_flash(void (*kernel)(Args), const Args& a, unsigned blocks, hipStream_t s) {
-  launch_kernel(kernel, blocks, kFlThreads, flash_lds<D>(), s, a);
-}
-
 }  // namespace
 
 hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k, const void* v, const int32_t* cu_q,
                          const int32_t* cu_k, void* out, hipStream_t s) {
   const int group = d.heads / d.kv_heads;
   // every sequence's last tile may be partly filled
-  const int64_t tiles = static_cast<int64_t>(d.tokens) * group / kFlRows + d.n_seqs;
+  auto blocks = [&](int rows) {
+    return static_cast<unsigned>((static_cast<int64_t>(d.tokens) * group / rows + d.n_seqs) * d.kv_heads);
+  };
   const PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                      static_cast<uint16_t*>(out), cu_q, cu_k, d.q_token, d.q_head, d.k_token, d.k_head, d.v_token,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
                      group, d.causal, kCus / d.kv_heads};
-  const unsigned blocks = static_cast<unsigned>(tiles * d.kv_heads);
-  if (d.head_dim == 64) launch_flash<64>(k_prompt<64>, a, blocks, s);
-  else launch_flash<128>(k_prompt<128>, a, blocks, s);
+  // At most a workgroup a CU: the time is that of the most keys, and two waves take them for
+  // 32 rows (heads 16 of 64 / 128: 2048 tokens 26.3 -> 22.5 / 35.9 -> 28.5 us, 32 rows
+  // behind 8192 keys 81.5 -> 66.2 / 108 -> 71), unless there are few (16 prompts of 128 tokens
+  // 7.5 either way / 9.9 -> 11.5) or the loads of them, which are twice as many, bound it (64 times 32 rows
+  // behind 2048 keys: 36 -> 48 / 62 -> 90)
+  const bool few = static_cast<int64_t>(d.tokens) * group * d.kv_heads <= kCus * kFlRows &&
+                   d.kv_tokens >= static_cast<int64_t>(d.n_seqs) * 4 * kFlKeys &&
+                   static_cast<int64_t>(d.kv_tokens) * d.kv_heads * d.head_dim <= kFewElements;
+  auto launch = [&](auto two, auto one, size_t lds) {
+    if (few) launch_kernel(two, blocks(kFlRows / 2), kFlThreads, lds, s, a);
+    else launch_kernel(one, blocks(kFlRows), kFlThreads, lds, s, a);
+  };
+  if (d.head_dim == 64) launch(k_prompt<64, 2>, k_prompt<64, 1>, flash_lds<64>());
+  else launch(k_prompt<128, 2>, k_prompt<128, 1>, flash_lds<128>());
   return hipGetLastError();
 }
 

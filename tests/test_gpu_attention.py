@@ -274,6 +274,55 @@ def test_prompt_bounds_outside_are_cut():
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128), (3, 3, 128), (5, 1, 64)])
+@pytest.mark.parametrize("lens,lens_k", [([290], [290]), ([5, 40, 0, 33], [700, 257, 300, 331]), ([90, 1], [20, 513])])
+def test_prompt_of_few_rows_and_many_keys(heads, kv, dim, lens, lens_k, causal):
+    g = gen(sum(lens_k) + heads)
+    q, k, v = normal(g, sum(lens), heads, dim), normal(g, sum(lens_k), kv, dim), normal(g, sum(lens_k), kv, dim)
+    got, (want, tol) = run_prompt(q, k, v, lens, lens_k, causal=causal)
+    assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("poison", [NAN, INF, -INF])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_of_many_keys_unseen_values_stay_unseen(dim, poison):
+    """As above, for rows whose keys two waves share: a poisoned key in either half of a tile."""
+    g = gen(26)
+    cu = [0, 290, 570]
+    q, k, v = normal(g, 570, 2, dim), normal(g, 570, 2, dim), normal(g, 570, 2, dim)
+    want, tol = O.prompt(q, k, v, cu, cu)
+    clean = torch.ones(570, 2, dim, dtype=torch.bool)
+    for at, end in ((270, 290), (290 + 200, 570), (290 + 250, 570)):
+        v[at, 1, 7] = poison
+        clean[at:end, 1, 7] = False
+    k[569, 0] = NAN                                              # seen by its own row alone
+    clean[569, 0] = False
+    got = dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), ints(cu)).cpu().double()
+    assert not torch.isfinite(got[~clean]).any()
+    assert ((got - want).abs() <= tol)[clean].all()
+
+
+@pytest.mark.parametrize("longest", [0, 700])
+def test_prompt_of_many_sequences(longest):
+    """More sequences than lanes, and one whose row tiles are more than lanes."""
+    lens = [(7 * i) % 10 for i in range(150)]
+    lens[77] = longest
+    g = gen(27)
+    t = sum(lens)
+    q, k, v = normal(g, t, 16, 64), normal(g, t, 1, 64), normal(g, t, 1, 64)
+    got, (want, tol) = run_prompt(q, k, v, lens)
+    assert_within(got, want, tol)
+
+
+def test_prompt_behind_very_many_keys():
+    g = gen(28)
+    lens, lens_k = [3, 2], [10, 40000]
+    q, k, v = normal(g, 5, 16, 64), normal(g, 40010, 1, 64), normal(g, 40010, 1, 64)
+    got, (want, tol) = run_prompt(q, k, v, lens, lens_k)
+    assert_within(got, want, tol)
+
+
 def test_prompt_long_rows():
     """2000 tokens: every row of a few heads against float64 on the device (tolerances as the oracle's)."""
     g = torch.Generator(device=DEV).manual_seed(25)
