@@ -172,6 +172,9 @@ static int check_paged(const char* fn, const dsk_paged_desc* d, const dsk_kv_cac
     return fail(DSK_EUNSUPPORTED, "%s: q_len=%d must be in [1, 16] and q_len * heads / kv_heads at most 64", fn, d->q_len);
   if (static_cast<int64_t>(d->batch) * d->q_len * d->heads > kMostBlocks)
     return fail(DSK_EUNSUPPORTED, "%s: batch * q_len * heads exceeds 2^23", fn);
+  const int64_t keys = static_cast<int64_t>(cache->max_pages) * cache->page_size;
+  if (static_cast<int64_t>(d->batch) * d->kv_heads * (keys / 128 + 1) >= INT32_MAX)
+    return fail(DSK_EUNSUPPORTED, "%s: batch * kv_heads * the keys of a table row exceed 2^38", fn);
   if (d->prefix_len < 0 || d->prefix_len >= (1 << 30))
     return fail(DSK_EINVAL, "%s: prefix_len=%d must be in [0, 2^30)", fn, d->prefix_len);
   if (!(d->scale > 0.0f) || !isfinite(d->scale)) return fail(DSK_EINVAL, "%s: scale must be positive and finite", fn);

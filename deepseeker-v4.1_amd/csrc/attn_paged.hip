@@ -66,53 +66,33 @@ __device__ __forceinline__ int units_of(const PagedArgs& a, int b) {
   return (length_of(a, b, bad) + kPgUnit - 1) / kPgUnit;
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  return static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)))) |
-         (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32);
+template <int V>
+struct Const { static constexpr int value = V; };
+
+// Sums over the lanes 0 .. lane, in six vector additions.
+__device__ __forceinline__ uint32_t sum_up_to_lane(uint32_t v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += __builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl.value, rows.value, 0xf, false);
+  };
+  add(Const<0x111>{}, Const<0xf>{});                 // the lane 1, 2, 4, 8 below, in rows of 16
+  add(Const<0x112>{}, Const<0xf>{});
+  add(Const<0x114>{}, Const<0xf>{});
+  add(Const<0x118>{}, Const<0xf>{});
+  add(Const<0x142>{}, Const<0xa>{});                 // lane 15 of the row below to rows 1 and 3
+  add(Const<0x143>{}, Const<0xc>{});                 // lane 31 to rows 2 and 3
+  return v;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
-  return uniform64(v);
+// Units of one key head, 64 sequences at a time: lane's own, and up to its own.
+// Fewer than 2^31 in all, times the key heads too.
+struct Units { uint32_t own, up_to; };
+__device__ __forceinline__ Units units_at(const PagedArgs& a, int b0) {
+  const int b = b0 + (threadIdx.x & 63);
+  const uint32_t n = b < a.batch ? units_of(a, b) : 0;
+  return Units{n, sum_up_to_lane(n)};
 }
-
-// Units of one key head over all sequences, and over those before `stop`; every
-// wave by itself.
-struct Totals { int64_t all, before; };
-__device__ __forceinline__ Totals unit_totals(const PagedArgs& a, int stop) {
-  int64_t all = 0, before = 0;
-  for (int b = threadIdx.x & 63; b < a.batch; b += 64) {
-    const int n = units_of(a, b);
-    all += n;
-    if (b < stop) before += n;
-  }
-  return Totals{wave_sum(all), wave_sum(before)};
-}
-
-// The sequence that unit u of one key head lies in (u < the units of all), and
-// the units before it; every wave by itself.
-__device__ __forceinline__ int find_seq(const PagedArgs& a, int64_t u, int64_t& before) {
-  const int lane = threadIdx.x & 63;
-  int64_t base = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int n = b0 + lane < a.batch ? units_of(a, b0 + lane) : 0;
-    int64_t incl = n;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int64_t o = __shfl_up(incl, s, 64);
-      if (lane >= s) incl += o;
-    }
-    const uint64_t past = __ballot(base + incl > u);
-    if (past) {
-      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      before = uniform64(base + __shfl(incl - n, l, 64));
-      return b0 + l;
-    }
-    base += uniform64(__shfl(incl, 63, 64));
-  }
-  before = base;
-  return a.batch - 1;
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 
 // LDS writes of a wave's lanes before the reads of others of its lanes.
@@ -386,27 +366,44 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 // Workgroup `share` of a.shares takes its share of all units.
 template <int D, int RT>
 __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, SegLds<D, RT, 4>& lds) {
-  const int64_t total = unit_totals(a, 0).all * a.kv_heads;
-  const int64_t quota = (total + a.shares - 1) / a.shares;
-  const int64_t u0 = share * quota, u1 = min(u0 + quota, total);
+  Units n;
+  uint32_t all = 0;                  // units of one key head
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    n = units_at(a, b0);
+    all += lane_value(n.up_to, 63);
+  }
+  const uint32_t total = all * a.kv_heads, quota = (total + a.shares - 1) / a.shares;
+  const uint32_t u0 = share * quota, u1 = min(u0 + quota, total);
   if (u0 >= u1) return;
-  int64_t before;                    // units of one key head in the sequences before b
-  int b = find_seq(a, u0 / a.kv_heads, before);
-  for (int64_t u = u0; u < u1;) {
+  // the sequence that u0 lies in, and the units of one key head in those before it
+  const uint32_t first_unit = u0 / a.kv_heads;
+  uint32_t before = 0;
+  int b = a.batch;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    if (a.batch > 64) n = units_at(a, b0);
+    const uint64_t past = __ballot(before + n.up_to > first_unit);
+    if (past) {
+      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      before += lane_value(n.up_to - n.own, l);
+      b = b0 + l;
+      break;
+    }
+    before += lane_value(n.up_to, 63);
+  }
+  for (uint32_t u = u0; u < u1 && b < a.batch;) {
     bool bad_len;
-    const int len = length_of(a, b, bad_len), nb = (len + kPgUnit - 1) / kPgUnit;
-    const int64_t first = before * a.kv_heads;
-    if (nb == 0 || u >= first + static_cast<int64_t>(nb) * a.kv_heads) {
+    const int len = length_of(a, b, bad_len);
+    const uint32_t nb = (len + kPgUnit - 1) / kPgUnit, first = before * a.kv_heads;
+    if (nb == 0 || u >= first + nb * a.kv_heads) {
       before += nb;
       ++b;
       continue;
     }
     // an item's first unit is kv_heads * before + h * its units
     const int h = static_cast<int>((u - first) / nb);
-    const int64_t item0 = first + static_cast<int64_t>(h) * nb;
-    const int k0 = static_cast<int>(u - item0);
-    const int k1 = static_cast<int>(min(static_cast<int64_t>(nb), u1 - item0));
-    const bool whole = k0 == 0 && k1 == nb;
+    const uint32_t item0 = first + h * nb;
+    const int k0 = static_cast<int>(u - item0), k1 = static_cast<int>(min(nb, u1 - item0));
+    const bool whole = k0 == 0 && k1 == static_cast<int>(nb);
     const int64_t slot = whole ? (a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h : -1)
                                : 2 * static_cast<int64_t>(share) + (u == u0 ? 0 : 1);
     segment<D, RT, 4>(a, b, h, len, bad_len, r0, k0, k1, slot, page_ids<4>(a, b, k0), lds);
@@ -539,27 +536,31 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   __shared__ float red[kRows][WPR];
   __shared__ f32x4 sums[kRows][kWays][kLanes];
   const int M = a.q_len * a.group, tid = threadIdx.x % kThreads, lane = threadIdx.x & 63, wave = tid >> 6;
-  const int mine = threadIdx.x / kThreads, row = blockIdx.x * kRows + mine;
+  const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), row = blockIdx.x * kRows + mine;
   const bool live = row < a.batch * a.kv_heads * M;
   const int r = row % M, item = row / M, h = item % a.kv_heads, b = live ? item / a.kv_heads : 0;
-  const Totals tt = unit_totals(a, b);
-  const int64_t total = tt.all * a.kv_heads;
-  const int64_t quota = (total + a.shares - 1) / a.shares;
+  uint32_t all = 0, before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const Units u = units_at(a, b0);
+    if (b >= b0 && b < b0 + 64) before = all + lane_value(u.up_to - u.own, b - b0);
+    all += lane_value(u.up_to, 63);
+  }
+  const uint32_t quota = (all * a.kv_heads + a.shares - 1) / a.shares;
   bool bad;
   const int len = length_of(a, b, bad), nb = (len + kPgUnit - 1) / kPgUnit;
-  const int64_t item0 = tt.before * a.kv_heads + static_cast<int64_t>(h) * nb;
-  const int64_t s0 = nb ? item0 / quota : 0, s1 = nb ? (item0 + nb - 1) / quota : -1;
+  const uint32_t item0 = before * a.kv_heads + h * nb;
+  const int s0 = nb ? item0 / quota : 0, s1 = nb ? (item0 + nb - 1) / quota : -1;
   const bool whole = nb > 0 && s0 == s1;
   if (WPR > 1 && whole && a.splits == 0) return;      // finished where it was computed
   const bool odd = nb && item0 % quota != 0;          // the first part is not its share's first
-  const int own = static_cast<int>(s1 - s0 + 1);
+  const int own = s1 - s0 + 1;
   const int parts = !live || (whole && a.splits == 0) ? 0 : own + a.splits;
   // row of part i among the partial rows; parts >= own are the prefix's
   auto row_of = [&](int i) -> int64_t {
     if (i >= own)
       return (static_cast<int64_t>(i - own) * a.kv_heads + h) * (static_cast<int64_t>(a.batch) * M) + static_cast<int64_t>(b) * M + r;
     const int64_t slot = whole ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h
-                               : 2 * (s0 + i) + (i == 0 && odd ? 1 : 0);
+                               : 2 * static_cast<int64_t>(s0 + i) + (i == 0 && odd ? 1 : 0);
     return slot * M + r;
   };
   auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };

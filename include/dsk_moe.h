@@ -416,7 +416,8 @@ typedef struct dsk_paged_desc {
  * zeros.  lens[s] < 0: an unused slot, zeros whatever its q holds.  Lengths beyond the
  * table row and page ids outside the cache are never followed: the rows that
  * would need them come out as NaN.  workspace: dsk_paged_attention_workspace_size
- * bytes, 256-byte aligned, no initialisation; one call at a time. */
+ * bytes, 256-byte aligned, no initialisation; one call at a time.  batch * kv_heads
+ * times the keys of a table row (whatever the lengths): below 2^38. */
 int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, size_t* bytes);
 int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, const void* q, const void* k_cache,
                         const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix,

@@ -132,6 +132,18 @@ def test_paged_refuses_pointers_and_space():
     assert call(paged_desc(), n=128) == -5
 
 
+def test_paged_refuses_more_work_than_it_counts():
+    """Units of 128 keys are counted in 31 bits, over the batch and the key heads."""
+    size = ctypes.c_size_t()
+    wide = cache(n_seqs=65535, page_size=256, max_pages=1 << 20, table_stride=1 << 20)
+    assert code("dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(batch=65535, kv_heads=8)), ctypes.byref(wide),
+                ctypes.byref(size)) == -3
+    for heads, pages in ((8, 1 << 11), (1, 1 << 14)):                  # just below 2^31
+        c = cache(n_seqs=65535, page_size=256, max_pages=pages - 1, table_stride=pages)
+        _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(batch=65535, heads=heads, kv_heads=heads)), ctypes.byref(c),
+                  ctypes.byref(size))
+
+
 def test_paged_workspace_grows_with_the_batch():
     size = lambda **kw: (lambda n: (_lib.call(  # noqa: E731
         "dsk_paged_attention_workspace_size", ctypes.byref(paged_desc(**kw)), ctypes.byref(cache(n_seqs=kw.get("batch", 4), max_pages=32, table_stride=32)),
