@@ -23,8 +23,8 @@
 // shares for a fixed number of workgroups, so ragged lengths cost no balance
 // and the lengths are read on the device (a captured launch follows them).  An
 // item that lies in one share is finished there; the parts of the others go
-// through float32 partial rows (o, m, l) and k_paged_join.  Tables of at most
-// kPgShort keys need neither: a workgroup of eight waves takes a whole item.
+// through float32 partial rows (o, m, l) and k_paged_join.  Short tables
+// need neither: a workgroup of eight waves takes a whole item.
 //
 // A prefix that the batch shares is a pass of its own over all of the batch's rows
 // (flash, attn_core.h), split along its keys; its workgroups come first in the
@@ -36,7 +36,9 @@ namespace {
 
 constexpr int kPgThreads = 256;
 constexpr int kPgUnit = 128;        // keys of a unit: 32 for each of four waves
-constexpr int kPgShort = 1024;      // keys of a table row that one workgroup takes alone
+constexpr int kPgShort = 512;       // keys of a table row that one workgroup takes alone
+constexpr int kPgShortMany = 1024;  // where there are kPgMany items
+constexpr int kPgMany = 512;
 constexpr int kPgShortWaves = 8;
 
 struct PagedArgs {
@@ -636,11 +638,19 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
   const int64_t M = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
   p.rt = M <= 16 ? 1 : 2;
   const int64_t items = static_cast<int64_t>(d.batch) * d.kv_heads, keys = static_cast<int64_t>(c.max_pages) * c.page_size;
-  p.alone = d.prefix_len == 0 && keys <= kPgShort;
+  // Up to kPgShort keys are two steps of a workgroup of eight waves, whose loads are all in flight at once: one
+  // sequence with 8 key heads of 128 takes 7.3 us for 260 keys, with shares and their join
+  // 9.3, but 9.9 against 9.3 for 517 and 14.6 against 9.3 for 1000.  Where items fill the
+  // machine without shares, the join is all that they would add (64 such sequences of 600 / 1000 keys: 30.2 / 44.5 us, 31.6 / 45.9
+  // with shares).
+  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany ? kPgShortMany : kPgShort);
   p.total = 256;
   if (p.alone) return p;
   const int64_t units = items * ((keys + kPgUnit - 1) / kPgUnit);
-  const int64_t most = p.rt == 1 ? 512 : 256;   // the workgroups that are resident at once
+  // the workgroups that are resident at once, two a CU (64 sequences of up to 8192 keys, 8 heads
+  // of 128: 81 us, 90 with 256 and 86 with 768); one a CU where registers allow no
+  // more, or beside a prefix's (36.5 us with 256, 39.4 with 512, 64 sequences behind 16385 keys)
+  const int64_t most = p.rt == 1 && d.prefix_len == 0 ? 512 : 256;
   p.shares = static_cast<int>(units < most ? units : most);
   const int64_t rows = static_cast<int64_t>(d.batch) * M;
   if (d.prefix_len > 0) {
