@@ -29,6 +29,10 @@
 // A prefix that the batch shares is a pass of its own over all of the batch's rows
 // (flash, attn_core.h), split along its keys; its workgroups come first in the
 // launch of the shares, so that its products run beside their loads.
+#include <math.h>
+
+#include <algorithm>
+
 #include "attn_core.h"
 
 namespace dsk {
@@ -417,7 +421,8 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
 // head h, split `split` of the keys.
 constexpr int kPreWaves = 4;
 constexpr int kPreRows = 32 * kPreWaves;
-constexpr int kPreBlocks = 256;      // workgroups of the prefix, about: one a CU
+constexpr int kPreBlocks = 256;      // workgroups of the prefix, at most about: one a CU (prefix of 16385 keys for 64
+                                     // sequences: 40 us, 45 with 128, 47 with 384, 50 with 512)
 constexpr int kPreChunk = 64;        // tiles whose places in the cache a wave holds at once
 
 template <int D>
@@ -657,7 +662,13 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
     p.row_tiles = static_cast<int>((rows + kPreRows - 1) / kPreRows);
     const int64_t blocks = static_cast<int64_t>(p.row_tiles) * d.kv_heads, tiles = (d.prefix_len + kFlKeys - 1) / kFlKeys;
     const int64_t want = (kPreBlocks + blocks - 1) / blocks;
-    p.splits = static_cast<int>(want < tiles ? want : tiles);
+    // A split's time are its tiles, about 1 us each (heads of 128), and it adds partial rows to write and to
+    // read, about 0.5 us for 2048 rows: least for the root of their ratio.  64 sequences
+    // with 32 heads of 128 behind 4096 keys: 29.4 us with 8 splits, 34.5 with 16; behind 2000 keys 20.5
+    // with 8, 23.5 with 16, 23.0 with 4; 16 sequences 17.8 with 32, 16.3 with 16, 17.0 with 8
+    const double best = sqrt(4096.0 * static_cast<double>(tiles) / static_cast<double>(rows * d.kv_heads));
+    const int64_t most = best < 1.0 ? 1 : static_cast<int64_t>(best + 0.5);
+    p.splits = static_cast<int>(std::min({want, most, tiles}));
   }
   const size_t own = (2 * static_cast<size_t>(p.shares) + (p.splits ? items : 0)) * M;
   const size_t pre = static_cast<size_t>(p.splits) * d.kv_heads * rows;
