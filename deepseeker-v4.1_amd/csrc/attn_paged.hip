@@ -26,9 +26,17 @@
 // through float32 partial rows (o, m, l) and k_paged_join.  Short tables
 // need neither: a workgroup of eight waves takes a whole item.
 //
+// 64 sequences of 1 to 8192 keys, 32 + 8 heads of 128: 74 us for 381 MB of cache (5.1 TB/s, as
+// a large copy) and 5 us for the join.  8 of up to 32768, 16 + 4 heads of 64, two tokens: 15 us
+// for 66 MB and 5.2 us: 512 workgroups of few loads each, so the start (lengths, pages,
+// keys, one after the other) and the join count.
+//
 // A prefix that the batch shares is a pass of its own over all of the batch's rows
 // (flash, attn_core.h), split along its keys; its workgroups come first in the
-// launch of the shares, so that its products run beside their loads.
+// launch of the shares, so that its products run beside their loads (a launch of its own: 51 against 41 us
+// for 16385 keys and 64 sequences).  There the kernel takes 29 us: 9 us from the launch to the
+// first tile's end and for 16.8 MB of partial rows, 1 us for each of 16 tiles, the rest the
+// shares' loads beside them; the join of 16 parts and the own keys' takes 7.5 us.
 #include <math.h>
 
 #include <algorithm>
@@ -509,7 +517,9 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged_prefix(co
   else shares<D, RT>(a, block % a.shares, 16 * RT * (block / a.shares), *reinterpret_cast<SegLds<D, RT, 4>*>(lds));
 }
 
-// A workgroup for 16 rows of an item; nothing is left to join.
+// A workgroup for 16 rows of an item; nothing is left to join.  260 keys of 8 heads of 128 take 7.3
+// us: the launch, length and page ids, keys, and the eight waves' parts through LDS, one
+// after the other.
 template <int D>
 __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const PagedArgs a) {
   __shared__ SegLds<D, 1, kPgShortWaves> lds;
@@ -667,8 +677,8 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
     // with 32 heads of 128 behind 4096 keys: 29.4 us with 8 splits, 34.5 with 16; behind 2000 keys 20.5
     // with 8, 23.5 with 16, 23.0 with 4; 16 sequences 17.8 with 32, 16.3 with 16, 17.0 with 8
     const double best = sqrt(4096.0 * static_cast<double>(tiles) / static_cast<double>(rows * d.kv_heads));
-    const int64_t most = best < 1.0 ? 1 : static_cast<int64_t>(best + 0.5);
-    p.splits = static_cast<int>(std::min({want, most, tiles}));
+    const int64_t balanced = best < 1.0 ? 1 : static_cast<int64_t>(best + 0.5);
+    p.splits = static_cast<int>(std::min({want, balanced, tiles}));
   }
   const size_t own = (2 * static_cast<size_t>(p.shares) + (p.splits ? items : 0)) * M;
   const size_t pre = static_cast<size_t>(p.splits) * d.kv_heads * rows;

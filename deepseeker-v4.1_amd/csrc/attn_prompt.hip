@@ -4,6 +4,13 @@
 // token by token: the heads of a group share every key tile that is loaded, a
 // short prompt of a few tokens fills a tile with its heads, and the causal edge
 // crosses few keys of a tile.
+//
+// 8192 tokens of 32 + 8 heads of 128 take 474 to 500 us (1.16 to 1.1 PFLOP/s, by the
+// card), bound by the products and the vector work beside them (flash).  16 ragged prompts
+// of 5375 tokens together, 16 + 4 heads of 64, take 25.7 us of which the machine's
+// work is 13: the longest prompt's last rows are 24 tiles in a row, and a CU that
+// holds two such workgroups takes 24 us for them.  17 tokens take 6 us: the launch, the
+// sequence bounds, then q and the first keys, one after the other.
 #include "attn_core.h"
 
 namespace dsk {
