@@ -658,7 +658,9 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
   // 9.3, but 9.9 against 9.3 for 517 and 14.6 against 9.3 for 1000.  Where items fill the
   // machine without shares, the join is all that they would add (64 such sequences of 600 / 1000 keys: 30.2 / 44.5 us, 31.6 / 45.9
   // with shares).
-  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany ? kPgShortMany : kPgShort);
+  // (a launch counts its threads in 32 bits)
+  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany ? kPgShortMany : kPgShort) &&
+            items * (64 * kPgShortWaves) < (int64_t{1} << 32);
   p.total = 256;
   if (p.alone) return p;
   const int64_t units = items * ((keys + kPgUnit - 1) / kPgUnit);

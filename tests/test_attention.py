@@ -151,6 +151,16 @@ def test_paged_workspace_grows_with_the_batch():
     assert 0 < size() < size(batch=8) and size() < size(prefix_len=1) and size() % 256 == 0
 
 
+def test_paged_items_for_more_threads_than_a_launch_counts():
+    """2^23 items in short tables: not one workgroup of 512 threads for each, but shares, which need partial rows."""
+    size = ctypes.c_size_t()
+    for batch, shares in ((8191, False), (8192, True)):
+        d = paged_desc(batch=batch, heads=1024, kv_heads=1024, head_dim=64, q_token=65536, q_head=64, o_token=65536, o_head=64)
+        c = cache(n_seqs=batch, page_size=16, max_pages=4, table_stride=4)
+        _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(d), ctypes.byref(c), ctypes.byref(size))
+        assert (size.value > 256) == shares
+
+
 def test_functions_refuse_cpu_tensors():
     q = torch.zeros(4, 8, 128, dtype=torch.bfloat16)
     i = torch.zeros(4, dtype=torch.int32)
