@@ -387,6 +387,28 @@ def test_paged_long_and_many(batch, longest):
     assert_within(got, want[:, 0], tol[:, 0])
 
 
+@pytest.mark.parametrize("batch,heads,kv,dim,q_len,width,longest,prefix", [
+    (150, 8, 2, 128, 1, 80, 300, 0), (70, 4, 1, 64, 2, 80, 1200, 0), (130, 8, 8, 64, 1, 60, 960, 0), (260, 8, 2, 128, 1, 64, 1024, 0),
+    (150, 8, 2, 64, 1, 80, 300, 200), (70, 8, 1, 128, 4, 80, 700, 100)])
+def test_paged_many_sequences(batch, heads, kv, dim, q_len, width, longest, prefix):
+    """More sequences than lanes over shares or in tables that a workgroup takes alone, long and empty ones among them;
+    their tables hold the same pages in different orders."""
+    page = 16
+    g = gen(batch + dim + width)
+    n_pages = width + 20
+    kc, vc = normal(g, n_pages, kv, page, dim), normal(g, n_pages, kv, page, dim)
+    table = torch.stack([torch.randperm(n_pages, generator=g)[:width] for _ in range(batch)]).to(I32)
+    lens = torch.randint(0, 40, (batch,), generator=g).to(I32)
+    lens[[0, 5, 63, 64, batch - 1]] = torch.tensor([longest, 0, longest, longest // 2, longest - 1], dtype=I32)
+    lens[lens > 0] = lens[lens > 0].clamp(min=q_len)
+    q = normal(g, batch, q_len, heads, dim)
+    pre = torch.randperm(n_pages, generator=g)[:-(-prefix // page)].to(I32)
+    kw = dict(prefix=pre.to(DEV), prefix_len=prefix) if prefix else {}
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), lens.to(DEV), **kw)
+    want, tol = O.paged(q, kc, vc, table, lens.tolist(), pre, prefix)
+    assert_within(got, want, tol)
+
+
 def test_paged_long_prefix():
     g = gen(31)
     table, kc, vc = paged_setup(g, [3, 1, 60], 60, 1, 1, 64, 128)
