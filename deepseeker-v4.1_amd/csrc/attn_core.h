@@ -14,7 +14,7 @@
 // A wave's tile of heads of 128 is 32 products of 32 cycles (16 for heads of 64) and about 200
 // vector instructions, an exponential, a multiply-add, an addition and half a maximum for every score,
 // that issue between them; both pipes together bound it: 0.84 us a tile where a wave has its
-// SIMD to itself, 0.92 for two tiles of two waves (64: 0.6 either way).  That is 1.1 to 1.16
+// SIMD to itself, 0.92 for two tiles of two waves (64: 0.6 either way).  That is 1.07 to 1.16
 // PFLOP/s over 8192 causal tokens of 32 heads (a library product of 8192^3: 1.23).  32 rows a
 // wave, since 64 halve the reads of LDS but spill with heads of 128 and take the same time a row
 // with 64.

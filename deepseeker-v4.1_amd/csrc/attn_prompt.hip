@@ -5,7 +5,7 @@
 // short prompt of a few tokens fills a tile with its heads, and the causal edge
 // crosses few keys of a tile.
 //
-// 8192 tokens of 32 + 8 heads of 128 take 474 to 500 us (1.16 to 1.1 PFLOP/s, by the
+// 8192 tokens of 32 + 8 heads of 128 take 473 to 515 us (1.16 to 1.07 PFLOP/s, by the
 // card), bound by the products and the vector work beside them (flash).  16 ragged prompts
 // of 5375 tokens together, 16 + 4 heads of 64, take 25.7 us of which the machine's
 // work is 13: the longest prompt's last rows are 24 tiles in a row, and a CU that
@@ -40,8 +40,9 @@ struct TilePlace { int q0, q1, k0, k1, at; };
 // Row tile `tile` of all (false: there are fewer), the most keys first, 64 sequences at a
 // time: tile i of a sequence has rank lo + i, lo for the keys before its first query, and
 // those of a high rank come first.  The rank is searched for by 64 lanes at once.
-// Workgroups are dealt out to the CUs in turn, two to each; where all of them
-// are there at once, the second of a CU is taken from the other end.
+// Workgroups are dealt out to the CUs in turn (the 257th comes to the first one's), so the
+// second of a CU is taken in the opposite order: 8192 tokens of 16 heads of 64 / 128 take 163 /
+// 262 us, 170 / 273 without, 4096 of 128 80 against 85.
 template <int ROWS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePlace& p) {
   const int lane = threadIdx.x & 63;
@@ -65,7 +66,7 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int tile, TilePla
       tile -= all;
       continue;
     }
-    if (a.n_seqs <= 64 && all <= 2 * a.first && tile >= a.first) tile = all - 1 - (tile - a.first);
+    if (a.n_seqs <= 64 && tile >= a.first && tile < 2 * a.first) tile = a.first + min(2 * a.first, all) - 1 - tile;
     for (;;) {
       const int l = 63 - __clzll(__ballot(count > tile));  // lane 0 always
       rank += l * step;
