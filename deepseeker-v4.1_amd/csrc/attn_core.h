@@ -225,12 +225,22 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   // fragment and the vector work that its time covers (8192 tokens, 32 heads of 128: 492 us as the
   // compiler orders it, 484 with the products' order, 476 with the loads of K
   // behind the first products)
+  // reads of V (two a fragment) in the place of those of K that are made already; of heads of 64 with
+  // half the keys there are few products to hide them behind (2048 tokens 22.8 -> 21.5 us; whole tiles need the
+  // registers for a third wave)
+  constexpr int kAhead = D == 64 && KT == 1 ? 3 : 1;
   auto order = [&]() {
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int i = 0; i < KT * KS; ++i) {
+    for (int i = 0; i < KT * KS - 4; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
       __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
     }
 #pragma unroll

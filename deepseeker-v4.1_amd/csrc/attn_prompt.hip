@@ -171,7 +171,7 @@ hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
                      group, d.causal, kCus / d.kv_heads};
   // At most a workgroup a CU: the time is that of the most keys, and two waves take them for
-  // 32 rows (heads 16 of 64 / 128: 2048 tokens 26.3 -> 22.5 / 35.9 -> 28.5 us, 32 rows
+  // 32 rows (heads 16 of 64 / 128: 2048 tokens 26.3 -> 21.5 / 35.9 -> 28.5 us, 32 rows
   // behind 8192 keys 81.5 -> 66.2 / 108 -> 71), unless there are few (16 prompts of 128 tokens
   // 7.5 either way / 9.9 -> 11.5) or the loads of them, which are twice as many, bound it (64 times 32 rows
   // behind 2048 keys: 36 -> 48 / 62 -> 90)
