@@ -170,12 +170,13 @@ hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k,
                      static_cast<uint16_t*>(out), cu_q, cu_k, d.q_token, d.q_head, d.k_token, d.k_head, d.v_token,
                      d.v_head, d.o_token, d.o_head, d.scale * kLog2e, d.tokens, d.kv_tokens, d.n_seqs, d.kv_heads,
                      group, d.causal, kCus / d.kv_heads};
-  // At most a workgroup a CU: the time is that of the most keys, and two waves take them for
-  // 32 rows (heads 16 of 64 / 128: 2048 tokens 26.3 -> 21.5 / 35.9 -> 28.5 us, 32 rows
-  // behind 8192 keys 81.5 -> 66.2 / 108 -> 71), unless there are few (16 prompts of 128 tokens
-  // 7.5 either way / 9.9 -> 11.5) or the loads of them, which are twice as many, bound it (64 times 32 rows
+  // Up to about one and a half workgroups a CU the time is that of the most keys, and two waves take
+  // them for 32 rows (16 heads of 64 / 128: 2048 tokens 26.3 -> 21.5 / 35.9 -> 28.5 us, 32 rows
+  // behind 8192 keys 81.5 -> 66.2 / 108 -> 71, prompts of 1500 and 1124 together 20.9 -> 17.6 / 29.6 -> 28.3, but
+  // three of 1500 24.1 -> 27.7 / 38 -> 47), unless there are few (16 prompts of 128 tokens
+  // 7.3 either way / 9.7 -> 11) or the loads of them, which are twice as many, bound it (64 times 32 rows
   // behind 2048 keys: 36 -> 48 / 62 -> 90)
-  const bool few = static_cast<int64_t>(d.tokens) * group * d.kv_heads <= kCus * kFlRows &&
+  const bool few = static_cast<int64_t>(d.tokens) * group * d.kv_heads <= kCus * kFlRows * 3 / 2 &&
                    d.kv_tokens >= static_cast<int64_t>(d.n_seqs) * 4 * kFlKeys &&
                    static_cast<int64_t>(d.kv_tokens) * d.kv_heads * d.head_dim <= kFewElements;
   auto launch = [&](auto two, auto one, size_t lds) {
