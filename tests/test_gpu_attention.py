@@ -679,6 +679,47 @@ def test_captured_steps_follow_the_lengths(prefix):
             assert torch.equal(step(), held), i                  # the eager step writes the same rows again
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_captured_prompts_follow_their_bounds(dim):
+    """A prompt step (norms, rotation, append, attention) captured once: replays on other rows and other bounds against
+    the eager calls, with eager work between them."""
+    g = gen(45)
+    t, heads, kv = 700, 8, 2
+    st = dict(qkv=normal(g, t, (heads + 2 * kv) * dim).to(DEV), pos=torch.zeros(t, dtype=I32, device=DEV),
+              seq=torch.zeros(t, dtype=I32, device=DEV), cu=ints([0, t, t, t]), table=torch.arange(3 * 44, dtype=I32).view(3, 44).to(DEV))
+    caches = [torch.zeros((140, kv, 16, dim), dtype=BF16, device=DEV) for _ in range(4)]
+    freq, _ = dsk_moe.rope_frequencies(dim)
+
+    def step(kc, vc):
+        q, k, v = (p.unflatten(1, (-1, dim)) for p in st["qkv"].split([heads * dim, kv * dim, kv * dim], 1))
+        kr = torch.zeros((t, kv, dim), dtype=BF16, device=DEV)
+        q = dsk_moe.kv_append(q, k, v, st["pos"], st["seq"], st["table"], kc, vc, freq, k_out=kr, q_out=torch.zeros((t, heads, dim), dtype=BF16, device=DEV))
+        return dsk_moe.prompt_attention(q, kr, v, st["cu"], out=torch.zeros_like(q))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*caches[:2])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*caches[:2])
+    for lens in ([700, 0, 0], [1, 300, 399], [0, 0, 0], [64, 65, 63], [350, 350, 0]):
+        n = sum(lens)
+        st["qkv"].copy_(normal(g, *st["qkv"].shape))
+        st["cu"].copy_(ints(cumulative(lens)))
+        st["pos"].copy_(ints([i for m in lens for i in range(m)] + [-1] * (t - n)))
+        st["seq"].copy_(ints([b for b, m in enumerate(lens) for _ in range(m)] + [0] * (t - n)))
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        want = step(*caches[2:])
+        assert torch.equal(got, want) and not got[n:].any(), lens
+        assert all(torch.equal(a, b) for a, b in zip(caches[:2], caches[2:])), lens
+        dsk_moe.prompt_attention(want[:50], want[:50, :kv].contiguous(), want[:50, :kv].contiguous(), ints([0, 20, 50]))   # eager work of another size
+
+
 def test_calls_on_two_streams():
     """Concurrent calls on two streams, each with its own scratch memory."""
     g = gen(50)
