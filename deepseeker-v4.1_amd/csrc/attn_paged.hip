@@ -53,6 +53,8 @@ constexpr int kPgShortMany = 1024;  // where there are kPgMany items
 constexpr int kPgMany = 512;
 constexpr int kPgShortWaves = 8;
 
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
 struct PagedArgs {
   const uint16_t* q;
   uint16_t* out;
@@ -60,6 +62,7 @@ struct PagedArgs {
   CacheView c;
   float* po;                        // partial rows [slot][M][D]
   float* pml;                       // [slot][M][2]: maximum (of scores times c), sum
+  i32x2* parts;                     // of an item with keys: its first slot, and how many parts to join
   float* pre_o;                     // prefix partials [split][kv head][batch * M][D]
   float* pre_ml;
   const int32_t* pages;             // of the prefix
@@ -420,6 +423,9 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
     const bool whole = k0 == 0 && k1 == static_cast<int>(nb);
     const int64_t slot = whole ? (a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h : -1)
                                : 2 * static_cast<int64_t>(share) + (u == u0 ? 0 : 1);
+    if (k0 == 0 && r0 == 0 && threadIdx.x == 0)
+      a.parts[b * a.kv_heads + h] =
+          i32x2{static_cast<int>(slot), whole ? (a.splits ? 1 : 0) : static_cast<int>((item0 + nb - 1) / quota) - share + 1};
     segment<D, RT, 4>(a, b, h, len, bad_len, r0, k0, k1, slot, page_ids<4>(a, b, k0), lds);
     u = item0 + k1;
   }
@@ -556,29 +562,18 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), row = blockIdx.x * kRows + mine;
   const bool live = row < a.batch * a.kv_heads * M;
   const int r = row % M, item = row / M, h = item % a.kv_heads, b = live ? item / a.kv_heads : 0;
-  uint32_t all = 0, before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const Units u = units_at(a, b0);
-    if (b >= b0 && b < b0 + 64) before = all + lane_value(u.up_to - u.own, b - b0);
-    all += lane_value(u.up_to, 63);
-  }
-  const uint32_t quota = (all * a.kv_heads + a.shares - 1) / a.shares;
+  const i32x2 of_item = ldg<i32x2>(a.parts + b * a.kv_heads + h);   // beside the length; nothing where there are no keys
   bool bad;
-  const int len = length_of(a, b, bad), nb = (len + kPgUnit - 1) / kPgUnit;
-  const uint32_t item0 = before * a.kv_heads + h * nb;
-  const int s0 = nb ? item0 / quota : 0, s1 = nb ? (item0 + nb - 1) / quota : -1;
-  const bool whole = nb > 0 && s0 == s1;
-  if (WPR > 1 && whole && a.splits == 0) return;      // finished where it was computed
-  const bool odd = nb && item0 % quota != 0;          // the first part is not its share's first
-  const int own = s1 - s0 + 1;
-  const int parts = !live || (whole && a.splits == 0) ? 0 : own + a.splits;
-  // row of part i among the partial rows; parts >= own are the prefix's
+  const int len = length_of(a, b, bad);
+  const bool done = len > 0 && of_item.y == 0;        // finished where it was computed
+  if (WPR > 1 && done) return;
+  const int own = len > 0 ? of_item.y : 0, parts = !live || done ? 0 : own + a.splits;
+  // row of part i among the partial rows: of a share its first (2 share) or last (2 share + 1) item, the
+  // later parts are the first of theirs; parts >= own are the prefix's
   auto row_of = [&](int i) -> int64_t {
     if (i >= own)
       return (static_cast<int64_t>(i - own) * a.kv_heads + h) * (static_cast<int64_t>(a.batch) * M) + static_cast<int64_t>(b) * M + r;
-    const int64_t slot = whole ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h
-                               : 2 * static_cast<int64_t>(s0 + i) + (i == 0 && odd ? 1 : 0);
-    return slot * M + r;
+    return static_cast<int64_t>(i == 0 ? of_item.x : (of_item.x | 1) - 1 + 2 * i) * M + r;
   };
   auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };
   // the first parts of every group of lanes, on their way beside the maxima and sums
@@ -629,7 +624,7 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   sums[mine][way][tid % kLanes] = y;
   if constexpr (WPR > 1) __syncthreads();
   else wave_fence();
-  if (way || !live || (whole && a.splits == 0)) return;
+  if (way || !live || done) return;
 #pragma unroll
   for (int w = 1; w < kWays; ++w) y += sums[mine][w][tid % kLanes];
   const int tok = r / a.group, hd = h * a.group + r % a.group;
@@ -644,7 +639,7 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
 struct PagedPlan {
   int rt, shares, splits, row_tiles;
   bool alone;                        // k_paged_short
-  size_t po, pml, pre_o, pre_ml, total;
+  size_t po, pml, parts, pre_o, pre_ml, total;
 };
 
 PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
@@ -686,7 +681,8 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
   const size_t pre = static_cast<size_t>(p.splits) * d.kv_heads * rows;
   p.po = 0;
   p.pml = up(p.po + own * d.head_dim * 4);
-  p.pre_o = up(p.pml + own * 8);
+  p.parts = up(p.pml + own * 8);
+  p.pre_o = up(p.parts + items * 8);
   p.pre_ml = up(p.pre_o + pre * d.head_dim * 4);
   p.total = up(p.pre_ml + pre * 8);
   return p;
@@ -722,7 +718,7 @@ hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const vo
   const PagedPlan p = plan_of(d, c);
   char* w = static_cast<char*>(ws);
   const PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, view,
-                    reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml),
+                    reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml), reinterpret_cast<i32x2*>(w + p.parts),
                     reinterpret_cast<float*>(w + p.pre_o), reinterpret_cast<float*>(w + p.pre_ml), prefix,
                     d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
                     d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits, p.row_tiles,
