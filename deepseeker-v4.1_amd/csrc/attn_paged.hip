@@ -28,7 +28,7 @@
 //
 // 64 sequences of 1 to 8192 keys, 32 + 8 heads of 128: 74 us for 381 MB of cache (5.1 TB/s, as
 // a large copy) and 5 us for the join.  8 of up to 32768, 16 + 4 heads of 64, two tokens: 15 us
-// for 66 MB and 5.2 us: 512 workgroups of few loads each, so the start (lengths, pages,
+// for 66 MB and 5 us: 512 workgroups of few loads each, so the start (lengths, pages,
 // keys, one after the other) and the join count.
 //
 // A prefix that the batch shares is a pass of its own over all of the batch's rows
@@ -36,7 +36,7 @@
 // launch of the shares, so that its products run beside their loads (a launch of its own: 51 against 41 us
 // for 16385 keys and 64 sequences).  There the kernel takes 29 us: 9 us from the launch to the
 // first tile's end and for 16.8 MB of partial rows, 1 us for each of 16 tiles, the rest the
-// shares' loads beside them; the join of 16 parts and the own keys' takes 7.5 us.
+// shares' loads beside them; the join of 16 parts and the own keys' takes 6.6 us.
 #include <math.h>
 
 #include <algorithm>
@@ -549,8 +549,9 @@ __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const Pag
 // row: their maxima and sums first, a part a lane, then groups of D / 4 lanes add up the
 // parts in a fixed order.  Also writes the rows of sequences without keys.
 // From kPgWaveRows rows on a wave each, since a workgroup then has little to do a row: 2048 rows of
-// 18 and of 2 parts of 128 take 7.7 and 5.7 us so, 10.6 and 8.1 with four waves; below, four
-// waves: 256 rows of 17 parts of 64 take 5.9 us, with one 7.8.
+// 18 parts of 128 take 6.6 us so, 7.4 with four waves (of 2 parts 5.3 either way); below, four
+// waves: 256 rows of 17 parts of 64 take 4.9 us, with one 7.4.  Most of it is the launch and
+// the loads after each other: length and place, maxima and sums beside the first parts.
 constexpr int kPgWaveRows = 1024;
 
 template <int D, int WPR>
