@@ -568,13 +568,16 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   const int len = length_of(a, b, bad);
   const bool done = len > 0 && of_item.y == 0;        // finished where it was computed
   if (WPR > 1 && done) return;
-  const int own = len > 0 ? of_item.y : 0, parts = !live || done ? 0 : own + a.splits;
+  // (kept inside the partial rows, also where a length has changed since the shares ran)
+  const int slot0 = min(max(of_item.x, 0), 2 * a.shares + (a.splits ? a.batch * a.kv_heads : 0) - 1);
+  const int own = len > 0 ? min(max(of_item.y, 1), max(a.shares - (slot0 >> 1), 1)) : 0;
+  const int parts = !live || done ? 0 : own + a.splits;
   // row of part i among the partial rows: of a share its first (2 share) or last (2 share + 1) item, the
   // later parts are the first of theirs; parts >= own are the prefix's
   auto row_of = [&](int i) -> int64_t {
     if (i >= own)
       return (static_cast<int64_t>(i - own) * a.kv_heads + h) * (static_cast<int64_t>(a.batch) * M) + static_cast<int64_t>(b) * M + r;
-    return static_cast<int64_t>(i == 0 ? of_item.x : (of_item.x | 1) - 1 + 2 * i) * M + r;
+    return static_cast<int64_t>(i == 0 ? slot0 : (slot0 | 1) - 1 + 2 * i) * M + r;
   };
   auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };
   // the first parts of every group of lanes, on their way beside the maxima and sums
