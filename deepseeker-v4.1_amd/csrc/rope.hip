@@ -18,7 +18,7 @@
 // keeps its 8 elements' factors, gamma cos and +-gamma' sin, in registers.  A
 // head then takes two multiply-adds an element, and the traffic bounds the
 // kernel: 8192 tokens of 32 + 8 + 8 heads of 128 into a cache take 36 us (5.6
-// TB/s), 4095 of 32 + 8 20.5 us (4.1 TB/s); a block for four tokens with the factors
+// TB/s), 4095 of 32 + 8 20 us (4.2 TB/s); a block for four tokens with the factors
 // from LDS for every head took 53 and 28 us.  Few tokens: a token's heads over
 // several waves, queries apart from keys and values, for the latency.
 #include "attn.h"
@@ -38,7 +38,7 @@ struct QkArgs {
   uint16_t *q_out, *k_out;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head, ko_token, ko_head;
   int32_t tokens, heads, kv_heads, rot_dim, rot_first, prefix_len, norm;
-  int32_t q_parts, kv_parts;         // waves of a token for queries, and for keys and values; 0: one for all
+  int32_t q_parts, kv_parts;         // waves of a token for queries, and for keys and values (kAll: one for all)
   float eps, mscale;
   CacheView cache;
   bool append;
@@ -63,8 +63,9 @@ struct Raw8 {
   }
 };
 
-// A lane's part of a head row: elements e .. e + 7 of 8 lanes (D 64) or 16 (D 128).
-template <int D, bool kBF16, bool kInter>
+// A lane's part of a head row: elements e .. e + 7 of 8 lanes (D 64) or 16 (D 128).  kAll: a
+// wave takes all heads of its token.
+template <int D, bool kBF16, bool kInter, bool kAll>
 __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a head row, rows of a wave
   __shared__ float2 turns[kQkWaves][D / 2];
@@ -77,9 +78,9 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   // half pairs: the elements that pair with the lane's own
   const int ep = kInter || !rotated ? e : (low ? e + half : e - half);
   // this lane's heads: row0, row0 + step, ..
-  const bool all = a.q_parts == 0, is_q = all || static_cast<int>(blockIdx.y) < a.q_parts;
+  const bool is_q = kAll || static_cast<int>(blockIdx.y) < a.q_parts;
   const int part = is_q ? blockIdx.y : blockIdx.y - a.q_parts;
-  const int row0 = part * kRows + wl / kLanes, step = (all ? 1 : is_q ? a.q_parts : a.kv_parts) * kRows;
+  const int row0 = part * kRows + wl / kLanes, step = (kAll ? 1 : is_q ? a.q_parts : a.kv_parts) * kRows;
 
   // heads row, row + step, .. of one tensor: kQkAhead of them
   struct Heads { Raw8<kBF16> x[kQkAhead], y[kQkAhead]; };
@@ -165,6 +166,14 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
     return u32x4{pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]), pack_bf16(z[4], z[5]), pack_bf16(z[6], z[7])};
   };
 
+  // Many tokens write more than L2 holds, past it: 8192 of 32 + 8 + 8 heads of 128, each call on
+  // tensors of its own, 47.4 -> 44.7 us, 4095 of 32 + 8 27 -> 20, 2048 13.7 -> 11.5; with the attention that reads
+  // them next, 8192 tokens 522 -> 517, 2048 to 4096 within 1 %.  Few tokens' rows are read next and
+  // stay (128 to 512 tokens with their attention: 0.2 us)
+  auto store = [&](uint16_t* p, const u32x4& x) {
+    if constexpr (kAll) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+    else *reinterpret_cast<u32x4*>(p) = x;
+  };
   // each wave reads its own angles alone: its LDS writes are done before
   __builtin_amdgcn_wave_barrier();
   float own[8], pair[8];
@@ -181,12 +190,12 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
 #pragma unroll
       for (int i = 0; i < kQkAhead; ++i)
         if (row + i * step < a.heads)
-          *reinterpret_cast<u32x4*>(a.q_out + t * a.qo_token + (row + i * step) * a.qo_head + e) = out[i];
+          store(a.q_out + t * a.qo_token + (row + i * step) * a.qo_head + e, out[i]);
       row = next;
     }
   }
-  if (row0 >= a.kv_heads || (is_q && !all)) return;
-  if (all) {
+  if (row0 >= a.kv_heads || (is_q && !kAll)) return;
+  if (kAll) {
     load(r, a.k, a.k_token, a.k_head, row0, a.kv_heads, true);
     if (slot >= 0) load(v, a.v, a.v_token, a.v_head, row0, a.kv_heads, false);
   }
@@ -201,13 +210,12 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
     for (int i = 0; i < kQkAhead; ++i) {
       const int h = row + i * step;
       if (h >= a.kv_heads) break;
-      if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + e) = out[i];
+      if (a.k_out) store(a.k_out + t * a.ko_token + h * a.ko_head + e, out[i]);
       if (slot >= 0) {
         const int64_t to = (slot + (static_cast<int64_t>(h) << a.cache.page_shift)) * D + e;
-        *reinterpret_cast<u32x4*>(a.cache.k + to) = out[i];
+        store(a.cache.k + to, out[i]);
         const Raw8<kBF16>& x = v.x[i];
-        *reinterpret_cast<u32x4*>(a.cache.v + to) =
-            u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+        store(a.cache.v + to, u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])});
       }
     }
     if (next < a.kv_heads && slot >= 0) load(v, a.v, a.v_token, a.v_head, next, a.kv_heads, false);
@@ -227,12 +235,13 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
   a.q_parts = q_parts;
   a.kv_parts = kv_parts;
   const dim3 grid((d.tokens + kQkWaves - 1) / kQkWaves, split ? q_parts + kv_parts : 1);
+  auto launch = [&](auto whole, auto parts) { launch_kernel(split ? parts : whole, grid, 64 * kQkWaves, 0, s, a); };
   if (d.dtype == DSK_DTYPE_BF16) {
-    if (d.interleaved) launch_kernel(k_qk<D, true, true>, grid, 64 * kQkWaves, 0, s, a);
-    else launch_kernel(k_qk<D, true, false>, grid, 64 * kQkWaves, 0, s, a);
+    if (d.interleaved) launch(k_qk<D, true, true, true>, k_qk<D, true, true, false>);
+    else launch(k_qk<D, true, false, true>, k_qk<D, true, false, false>);
   } else {
-    if (d.interleaved) launch_kernel(k_qk<D, false, true>, grid, 64 * kQkWaves, 0, s, a);
-    else launch_kernel(k_qk<D, false, false>, grid, 64 * kQkWaves, 0, s, a);
+    if (d.interleaved) launch(k_qk<D, false, true, true>, k_qk<D, false, true, false>);
+    else launch(k_qk<D, false, false, true>, k_qk<D, false, false, false>);
   }
 }
 
