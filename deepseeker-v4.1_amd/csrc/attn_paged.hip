@@ -283,9 +283,10 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
         // output's own rounding of 2^-9
         p[rt] = as_bf16x8(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
       }
-      // rows of several tokens see different keys here: are all the values finite?
+      // keys that a row does not see, or places behind the last key (that key's values again): are all
+      // the values finite?
       bool finite = true;
-      if (masked && a.q_len > 1) {
+      if (masked) {
         uint32_t bits = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)

@@ -880,3 +880,29 @@ def test_decoder_refuses():
     for heads, kv in ((8, 3), (7, 7), (0, 0)):
         with pytest.raises(ValueError):
             dsk_moe.Attention(a.w_qkv, a.w_o, heads, kv)
+
+
+@pytest.mark.parametrize("width,prefix", [(16, 0), (80, 0), (16, 50)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_shows_an_infinite_value_as_it_is(dim, width, prefix):
+    """One token a sequence: an infinite value among its last keys gives that infinity whatever the length leaves
+    empty of the last 32 keys, a NaN gives NaN, and the other elements stay as they were."""
+    g = gen(38 + dim)
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 48, 100, 127, 128, 129, 190]
+    used = [-(-n // 16) for n in lens]
+    table, kc, vc = paged_setup(g, used + [4], max(max(used), width), 0, 1, 16, dim)
+    pre, table = table[-1, :4], table[:-1]
+    q = normal(g, len(lens), 4, dim)
+    want, tol = O.paged(q[:, None], kc, vc, table, lens, pre, prefix)
+    want, tol = want[:, 0], tol[:, 0]
+    for b, n in enumerate(lens):                                 # at the last key, and one before it
+        for j, at, x in ((n - 1, 3, INF), (n - 1, 9, -INF), (n - 1, 20, NAN), (max(0, n - 2), 5, INF)):
+            vc[table[b, j // 16], 0, j % 16, at] = x
+    for at, x in ((3, INF), (9, -INF), (20, NAN), (5, INF)):
+        want[..., at] = x
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints(lens),
+                                  prefix=pre.to(DEV) if prefix else None, prefix_len=prefix).cpu().double()
+    assert torch.equal(got[..., [3, 5, 9]], want[..., [3, 5, 9]])
+    assert got[..., 20].isnan().all()
+    rest = [i for i in range(dim) if i not in (3, 5, 9, 20)]
+    assert ((got - want).abs() <= tol)[..., rest].all()
