@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
@@ -363,6 +363,10 @@ class PromptStep:
     table: torch.Tensor
     cu: torch.Tensor
 
+    def idle(self) -> PromptStep:
+        """A step of the same sizes that has no sequences and keeps nothing."""
+        return replace(self, positions=torch.full_like(self.positions, -1), cu=torch.zeros_like(self.cu))
+
 
 @dataclass
 class DecodeStep:
@@ -377,6 +381,10 @@ class DecodeStep:
     q_len: int = 1
     prefix: torch.Tensor | None = None
     prefix_len: int = 0
+
+    def idle(self) -> DecodeStep:
+        """A step of the same sizes whose slots are all unused: it keeps nothing."""
+        return replace(self, positions=torch.full_like(self.positions, -1), lens=torch.full_like(self.lens, -1))
 
 
 class Attention:

@@ -122,8 +122,8 @@ class MoEStack:
         """Record the stack for ``tokens`` rows as one HIP graph (static input / output
         buffers).  The graph owns its workspace (sized for the largest layer), so
         later eager calls of any size, or other captures, cannot move it.  With
-        attention sublayers: on ``step``'s tensors, which must stay where they are
-        (the warm-up writes cache rows at the positions that they hold)."""
+        attention sublayers: on ``step``'s tensors, which must stay where they are;
+        the capture itself keeps nothing in the caches, whatever they hold."""
         dev = self.layers[0].gate_w.device
         hidden = self.layers[0].gate_w.shape[1]
         self._x = torch.zeros((tokens, hidden), dtype=dtype, device=dev)
@@ -133,8 +133,9 @@ class MoEStack:
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
+            idle = step.idle() if step is not None else None
             for _ in range(warmup):
-                self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=step)
+                self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=idle)
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         self._step = step                # the graph reads its tensors

@@ -906,3 +906,45 @@ def test_decode_shows_an_infinite_value_as_it_is(dim, width, prefix):
     assert got[..., 20].isnan().all()
     rest = [i for i in range(dim) if i not in (3, 5, 9, 20)]
     assert ((got - want).abs() <= tol)[..., rest].all()
+
+
+def test_capture_leaves_the_cache_alone():
+    """Prompts, then a captured decode step, as documented: the capture keeps nothing in the caches, and the replays follow
+    the eager steps bit for bit.  An unused slot's table row names the page of a live sequence, which stays as it is."""
+    g, stack = make_decoder(64)
+    table = (torch.randperm(60, generator=g)[:48].view(4, 12) + 1).to(I32)
+    table[0, 0], table[2] = 0, 0                                  # slot 2 is unused; page 0 is sequence 0's first
+    table = table.to(DEV)
+    rows = [20, 1, 0, 33]
+    ar = torch.cat([torch.arange(n) for n in rows]).to(I32).to(DEV)
+    seq = torch.repeat_interleave(torch.arange(4), torch.tensor(rows)).to(I32).to(DEV)
+    stack(normal(g, 54, 1024).to(DEV), step=dsk_moe.PromptStep(ar, seq, table, ints(cumulative(rows))))
+    caches = [c for a in stack.attention for c in (a.k_cache, a.v_cache)]
+    held = [c.clone() for c in caches]
+    xs = [normal(g, 4, 1024).to(DEV) for _ in range(3)]
+
+    def fresh():
+        return dsk_moe.DecodeStep(ints([19, 0, -1, 32]), ints([0, 1, 2, 3]), table, ints([20, 1, -1, 33]))
+
+    def advance(step):
+        live = (step.lens >= 0).int()
+        step.positions += live
+        step.lens += live
+
+    step, want = fresh(), []
+    for x in xs:
+        advance(step)
+        want.append(stack(x, step=step).clone())
+    after = [c.clone() for c in caches]
+    for c, h in zip(caches, held):
+        c.copy_(h)
+    step = fresh()
+    stack.capture(4, step=step)
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, h) for c, h in zip(caches, held)), "the capture wrote to the cache"
+    assert step.positions.tolist() == [19, 0, -1, 32] and step.lens.tolist() == [20, 1, -1, 33]
+    for x, w in zip(xs, want):
+        advance(step)
+        assert torch.equal(stack.replay(x), w)
+        torch.cuda.synchronize()
+    assert all(torch.equal(c, a) for c, a in zip(caches, after))
