@@ -189,11 +189,11 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     const int32_t* trow = a.c.table + b * a.c.table_stride;
     const int last_tile = (len - 1) >> 4;
     int ids = first_ids, ids0 = k0;   // lane 2 i + kt: the page of tile kt of step ids0 + i
-    bool bad = false;
+    int bad_tile = INT32_MAX;         // the lane's first 16 keys on a page outside the cache
     auto check_ids = [&]() {
-      const int step = ids0 + (lane >> 1);
+      const int step = ids0 + (lane >> 1), tile = step * (2 * W) + 2 * wave + (lane & 1);
       const bool out_of = ids < 0 || ids >= a.c.n_pages;
-      bad = bad || (out_of && step < k1 && step * (2 * W) + 2 * wave + (lane & 1) <= last_tile);
+      if (out_of && step < k1 && tile <= last_tile) bad_tile = min(bad_tile, tile);
       if (out_of) ids = 0;
     };
     check_ids();
@@ -321,12 +321,15 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     if (kk < k1) compute(s0, kk);
 
     // the waves' parts
-    const bool any_bad = __any(bad);
+    const bool any_bad = __any(bad_tile != INT32_MAX);
+    if (any_bad)
+#pragma unroll
+      for (int s = 32; s >= 1; s >>= 1) bad_tile = min(bad_tile, __shfl_xor(bad_tile, s, 64));
     __syncthreads();                 // the last segment's reads of LDS are done
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       l[rt] = sum_across32(sum_across16(l[rt]));
-      if (any_bad) l[rt] = __builtin_nanf("");
+      if (any_bad && (lim[rt] >> 4) >= bad_tile) l[rt] = __builtin_nanf("");   // the rows that see such keys
       if (g == 0) {
         lds.ml[wave][16 * rt + n16][0] = m[rt];
         lds.ml[wave][16 * rt + n16][1] = l[rt];

@@ -413,9 +413,9 @@ typedef struct dsk_paged_desc {
  * before) after the prefix_len keys of the pages prefix[0 ..], which are read
  * once for the whole batch.  Query i of q_len sees the prefix and its
  * sequence's keys j <= lens[s] - q_len + i; a query that sees no key gives
- * zeros.  lens[s] < 0: an unused slot, zeros whatever its q holds.  Lengths beyond the
- * table row and page ids outside the cache are never followed: the rows that
- * would need them come out as NaN.  workspace: dsk_paged_attention_workspace_size
+ * zeros.  lens[s] < 0: an unused slot, zeros whatever its q holds.  Page ids outside the
+ * cache and lengths beyond the table row are never followed: the queries that see a
+ * key on such a page, and all of a sequence with such a length, come out as NaN.  workspace: dsk_paged_attention_workspace_size
  * bytes, 256-byte aligned, no initialisation; one call at a time.  batch * kv_heads
  * times the keys of a table row (whatever the lengths): below 2^38. */
 int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, size_t* bytes);

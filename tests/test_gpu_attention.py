@@ -948,3 +948,24 @@ def test_capture_leaves_the_cache_alone():
         assert torch.equal(stack.replay(x), w)
         torch.cuda.synchronize()
     assert all(torch.equal(c, a) for c, a in zip(caches, after))
+
+
+@pytest.mark.parametrize("width,prefix", [(6, 0), (80, 0), (6, 33)])
+def test_paged_rows_that_need_no_bad_page(width, prefix):
+    """Of a verify step's tokens, those that see a key on a page outside the cache are NaN; those before them are not,
+    and those that see no key are zero."""
+    g = gen(39)
+    n, q_len = [50, 48, 2, 83], 4
+    table, kc, vc = paged_setup(g, [6, 6, 6, 6, 3], max(width, 6), 0, 2, 16, 64)
+    pre, table = table[-1, :3], table[:-1]
+    bad = table.clone()
+    bad[0, 3], bad[1, 2], bad[2, 0], bad[3, 5], bad[3, 1] = 1 << 30, -1, 99, 1 << 20, -5
+    q = normal(g, 4, q_len, 6, 64)
+    kw = dict(prefix=pre.to(DEV), prefix_len=prefix) if prefix else {}
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bad.to(DEV), ints(n), **kw)
+    want, tol = O.paged(q, kc, vc, table, n, pre, prefix)
+    needs = torch.tensor([[False, False, True, True], [True] * 4, [False, False, True, True], [True] * 4])
+    assert got[needs.to(DEV)].isnan().all()
+    assert_within(got.cpu()[~needs], want[~needs], tol[~needs])
+    if not prefix:
+        assert not got[2, :2].any()
