@@ -49,6 +49,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
+// c + lo + hi of a pair of bf16, in float32 (one instruction on gfx950).
+__device__ __forceinline__ float add_bf16_pair(uint32_t two, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}, c, false);
+}
+
 // max / sum with the lane 32 (16) lanes away, in one instruction each.
 __device__ __forceinline__ float max_across32(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

@@ -12,7 +12,7 @@
 // every 16 lanes).
 //
 // A wave's tile of heads of 128 is 32 products of 32 cycles (16 for heads of 64) and about 200
-// vector instructions, an exponential, a multiply-add, an addition and half a maximum for every score,
+// vector instructions, an exponential, a multiply-add and half a maximum, rounding and sum for every score,
 // that issue between them; both pipes together bound it: 0.84 us a tile where a wave has its
 // SIMD to itself, 0.92 for two tiles of two waves (64: 0.6 either way).  That is 1.07 to 1.16
 // PFLOP/s over 8192 causal tokens of 32 heads (a library product of 8192^3: 1.23).  32 rows a
@@ -191,18 +191,27 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   };
   auto weights = [&](const f32x16 (&s)[KT], bf16x8 (&p)[2 * KT]) {
     const float mu = st.m == kNegInf ? 0.0f : st.m;
+    u32x4 w[2 * KT];
 #pragma unroll
     for (int s4 = 0; s4 < 2 * KT; ++s4) {
-      float e[8];
+      // p to bf16: at most 2^-8 of each, of random sign over the keys, next to the output's own
+      // rounding of 2^-8.  As the sum of two bf16, with two products each, 8192 tokens of 32 heads of 128
+      // take 695 instead of 488 us, 16 prompts of 5375 tokens together 37 instead of 25.5.
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + i] * c2 - mu);
-        st.l += e[i];
-      }
-      // p to bf16: at most 2^-8 of each, of random sign over the keys, next to the
-      // output's own rounding of 2^-8
-      p[s4] = as_bf16x8(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
+      for (int i = 0; i < 4; ++i)
+        w[s4][i] = pack_bf16(__builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i] * c2 - mu),
+                             __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu));
+      p[s4] = as_bf16x8(w[s4]);
     }
+    // the sum is that of the rounded weights, which the product uses: a row whose visible values are all the
+    // same gives that value (8192 tokens 470 -> 474 us; the rounded weights added one by one 4.5 % more than the
+    // unrounded ones)
+    float sum[4];
+#pragma unroll
+    for (int s4 = 0; s4 < 2 * KT; ++s4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = add_bf16_pair(w[s4][i], s4 == 0 ? 0.0f : sum[i]);
+    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
   auto values = [&](const char* vl, const bf16x8 (&p)[2 * KT]) {
 #pragma unroll
@@ -235,19 +244,19 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
     for (int i = 0; i < KT * KS - 4; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 24 / KS, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 40 / KS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 24 / KS, 0);
     }
 #pragma unroll
     for (int i = 0; i < KT * D / 16; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 384 / D, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 640 / D, 0);
     }
   };
   f32x16 s[KT];

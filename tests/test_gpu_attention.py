@@ -969,3 +969,30 @@ def test_paged_rows_that_need_no_bad_page(width, prefix):
     assert_within(got.cpu()[~needs], want[~needs], tol[~needs])
     if not prefix:
         assert not got[2, :2].any()
+
+
+# ------------------------------------------------------------------ the weights' sum
+def constant_values(g, dim, n, special):
+    """(q [64, 2, dim], k [n, 1, dim], v [1, 1, dim]): all keys but one score 0 and that one x, up to 8, for the first head's rows
+    (scale ln 2), a little more or less for the second's.  Its weight is 2^x beside the others' 1, so the reference point of the exponentials
+    stays where they have put it."""
+    v = normal(g, 1, 1, dim)
+    v[..., :8] = torch.tensor([1.9921875, 1.0, 1.0078125, 1.984375, -1.9921875, 255.0, 0.49609375, 3.984375])
+    k = torch.zeros(n, 1, dim, dtype=BF16)
+    k[special, 0, 0] = 1.0
+    q = torch.zeros(64, 2, dim, dtype=BF16)
+    q[:, 0, 0] = torch.linspace(0.1, 7.9, 64).to(BF16)
+    q[:, 1] = normal(g, 64, dim) * 0.2
+    return q, k, v
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,special", [(65, 64), (200, 128), (700, 650)])
+def test_prompt_gives_constant_values_as_they_are(dim, n, special):
+    """Where every visible value is the same, so is the result, bit for bit, whatever the weights: their sum is that of
+    the weights as the product uses them.  (Sums in float32 are off by less than 2 n 2^-24, far below the half step of
+    2^-9 that would change a bf16.)"""
+    q, k, v = constant_values(gen(52), dim, n, special)
+    got = dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.expand(n, 1, dim).contiguous().to(DEV), ints([0, 64]), ints([0, n]),
+                                   causal=False, scale=math.log(2.0))
+    assert torch.equal(got.cpu(), v.expand(64, 2, dim))
