@@ -54,6 +54,7 @@ constexpr int kPgMany = 512;
 constexpr int kPgShortWaves = 8;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct PagedArgs {
   const uint16_t* q;
@@ -243,7 +244,7 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
       const int key0 = kk * kUnit + 32 * wave;
       if (key0 >= len) return;
       const bool masked = key0 + 31 > len - a.q_len;
-      bf16x8 p[RT];
+      bf16x8 p[RT], rest[RT];         // the weights: bf16, and what that rounds off
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         f32x4 x[2];
@@ -279,21 +280,26 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
           e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
           l[rt] += e[i];
         }
-        // p to bf16: relative 2^-9 each, of random sign over the keys, next to the
-        // output's own rounding of 2^-9
-        p[rt] = as_bf16x8(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
-      }
-      // keys that a row does not see, or places behind the last key (that key's values again): are all
-      // the values finite?
-      bool finite = true;
-      if (masked) {
-        uint32_t bits = 0;
+        // as the sum of two bf16: 2^-16 of each is left, far below the output's own rounding of 2^-8
+        u32x4 w, u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < VW / 2; ++i) bits |= nonfinite_bits(s.v[j][i]);
-        finite = !__any(bits != 0);
+        for (int i = 0; i < 4; ++i) {
+          w[i] = pack_bf16(e[2 * i], e[2 * i + 1]);
+          u[i] = pack_bf16(e[2 * i] - __uint_as_float(w[i] << 16), e[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+        }
+        p[rt] = as_bf16x8(w);
+        rest[rt] = as_bf16x8(u);
       }
+      // An infinite value times a weight's rest, which may be zero or negative, or the weight zero of a key that a
+      // row does not see or of a place behind the last key (that key's values again), would be NaN: are
+      // all the values finite?  The largest exponents of the pairs tell (decode_64 0.5 us more than without).
+      u16x2 largest = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < VW / 2; ++i)
+          largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, s.v[j][i] & 0x7f807f80u));
+      const bool finite = !__any(nonfinite_bits(__builtin_bit_cast(uint32_t, largest)) != 0);
       if (!finite) add_nonfinite(kk);
 #pragma unroll
       for (int t = 0; t < VW; ++t) {
@@ -305,7 +311,7 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), p[rt], o[rt][t]);
+        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), rest[rt], mfma16(as_bf16x8(w), p[rt], o[rt][t]));
       }
     };
 

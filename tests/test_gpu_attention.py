@@ -996,3 +996,34 @@ def test_prompt_gives_constant_values_as_they_are(dim, n, special):
     got = dsk_moe.prompt_attention(q.to(DEV), k.to(DEV), v.expand(n, 1, dim).contiguous().to(DEV), ints([0, 64]), ints([0, n]),
                                    causal=False, scale=math.log(2.0))
     assert torch.equal(got.cpu(), v.expand(64, 2, dim))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,special", [(65, 64), (200, 128), (700, 650)])
+@pytest.mark.parametrize("wide,prefix", [(False, False), (True, False), (False, True)])
+def test_paged_gives_constant_values_as_they_are(dim, n, special, wide, prefix):
+    q, k, v = constant_values(gen(53), dim, n, special)
+    pages = -(-n // 16)
+    kc = torch.zeros(pages, 1, 16, dim, dtype=BF16)
+    kc[special // 16, 0, special % 16] = k[special, 0]
+    vc = v.view(1, 1, 1, dim).expand(pages, 1, 16, dim).contiguous()
+    table = torch.zeros(64, 100 if wide else pages, dtype=I32)
+    table[:, :pages] = torch.arange(pages)
+    pre = dict(prefix=torch.arange(pages, dtype=I32).to(DEV), prefix_len=n) if prefix else {}
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints([3 if prefix else n] * 64), scale=math.log(2.0), **pre)
+    assert torch.equal(got.cpu(), v.expand(64, 2, dim))
+
+
+@pytest.mark.parametrize("heads,kv,dim,q_len,width,lens", [(8, 2, 128, 1, 40, [1, 2, 33, 500, 639]), (4, 1, 64, 2, 40, [2, 3, 33, 500, 639]),
+                                                          (4, 2, 128, 1, 400, [1, 2, 33, 500, 6000]), (40, 1, 64, 1, 400, [1, 2, 33, 500, 6000])])
+def test_paged_weights_keep_their_digits(heads, kv, dim, q_len, width, lens):
+    """Own keys: the weights enter the product with 2^-16 of each at most left out, so the result's own rounding is nearly
+    all of the error (the float32 sums as in the oracle's tolerance)."""
+    g = gen(54 + dim)
+    table, kc, vc = paged_setup(g, [-(-n // 16) for n in lens], width, 0, kv, 16, dim)
+    q = normal(g, len(lens), q_len, heads, dim)
+    got = dsk_moe.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table.to(DEV), ints(lens)).cpu().double()
+    want, tol = O.paged(q, kc, vc, table, lens)
+    # without the 2^-8 of each weight that the oracle allows
+    size = O.paged(q, kc, vc.abs(), table, lens)[0]
+    assert ((got - want).abs() <= tol - size * (2.0 ** -8 - 2.0 ** -16)).all()
