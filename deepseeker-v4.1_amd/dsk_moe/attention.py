@@ -106,7 +106,8 @@ def _out_strides(out: torch.Tensor | None, shape: tuple, dev: torch.device, what
 
 # A call's checks depend on its tensors' sizes, strides, types and devices and on its numbers alone, so what they
 # found -- a plan: the device, the entry point and its descriptors; no tensor, no address -- serves later calls of the
-# same kind.  A decode step's host work is then a third of that of checking each time (18 us a call).
+# same kind.  A number given as something else (a tensor, say, which may change) is read at every call.  A decode step's
+# host work is then a third of that of checking each time (18 us a call).
 _plans: dict[str, dict[tuple, tuple]] = {"qk": {}, "append": {}, "prompt": {}, "paged": {}}
 _MOST_PLANS = 1024
 _CONTIGUOUS = torch.contiguous_format
@@ -192,8 +193,8 @@ def _qk_plan(q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, tabl
         ko = _out_strides(k_out, k.shape, dev, "k_out")
     ks = k.stride()
     desc = _lib.QkDesc(tokens, heads, kv_heads, dim, _lib.DTYPE_BF16 if k.dtype == _BF16 else _lib.DTYPE_F32,
-                            1 if norm else 0, rot, int(rot_first), 1 if interleaved else 0, int(prefix_len), float(eps),
-                            float(mscale), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], *qo, *ko)
+                            1 if norm else 0, rot, rot_first, 1 if interleaved else 0, prefix_len, eps,
+                            mscale, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], *qo, *ko)
     lib = _lib.load()
     if v is None:
         return lib.dsk_qk_norm_rope, dev, ctypes.byref(desc), None
@@ -209,6 +210,8 @@ def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tenso
     elements rot_first .. rot_first + 2 len(freq) by positions[t] * freq (``interleaved``: pairs (2i, 2i+1), otherwise (i,
     i + len(freq))), in one pass.  q and k bf16 or float32; the results bf16.  Tokens at negative positions are left out
     (their output rows are not written).  q_out / k_out may be q / k themselves."""
+    if not (type(mscale) is type(eps) is float and type(interleaved) is type(norm) is bool and type(rot_first) is int):
+        interleaved, rot_first, mscale, norm, eps = bool(interleaved), int(rot_first), float(mscale), bool(norm), float(eps)
     key = (_sig(q), _sig(k), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out),
            interleaved, rot_first, mscale, norm, eps)
     plan = _plans["qk"].get(key)
@@ -235,6 +238,10 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, position
     positions[t] - prefix_len of sequence seq[t] (int32), whose pages are table[seq[t]].  Returns q's result; the keys
     are also written to ``k_out`` if given.  Tokens outside the table or with a page outside the cache are not kept; two
     tokens of one call must not share a row."""
+    if not (type(mscale) is type(eps) is float and type(interleaved) is type(norm) is bool and type(rot_first) is int):
+        interleaved, rot_first, mscale, norm, eps = bool(interleaved), int(rot_first), float(mscale), bool(norm), float(eps)
+    if type(prefix_len) is not int:
+        prefix_len = int(prefix_len)
     key = (_sig(q), _sig(k), _sig(v), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out),
            _sig(seq), _sig(table), _sig(k_cache), _sig(v_cache), interleaved, rot_first, mscale, norm, eps, prefix_len)
     plan = _plans["append"].get(key)
@@ -261,7 +268,7 @@ def _prompt_plan(q, k, v, cu_q, cu_k, out, causal, scale):
     _exact(cu_q, "cu_q", _I32, n, dev)
     _exact(cu_k, "cu_k", _I32, n, dev)
     desc = _lib.PromptDesc(tokens, k.shape[0], n - 1, heads, k.shape[1], dim, 1 if causal else 0,
-                           float(scale) if scale is not None else dim ** -0.5,
+                           scale if scale is not None else dim ** -0.5,
                            *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_out_strides(out, q.shape, dev, "out"))
     return _lib.load().dsk_prompt_attention, dev, ctypes.byref(desc)
 
@@ -274,6 +281,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     head_dim ** -0.5.  Rows of ``out`` behind the last sequence are left as they were."""
     if cu_k is None:
         cu_k = cu_q
+    if type(causal) is not bool or not (scale is None or type(scale) is float):
+        causal, scale = bool(causal), float(scale) if scale is not None else None
     key = (_sig(q), _sig(k), _sig(v), _sig(cu_q), _sig(cu_k), _sig(out), causal, scale)
     plan = _plans["prompt"].get(key)
     if plan is None:
@@ -316,8 +325,8 @@ def _paged_plan(q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale
         _vector(prefix, "prefix", _I32, -(-prefix_len // k_cache.shape[2]), dev)
     if out is not None and q.dim() == 4:
         out = _token_rows(out, q_len, "out")
-    desc = _lib.PagedDesc(batch, q_len, heads, kv_heads, dim, int(prefix_len),
-                          float(scale) if scale is not None else dim ** -0.5, *rows.stride()[:2],
+    desc = _lib.PagedDesc(batch, q_len, heads, kv_heads, dim, prefix_len,
+                          scale if scale is not None else dim ** -0.5, *rows.stride()[:2],
                           *_out_strides(out, rows.shape, dev, "out"))
     cache = ctypes.byref(_cache(k_cache, table))
     n = ctypes.c_size_t(0)
@@ -334,6 +343,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``prefix_len`` keys that all sequences see first, read once for the batch.  The result has q's shape.  ``workspace``:
     uint8, 256-byte aligned, as large as ``dsk_paged_attention_workspace_size`` says, for one call at a time; otherwise
     allocated (inside a graph capture, in the graph's pool)."""
+    if type(prefix_len) is not int or not (scale is None or type(scale) is float):
+        prefix_len, scale = int(prefix_len), float(scale) if scale is not None else None
     key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(table), _sig(lens), _sig(prefix), _sig(out), prefix_len, scale)
     plan = _plans["paged"].get(key)
     if plan is None:

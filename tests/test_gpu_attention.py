@@ -1027,3 +1027,21 @@ def test_paged_weights_keep_their_digits(heads, kv, dim, q_len, width, lens):
     # without the 2^-8 of each weight that the oracle allows
     size = O.paged(q, kc, vc.abs(), table, lens)[0]
     assert ((got - want).abs() <= tol - size * (2.0 ** -8 - 2.0 ** -16)).all()
+
+
+def test_numbers_given_as_tensors_are_read_at_every_call():
+    g = gen(51)
+    q, k = normal(g, 5, 2, 64).to(DEV), normal(g, 5, 2, 64).to(DEV)
+    pos, cu, freq = torch.arange(5, dtype=I32, device=DEV), ints([0, 5]), dsk_moe.rope_frequencies(64)[0]
+    table, lens = ints([[0]]), ints([5])
+    cache = normal(g, 1, 2, 16, 64).to(DEV)
+    number = torch.tensor(1.0)
+    for x in (1.0, 0.25):
+        number.fill_(x)
+        for a, b in zip(dsk_moe.qk_norm_rope(q, k, pos, freq, mscale=number), dsk_moe.qk_norm_rope(q, k, pos, freq, mscale=x)):
+            assert torch.equal(a, b), x
+        for a, b in zip(dsk_moe.qk_norm_rope(q, k, pos, freq, eps=number), dsk_moe.qk_norm_rope(q, k, pos, freq, eps=x)):
+            assert torch.equal(a, b), x
+        assert torch.equal(dsk_moe.prompt_attention(q, k, k, cu, scale=number), dsk_moe.prompt_attention(q, k, k, cu, scale=x)), x
+        assert torch.equal(dsk_moe.paged_attention(q[:1], cache, cache, table, lens, scale=number),
+                           dsk_moe.paged_attention(q[:1], cache, cache, table, lens, scale=x)), x
