@@ -366,13 +366,29 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 # ------------------------------------------------------------------ a sublayer
 @dataclass
 class PromptStep:
-    """Whole prompts, packed: token t is at positions[t] of sequence seq[t], whose pages are table[seq[t]]; sequence s has
-    the rows cu[s] .. cu[s+1] (all int32 on the device).  Rows behind the last sequence have position -1."""
+    """Whole prompts, packed: prompt i has the rows cu[i] .. cu[i+1]; token t is at positions[t] of sequence seq[t], whose
+    pages are table[seq[t]] (all int32 on the device).  A prompt's tokens attend over its own keys alone, so its
+    positions are 0, 1, ..; rows of no prompt have position -1.  A step with other positions (a prompt's later part,
+    which would not see the keys kept before, or a prompt behind a shared prefix) is refused when it is made, by
+    one look at the device's values; inside a graph capture, and of values written later, nothing is looked at."""
 
     positions: torch.Tensor
     seq: torch.Tensor
     table: torch.Tensor
     cu: torch.Tensor
+
+    def __post_init__(self):
+        if self.positions.is_cuda and torch.cuda.is_current_stream_capturing():
+            return
+        n, t = self.cu.numel() - 1, self.positions.numel()
+        if n < 1 or t < 1:
+            return                       # the calls refuse these themselves
+        at = torch.arange(t, device=self.positions.device)
+        own = torch.searchsorted(self.cu[1:].long().contiguous(), at, right=True).clamp(max=n - 1)
+        inside = (at >= self.cu[0]) & (at < self.cu[-1])
+        whole = torch.where(inside, self.positions == at - self.cu.long()[own], self.positions < 0).all()
+        if not bool(whole & (self.cu[1:] >= self.cu[:-1]).all() & (self.cu[0] >= 0) & (self.cu[-1] <= t)):
+            raise ValueError("a PromptStep takes whole prompts: positions 0, 1, .. in the rows cu[i] .. cu[i+1], and -1 in others")
 
     def idle(self) -> PromptStep:
         """A step of the same sizes that has no sequences and keeps nothing."""

@@ -211,3 +211,14 @@ def test_oracle_attention_against_torch():
     assert torch.allclose(o, want.transpose(0, 1), atol=1e-12)
     o, _ = O.attention(q, k, v, torch.tensor([-2, -1, 0, 1, 2]), 0.25)
     assert not o[:2].any() and torch.allclose(o[2], v[0])
+
+
+def test_prompt_steps_are_whole_prompts():
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    step = lambda pos, cu: dsk_moe.PromptStep(ints(pos), ints([0] * len(pos)), ints([[0]]), ints(cu))  # noqa: E731
+    for pos, cu in (([0, 1, 2, 0, -1], [0, 3, 4]), ([0], [0, 1]), ([0, 1, 0], [0, 0, 2, 2, 3]), ([-1, -1], [0, 0])):
+        idle = step(pos, cu).idle()
+        assert idle.positions.tolist() == [-1] * len(pos) and idle.cu.tolist() == [0] * len(cu)
+    for pos, cu in (([4, 5], [0, 2]), ([0, 1, 3, 4], [0, 2, 4]), ([0, 1, 2], [0, 2]), ([0, -1], [0, 2]), ([0, 1], [0, 3]), ([0, 1], [0, 2, 1])):
+        with pytest.raises(ValueError, match="whole prompts"):
+            step(pos, cu)

@@ -1045,3 +1045,22 @@ def test_numbers_given_as_tensors_are_read_at_every_call():
         assert torch.equal(dsk_moe.prompt_attention(q, k, k, cu, scale=number), dsk_moe.prompt_attention(q, k, k, cu, scale=x)), x
         assert torch.equal(dsk_moe.paged_attention(q[:1], cache, cache, table, lens, scale=number),
                            dsk_moe.paged_attention(q[:1], cache, cache, table, lens, scale=x)), x
+
+
+def test_prompt_step_of_a_part_of_a_prompt_is_refused():
+    """The sublayer's prompts attend over their own keys alone: a step that starts behind kept keys would leave those out."""
+    seq, table = ints([0, 0, 0, 1, 1, 0]), ints([[0, 1], [2, 3]])
+
+    def step(pos, cu):
+        return dsk_moe.PromptStep(ints(pos), seq, table, ints(cu))
+
+    step([0, 1, 2, 0, 1, -1], [0, 3, 5])
+    step([0, 1, 2, 0, 1, -1], [0, 0, 3, 3, 5, 5])
+    step([-1, 0, 1, 0, 1, -1], [1, 3, 5])
+    step([-1] * 6, [0, 0, 0])
+    for pos, cu in (([7, 8, 9, 0, 1, -1], [0, 3, 5]), ([0, 1, 2, 16, 17, -1], [0, 3, 5]), ([0, 2, 1, 0, 1, -1], [0, 3, 5]),
+                    ([0, 1, -1, 0, 1, -1], [0, 3, 5]), ([0, 1, 2, 0, 1, 2], [0, 3, 5]), ([0, 1, 2, 0, 1, -1], [0, 3, 6]),
+                    ([0, 1, 2, 0, 1, -1], [0, 3, 7]), ([0, 1, 2, 0, 1, -1], [0, 3, 2]), ([0, 1, 2, 0, 1, -1], [-1, 3, 5]),
+                    ([0, 1, 2, 0, 1, -1], [1, 3, 5])):
+        with pytest.raises(ValueError, match="whole prompts"):
+            step(pos, cu)
