@@ -20,24 +20,31 @@ int check_heads(const char* fn, int heads, int kv_heads, int head_dim) {
   return DSK_OK;
 }
 
+constexpr int64_t kMostStride = int64_t{1} << 40;
+
 // Strides of `what`: rows of 16-byte pieces, `unit` elements each.
 int check_strides(const char* fn, const char* what, int64_t token, int64_t head, int unit) {
-  constexpr int64_t kMost = int64_t{1} << 40;
   if (token % unit || head % unit)
     return fail(DSK_EALIGN, "%s: strides of %s (%lld, %lld) must be multiples of %d elements", fn, what,
                 static_cast<long long>(token), static_cast<long long>(head), unit);
-  if (token < 0 || head < 0 || token > kMost || head > kMost)
+  if (token < 0 || head < 0 || token > kMostStride || head > kMostStride)
     return fail(DSK_EINVAL, "%s: strides of %s (%lld, %lld) out of range", fn, what, static_cast<long long>(token),
                 static_cast<long long>(head));
   return DSK_OK;
 }
 
 // Rows that are written: no two heads or tokens may share elements.
-int check_out(const char* fn, const char* what, int64_t token, int64_t head, int heads, int head_dim) {
-  const bool inner = head >= head_dim && token >= head * (heads - 1) + head_dim;   // heads of a token together
-  const bool single = heads == 1 && token >= head_dim;
-  const bool outer = token >= head_dim && head >= token;                            // tokens of a head together
-  if (!inner && !single && !outer)
+int check_out(const char* fn, const char* what, int64_t token, int64_t head, int64_t tokens, int heads, int head_dim) {
+  const bool in_range = token >= 0 && head >= 0 && token <= kMostStride && head <= kMostStride;   // else refused below
+  bool apart = !in_range || ((tokens == 1 || token >= head_dim) && (heads == 1 || head >= head_dim));
+  if (in_range && apart && tokens > 1 && heads > 1 && token < head * (heads - 1) + head_dim) {
+    // a token's heads do not lie together: the tokens next to a distance of i heads, before and behind it
+    for (int64_t i = 1; i < heads && apart; ++i) {
+      const int64_t before = i * head / token, rest = i * head % token;
+      apart = (before >= tokens || rest >= head_dim) && (before + 1 >= tokens || token - rest >= head_dim);
+    }
+  }
+  if (!apart)
     return fail(DSK_EINVAL, "%s: rows of %s overlap (strides %lld, %lld)", fn, what, static_cast<long long>(token),
                 static_cast<long long>(head));
   return check_strides(fn, what, token, head, 8);
@@ -92,7 +99,7 @@ int check_qk(const char* fn, const dsk_qk_desc* d, const void* q, const void* k,
   const int unit = d->dtype == DSK_DTYPE_BF16 ? 8 : 4;
   int rc = d->heads ? check_strides(fn, "q", d->q_token, d->q_head, unit) : DSK_OK;
   if (!rc) rc = check_strides(fn, "k", d->k_token, d->k_head, unit);
-  if (!rc && d->heads) rc = check_out(fn, "q_out", d->qo_token, d->qo_head, d->heads, d->head_dim);
+  if (!rc && d->heads) rc = check_out(fn, "q_out", d->qo_token, d->qo_head, d->tokens, d->heads, d->head_dim);
   return rc;
 }
 
@@ -107,7 +114,7 @@ int dsk_qk_norm_rope(const dsk_qk_desc* d, const void* q, const void* k, const i
   if (rc) return rc;
   if (!k_out) return fail(DSK_EINVAL, "%s: k_out is NULL", fn);
   if (!aligned(k_out, 16)) return fail(DSK_EALIGN, "%s: k_out must be 16-byte aligned", fn);
-  rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->kv_heads, d->head_dim);
+  rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->tokens, d->kv_heads, d->head_dim);
   if (rc) return rc;
   return hip_check(launch_qk(*d, q, k, nullptr, positions, nullptr, freq, q_gamma, k_gamma, nullptr, q_out, k_out,
                              static_cast<hipStream_t>(stream)), fn);
@@ -127,7 +134,7 @@ int dsk_kv_append(const dsk_qk_desc* d, const dsk_kv_cache* cache, const void* q
   rc = check_cache(fn, cache);
   if (!rc) rc = check_cache_pointers(fn, k_cache, v_cache, table);
   if (!rc) rc = check_strides(fn, "v", d->v_token, d->v_head, d->dtype == DSK_DTYPE_BF16 ? 8 : 4);
-  if (!rc && k_out) rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->kv_heads, d->head_dim);
+  if (!rc && k_out) rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->tokens, d->kv_heads, d->head_dim);
   if (rc) return rc;
   const CacheView view = cache_view(*cache, k_cache, v_cache, table);
   return hip_check(launch_qk(*d, q, k, v, positions, seq, freq, q_gamma, k_gamma, &view, q_out, k_out,
@@ -154,7 +161,7 @@ int dsk_prompt_attention(const dsk_prompt_desc* d, const void* q, const void* k,
   rc = check_strides(fn, "q", d->q_token, d->q_head, 8);
   if (!rc) rc = check_strides(fn, "k", d->k_token, d->k_head, 8);
   if (!rc) rc = check_strides(fn, "v", d->v_token, d->v_head, 8);
-  if (!rc) rc = check_out(fn, "out", d->o_token, d->o_head, d->heads, d->head_dim);
+  if (!rc) rc = check_out(fn, "out", d->o_token, d->o_head, d->tokens, d->heads, d->head_dim);
   if (!rc && (d->k_token >= (1 << 26) || d->v_token >= (1 << 26)))
     rc = fail(DSK_EUNSUPPORTED, "%s: token strides of k and v must stay below 2^26", fn);
   if (rc) return rc;
@@ -179,7 +186,7 @@ static int check_paged(const char* fn, const dsk_paged_desc* d, const dsk_kv_cac
     return fail(DSK_EINVAL, "%s: prefix_len=%d must be in [0, 2^30)", fn, d->prefix_len);
   if (!(d->scale > 0.0f) || !isfinite(d->scale)) return fail(DSK_EINVAL, "%s: scale must be positive and finite", fn);
   rc = check_strides(fn, "q", d->q_token, d->q_head, 8);
-  if (!rc) rc = check_out(fn, "out", d->o_token, d->o_head, d->heads, d->head_dim);
+  if (!rc) rc = check_out(fn, "out", d->o_token, d->o_head, static_cast<int64_t>(d->batch) * d->q_len, d->heads, d->head_dim);
   return rc;
 }
 

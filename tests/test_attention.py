@@ -222,3 +222,45 @@ def test_prompt_steps_are_whole_prompts():
     for pos, cu in (([4, 5], [0, 2]), ([0, 1, 3, 4], [0, 2, 4]), ([0, 1, 2], [0, 2]), ([0, -1], [0, 2]), ([0, 1], [0, 3]), ([0, 1], [0, 2, 1])):
         with pytest.raises(ValueError, match="whole prompts"):
             step(pos, cu)
+
+
+def overlaps(token, head, tokens, heads, dim):
+    at = sorted(t * token + h * head for t in range(tokens) for h in range(heads))
+    return any(b - a < dim for a, b in zip(at, at[1:]))
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (1, 4), (2, 1), (2, 2), (3, 4), (10, 2), (12, 8)])
+def test_outputs_whose_rows_overlap_are_refused(tokens, heads):
+    """Every output, over strides from none to far apart, against all rows' places (a NULL input, which is looked for before or
+    behind the strides, ends the others)."""
+    d, refused = 64, 0
+    n = ctypes.c_size_t()
+    strides = [0, 8, 56, 64, 72, 96, 128, 192, 256, 264, 384, 512, 576, 640, 704, 768, 1024, 1280, 2048]
+    for token in strides:
+        for head in strides:
+            want = overlaps(token, head, tokens, heads, d)
+            refused += want
+            p = prompt_desc(tokens=tokens, heads=heads, kv_heads=heads, o_token=token, o_head=head, k_token=1 << 26)
+            with pytest.raises(_lib.DskError) as e:
+                _lib.call("dsk_prompt_attention", ctypes.byref(p), P, P, P, P, P, P, None)
+            assert ("rows of out overlap" in str(e.value)) == want, (token, head)
+            for q_len in ({1, tokens} if tokens < 10 else {1, 2}):
+                if tokens % q_len:
+                    continue
+                batch = tokens // q_len
+                g = paged_desc(batch=batch, q_len=q_len, heads=heads, kv_heads=heads, head_dim=d, o_token=token, o_head=head)
+                c = cache(n_seqs=batch)
+                if want:
+                    assert code("dsk_paged_attention_workspace_size", ctypes.byref(g), ctypes.byref(c), ctypes.byref(n)) == -1
+                else:
+                    _lib.call("dsk_paged_attention_workspace_size", ctypes.byref(g), ctypes.byref(c), ctypes.byref(n))
+            r = qk_desc(tokens=tokens, heads=heads, kv_heads=heads, head_dim=d, rot_dim=32, qo_token=token, qo_head=head)
+            with pytest.raises(_lib.DskError) as e:
+                _lib.call("dsk_qk_norm_rope", ctypes.byref(r), P, P, P, P, P, P, P, None, None)
+            assert ("rows of q_out overlap" in str(e.value)) == want, (token, head)
+            if want:
+                r = qk_desc(tokens=tokens, heads=heads, kv_heads=heads, head_dim=d, rot_dim=32, qo_token=heads * d, qo_head=d, ko_token=token,
+                            ko_head=head)
+                assert rope_code(r) == -1
+                assert code("dsk_kv_append", ctypes.byref(r), ctypes.byref(cache()), *[P] * 13, None) == -1
+    assert refused or tokens * heads == 1
