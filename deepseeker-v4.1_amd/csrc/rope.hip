@@ -21,6 +21,8 @@
 // TB/s), 4095 of 32 + 8 20 us (4.2 TB/s); a block for four tokens with the factors
 // from LDS for every head took 53 and 28 us.  Few tokens: a token's heads over
 // several waves, queries apart from keys and values, for the latency.
+#include <type_traits>
+
 #include "attn.h"
 
 namespace dsk {
@@ -64,8 +66,8 @@ struct Raw8 {
 };
 
 // A lane's part of a head row: elements e .. e + 7 of 8 lanes (D 64) or 16 (D 128).  kAll: a
-// wave takes all heads of its token.
-template <int D, bool kBF16, bool kInter, bool kAll>
+// wave takes all heads of its token.  kPast: queries and rows of the cache are written past L2.
+template <int D, bool kBF16, bool kInter, bool kAll, bool kPast>
 __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a head row, rows of a wave
   __shared__ float2 turns[kQkWaves][D / 2];
@@ -166,12 +168,8 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
     return u32x4{pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]), pack_bf16(z[4], z[5]), pack_bf16(z[6], z[7])};
   };
 
-  // Many tokens write more than L2 holds, past it: 8192 of 32 + 8 + 8 heads of 128, each call on
-  // tensors of its own, 47.4 -> 44.7 us, 4095 of 32 + 8 27 -> 20, 2048 13.7 -> 11.5; with the attention that reads
-  // them next, 8192 tokens 522 -> 517, 2048 to 4096 within 1 %.  Few tokens' rows are read next and
-  // stay (128 to 512 tokens with their attention: 0.2 us)
   auto store = [&](uint16_t* p, const u32x4& x) {
-    if constexpr (kAll) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+    if constexpr (kPast) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
     else *reinterpret_cast<u32x4*>(p) = x;
   };
   // each wave reads its own angles alone: its LDS writes are done before
@@ -210,7 +208,7 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
     for (int i = 0; i < kQkAhead; ++i) {
       const int h = row + i * step;
       if (h >= a.kv_heads) break;
-      if (a.k_out) store(a.k_out + t * a.ko_token + h * a.ko_head + e, out[i]);
+      if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + e) = out[i];   // read many times next
       if (slot >= 0) {
         const int64_t to = (slot + (static_cast<int64_t>(h) << a.cache.page_shift)) * D + e;
         store(a.cache.k + to, out[i]);
@@ -223,11 +221,21 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   }
 }
 
+// Calls that write this many bytes write queries and rows of the cache past L2: on tensors of its own each,
+// 32 + 8 + 8 heads of 128, 512 tokens (6 MB) take 7.0 -> 6.6 us, 1024 10.6 -> 7.9, 2048 18.4 -> 16.4, 8192 49.2 -> 46.8, and with the prompt
+// attention behind them 19.8 -> 19.0, 30.6 -> 29.3, 63.1 -> 63.3, 563 -> 566; 12 + 12 + 12 of 64, 1500 tokens (6.6 MB) 8.0 -> 7.2, 26.3 ->
+// 25.5; 64 + 8 + 8 of 128, 2048 tokens 25.2 -> 23.4, 105 -> 110.  Fewer are read next and stay: 512 tokens of 16 + 4 + 4 heads
+// of 64 (1.5 MB) 5.0 either way, 14.7 -> 14.9; 256 of 12 + 12 + 12 (1.1 MB) 12.8 -> 13.0.  k_out's rows, which the attention
+// reads for every row tile, always stay: past L2 they cost it up to 16 % (3000 tokens of 12 + 12 + 12: 43.9 -> 50.5).
+constexpr int64_t kPastL2 = 4 << 20;
+
 template <int D>
 void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
   constexpr int kRows = 64 / (D / 8);
-  // few tokens: a token's heads over several waves, kQkAhead heads to a group of lanes;
-  // from 4096 waves of whole tokens on the chip is full
+  // Few tokens: a token's heads over several waves, kQkAhead heads to a group of lanes (1024 tokens, whole ones
+  // against those: 32 + 8 + 8 heads of 128 11.0 and 7.9 us, 12 + 12 + 12 of 64 7.5 and 5.9, 4 + 1 + 1 8.2 and 5.4; 2048: 15.7 and
+  // 14.7, 8.5 and 9.4, 8.3 and 9.9; 8192: 45.7 and 50.8, 28.0 and 29.1, 19.8 and 22.2).  Without queries there is little to
+  // spread (16 tokens 4.4 and 4.5, 2048 6.6 and 6.7).
   const int per = kRows * kQkAhead;
   const bool split = d.tokens < 2048 && d.heads > 0;
   const int q_parts = split ? (d.heads + per - 1) / per : 0, kv_parts = split ? (d.kv_heads + per - 1) / per : 0;
@@ -235,13 +243,21 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
   a.q_parts = q_parts;
   a.kv_parts = kv_parts;
   const dim3 grid((d.tokens + kQkWaves - 1) / kQkWaves, split ? q_parts + kv_parts : 1);
-  auto launch = [&](auto whole, auto parts) { launch_kernel(split ? parts : whole, grid, 64 * kQkWaves, 0, s, a); };
+  const int64_t rows = static_cast<int64_t>(d.tokens) * (d.heads + (a.k_out ? d.kv_heads : 0) + (a.append ? 2 * d.kv_heads : 0));
+  const bool past = rows * D * 2 >= kPastL2;
+  auto launch = [&](auto whole, auto parts, auto whole_past, auto parts_past) {
+    launch_kernel(past ? (split ? parts_past : whole_past) : (split ? parts : whole), grid, 64 * kQkWaves, 0, s, a);
+  };
+  auto form = [&](auto bf16, auto inter) {
+    constexpr bool kB = decltype(bf16)::value, kI = decltype(inter)::value;
+    launch(k_qk<D, kB, kI, true, false>, k_qk<D, kB, kI, false, false>, k_qk<D, kB, kI, true, true>, k_qk<D, kB, kI, false, true>);
+  };
   if (d.dtype == DSK_DTYPE_BF16) {
-    if (d.interleaved) launch(k_qk<D, true, true, true>, k_qk<D, true, true, false>);
-    else launch(k_qk<D, true, false, true>, k_qk<D, true, false, false>);
+    if (d.interleaved) form(std::true_type{}, std::true_type{});
+    else form(std::true_type{}, std::false_type{});
   } else {
-    if (d.interleaved) launch(k_qk<D, false, true, true>, k_qk<D, false, true, false>);
-    else launch(k_qk<D, false, false, true>, k_qk<D, false, false, false>);
+    if (d.interleaved) form(std::false_type{}, std::true_type{});
+    else form(std::false_type{}, std::false_type{});
   }
 }
 
