@@ -203,15 +203,18 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
                              __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu));
       p[s4] = as_bf16x8(w[s4]);
     }
-    // the sum is that of the rounded weights, which the product uses: a row whose visible values are all the
-    // same gives that value (8192 tokens 470 -> 474 us; the rounded weights added one by one 4.5 % more than the
-    // unrounded ones)
-    float sum[4];
+    // The sum is that of the rounded weights, which the product uses: a row whose visible values are all the
+    // same gives that value.  8192 tokens of 32 heads take 470 -> 474 us for it, six prompts of 1500 of 16
+    // 74.4 -> 76.4, shorter ones the same; the rounded weights added one by one 4.5 % more.
+    float even = 0.0f, odd = 0.0f;
 #pragma unroll
     for (int s4 = 0; s4 < 2 * KT; ++s4)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = add_bf16_pair(w[s4][i], s4 == 0 ? 0.0f : sum[i]);
-    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      for (int i = 0; i < 4; i += 2) {
+        even = add_bf16_pair(w[s4][i], even);
+        odd = add_bf16_pair(w[s4][i + 1], odd);
+      }
+    st.l += even + odd;
   };
   auto values = [&](const char* vl, const bf16x8 (&p)[2 * KT]) {
 #pragma unroll
@@ -238,25 +241,28 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   // half the keys there are few products to hide them behind (2048 tokens 22.8 -> 21.5 us; whole tiles need the
   // registers for a third wave)
   constexpr int kAhead = D == 64 && KT == 1 ? 3 : 1;
+  // vector instructions behind each of the first and of the second products (2048 tokens, 16 heads of 64: 23.8 us with 6 and
+  // 10, 22.1 with 10 and 10; 8192, 32 of 128: 498 with 3 and 4, 502 with 4 and 4)
+  constexpr int kFirst = D == 64 ? 10 : 3, kSecond = D == 64 ? 10 : 4;
   auto order = [&]() {
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
     for (int i = 0; i < KT * KS - 4; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 24 / KS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, kFirst, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 24 / KS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, kFirst, 0);
     }
 #pragma unroll
     for (int i = 0; i < KT * D / 16; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 640 / D, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, kSecond, 0);
     }
   };
   f32x16 s[KT];
