@@ -138,7 +138,10 @@ class MoEStack:
                 self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=idle)
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
-        self._step = step                # the graph reads its tensors
+        # what the graph reads and writes stays as long as the graph
+        self._step = step
+        self._caches = [(a, a.k_cache, a.v_cache) for a in self.attention or ()]
+        self._weights = [(a.w_qkv, a.w_o) for a in self.attention or ()]
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph):
             self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=step)
@@ -149,6 +152,8 @@ class MoEStack:
         returns the static output buffer."""
         if self._graph is None:
             raise RuntimeError("capture() the stack first")
+        if any(a.k_cache is not k or a.v_cache is not v for a, k, v in self._caches):
+            raise RuntimeError("an attention layer has another cache than the graph's: capture() the stack again")
         if x is not None:
             self._x.copy_(x)
         self._graph.replay()

@@ -1064,3 +1064,41 @@ def test_prompt_step_of_a_part_of_a_prompt_is_refused():
                     ([0, 1, 2, 0, 1, -1], [1, 3, 5])):
         with pytest.raises(ValueError, match="whole prompts"):
             step(pos, cu)
+
+
+def test_replay_with_another_cache_is_refused():
+    """A graph writes to the caches that its layers had: a layer's new one needs a new capture."""
+    g, stack = make_decoder(65, n=1)
+    step = dsk_moe.DecodeStep(ints([0]), ints([0]), ints([[0]]), ints([1]))
+    x = normal(g, 1, 1024).to(DEV)
+    stack.capture(1, step=step)
+    want = stack.replay(x).clone()
+    stack.attention[0].new_cache(4, 16)
+    with pytest.raises(RuntimeError, match="capture"):
+        stack.replay(x)
+    stack.capture(1, step=step)
+    assert torch.equal(stack.replay(x), want) and stack.attention[0].k_cache[0, :, 0].any()
+
+
+def test_two_captured_decoders_at_once():
+    """Two stacks' graphs replayed on two streams at the same time: each gives what it gives alone."""
+    stacks = []
+    for seed in (70, 71):
+        g, stack = make_decoder(seed)
+        for a in stack.attention:
+            for c in (a.k_cache, a.v_cache):
+                c.copy_(normal(g, *c.shape))
+        table = torch.randperm(70, generator=g)[:48].view(4, 12).to(I32).to(DEV)
+        stack.capture(4, step=dsk_moe.DecodeStep(ints([3, 100, 40, 17]), ints([0, 1, 2, 3]), table, ints([4, 101, 41, 18])))
+        x = normal(g, 4, 1024).to(DEV)
+        stacks.append((stack, x, stack.replay(x).clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for (stack, x, _), s in zip(stacks, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    stack.replay(x)
+        torch.cuda.synchronize()
+        for stack, x, want in stacks:
+            assert torch.equal(stack._out, want)
