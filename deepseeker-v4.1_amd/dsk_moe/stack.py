@@ -126,6 +126,7 @@ class MoEStack:
         the capture itself keeps nothing in the caches, whatever they hold."""
         dev = self.layers[0].gate_w.device
         hidden = self.layers[0].gate_w.shape[1]
+        self._graph = None               # an earlier graph goes with its buffers, also if this capture fails
         self._x = torch.zeros((tokens, hidden), dtype=dtype, device=dev)
         self._out = torch.empty_like(self._x)
         self._bufs = self._buffers(self._x)
@@ -142,10 +143,11 @@ class MoEStack:
         self._step = step
         self._caches = [(a, a.k_cache, a.v_cache) for a in self.attention or ()]
         self._weights = [(a.w_qkv, a.w_o) for a in self.attention or ()]
-        self._graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self._graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self.forward(self._x, out=self._out, bufs=self._bufs, ws=self._ws, step=step)
         torch.cuda.synchronize(dev)
+        self._graph = graph
 
     def replay(self, x: torch.Tensor | None = None) -> torch.Tensor:
         """Run the captured stack (on ``x`` copied into the static input if given);

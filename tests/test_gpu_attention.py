@@ -1102,3 +1102,19 @@ def test_two_captured_decoders_at_once():
         torch.cuda.synchronize()
         for stack, x, want in stacks:
             assert torch.equal(stack._out, want)
+
+
+def test_failed_capture_leaves_no_graph():
+    """A capture that raises has replaced the buffers that an earlier graph used: there is nothing to replay then."""
+    g, stack = make_decoder(66, n=1)
+    step = dsk_moe.DecodeStep(ints([0]), ints([0]), ints([[0]]), ints([1]))
+    x = normal(g, 1, 1024).to(DEV)
+    stack.capture(1, step=step)
+    want = stack.replay(x).clone()
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError):
+        stack.capture(2, step=step)                              # two rows for one sequence
+    with pytest.raises(RuntimeError, match="capture"):
+        stack.replay()
+    stack.capture(1, step=step)
+    assert torch.equal(stack.replay(x), want)
