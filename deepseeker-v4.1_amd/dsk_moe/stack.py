@@ -69,6 +69,8 @@ class MoEStack:
             raise ValueError("a stack needs at least one layer")
         if attention is not None and len(attention) != len(layers):
             raise ValueError(f"{len(attention)} attention sublayers for {len(layers)} layers")
+        if attention_gammas is not None and (attention is None or len(attention_gammas) != len(layers)):
+            raise ValueError("attention_gammas: one for each of the attention sublayers")
         self.attention = list(attention) if attention is not None else None
         self.attention_gammas = attention_gammas if attention_gammas is not None else [None] * len(layers)
         self.layers, self.eps = list(layers), float(eps)
@@ -118,7 +120,7 @@ class MoEStack:
     __call__ = forward
 
     def capture(self, tokens: int, dtype: torch.dtype = torch.bfloat16, warmup: int = 2,
-                step: DecodeStep | None = None) -> None:
+                step: PromptStep | DecodeStep | None = None) -> None:
         """Record the stack for ``tokens`` rows as one HIP graph (static input / output
         buffers).  The graph owns its workspace (sized for the largest layer), so
         later eager calls of any size, or other captures, cannot move it.  With

@@ -1118,3 +1118,35 @@ def test_failed_capture_leaves_no_graph():
         stack.replay()
     stack.capture(1, step=step)
     assert torch.equal(stack.replay(x), want)
+
+
+def test_captured_prompts_of_the_stack():
+    """A prompt step captured: nothing is kept by the capture; replays follow the step's tensors, against the eager stack."""
+    g, stack = make_decoder(67)
+    caches = [c for a in stack.attention for c in (a.k_cache, a.v_cache)]
+    table = torch.randperm(60, generator=g)[:24].view(2, 12).to(I32).to(DEV)
+    step = dsk_moe.PromptStep(ints(list(range(20)) + [-1] * 20), ints([0] * 20 + [1] * 20), table, ints([0, 20, 20]))
+    stack.capture(40, step=step)
+    torch.cuda.synchronize()
+    assert not any(c.any() for c in caches)
+    for a, b in ((20, 20), (1, 30), (37, 0)):
+        step.positions.copy_(ints(list(range(a)) + list(range(b)) + [-1] * (40 - a - b)))
+        step.seq.copy_(ints([0] * a + [1] * (40 - a)))
+        step.cu.copy_(ints([0, a, a + b]))
+        x = normal(g, 40, 1024).to(DEV)
+        for c in caches:
+            c.zero_()
+        got = stack.replay(x).clone()
+        torch.cuda.synchronize()
+        held = [c.clone() for c in caches]
+        for c in caches:
+            c.zero_()
+        want = stack(x, step=step)
+        assert torch.equal(got, want) and all(torch.equal(c, h) for c, h in zip(caches, held))
+
+
+def test_decoder_refuses_gammas_without_their_sublayers():
+    g, stack = make_decoder(68, n=2)
+    for kw in (dict(attention_gammas=stack.attention_gammas), dict(attention=stack.attention, attention_gammas=stack.attention_gammas[:1])):
+        with pytest.raises(ValueError, match="attention_gammas"):
+            dsk_moe.MoEStack(stack.layers, **kw)
