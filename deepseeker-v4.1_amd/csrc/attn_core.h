@@ -11,7 +11,7 @@
 // operand, comes from LDS with transposing reads (four keys by 16 elements in
 // every 16 lanes).
 //
-// A wave's tile of heads of 128 is 32 products of 32 cycles (16 for heads of 64) and about 200
+// A wave's tile of heads of 128 is 32 products of 32 cycles (16 for heads of 64) and about 140
 // vector instructions, an exponential, a multiply-add and half a maximum, rounding and sum for every score,
 // that issue between them; both pipes together bound it: 0.84 us a tile where a wave has its
 // SIMD to itself, 0.92 for two tiles of two waves (64: 0.6 either way).  That is 1.07 to 1.16

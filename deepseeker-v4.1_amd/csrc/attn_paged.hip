@@ -4,8 +4,8 @@
 //
 // The M = q_len * heads / kv_heads query rows that share a key head are the
 // columns of 16-wide MFMA tiles; each 32 keys of a wave cost 2 D/32 products
-// for K q^T and D/16 for V^T p^T and 4 D bytes of cache per key, so the stream
-// of the cache bounds the kernel and everything else has to stay out of its
+// for K q^T and 2 D/16 for V^T p^T (p as two bf16) and 4 D bytes of cache per key, so the
+// stream of the cache bounds the kernel and everything else has to stay out of its
 // way: K and V go straight into registers (no LDS, no barrier in the loop).
 //
 // S^T = K q^T comes out with a query row in every lane (column lane & 15) and

@@ -5,7 +5,7 @@
 // short prompt of a few tokens fills a tile with its heads, and the causal edge
 // crosses few keys of a tile.
 //
-// 8192 tokens of 32 + 8 heads of 128 take 473 to 515 us (1.16 to 1.07 PFLOP/s, by the
+// 8192 tokens of 32 + 8 heads of 128 take 474 to 515 us (1.16 to 1.07 PFLOP/s, by the
 // card), bound by the products and the vector work beside them (flash).  16 ragged prompts
 // of 5375 tokens together, 16 + 4 heads of 64, take 25.7 us of which the machine's
 // work is 13: the longest prompt's last rows are 24 tiles in a row, and a CU that

@@ -59,7 +59,9 @@ def attention(q, k, v, last, scale):
     """(o, tol) of q [Lq, heads, D] over k, v [Lk, kv heads, D]; query i sees the keys 0..last[i] (none: zeros).
 
     Roundings: p (the weight before normalisation) to bf16, 2^-8 of each term; the scores' sums of D products and
-    the sums over the keys in float32, at most n and D steps of them; the result to bf16."""
+    the sums over the keys in float32, at most n and D steps of them; the result to bf16.  Where the kernels divide by the
+    sum of the rounded weights, a term's rounding counts with |v - o| instead of |v|: less, but where nearly all of the value is
+    that of keys of little weight, and all roundings fall the worst way, up to o's half step more."""
     q, k, v = q.to(F64), k.to(F64), v.to(F64)
     heads, kv = q.shape[1], k.shape[1]
     o, tol = torch.zeros_like(q), torch.zeros_like(q)
