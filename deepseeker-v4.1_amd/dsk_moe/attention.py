@@ -371,7 +371,8 @@ class PromptStep:
     pages are table[seq[t]] (all int32 on the device).  A prompt's tokens attend over its own keys alone, so its
     positions are 0, 1, ..; rows of no prompt have position -1.  A step with other positions (a prompt's later part,
     which would not see the keys kept before, or a prompt behind a shared prefix) is refused when it is made, by
-    one look at the device's values (40 us, 65 for 8192 tokens); inside a graph capture, and of values written later, nothing is looked at."""
+    one look at the device's values (40 us, 65 for 8192 tokens); inside a graph capture, and of values written
+    later, nothing is looked at."""
 
     positions: torch.Tensor
     seq: torch.Tensor
