@@ -143,6 +143,7 @@ class MoEStack:
         torch.cuda.synchronize(dev)
         # what the graph reads and writes stays as long as the graph
         self._step = step
+        self._places = [(k, v) for k, v in vars(step).items() if isinstance(v, torch.Tensor)] if step is not None else []
         self._caches = [(a, a.k_cache, a.v_cache) for a in self.attention or ()]
         self._weights = [(a.w_qkv, a.w_o) for a in self.attention or ()]
         graph = torch.cuda.CUDAGraph()
@@ -158,6 +159,8 @@ class MoEStack:
             raise RuntimeError("capture() the stack first")
         if any(a.k_cache is not k or a.v_cache is not v for a, k, v in self._caches):
             raise RuntimeError("an attention layer has another cache than the graph's: capture() the stack again")
+        if any(getattr(self._step, k) is not v for k, v in self._places):
+            raise RuntimeError("the step has other tensors than the graph's: write into those, or capture() the stack again")
         if x is not None:
             self._x.copy_(x)
         self._graph.replay()

@@ -1150,3 +1150,21 @@ def test_decoder_refuses_gammas_without_their_sublayers():
     for kw in (dict(attention_gammas=stack.attention_gammas), dict(attention=stack.attention, attention_gammas=stack.attention_gammas[:1])):
         with pytest.raises(ValueError, match="attention_gammas"):
             dsk_moe.MoEStack(stack.layers, **kw)
+
+
+def test_replay_of_a_step_with_other_tensors_is_refused():
+    """A graph reads the tensors that its step had: new ones in the step would not be seen."""
+    g, stack = make_decoder(69, n=1)
+    step = dsk_moe.DecodeStep(ints([0]), ints([0]), ints([[0]]), ints([1]))
+    x = normal(g, 1, 1024).to(DEV)
+    stack.capture(1, step=step)
+    stack.replay(x)
+    held = step.positions
+    step.positions = step.positions + 1
+    with pytest.raises(RuntimeError, match="other tensors"):
+        stack.replay(x)
+    step.positions = held
+    held += 1
+    step.lens += 1
+    got = stack.replay(x).clone()
+    assert torch.equal(got, stack(x, step=step))
