@@ -72,14 +72,34 @@ __device__ __forceinline__ float sum_across16(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// What a call has beside the plain ones' arguments: positions on several axes (axis: of each pair), the
+// tokens' rows in the cache, the cache's scales and its keys' weights.
+struct QkMore {
+  const int32_t *axis = nullptr, *rows = nullptr;
+  int64_t axis_stride = 0;
+  int32_t n_axes = 1;
+  uint8_t *k_scale = nullptr, *v_scale = nullptr;
+  float* key_weights = nullptr;
+};
 hipError_t launch_qk(const dsk_qk_desc& d, const void* q, const void* k, const void* v, const int32_t* positions,
                      const int32_t* seq, const double* freq, const float* q_gamma, const float* k_gamma,
-                     const CacheView* cache, void* q_out, void* k_out, hipStream_t s);   // cache: null, no append
+                     const CacheView* cache, const QkMore& more, void* q_out, void* k_out,
+                     hipStream_t s);   // cache: null, no append
 
+// What a decode step's cache has beside its rows (f8: scales, weigh: its keys' weights).
+struct PagedMore {
+  bool f8 = false, weigh = false;
+  const uint8_t *k_scale = nullptr, *v_scale = nullptr;
+  float* key_weights = nullptr;
+};
 // Workspace of dsk_paged_attention, in bytes.
-size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c);
-hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const void* q, const CacheView& view,
+size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more);
+hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more, const void* q, const CacheView& view,
                         const int32_t* lens, const int32_t* prefix, void* out, void* ws, hipStream_t s);
+// Workspace of dsk_kv_evict, in bytes (codes: a cache in 8 bits).
+size_t evict_workspace(const dsk_evict_desc& d, const dsk_kv_cache& c, bool codes);
+hipError_t launch_evict(const dsk_evict_desc& d, const dsk_kv_cache& c, const CacheView& view, uint8_t* k_scale, uint8_t* v_scale,
+                        float* weights, const int32_t* lens, int32_t* lens_out, void* ws, hipStream_t s);
 hipError_t launch_prompt(const dsk_prompt_desc& d, const void* q, const void* k, const void* v, const int32_t* cu_q,
                          const int32_t* cu_k, void* out, hipStream_t s);
 

@@ -103,28 +103,43 @@ int check_qk(const char* fn, const dsk_qk_desc* d, const void* q, const void* k,
   return rc;
 }
 
-}  // namespace
+int check_axes(const char* fn, const dsk_qk_desc& d, const dsk_rope_axes& axes, QkMore& more) {
+  if (axes.n_axes < 1 || axes.n_axes > 8) return fail(DSK_EINVAL, "%s: n_axes=%d must be in [1, 8]", fn, axes.n_axes);
+  if (!axes.axis) return fail(DSK_EINVAL, "%s: axis is NULL", fn);
+  if (!aligned(axes.axis, 4)) return fail(DSK_EALIGN, "%s: axis must be 4-byte aligned", fn);
+  if (d.rot_dim == 0) return fail(DSK_EINVAL, "%s: axes without a rotation", fn);
+  if (axes.axis_stride < (axes.n_axes > 1 ? d.tokens : 0) || axes.axis_stride > kMostStride)
+    return fail(DSK_EINVAL, "%s: axis_stride=%lld must be at least tokens=%d, and in range", fn, static_cast<long long>(axes.axis_stride), d.tokens);
+  more.axis = axes.axis;
+  more.axis_stride = axes.axis_stride;
+  more.n_axes = axes.n_axes;
+  return DSK_OK;
+}
 
-extern "C" {
+int check_extra(const char* fn, const dsk_kv_extra& x) {
+  if (!x.k_scale != !x.v_scale) return fail(DSK_EINVAL, "%s: k_scale and v_scale go together", fn);
+  if (!aligned(x.key_weights, 4)) return fail(DSK_EALIGN, "%s: key_weights must be 4-byte aligned", fn);
+  return DSK_OK;
+}
 
-int dsk_qk_norm_rope(const dsk_qk_desc* d, const void* q, const void* k, const int32_t* positions, const double* freq,
-                     const float* q_gamma, const float* k_gamma, void* q_out, void* k_out, void* stream) {
-  const char* fn = "dsk_qk_norm_rope";
+int norm_rope(const char* fn, const dsk_qk_desc* d, const dsk_rope_axes* axes, const void* q, const void* k, const int32_t* positions,
+              const double* freq, const float* q_gamma, const float* k_gamma, void* q_out, void* k_out, void* stream) {
   int rc = check_qk(fn, d, q, k, positions, freq, q_gamma, k_gamma, q_out);
+  QkMore more;
+  if (!rc && axes) rc = check_axes(fn, *d, *axes, more);
   if (rc) return rc;
   if (!k_out) return fail(DSK_EINVAL, "%s: k_out is NULL", fn);
   if (!aligned(k_out, 16)) return fail(DSK_EALIGN, "%s: k_out must be 16-byte aligned", fn);
   rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->tokens, d->kv_heads, d->head_dim);
   if (rc) return rc;
-  return hip_check(launch_qk(*d, q, k, nullptr, positions, nullptr, freq, q_gamma, k_gamma, nullptr, q_out, k_out,
+  return hip_check(launch_qk(*d, q, k, nullptr, positions, nullptr, freq, q_gamma, k_gamma, nullptr, more, q_out, k_out,
                              static_cast<hipStream_t>(stream)), fn);
 }
 
-int dsk_kv_append(const dsk_qk_desc* d, const dsk_kv_cache* cache, const void* q, const void* k, const void* v,
-                  const int32_t* positions, const int32_t* seq, const double* freq, const float* q_gamma,
-                  const float* k_gamma, void* k_cache, void* v_cache, const int32_t* table, void* q_out, void* k_out,
-                  void* stream) {
-  const char* fn = "dsk_kv_append";
+int append(const char* fn, const dsk_qk_desc* d, const dsk_kv_cache* cache, const dsk_rope_axes* axes, const dsk_kv_extra* extra,
+           const void* q, const void* k, const void* v, const int32_t* positions, const int32_t* seq, const int32_t* rows,
+           const double* freq, const float* q_gamma, const float* k_gamma, void* k_cache, void* v_cache, const int32_t* table,
+           void* q_out, void* k_out, void* stream) {
   int rc = check_qk(fn, d, q, k, positions, freq, q_gamma, k_gamma, q_out);
   if (rc) return rc;
   if (!v || !seq) return fail(DSK_EINVAL, "%s: v or seq is NULL", fn);
@@ -135,10 +150,54 @@ int dsk_kv_append(const dsk_qk_desc* d, const dsk_kv_cache* cache, const void* q
   if (!rc) rc = check_cache_pointers(fn, k_cache, v_cache, table);
   if (!rc) rc = check_strides(fn, "v", d->v_token, d->v_head, d->dtype == DSK_DTYPE_BF16 ? 8 : 4);
   if (!rc && k_out) rc = check_out(fn, "k_out", d->ko_token, d->ko_head, d->tokens, d->kv_heads, d->head_dim);
+  QkMore more;
+  if (!rc && axes) rc = check_axes(fn, *d, *axes, more);
+  if (!rc && extra) rc = check_extra(fn, *extra);
   if (rc) return rc;
+  if (rows && d->prefix_len) return fail(DSK_EINVAL, "%s: rows are given, so prefix_len=%d must be 0", fn, d->prefix_len);
+  if (!aligned(rows, 4)) return fail(DSK_EALIGN, "%s: rows must be 4-byte aligned", fn);
+  more.rows = rows;
+  if (extra) {
+    more.k_scale = extra->k_scale;
+    more.v_scale = extra->v_scale;
+    more.key_weights = extra->key_weights;
+  }
   const CacheView view = cache_view(*cache, k_cache, v_cache, table);
-  return hip_check(launch_qk(*d, q, k, v, positions, seq, freq, q_gamma, k_gamma, &view, q_out, k_out,
+  return hip_check(launch_qk(*d, q, k, v, positions, seq, freq, q_gamma, k_gamma, &view, more, q_out, k_out,
                              static_cast<hipStream_t>(stream)), fn);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsk_qk_norm_rope(const dsk_qk_desc* d, const void* q, const void* k, const int32_t* positions, const double* freq,
+                     const float* q_gamma, const float* k_gamma, void* q_out, void* k_out, void* stream) {
+  return norm_rope("dsk_qk_norm_rope", d, nullptr, q, k, positions, freq, q_gamma, k_gamma, q_out, k_out, stream);
+}
+
+int dsk_qk_norm_rope_axes(const dsk_qk_desc* d, const dsk_rope_axes* axes, const void* q, const void* k, const int32_t* positions,
+                          const double* freq, const float* q_gamma, const float* k_gamma, void* q_out, void* k_out,
+                          void* stream) {
+  const char* fn = "dsk_qk_norm_rope_axes";
+  if (!axes) return fail(DSK_EINVAL, "%s: axes is NULL", fn);
+  return norm_rope(fn, d, axes, q, k, positions, freq, q_gamma, k_gamma, q_out, k_out, stream);
+}
+
+int dsk_kv_append(const dsk_qk_desc* d, const dsk_kv_cache* cache, const void* q, const void* k, const void* v,
+                  const int32_t* positions, const int32_t* seq, const double* freq, const float* q_gamma,
+                  const float* k_gamma, void* k_cache, void* v_cache, const int32_t* table, void* q_out, void* k_out,
+                  void* stream) {
+  return append("dsk_kv_append", d, cache, nullptr, nullptr, q, k, v, positions, seq, nullptr, freq, q_gamma, k_gamma, k_cache,
+                v_cache, table, q_out, k_out, stream);
+}
+
+int dsk_kv_append_extra(const dsk_qk_desc* d, const dsk_kv_cache* cache, const dsk_rope_axes* axes, const dsk_kv_extra* extra,
+                        const void* q, const void* k, const void* v, const int32_t* positions, const int32_t* seq,
+                        const int32_t* rows, const double* freq, const float* q_gamma, const float* k_gamma, void* k_cache,
+                        void* v_cache, const int32_t* table, void* q_out, void* k_out, void* stream) {
+  return append("dsk_kv_append_extra", d, cache, axes, extra, q, k, v, positions, seq, rows, freq, q_gamma, k_gamma, k_cache,
+                v_cache, table, q_out, k_out, stream);
 }
 
 int dsk_prompt_attention(const dsk_prompt_desc* d, const void* q, const void* k, const void* v, const int32_t* cu_q,
@@ -190,19 +249,35 @@ static int check_paged(const char* fn, const dsk_paged_desc* d, const dsk_kv_cac
   return rc;
 }
 
-int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, size_t* bytes) {
-  const char* fn = "dsk_paged_attention_workspace_size";
+static int paged_more(const char* fn, const dsk_kv_extra* extra, PagedMore& more) {
+  if (!extra) return fail(DSK_EINVAL, "%s: extra is NULL", fn);
+  const int rc = check_extra(fn, *extra);
+  more = PagedMore{extra->k_scale != nullptr, extra->key_weights != nullptr, extra->k_scale, extra->v_scale, extra->key_weights};
+  return rc;
+}
+
+static int paged_workspace_size(const char* fn, const dsk_paged_desc* d, const dsk_kv_cache* cache, const PagedMore& more, size_t* bytes) {
   int rc = check_paged(fn, d, cache);
   if (rc) return rc;
   if (!bytes) return fail(DSK_EINVAL, "%s: bytes is NULL", fn);
-  *bytes = paged_workspace(*d, *cache);
+  *bytes = paged_workspace(*d, *cache, more);
   return DSK_OK;
 }
 
-int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, const void* q, const void* k_cache,
-                        const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix,
-                        void* out, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "dsk_paged_attention";
+int dsk_paged_attention_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, size_t* bytes) {
+  return paged_workspace_size("dsk_paged_attention_workspace_size", d, cache, PagedMore{}, bytes);
+}
+
+int dsk_paged_attention_extra_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, size_t* bytes) {
+  const char* fn = "dsk_paged_attention_extra_workspace_size";
+  PagedMore more;
+  const int rc = paged_more(fn, extra, more);
+  return rc ? rc : paged_workspace_size(fn, d, cache, more, bytes);
+}
+
+static int paged(const char* fn, const dsk_paged_desc* d, const dsk_kv_cache* cache, const PagedMore& more, const void* q,
+                 const void* k_cache, const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix, void* out,
+                 void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_paged(fn, d, cache);
   if (rc) return rc;
   rc = check_cache_pointers(fn, k_cache, v_cache, table);
@@ -212,10 +287,71 @@ int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, cons
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 256))
     return fail(DSK_EALIGN, "%s: q and out must be 16-byte, the workspace 256-byte aligned", fn);
   if (!aligned(lens, 4) || !aligned(prefix, 4)) return fail(DSK_EALIGN, "%s: lens and prefix must be 4-byte aligned", fn);
-  if (workspace_bytes < paged_workspace(*d, *cache))
-    return fail(DSK_ESPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, paged_workspace(*d, *cache));
+  const size_t need = paged_workspace(*d, *cache, more);
+  if (workspace_bytes < need) return fail(DSK_ESPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, need);
   const CacheView view = cache_view(*cache, const_cast<void*>(k_cache), const_cast<void*>(v_cache), table);
-  return hip_check(launch_paged(*d, *cache, q, view, lens, prefix, out, workspace, static_cast<hipStream_t>(stream)), fn);
+  return hip_check(launch_paged(*d, *cache, more, q, view, lens, prefix, out, workspace, static_cast<hipStream_t>(stream)), fn);
+}
+
+int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, const void* q, const void* k_cache,
+                        const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix,
+                        void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  return paged("dsk_paged_attention", d, cache, PagedMore{}, q, k_cache, v_cache, table, lens, prefix, out, workspace, workspace_bytes,
+               stream);
+}
+
+int dsk_paged_attention_extra(const dsk_paged_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, const void* q,
+                              const void* k_cache, const void* v_cache, const int32_t* table, const int32_t* lens,
+                              const int32_t* prefix, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "dsk_paged_attention_extra";
+  PagedMore more;
+  const int rc = paged_more(fn, extra, more);
+  return rc ? rc : paged(fn, d, cache, more, q, k_cache, v_cache, table, lens, prefix, out, workspace, workspace_bytes, stream);
+}
+
+static int check_evict(const char* fn, const dsk_evict_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra) {
+  if (!d) return fail(DSK_EINVAL, "%s: desc is NULL", fn);
+  if (!extra) return fail(DSK_EINVAL, "%s: extra is NULL", fn);
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return fail(DSK_EUNSUPPORTED, "%s: head_dim=%d, 64 and 128 are built", fn, d->head_dim);
+  if (d->kv_heads < 1 || d->kv_heads > 1024) return fail(DSK_EINVAL, "%s: kv_heads=%d must be in [1, 1024]", fn, d->kv_heads);
+  int rc = check_cache(fn, cache);
+  if (!rc) rc = check_extra(fn, *extra);
+  if (rc) return rc;
+  if (d->keep < 1 || d->first < 0 || d->recent < 0 || static_cast<int64_t>(d->first) + d->recent > d->keep)
+    return fail(DSK_EINVAL, "%s: keep=%d must be >= 1 and hold first=%d and recent=%d, both >= 0", fn, d->keep, d->first, d->recent);
+  // a launch counts its threads in 32 bits, 1024 for an item
+  if (static_cast<int64_t>(cache->n_seqs) * d->kv_heads >= (1 << 22))
+    return fail(DSK_EUNSUPPORTED, "%s: sequences * kv_heads must stay below 2^22", fn);
+  return DSK_OK;
+}
+
+int dsk_kv_evict_workspace_size(const dsk_evict_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, size_t* bytes) {
+  const char* fn = "dsk_kv_evict_workspace_size";
+  const int rc = check_evict(fn, d, cache, extra);
+  if (rc) return rc;
+  if (!bytes) return fail(DSK_EINVAL, "%s: bytes is NULL", fn);
+  *bytes = evict_workspace(*d, *cache, extra->k_scale != nullptr);
+  return DSK_OK;
+}
+
+int dsk_kv_evict(const dsk_evict_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, void* k_cache, void* v_cache,
+                 const int32_t* table, const int32_t* lens, int32_t* lens_out, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  const char* fn = "dsk_kv_evict";
+  int rc = check_evict(fn, d, cache, extra);
+  if (!rc) rc = check_cache_pointers(fn, k_cache, v_cache, table);
+  if (rc) return rc;
+  if (!extra->key_weights || !lens || !lens_out || !workspace) return fail(DSK_EINVAL, "%s: NULL pointer argument", fn);
+  if (!aligned(lens, 4) || !aligned(lens_out, 4)) return fail(DSK_EALIGN, "%s: lens and lens_out must be 4-byte aligned", fn);
+  if (!aligned(workspace, 256)) return fail(DSK_EALIGN, "%s: the workspace must be 256-byte aligned", fn);
+  if (lens_out != lens && lens_out < lens + cache->n_seqs && lens < lens_out + cache->n_seqs)
+    return fail(DSK_EINVAL, "%s: lens_out overlaps lens", fn);
+  const size_t need = evict_workspace(*d, *cache, extra->k_scale != nullptr);
+  if (workspace_bytes < need) return fail(DSK_ESPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, need);
+  const CacheView view = cache_view(*cache, k_cache, v_cache, table);
+  return hip_check(launch_evict(*d, *cache, view, extra->k_scale, extra->v_scale, extra->key_weights, lens, lens_out, workspace,
+                                static_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

@@ -40,14 +40,20 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_core.h"
+#include "kv8.h"
 
 namespace dsk {
 namespace {
 
 constexpr int kPgThreads = 256;
-constexpr int kPgUnit = 128;        // keys of a unit: 32 for each of four waves
+// Keys of a wave's step: the bytes in flight are the same with codes of half the size.
+template <bool F8>
+constexpr int step_keys() { return F8 ? 64 : 32; }
+template <bool F8>
+constexpr int unit_keys() { return 4 * step_keys<F8>(); }   // keys of a unit: a step of each of four waves
 constexpr int kPgShort = 512;       // keys of a table row that one workgroup takes alone
 constexpr int kPgShortMany = 1024;  // where there are kPgMany items
 constexpr int kPgMany = 512;
@@ -71,6 +77,11 @@ struct PagedArgs {
   float c2;                         // scale * log2(e)
   int32_t batch, q_len, kv_heads, group, prefix, shares, splits;
   int32_t row_tiles, prefix_blocks; // of the prefix: tiles of all rows, workgroups
+  const uint8_t *k_scale, *v_scale; // of a cache in 8 bits
+  uint16_t *pre_k, *pre_v;          // of such a cache, the prefix's pages as bf16
+  float* weights;                   // of the cache's rows, to be added to, or null; then also:
+  float* scores;                    // [item][key of the table row][M], times c
+  float* lse;                       // [item][M]: log2 of the sum of 2^score (infinite: the row sees no key)
 };
 
 // Keys of sequence b that the cache can hold; `bad` if lens[b] claims more.
@@ -79,9 +90,10 @@ __device__ __forceinline__ int length_of(const PagedArgs& a, int b, bool& bad) {
   bad = n > cap;
   return min(max(n, 0), cap);
 }
+template <int U>
 __device__ __forceinline__ int units_of(const PagedArgs& a, int b) {
   bool bad;
-  return (length_of(a, b, bad) + kPgUnit - 1) / kPgUnit;
+  return (length_of(a, b, bad) + U - 1) / U;
 }
 
 template <int V>
@@ -104,9 +116,10 @@ __device__ __forceinline__ uint32_t sum_up_to_lane(uint32_t v) {
 // Units of one key head, 64 sequences at a time: lane's own, and up to its own.
 // Fewer than 2^31 in all, times the key heads too.
 struct Units { uint32_t own, up_to; };
+template <int U>
 __device__ __forceinline__ Units units_at(const PagedArgs& a, int b0) {
   const int b = b0 + (threadIdx.x & 63);
-  const uint32_t n = b < a.batch ? units_of(a, b) : 0;
+  const uint32_t n = b < a.batch ? units_of<U>(a, b) : 0;
   return Units{n, sum_up_to_lane(n)};
 }
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
@@ -120,23 +133,41 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int D>
-struct Step {                       // one wave's 32 keys
-  u32x4 k[2][D / 32];
-  uint32_t v[8][D / 32];            // VW = D / 16 elements of 8 keys
+template <int D, bool F8>
+struct Step {                       // one wave's keys, in tiles of 16
+  static constexpr int kTiles = step_keys<F8>() / 16, kPieces = D / (F8 ? 64 : 32);
+  u32x4 k[kTiles][kPieces];
+  uint32_t v[4 * kTiles][kPieces];  // VW = D / 16 elements of 4 keys of each
 };
 
-template <int VW>
-__device__ __forceinline__ void load_v(uint32_t (&v)[VW / 2], const uint16_t* p) {
-  if constexpr (VW == 8) {
+template <int N>
+__device__ __forceinline__ void load_v(uint32_t (&v)[N], const void* p) {
+  if constexpr (N == 4) {
     const u32x4 r = ldg16(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = r[i];
-  } else {
+  } else if constexpr (N == 2) {
     const u32x2 r = ldg<u32x2>(p);
     v[0] = r[0];
     v[1] = r[1];
+  } else {
+    v[0] = ldg<uint32_t>(p);
   }
+}
+
+// bf16 values of four keys a tile, element t of each: slots 0..3 (4..7) of a product's A operand from tile 0 (1).
+// Codes: four elements of four keys are a 4 x 4 of bytes; bytes of one element together, then to bf16.
+template <int VW>
+__device__ __forceinline__ void values_of(const uint32_t (&v)[4][VW / 4], float scale, u32x2 (&w)[VW]) {
+#pragma unroll
+  for (int i = 0; i < VW / 4; ++i)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) {
+      const uint32_t sel = hi ? 0x07030602u : 0x05010400u;
+      const uint32_t a = __builtin_amdgcn_perm(v[1][i], v[0][i], sel), b = __builtin_amdgcn_perm(v[3][i], v[2][i], sel);
+      w[4 * i + 2 * hi] = codes_to_bf16(__builtin_amdgcn_perm(b, a, 0x05040100u), scale);
+      w[4 * i + 2 * hi + 1] = codes_to_bf16(__builtin_amdgcn_perm(b, a, 0x07060302u), scale);
+    }
 }
 
 // LDS of a segment of W waves: their rows, then maxima and sums.
@@ -146,23 +177,28 @@ struct SegLds {
   float ml[W][16 * RT][2];
 };
 
-// Lane 2 i + kt: the page of the wave's 16-key tile kt in step kk + i (the table row's
+// Lane T i + kt: the page of the wave's 16-key tile kt of T in step kk + i (the table row's
 // last one behind its end; the sequence's length need not be known yet).
-template <int W>
+template <int W, int T>
 __device__ __forceinline__ int page_ids(const PagedArgs& a, int b, int kk) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t tile = (static_cast<int64_t>(kk) + (lane >> 1)) * (2 * W) + 2 * wave + (lane & 1);
+  const int64_t tile = (static_cast<int64_t>(kk) + lane / T) * (T * W) + T * wave + lane % T;
   const int page = static_cast<int>(min(tile >> (a.c.page_shift - 4), static_cast<int64_t>(a.c.max_pages - 1)));
   return ldg<int32_t>(a.c.table + b * a.c.table_stride + page);
 }
 
-// Units [k0, k1) of the keys of item (b, h), in units of 32 W keys, for the rows from
+// Units [k0, k1) of the keys of item (b, h), in units of a step of W waves, for the rows from
 // r0 on: to `out` (slot < 0: they are all of the item's) or to the partial rows of `slot`.
 // first_ids: page_ids of k0.
-template <int D, int RT, int W>
+//
+// F8: a cache in 8 bits.  A lane's piece of a key is D / 4 codes, of which product ks takes 8 (queries
+// are held in the same order), so that K too comes in 16-byte loads; a 16-key tile is a block of one scale, which the
+// conversion to bf16 applies.  kWeigh: scores are kept for k_key_weights.
+template <int D, int RT, int W, bool F8, bool kWeigh>
 __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int len, bool bad_len, int r0, int k0, int k1,
                                         int64_t slot, int first_ids, SegLds<D, RT, W>& lds) {
-  constexpr int VW = D / 16, KS = D / 32, kUnit = 32 * W;
+  using S = Step<D, F8>;
+  constexpr int VW = D / 16, KS = D / 32, kKeys = step_keys<F8>(), kUnit = kKeys * W, T = S::kTiles;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
   const int M = a.q_len * a.group;
@@ -172,10 +208,10 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = min(r0 + 16 * rt + n16, M - 1), tok = r / a.group, hd = h * a.group + r % a.group;
-      const uint16_t* p = a.q + (static_cast<int64_t>(b) * a.q_len + tok) * a.q_token + hd * a.q_head + 8 * g;
+      const uint16_t* p = a.q + (static_cast<int64_t>(b) * a.q_len + tok) * a.q_token + hd * a.q_head + (F8 ? D / 4 : 8) * g;
       lim[rt] = len - a.q_len + tok;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) q[rt][ks] = as_bf16x8(ldg16(p + 32 * ks));
+      for (int ks = 0; ks < KS; ++ks) q[rt][ks] = as_bf16x8(ldg16(p + (F8 ? 8 : 32) * ks));
     }
     f32x4 o[RT][VW];
     float m[RT], l[RT];
@@ -189,80 +225,146 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 
     const int32_t* trow = a.c.table + b * a.c.table_stride;
     const int last_tile = (len - 1) >> 4;
-    int ids = first_ids, ids0 = k0;   // lane 2 i + kt: the page of tile kt of step ids0 + i
+    int ids = first_ids, ids0 = k0;   // lane T i + kt: the page of tile kt of step ids0 + i
     int bad_tile = INT32_MAX;         // the lane's first 16 keys on a page outside the cache
+    // F8: scale bytes of the lane's tile, and those of the ids before, which a step may still need
+    uint32_t k_byte = 0, v_byte = 0, old_k_byte = 0, old_v_byte = 0;
+    int old0 = k0;
     auto check_ids = [&]() {
-      const int step = ids0 + (lane >> 1), tile = step * (2 * W) + 2 * wave + (lane & 1);
+      const int step = ids0 + lane / T, tile = step * (T * W) + T * wave + lane % T;
       const bool out_of = ids < 0 || ids >= a.c.n_pages;
       if (out_of && step < k1 && tile <= last_tile) bad_tile = min(bad_tile, tile);
       if (out_of) ids = 0;
+      if constexpr (F8) {
+        const int64_t at = ((static_cast<int64_t>(ids) * a.kv_heads + h) << (a.c.page_shift - 4)) +
+                           (tile & ((1 << (a.c.page_shift - 4)) - 1));
+        old_k_byte = k_byte;
+        old_v_byte = v_byte;
+        k_byte = ldg<uint8_t>(a.k_scale + at);
+        v_byte = ldg<uint8_t>(a.v_scale + at);
+      }
     };
     check_ids();
-    auto load = [&](Step<D>& s, int kk) {
-      if (kk - ids0 >= 32) {
+    auto load = [&](S& s, int kk) {
+      if (kk - ids0 >= 64 / T) {
+        old0 = ids0;
         ids0 = kk;
-        ids = page_ids<W>(a, b, kk);
+        ids = page_ids<W, T>(a, b, kk);
         check_ids();
       }
-      const int tile0 = kk * (2 * W) + 2 * wave;
+      const int tile0 = kk * (T * W) + T * wave;
       if (tile0 > last_tile) return;                  // none of the wave's keys in this step
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+      for (int kt = 0; kt < T; ++kt) {
         const int tile = min(tile0 + kt, last_tile);
-        const int id = __builtin_amdgcn_readlane(ids, 2 * (kk - ids0) + tile - tile0);
+        const int id = __builtin_amdgcn_readlane(ids, T * (kk - ids0) + tile - tile0);
         const int last_row = len - 1 - tile * 16;     // rows past the length: the last one again
         const int row0 = (tile * 16) & ((1 << a.c.page_shift) - 1);
         const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + row0) * D;
-        const uint16_t* kp = a.c.k + base + min(n16, last_row) * D + 8 * g;
+        if constexpr (F8) {
+          const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.c.k) + base + min(n16, last_row) * D + D / 4 * g;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s.k[kt][ks] = ldg16(kp + 32 * ks);
+          for (int i = 0; i < S::kPieces; ++i) s.k[kt][i] = ldg16(kp + 16 * i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          load_v<VW>(s.v[4 * kt + j], a.c.v + base + min(4 * g + j, last_row) * D + VW * n16);
+          for (int j = 0; j < 4; ++j)
+            load_v(s.v[4 * kt + j], reinterpret_cast<const uint8_t*>(a.c.v) + base + min(4 * g + j, last_row) * D + VW * n16);
+        } else {
+          const uint16_t* kp = a.c.k + base + min(n16, last_row) * D + 8 * g;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s.k[kt][ks] = ldg16(kp + 32 * ks);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) load_v(s.v[4 * kt + j], a.c.v + base + min(4 * g + j, last_row) * D + VW * n16);
+        }
       }
     };
     // rarely: infinite and NaN values of step kk, to the rows that see them (the
     // products then leave them out)
     auto add_nonfinite = [&](int kk) {
 #pragma unroll 1
-      for (int key = kk * kUnit + 32 * wave, end = min(key + 32, len); key < end; ++key) {
+      for (int key = kk * kUnit + kKeys * wave, end = min(key + kKeys, len); key < end; ++key) {
         int id = ldg<int32_t>(trow + (key >> a.c.page_shift));
         if (id < 0 || id >= a.c.n_pages) id = 0;
         const int in_page = key & ((1 << a.c.page_shift) - 1);
-        const uint16_t* vp = a.c.v + (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page) * D;
+        const int64_t row = ((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + in_page;
+        const bool no_scale = F8 && ldg<uint8_t>(a.v_scale + (F8 ? row / kScaleRows : 0)) > kMostScale;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int t = 0; t < VW; ++t) {
-            const float x = nonfinite_only(ldg<uint16_t>(vp + VW * (4 * g + r) + t));
+            float x;
+            if constexpr (F8) {
+              const uint32_t c = ldg<uint8_t>(reinterpret_cast<const uint8_t*>(a.c.v) + row * D + VW * (4 * g + r) + t);
+              x = no_scale || (c & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.0f;
+            } else {
+              x = nonfinite_only(ldg<uint16_t>(a.c.v + row * D + VW * (4 * g + r) + t));
+            }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) o[rt][t][r] += key <= lim[rt] ? x : 0.0f;
           }
       }
     };
-    auto compute = [&](const Step<D>& s, int kk) {
-      const int key0 = kk * kUnit + 32 * wave;
+    auto compute = [&](const S& s, int kk) {
+      const int key0 = kk * kUnit + kKeys * wave;
       if (key0 >= len) return;
-      const bool masked = key0 + 31 > len - a.q_len;
-      bf16x8 p[RT], rest[RT];         // the weights: bf16, and what that rounds off
+      const bool masked = key0 + kKeys - 1 > len - a.q_len;
+      float k_scale[T], v_scale[T];
+      bool good_scales = true;
+      if constexpr (F8) {
+        const bool old = kk < ids0;
+        const uint32_t kb = old ? old_k_byte : k_byte, vb = old ? old_v_byte : v_byte;
+        const int tile0 = key0 >> 4;
+#pragma unroll
+        for (int kt = 0; kt < T; ++kt) {
+          const int at = T * (kk - (old ? old0 : ids0)) + min(tile0 + kt, last_tile) - tile0;
+          k_scale[kt] = scale_of(lane_value(kb, at));
+          const uint32_t byte = lane_value(vb, at);
+          good_scales = good_scales && byte <= kMostScale;
+          v_scale[kt] = scale_of(byte);
+        }
+      }
+      bf16x8 p[RT][T / 2], rest[RT][T / 2];   // the weights: bf16, and what that rounds off
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        f32x4 x[2];
+        f32x4 x[T];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < T; ++kt) {
           x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) x[kt] = mfma16(as_bf16x8(s.k[kt][ks]), q[rt][ks], x[kt]);
+          for (int ks = 0; ks < KS; ++ks) {
+            u32x4 key;
+            if constexpr (F8) {
+              const u32x4 c = s.k[kt][ks / 2];
+              const u32x2 lo = codes_to_bf16(c[2 * (ks & 1)], k_scale[kt]), hi = codes_to_bf16(c[2 * (ks & 1) + 1], k_scale[kt]);
+              key = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+              key = s.k[kt][ks];
+            }
+            x[kt] = mfma16(as_bf16x8(key), q[rt][ks], x[kt]);
+          }
         }
         if (masked) {
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
+          for (int kt = 0; kt < T; ++kt)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (key0 + 16 * kt + 4 * g + r > lim[rt]) x[kt][r] = kNegInf;
         }
-        float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                          fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        if constexpr (kWeigh) {
+          const int row = r0 + 16 * rt + n16;
+          const int64_t item = static_cast<int64_t>(b) * a.kv_heads + h;
+          float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + key0) * M + row;
+          if (row < M)
+#pragma unroll
+            for (int kt = 0; kt < T; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int i = 16 * kt + 4 * g + r;
+                if (key0 + i < len) to[static_cast<int64_t>(i) * M] = x[kt][r] * a.c2;
+              }
+        }
+        float top = kNegInf;
+#pragma unroll
+        for (int kt = 0; kt < T; ++kt) top = fmaxf(top, fmaxf(fmaxf(x[kt][0], x[kt][1]), fmaxf(x[kt][2], x[kt][3])));
         top = max_across32(max_across16(top)) * a.c2;
         // the reference point follows the maximum once it lags by more than 2^8
         if (__any(top > m[rt] + 8.0f)) {
@@ -274,48 +376,80 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
           for (int t = 0; t < VW; ++t) o[rt][t] *= f;
         }
         const float mu = m[rt] == kNegInf ? 0.0f : m[rt];
-        float e[8];
+        float e[4 * T];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4 * T; ++i) {
           e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
           l[rt] += e[i];
         }
         // as the sum of two bf16: 2^-16 of each is left, far below the output's own rounding of 2^-8
-        u32x4 w, u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = pack_bf16(e[2 * i], e[2 * i + 1]);
-          u[i] = pack_bf16(e[2 * i] - __uint_as_float(w[i] << 16), e[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+        for (int hh = 0; hh < T / 2; ++hh) {
+          u32x4 w, u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e0 = e[8 * hh + 2 * i], e1 = e[8 * hh + 2 * i + 1];
+            w[i] = pack_bf16(e0, e1);
+            u[i] = pack_bf16(e0 - __uint_as_float(w[i] << 16), e1 - __uint_as_float(w[i] & 0xffff0000u));
+          }
+          p[rt][hh] = as_bf16x8(w);
+          rest[rt][hh] = as_bf16x8(u);
         }
-        p[rt] = as_bf16x8(w);
-        rest[rt] = as_bf16x8(u);
       }
       // An infinite value times a weight's rest, which may be zero or negative, or the weight zero of a key that a
       // row does not see or of a place behind the last key (that key's values again), would be NaN: are
       // all the values finite?  The largest exponents of the pairs tell (decode_64 0.5 us more than without).
-      u16x2 largest = {0, 0};
+      // Codes have no infinity, and a NaN that every row sees may go through the products: there the question is
+      // for the last keys alone.
+      bool finite = true;
+      if constexpr (F8) {
+        if (masked) {
+          uint32_t bits = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 4 * T; ++j)
 #pragma unroll
-        for (int i = 0; i < VW / 2; ++i)
-          largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, s.v[j][i] & 0x7f807f80u));
-      const bool finite = !__any(nonfinite_bits(__builtin_bit_cast(uint32_t, largest)) != 0);
+            for (int i = 0; i < S::kPieces; ++i) bits |= nan_codes(s.v[j][i]);
+          finite = good_scales && !__any(bits != 0);
+        }
+      } else {
+        u16x2 largest = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 4 * T; ++j)
+#pragma unroll
+          for (int i = 0; i < VW / 2; ++i)
+            largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, s.v[j][i] & 0x7f807f80u));
+        finite = !__any(nonfinite_bits(__builtin_bit_cast(uint32_t, largest)) != 0);
+      }
       if (!finite) add_nonfinite(kk);
 #pragma unroll
-      for (int t = 0; t < VW; ++t) {
-        const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
-        u32x4 w;
+      for (int hh = 0; hh < T / 2; ++hh) {
+        u32x2 w0[VW], w1[VW];
+        if constexpr (F8) {
+          values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[8 * hh]), v_scale[2 * hh], w0);
+          values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[8 * hh + 4]), v_scale[2 * hh + 1], w1);
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(s.v[2 * i + 1][t / 2], s.v[2 * i][t / 2], sel);
-        if (!finite)
+        for (int t = 0; t < VW; ++t) {
+          u32x4 w;
+          if constexpr (F8) {
+            w = u32x4{w0[t][0], w0[t][1], w1[t][0], w1[t][1]};
+          } else {
+            const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
+            for (int i = 0; i < 4; ++i)
+              w[i] = __builtin_amdgcn_perm(s.v[8 * hh + 2 * i + 1][t / 2], s.v[8 * hh + 2 * i][t / 2], sel);
+          }
+          if (!finite)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), rest[rt], mfma16(as_bf16x8(w), p[rt], o[rt][t]));
+            for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            o[rt][t] = mfma16(as_bf16x8(w), rest[rt][hh], mfma16(as_bf16x8(w), p[rt][hh], o[rt][t]));
+        }
       }
     };
 
-    Step<D> s0, s1;
+    S s0, s1;
     load(s0, k0);
     int kk = k0;
     for (; kk + 1 < k1; kk += 2) {
@@ -376,6 +510,8 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
           const int tok = r / a.group, hd = h * a.group + r % a.group;
           const bool sees = len - a.q_len + tok >= 0 || ll != ll;   // else no key: zeros
           const float inv = 1.0f / ll;
+          if constexpr (kWeigh)
+            if (d0 == 0) a.lse[(static_cast<int64_t>(b) * a.kv_heads + h) * M + r] = sees ? mm + log2f(ll) : -kNegInf;
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = sees ? y[i] * inv : 0.0f;
           *reinterpret_cast<u32x4*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
@@ -391,12 +527,13 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 }
 
 // Workgroup `share` of a.shares takes its share of all units.
-template <int D, int RT>
+template <int D, int RT, bool F8, bool kWeigh>
 __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, SegLds<D, RT, 4>& lds) {
+  constexpr int kUnit = unit_keys<F8>(), T = Step<D, F8>::kTiles;
   Units n;
   uint32_t all = 0;                  // units of one key head
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    n = units_at(a, b0);
+    n = units_at<kUnit>(a, b0);
     all += lane_value(n.up_to, 63);
   }
   const uint32_t total = all * a.kv_heads, quota = (total + a.shares - 1) / a.shares;
@@ -407,7 +544,7 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
   uint32_t before = 0;
   int b = a.batch;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (a.batch > 64) n = units_at(a, b0);
+    if (a.batch > 64) n = units_at<kUnit>(a, b0);
     const uint64_t past = __ballot(before + n.up_to > first_unit);
     if (past) {
       const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
@@ -420,7 +557,7 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
   for (uint32_t u = u0; u < u1 && b < a.batch;) {
     bool bad_len;
     const int len = length_of(a, b, bad_len);
-    const uint32_t nb = (len + kPgUnit - 1) / kPgUnit, first = before * a.kv_heads;
+    const uint32_t nb = (len + kUnit - 1) / kUnit, first = before * a.kv_heads;
     if (nb == 0 || u >= first + nb * a.kv_heads) {
       before += nb;
       ++b;
@@ -436,7 +573,7 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
     if (k0 == 0 && r0 == 0 && threadIdx.x == 0)
       a.parts[b * a.kv_heads + h] =
           i32x2{static_cast<int>(slot), whole ? (a.splits ? 1 : 0) : static_cast<int>((item0 + nb - 1) / quota) - share + 1};
-    segment<D, RT, 4>(a, b, h, len, bad_len, r0, k0, k1, slot, page_ids<4>(a, b, k0), lds);
+    segment<D, RT, 4, F8, kWeigh>(a, b, h, len, bad_len, r0, k0, k1, slot, page_ids<4, T>(a, b, k0), lds);
     u = item0 + k1;
   }
 }
@@ -449,7 +586,7 @@ constexpr int kPreBlocks = 256;      // workgroups of the prefix, at most about:
                                      // sequences: 40 us, 45 with 128, 47 with 384, 50 with 512)
 constexpr int kPreChunk = 64;        // tiles whose places in the cache a wave holds at once
 
-template <int D>
+template <int D, bool F8>
 __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
@@ -475,17 +612,20 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
   for (int c0 = t0; c0 < t1; c0 += kPreChunk) {
     const int c1 = min(c0 + kPreChunk, t1), row = wave * (kFlKeys / kPreWaves);
     const int key = min((c0 + lane) * kFlKeys + row, a.prefix - 1);
-    int id = ldg<int32_t>(a.pages + (key >> a.c.page_shift));
-    const bool out_of = id < 0 || id >= a.c.n_pages;
-    bad |= __ballot(out_of && c0 + lane < c1);
-    if (out_of) id = 0;
+    int id = key >> a.c.page_shift;
+    if constexpr (!F8) {
+      id = ldg<int32_t>(a.pages + id);
+      const bool out_of = id < 0 || id >= a.c.n_pages;
+      bad |= __ballot(out_of && c0 + lane < c1);
+      if (out_of) id = 0;
+    }
     const int64_t at = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))) * D;
     const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
     auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
       const uint32_t lo = __builtin_amdgcn_readlane(at_lo, t - c0), hi = __builtin_amdgcn_readlane(at_hi, t - c0);
       const int64_t base = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-      kp = a.c.k + base;
-      vp = a.c.v + base;
+      kp = (F8 ? a.pre_k : a.c.k) + base;
+      vp = (F8 ? a.pre_v : a.c.v) + base;
       last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
     };
     if (c0 > t0) __syncthreads();      // the last chunk's reads of LDS are done
@@ -518,34 +658,34 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
   if (hf == 0 && wr0 + n < rows) *reinterpret_cast<float2*>(a.pre_ml + (at0 + n) * 2) = float2{st.m, l};
 }
 
-template <int D, int RT>
+template <int D, int RT, bool F8, bool kWeigh>
 __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged(const PagedArgs a) {
   __shared__ SegLds<D, RT, 4> lds;
-  shares<D, RT>(a, blockIdx.x, 16 * RT * blockIdx.y, lds);
+  shares<D, RT, F8, kWeigh>(a, blockIdx.x, 16 * RT * blockIdx.y, lds);
 }
 
 // The prefix's workgroups, then the shares (more than 32 rows: a half of the rows each).
-template <int D, int RT>
+template <int D, int RT, bool F8, bool kWeigh>
 __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged_prefix(const PagedArgs a) {
   extern __shared__ __align__(16) char lds[];
   const int block = blockIdx.x - a.prefix_blocks;
-  if (block < 0) prefix_part<D>(a, blockIdx.x, lds);
-  else shares<D, RT>(a, block % a.shares, 16 * RT * (block / a.shares), *reinterpret_cast<SegLds<D, RT, 4>*>(lds));
+  if (block < 0) prefix_part<D, F8>(a, blockIdx.x, lds);
+  else shares<D, RT, F8, kWeigh>(a, block % a.shares, 16 * RT * (block / a.shares), *reinterpret_cast<SegLds<D, RT, 4>*>(lds));
 }
 
 // A workgroup for 16 rows of an item; nothing is left to join.  260 keys of 8 heads of 128 take 7.3
 // us: the launch, length and page ids, keys, and the eight waves' parts through LDS, one
 // after the other.
-template <int D>
+template <int D, bool F8, bool kWeigh>
 __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const PagedArgs a) {
   __shared__ SegLds<D, 1, kPgShortWaves> lds;
-  constexpr int kUnit = 32 * kPgShortWaves;
+  constexpr int kUnit = step_keys<F8>() * kPgShortWaves;
   const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, M = a.q_len * a.group, r0 = 16 * blockIdx.y;
-  const int ids = page_ids<kPgShortWaves>(a, b, 0);   // on its way beside the length
+  const int ids = page_ids<kPgShortWaves, Step<D, F8>::kTiles>(a, b, 0);   // on its way beside the length
   bool bad_len;
   const int len = length_of(a, b, bad_len);
   if (len > 0) {
-    segment<D, 1, kPgShortWaves>(a, b, h, len, bad_len, r0, 0, (len + kUnit - 1) / kUnit, -1, ids, lds);
+    segment<D, 1, kPgShortWaves, F8, kWeigh>(a, b, h, len, bad_len, r0, 0, (len + kUnit - 1) / kUnit, -1, ids, lds);
     return;
   }
   for (int i = threadIdx.x; i < (min(M, r0 + 16) - r0) * (D / 8); i += 64 * kPgShortWaves) {
@@ -564,7 +704,7 @@ __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const Pag
 // the loads after each other: length and place, maxima and sums beside the first parts.
 constexpr int kPgWaveRows = 1024;
 
-template <int D, int WPR>
+template <int D, int WPR, bool kWeigh>
 __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   constexpr int kLanes = D / 4, kThreads = 64 * WPR, kWays = kThreads / kLanes, kRows = kPgThreads / kThreads;
   __shared__ float red[kRows][WPR];
@@ -644,19 +784,87 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
   const int tok = r / a.group, hd = h * a.group + r % a.group;
   // no key, or an unused slot (its q may hold anything): zeros
   const bool sees = a.lens[b] >= 0 && (a.prefix > 0 || len - a.q_len + tok >= 0 || ll != ll);
+  if constexpr (kWeigh)
+    if (d0 == 0) a.lse[static_cast<int64_t>(item) * M + r] = sees ? top + log2f(ll) : -kNegInf;
   y = sees ? y * (1.0f / ll) : f32x4{0.f, 0.f, 0.f, 0.f};
   *reinterpret_cast<u32x2*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
       u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
 }
 
-// Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's.
+// Adds to every key's weight what the item's rows gave it, in their order: 2^(score - lse) of each.
+// Workgroups of an item take its keys in turn.  M float32 a key and head are written by the scores' kernel and
+// read here, against 4 D bytes of its key and value (2 D in 8 bits).
+constexpr int kKwRows = 64;          // most rows of an item
+
+__global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, int each) {
+  __shared__ float lse[kKwRows];
+  const int item = blockIdx.x / each, part = blockIdx.x % each, b = item / a.kv_heads, h = item % a.kv_heads, M = a.q_len * a.group;
+  bool bad;
+  const int len = length_of(a, b, bad);
+  if (bad || len <= part * kPgThreads) return;
+  if (static_cast<int>(threadIdx.x) < M) lse[threadIdx.x] = a.lse[static_cast<int64_t>(item) * M + threadIdx.x];
+  __syncthreads();
+  const int64_t cap = static_cast<int64_t>(a.c.max_pages) << a.c.page_shift;
+  for (int key = part * kPgThreads + threadIdx.x; key < len; key += each * kPgThreads) {
+    const int id = ldg<int32_t>(a.c.table + b * a.c.table_stride + (key >> a.c.page_shift));
+    const float* x = a.scores + (item * cap + key) * M;
+    float sum = 0.0f;
+    auto add = [&](float score, int r) {
+      // a key that the row does not see, whatever the row is
+      sum += score == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(score - lse[r]);
+    };
+    if (M % 4 == 0) {
+      for (int r = 0; r < M; r += 4) {
+        const f32x4 v = ldg<f32x4>(x + r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(v[i], r + i);
+      }
+    } else {
+      for (int r = 0; r < M; ++r) add(ldg<float>(x + r), r);
+    }
+    if (id >= 0 && id < a.c.n_pages)
+      a.weights[((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))] += sum;
+  }
+}
+
+// The prefix's pages of a cache in 8 bits as bf16 (exact), one after the other; NaN for one outside the cache.
+template <int D>
+__global__ __launch_bounds__(kPgThreads) void k_prefix_values(const PagedArgs a) {
+  const int rows = a.kv_heads << a.c.page_shift;     // of a page, with all heads
+  const int64_t all = static_cast<int64_t>((a.prefix + (1 << a.c.page_shift) - 1) >> a.c.page_shift) * rows * (D / 16);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPgThreads + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kPgThreads) {
+    const int64_t at = i / (D / 16);                 // row of all
+    const int page = static_cast<int>(at / rows), row = static_cast<int>(at % rows), e = 16 * static_cast<int>(i % (D / 16));
+    const int id = a.pages[page];
+    const bool bad = id < 0 || id >= a.c.n_pages;
+    const int64_t from = static_cast<int64_t>(bad ? 0 : id) * rows + row, to = at * D + e;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const u32x4 c = ldg16(reinterpret_cast<const uint8_t*>(w ? a.c.v : a.c.k) + from * D + e);
+      const float scale = bad ? __builtin_nanf("") : scale_of(ldg<uint8_t>((w ? a.v_scale : a.k_scale) + from / kScaleRows));
+      u32x4 y[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x2 t = codes_to_bf16(c[j], scale);
+        y[j / 2][2 * (j & 1)] = bad ? 0x7fc07fc0u : t[0];
+        y[j / 2][2 * (j & 1) + 1] = bad ? 0x7fc07fc0u : t[1];
+      }
+      u32x4* dst = reinterpret_cast<u32x4*>((w ? a.pre_v : a.pre_k) + to);
+      dst[0] = y[0];
+      dst[1] = y[1];
+    }
+  }
+}
+
+// Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's, then
+// scores, and the prefix's pages.
 struct PagedPlan {
   int rt, shares, splits, row_tiles;
   bool alone;                        // k_paged_short
-  size_t po, pml, parts, pre_o, pre_ml, total;
+  size_t po, pml, parts, pre_o, pre_ml, scores, lse, pre_k, pre_v, total;
 };
 
-PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
+PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more) {
   PagedPlan p{};
   auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
   const int64_t M = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
@@ -671,8 +879,25 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
   p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany ? kPgShortMany : kPgShort) &&
             items * (64 * kPgShortWaves) < (int64_t{1} << 32);
   p.total = 256;
-  if (p.alone) return p;
-  const int64_t units = items * ((keys + kPgUnit - 1) / kPgUnit);
+  // behind what the call needs otherwise
+  auto add_more = [&]() {
+    if (more.weigh) {
+      p.scores = p.total;
+      p.lse = up(p.scores + static_cast<size_t>(items) * keys * M * 4);
+      p.total = up(p.lse + static_cast<size_t>(items) * M * 4);
+    }
+    if (more.f8 && d.prefix_len > 0) {
+      const size_t pages = (d.prefix_len + static_cast<size_t>(c.page_size) - 1) / c.page_size;
+      const size_t bytes = pages * d.kv_heads * c.page_size * d.head_dim * 2;
+      p.pre_k = p.total;
+      p.pre_v = up(p.pre_k + bytes);
+      p.total = up(p.pre_v + bytes);
+    }
+    return p;
+  };
+  if (p.alone) return add_more();
+  const int unit = more.f8 ? unit_keys<true>() : unit_keys<false>();
+  const int64_t units = items * ((keys + unit - 1) / unit);
   // the workgroups that are resident at once, two a CU (64 sequences of up to 8192 keys, 8 heads
   // of 128: 81 us, 90 with 256 and 86 with 768); one a CU where registers allow no
   // more, or beside a prefix's (36.5 us with 256, 39.4 with 512, 64 sequences behind 16385 keys)
@@ -699,51 +924,72 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c) {
   p.pre_o = up(p.parts + items * 8);
   p.pre_ml = up(p.pre_o + pre * d.head_dim * 4);
   p.total = up(p.pre_ml + pre * 8);
-  return p;
+  return add_more();
 }
 
-template <int D, int RT>
+// Workgroups of k_key_weights, at least about.
+constexpr int kKwBlocks = 2048;
+
+template <int D, int RT, bool F8, bool kWeigh>
 void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
   const int M = a.q_len * a.group;
   // more than 32 rows: every share (item) twice, a half of the rows each, which reads the cache twice (four row
   // tiles spill registers): 64 sequences of 4096 keys of one head of 128 take 40 us for 32 rows, 63 for 48, 65 for 64
   const int halves = (M + 16 * RT - 1) / (16 * RT);
   if (p.alone) {
-    launch_kernel(k_paged_short<D>, dim3(a.batch * a.kv_heads, (M + 15) / 16), 64 * kPgShortWaves, 0, s, a);
+    launch_kernel(k_paged_short<D, F8, kWeigh>, dim3(a.batch * a.kv_heads, (M + 15) / 16), 64 * kPgShortWaves, 0, s, a);
     return;
   }
   if (p.splits) {
+    if constexpr (F8) {
+      const int64_t rows = static_cast<int64_t>((a.prefix + (1 << a.c.page_shift) - 1) >> a.c.page_shift) * (a.kv_heads << a.c.page_shift);
+      const int64_t blocks = (rows * (D / 16) + kPgThreads - 1) / kPgThreads;
+      launch_kernel(k_prefix_values<D>, static_cast<uint32_t>(std::min<int64_t>(blocks, 4096)), kPgThreads, 0, s, a);
+    }
     constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D>();
-    launch_kernel(k_paged_prefix<D, RT>, a.prefix_blocks + p.shares * halves, kPgThreads, lds, s, a);
+    launch_kernel(k_paged_prefix<D, RT, F8, kWeigh>, a.prefix_blocks + p.shares * halves, kPgThreads, lds, s, a);
   } else {
-    launch_kernel(k_paged<D, RT>, dim3(p.shares, halves), kPgThreads, 0, s, a);
+    launch_kernel(k_paged<D, RT, F8, kWeigh>, dim3(p.shares, halves), kPgThreads, 0, s, a);
   }
   const int rows = a.batch * a.kv_heads * M;
-  if (rows >= kPgWaveRows) launch_kernel(k_paged_join<D, 1>, (rows + 3) / 4, kPgThreads, 0, s, a);
-  else launch_kernel(k_paged_join<D, 4>, rows, kPgThreads, 0, s, a);
+  if (rows >= kPgWaveRows) launch_kernel(k_paged_join<D, 1, kWeigh>, (rows + 3) / 4, kPgThreads, 0, s, a);
+  else launch_kernel(k_paged_join<D, 4, kWeigh>, rows, kPgThreads, 0, s, a);
+}
+
+template <int D, bool F8, bool kWeigh>
+void launch_paged_d(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
+  if (p.rt == 1) launch_paged_rt<D, 1, F8, kWeigh>(p, a, s);
+  else launch_paged_rt<D, 2, F8, kWeigh>(p, a, s);
+  if constexpr (kWeigh) {
+    const int items = a.batch * a.kv_heads, keys = a.c.max_pages << a.c.page_shift;
+    const int each = std::min((kKwBlocks + items - 1) / items, (keys + kPgThreads - 1) / kPgThreads);
+    launch_kernel(k_key_weights, items * each, kPgThreads, 0, s, a, each);
+  }
 }
 
 }  // namespace
 
-size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c) { return plan_of(d, c).total; }
+size_t paged_workspace(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more) { return plan_of(d, c, more).total; }
 
-hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const void* q, const CacheView& view,
+hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more, const void* q, const CacheView& view,
                         const int32_t* lens, const int32_t* prefix, void* out, void* ws, hipStream_t s) {
-  const PagedPlan p = plan_of(d, c);
+  const PagedPlan p = plan_of(d, c, more);
   char* w = static_cast<char*>(ws);
   const PagedArgs a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lens, view,
                     reinterpret_cast<float*>(w + p.po), reinterpret_cast<float*>(w + p.pml), reinterpret_cast<i32x2*>(w + p.parts),
                     reinterpret_cast<float*>(w + p.pre_o), reinterpret_cast<float*>(w + p.pre_ml), prefix,
                     d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
                     d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits, p.row_tiles,
-                    p.row_tiles * p.splits * d.kv_heads};
-  if (d.head_dim == 64) {
-    if (p.rt == 1) launch_paged_rt<64, 1>(p, a, s);
-    else launch_paged_rt<64, 2>(p, a, s);
-  } else {
-    if (p.rt == 1) launch_paged_rt<128, 1>(p, a, s);
-    else launch_paged_rt<128, 2>(p, a, s);
-  }
+                    p.row_tiles * p.splits * d.kv_heads, more.k_scale, more.v_scale, reinterpret_cast<uint16_t*>(w + p.pre_k),
+                    reinterpret_cast<uint16_t*>(w + p.pre_v), more.key_weights, reinterpret_cast<float*>(w + p.scores),
+                    reinterpret_cast<float*>(w + p.lse)};
+  auto form = [&](auto f8, auto weigh) {
+    constexpr bool kF = decltype(f8)::value, kW = decltype(weigh)::value;
+    if (d.head_dim == 64) launch_paged_d<64, kF, kW>(p, a, s);
+    else launch_paged_d<128, kF, kW>(p, a, s);
+  };
+  if (more.f8) more.weigh ? form(std::true_type{}, std::true_type{}) : form(std::true_type{}, std::false_type{});
+  else more.weigh ? form(std::false_type{}, std::true_type{}) : form(std::false_type{}, std::false_type{});
   return hipGetLastError();
 }
 

@@ -21,9 +21,13 @@
 // TB/s), 4095 of 32 + 8 20 us (4.2 TB/s); a block for four tokens with the factors
 // from LDS for every head took 53 and 28 us.  Few tokens: a token's heads over
 // several waves, queries apart from keys and values, for the latency.
+//
+// Keys and values for a cache in 8 bits: a block's scale needs the largest element of all its rows, so
+// a workgroup takes the tokens of whole blocks (append_codes), beside those of the
+// queries in one launch.
 #include <type_traits>
 
-#include "attn.h"
+#include "kv8.h"
 
 namespace dsk {
 namespace {
@@ -35,6 +39,8 @@ typedef f32x4 f32x4_a4 __attribute__((aligned(4)));   // gammas may start anywhe
 struct QkArgs {
   const void *q, *k, *v;
   const int32_t *positions, *seq;
+  const int32_t *axis, *rows;        // axis of each pair, cache row of each token, or null
+  int64_t axis_stride;
   const double* freq;
   const float *q_gamma, *k_gamma;
   uint16_t *q_out, *k_out;
@@ -44,7 +50,39 @@ struct QkArgs {
   float eps, mscale;
   CacheView cache;
   bool append;
+  int32_t n_axes;
+  float* key_weights;                // of the cache's rows, or null
+  uint8_t *k_scale, *v_scale;        // of a cache in 8 bits
+  int32_t windows, code_parts;       // workgroups for it: of kWindow tokens, times parts of the heads
 };
+
+// Whether token t, at pos on the first axis, is one of padding.
+__device__ __forceinline__ bool left_out(const QkArgs& a, int64_t t, int pos) {
+  bool out = pos < 0;
+  for (int x = 1; x < a.n_axes; ++x) out |= a.positions[x * a.axis_stride + t] < 0;
+  return out;
+}
+// Cosine and sine of pair i's angle, times mscale; a pair of no axis does not turn.
+__device__ __forceinline__ float2 turn_of(const QkArgs& a, int64_t t, int pos, int i) {
+  if (a.axis) {
+    const int x = a.axis[i];
+    pos = x >= 0 && x < a.n_axes ? a.positions[x * a.axis_stride + t] : 0;
+  }
+  double c = static_cast<double>(pos) * (a.freq[i] * 0.15915494309189533577);   // turns: / (2 pi)
+  c -= rint(c);
+  float sn, cs;
+  sincospif(2.0f * static_cast<float>(c), &sn, &cs);
+  return float2{cs * a.mscale, sn * a.mscale};
+}
+// Row of token t among all rows of the cache with one head, or -1.
+__device__ __forceinline__ int64_t slot_of(const QkArgs& a, int64_t t, int pos) {
+  const int sq = a.seq[t];
+  const int64_t at = a.rows ? a.rows[t] : static_cast<int64_t>(pos) - a.prefix_len, page = at >> a.cache.page_shift;
+  if (sq < 0 || sq >= a.cache.n_seqs || at < 0 || page >= a.cache.max_pages) return -1;
+  const int id = a.cache.table[sq * a.cache.table_stride + page];
+  if (id < 0 || id >= a.cache.n_pages) return -1;
+  return ((static_cast<int64_t>(id) * a.kv_heads) << a.cache.page_shift) + (at & ((1 << a.cache.page_shift) - 1));
+}
 
 // 8 elements as they lie in memory.
 template <bool kBF16>
@@ -65,23 +103,225 @@ struct Raw8 {
   }
 };
 
+// The rotation as a lane sees it: its elements e .. e + 7, and those that pair with them.
+template <bool kInter>
+struct Pairs {
+  int e, er, ep, half;
+  bool rotated, low;
+  __device__ __forceinline__ Pairs(const QkArgs& a, int lane) {
+    e = 8 * lane;
+    half = a.rot_dim / 2;
+    er = e - a.rot_first;                             // this lane's first element among the rotated
+    rotated = er >= 0 && er < a.rot_dim;
+    low = er < half;
+    ep = kInter || !rotated ? e : (low ? e + half : e - half);   // half pairs: the elements that pair with the lane's own
+  }
+  // own[j] x[j] + pair[j] y[j] is element j, before the norm's factor: gamma alone where
+  // nothing turns, gamma cos and -+gamma' sin (interleaved: of the lane's other element) where it does
+  __device__ __forceinline__ void factors(const float* gamma, const float2* turn, float (&own)[8], float (&pair)[8]) const {
+    float g[8], gp[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = gp[j] = 1.0f;
+    if (gamma) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const f32x4 u = *reinterpret_cast<const f32x4_a4*>(gamma + e + j), v = *reinterpret_cast<const f32x4_a4*>(gamma + ep + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { g[j + i] = u[i]; gp[j + i] = v[i]; }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // (read whether it turns or not, since a branch around each read waits for it: 8192 tokens 44.2 -> 43.1 us)
+      const int pr = kInter ? er / 2 + j / 2 : (low ? er : er - half) + j;
+      const float2 read = turn[rotated ? pr : 0], cs = rotated ? read : float2{1.0f, 0.0f};
+      own[j] = g[j] * cs.x;
+      if constexpr (kInter) pair[j] = j & 1 ? g[j - 1] * cs.y : -(g[j + 1] * cs.y);
+      else pair[j] = (low ? -cs.y : cs.y) * gp[j];
+    }
+  }
+};
+// Eight elements of a head row that D / 8 lanes hold, normed and rotated.
+template <int D, bool kBF16, bool kInter>
+__device__ __forceinline__ void norm_turn(bool norm, float eps, bool rotated, const Raw8<kBF16>& x, const Raw8<kBF16>& y, const float (&own)[8],
+                                          const float (&pair)[8], float (&z)[8]) {
+  float rstd = 1.0f;
+  if (norm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+#pragma unroll
+    for (int m = D / 16; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
+    rstd = rsqrtf(ss * (1.0f / D) + eps);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // the other one's product only where something turns: it may be infinite
+    const float other = kInter ? x[j ^ 1] : y[j];
+    z[j] = x[j] * own[j];
+    if (rotated) z[j] += other * pair[j];
+    z[j] *= rstd;
+  }
+}
+__device__ __forceinline__ u32x4 pack8(const float (&z)[8]) {
+  return u32x4{pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]), pack_bf16(z[4], z[5]), pack_bf16(z[6], z[7])};
+}
+
+// Keys and values of a cache in 8 bits.  The tokens of a call that go to one block of 16 rows stand
+// next to each other; the workgroup of the first one's window of 16 tokens takes them all (kSlots: up to
+// 15 behind its window).  A row lies in D / 8 lanes as elsewhere, its largest magnitude goes to the
+// block's by way of LDS, and with that the block's scale is known before a code is made.
+constexpr int kWindow = 16, kSlots = 2 * kWindow;
+
+template <int D>
+struct CodeLds {
+  float2 turn[kSlots][D / 2];
+  int64_t slot[kSlots];
+  int lead[kSlots];                  // first token of the block; kSkip, or kCopy: for k_out alone
+  uint32_t rows[kSlots];             // of the block that begins here: its rows that the call brings
+  uint32_t top[3][2][kSlots];        // largest magnitudes, of three heads in turn
+};
+constexpr int kSkip = -1, kCopy = -2;
+
+template <int D, bool kBF16, bool kInter>
+__device__ __forceinline__ void append_codes(const QkArgs& a, int block) {
+  __shared__ CodeLds<D> s;
+  constexpr int kLanes = D / 8, kRows = 64 * kQkWaves / kLanes, kPasses = kSlots / kRows;
+  const int tid = threadIdx.x, lane = tid % kLanes, part = block % a.code_parts;
+  const int64_t t0 = static_cast<int64_t>(block / a.code_parts) * kWindow;
+  if (tid < 64) {                    // lane 1 + i: token t0 + i
+    const int i = tid - 1;
+    const int64_t t = t0 + i;
+    int64_t slot = -1;
+    bool live = false;
+    if (i < kSlots && t >= 0 && t < a.tokens) {
+      const int pos = a.positions[t];
+      live = !left_out(a, t, pos);
+      if (live) slot = slot_of(a, t, pos);
+    }
+    const int64_t key = slot < 0 ? -1 : slot / kScaleRows, before = __shfl_up(key, 1, 64);
+    const uint64_t starts = __ballot(tid > 0 && (key < 0 || key != before));
+    const uint64_t mine = starts & ((2ull << tid) - 1);
+    const int first = mine ? 62 - __clzll(static_cast<long long>(mine)) : -1;
+    if (i >= 0 && i < kSlots) {
+      s.slot[i] = slot;
+      s.rows[i] = 0;
+      s.lead[i] = key >= 0 ? (first >= 0 && first < kWindow ? first : kSkip) : (live && i < kWindow ? kCopy : kSkip);
+    }
+  } else {
+    for (int i = tid - 64; i < 3 * 2 * kSlots; i += 64 * (kQkWaves - 1)) (&s.top[0][0][0])[i] = 0;
+  }
+  __syncthreads();
+  if (tid < kSlots && s.lead[tid] >= 0) atomicOr(&s.rows[s.lead[tid]], 1u << (s.slot[tid] & (kScaleRows - 1)));
+  const int half = a.rot_dim / 2;
+  for (int i = tid; i < kSlots * half; i += 64 * kQkWaves) {
+    const int64_t t = t0 + i / half;
+    if (s.lead[i / half] != kSkip) s.turn[i / half][i % half] = turn_of(a, t, a.positions[t], i % half);
+  }
+  __syncthreads();
+  const Pairs<kInter> pairs(a, lane);
+  int lead[kPasses];
+  int64_t slot[kPasses];
+  float own[kPasses][8], pair[kPasses][8];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int i = p * kRows + tid / kLanes;
+    lead[p] = s.lead[i];
+    slot[p] = s.slot[i];
+    if (lead[p] != kSkip) pairs.factors(a.k_gamma, s.turn[i], own[p], pair[p]);
+  }
+  int buffer = 0;
+  for (int h = part; h < a.kv_heads; h += a.code_parts, buffer = buffer == 2 ? 0 : buffer + 1) {
+    float z[kPasses][2][8];          // keys, values
+    int old[kPasses][2];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int i = p * kRows + tid / kLanes;
+      const int64_t t = t0 + i;
+      if (lead[p] == kSkip) continue;                 // (all lanes of a row alike)
+      Raw8<kBF16> x, y, v;
+      x.load(a.k, t * a.k_token + h * a.k_head + pairs.e);
+      if (!kInter) y.load(a.k, t * a.k_token + h * a.k_head + pairs.ep);
+      if (lead[p] >= 0) {
+        v.load(a.v, t * a.v_token + h * a.v_head + pairs.e);
+        const int64_t at = (slot[p] + (static_cast<int64_t>(h) << a.cache.page_shift)) / kScaleRows;
+        old[p][0] = min(static_cast<int>(a.k_scale[at]), 254);
+        old[p][1] = min(static_cast<int>(a.v_scale[at]), 254);
+      }
+      norm_turn<D, kBF16, kInter>(a.norm, a.eps, pairs.rotated, x, y, own[p], pair[p], z[p][0]);
+      if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + pairs.e) = pack8(z[p][0]);
+      if (lead[p] < 0) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[p][1][j] = v[j];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_or(fabsf(z[p][w][j]), 0.0f));
+#pragma unroll
+        for (int m = kLanes / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+        if (lane == 0) atomicMax(&s.top[buffer][w][lead[p]], __float_as_uint(top));
+      }
+    }
+    __syncthreads();
+    // those of the head after next: read before the barrier above, used behind the next
+    if (tid < 2 * kSlots) (&s.top[buffer == 0 ? 2 : buffer - 1][0][0])[tid] = 0;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      if (lead[p] < 0) continue;
+      const int i = p * kRows + tid / kLanes;
+      const int64_t row = slot[p] + (static_cast<int64_t>(h) << a.cache.page_shift);
+      const uint32_t here = s.rows[lead[p]];
+      const bool fresh = here & 1;
+      if (a.key_weights && lane == 0) a.key_weights[row] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        uint8_t* codes = reinterpret_cast<uint8_t*>(w ? a.cache.v : a.cache.k);
+        const int want = scale_byte(__uint_as_float(s.top[buffer][w][lead[p]])), b = fresh ? want : max(want, old[p][w]);
+        *reinterpret_cast<u32x2*>(codes + row * D + pairs.e) = to_codes(z[p][w], inverse_scale(b));
+        if (i != lead[p]) continue;
+        if (lane == 0) (w ? a.v_scale : a.k_scale)[row / kScaleRows] = static_cast<uint8_t>(b);
+        if (fresh || b <= old[p][w]) continue;
+        // the block's other rows, in the larger scale
+        const float f = scale_step(old[p][w], b);
+        uint8_t* rows = codes + row / kScaleRows * kScaleRows * D + pairs.e;
+        for (int r = 0; r < kScaleRows; ++r) {
+          if (here >> r & 1) continue;
+          u32x2* c = reinterpret_cast<u32x2*>(rows + r * D);
+          *c = u32x2{rescale4((*c)[0], f), rescale4((*c)[1], f)};
+        }
+      }
+    }
+  }
+}
+
 // A lane's part of a head row: elements e .. e + 7 of 8 lanes (D 64) or 16 (D 128).  kAll: a
 // wave takes all heads of its token.  kPast: queries and rows of the cache are written past L2.
-template <int D, bool kBF16, bool kInter, bool kAll, bool kPast>
+// kCodes: a cache in 8 bits, whose workgroups come first; then the queries'.
+template <int D, bool kBF16, bool kInter, bool kAll, bool kPast, bool kCodes>
 __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a head row, rows of a wave
   __shared__ float2 turns[kQkWaves][D / 2];
+  int bx = blockIdx.x, by = blockIdx.y;
+  if constexpr (kCodes) {
+    bx -= a.windows * a.code_parts;
+    if (bx < 0) {
+      append_codes<D, kBF16, kInter>(a, blockIdx.x);
+      return;
+    }
+    by = bx % a.q_parts;
+    bx /= a.q_parts;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wl = threadIdx.x & 63;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kQkWaves + wave;
+  const int64_t t = static_cast<int64_t>(bx) * kQkWaves + wave;
   if (t >= a.tokens) return;
-  const int lane = wl % kLanes, e = 8 * lane;
-  const int half = a.rot_dim / 2, er = e - a.rot_first;       // this lane's first element among the rotated
-  const bool rotated = er >= 0 && er < a.rot_dim, low = er < half;
-  // half pairs: the elements that pair with the lane's own
-  const int ep = kInter || !rotated ? e : (low ? e + half : e - half);
+  const int lane = wl % kLanes;
+  const Pairs<kInter> pairs(a, lane);
+  const int e = pairs.e, ep = pairs.ep, half = pairs.half;
+  const bool rotated = pairs.rotated;
   // this lane's heads: row0, row0 + step, ..
-  const bool is_q = kAll || static_cast<int>(blockIdx.y) < a.q_parts;
-  const int part = is_q ? blockIdx.y : blockIdx.y - a.q_parts;
+  const bool is_q = kAll || kCodes || by < a.q_parts;
+  const int part = is_q ? by : by - a.q_parts;
   const int row0 = part * kRows + wl / kLanes, step = (kAll ? 1 : is_q ? a.q_parts : a.kv_parts) * kRows;
 
   // heads row, row + step, .. of one tensor: kQkAhead of them
@@ -103,69 +343,16 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   }
 
   const int pos = a.positions[t];
-  if (pos < 0) return;                                // a token of padding
+  if (left_out(a, t, pos)) return;
   float2* turn = turns[wave];
-  if (wl < half) {
-    double c = static_cast<double>(pos) * (a.freq[wl] * 0.15915494309189533577);   // turns: / (2 pi)
-    c -= rint(c);
-    float sn, cs;
-    sincospif(2.0f * static_cast<float>(c), &sn, &cs);
-    turn[wl] = float2{cs * a.mscale, sn * a.mscale};
-  }
-  // the token's row of the cache, or none
-  int64_t slot = -1;
-  if (a.append) {
-    const int sq = a.seq[t];
-    const int64_t at = static_cast<int64_t>(pos) - a.prefix_len, page = at >> a.cache.page_shift;
-    if (sq >= 0 && sq < a.cache.n_seqs && at >= 0 && page < a.cache.max_pages) {
-      const int id = a.cache.table[sq * a.cache.table_stride + page];
-      if (id >= 0 && id < a.cache.n_pages)
-        slot = ((static_cast<int64_t>(id) * a.kv_heads) << a.cache.page_shift) + (at & ((1 << a.cache.page_shift) - 1));
-    }
-  }
+  if (wl < half) turn[wl] = turn_of(a, t, pos, wl);
+  const int64_t slot = !kCodes && a.append ? slot_of(a, t, pos) : -1;   // the token's row of the cache, or none
 
-  // own[j] x[j] + pair[j] y[j] is element j, before the norm's factor: gamma alone where
-  // nothing turns, gamma cos and -+gamma' sin (interleaved: of the lane's other element) where it does
-  auto factors = [&](const float* gamma, float (&own)[8], float (&pair)[8]) {
-    float g[8], gp[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = gp[j] = 1.0f;
-    if (gamma) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const f32x4 u = *reinterpret_cast<const f32x4_a4*>(gamma + e + j), v = *reinterpret_cast<const f32x4_a4*>(gamma + ep + j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { g[j + i] = u[i]; gp[j + i] = v[i]; }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int pr = kInter ? er / 2 + j / 2 : (low ? er : er - half) + j;
-      const float2 cs = rotated ? turn[pr] : float2{1.0f, 0.0f};
-      own[j] = g[j] * cs.x;
-      if constexpr (kInter) pair[j] = j & 1 ? g[j - 1] * cs.y : -(g[j + 1] * cs.y);
-      else pair[j] = (low ? -cs.y : cs.y) * gp[j];
-    }
-  };
+  auto factors = [&](const float* gamma, float (&own)[8], float (&pair)[8]) { pairs.factors(gamma, turn, own, pair); };
   auto normed = [&](const Raw8<kBF16>& x, const Raw8<kBF16>& y, const float (&own)[8], const float (&pair)[8]) {
-    float rstd = 1.0f, z[8];
-    if (a.norm) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-#pragma unroll
-      for (int m = kLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
-      rstd = rsqrtf(ss * (1.0f / D) + a.eps);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // the other one's product only where something turns: it may be infinite
-      const float other = kInter ? x[j ^ 1] : y[j];
-      z[j] = x[j] * own[j];
-      if (rotated) z[j] += other * pair[j];
-      z[j] *= rstd;
-    }
-    return u32x4{pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]), pack_bf16(z[4], z[5]), pack_bf16(z[6], z[7])};
+    float z[8];
+    norm_turn<D, kBF16, kInter>(a.norm, a.eps, rotated, x, y, own, pair, z);
+    return pack8(z);
   };
 
   auto store = [&](uint16_t* p, const u32x4& x) {
@@ -192,7 +379,7 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
       row = next;
     }
   }
-  if (row0 >= a.kv_heads || (is_q && !kAll)) return;
+  if (kCodes || row0 >= a.kv_heads || (is_q && !kAll)) return;
   if (kAll) {
     load(r, a.k, a.k_token, a.k_head, row0, a.kv_heads, true);
     if (slot >= 0) load(v, a.v, a.v_token, a.v_head, row0, a.kv_heads, false);
@@ -211,6 +398,7 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
       if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + e) = out[i];   // read many times next
       if (slot >= 0) {
         const int64_t to = (slot + (static_cast<int64_t>(h) << a.cache.page_shift)) * D + e;
+        if (a.key_weights && lane == 0) a.key_weights[to / D] = 0.0f;
         store(a.cache.k + to, out[i]);
         const Raw8<kBF16>& x = v.x[i];
         store(a.cache.v + to, u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])});
@@ -228,6 +416,9 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
 // of 64 (1.5 MB) 5.0 either way, 14.7 -> 14.9; 256 of 12 + 12 + 12 (1.1 MB) 12.8 -> 13.0.  k_out's rows, which the attention
 // reads for every row tile, always stay: past L2 they cost it up to 16 % (3000 tokens of 12 + 12 + 12: 43.9 -> 50.5).
 constexpr int64_t kPastL2 = 4 << 20;
+
+// Workgroups for the keys and values of a cache in 8 bits, at least about: a head's, until there are these.
+constexpr int kCodeBlocks = 512;
 
 template <int D>
 void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
@@ -250,7 +441,18 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
   };
   auto form = [&](auto bf16, auto inter) {
     constexpr bool kB = decltype(bf16)::value, kI = decltype(inter)::value;
-    launch(k_qk<D, kB, kI, true, false>, k_qk<D, kB, kI, false, false>, k_qk<D, kB, kI, true, true>, k_qk<D, kB, kI, false, true>);
+    if (!a.k_scale) {
+      launch(k_qk<D, kB, kI, true, false, false>, k_qk<D, kB, kI, false, false, false>, k_qk<D, kB, kI, true, true, false>,
+             k_qk<D, kB, kI, false, true, false>);
+      return;
+    }
+    a.windows = (d.tokens + kWindow - 1) / kWindow;
+    const int want = (kCodeBlocks + a.windows - 1) / a.windows;
+    a.code_parts = want < d.kv_heads ? want : d.kv_heads;
+    if (!split) a.q_parts = d.heads > 0 ? 1 : 0;
+    const int64_t blocks = static_cast<int64_t>(a.windows) * a.code_parts + static_cast<int64_t>(grid.x) * a.q_parts;
+    launch_kernel(past ? k_qk<D, kB, kI, false, true, true> : k_qk<D, kB, kI, false, false, true>, dim3(static_cast<uint32_t>(blocks)),
+                  64 * kQkWaves, 0, s, a);
   };
   if (d.dtype == DSK_DTYPE_BF16) {
     if (d.interleaved) form(std::true_type{}, std::true_type{});
@@ -265,11 +467,12 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
 
 hipError_t launch_qk(const dsk_qk_desc& d, const void* q, const void* k, const void* v, const int32_t* positions,
                      const int32_t* seq, const double* freq, const float* q_gamma, const float* k_gamma,
-                     const CacheView* cache, void* q_out, void* k_out, hipStream_t s) {
-  QkArgs a{q, k, v, positions, seq, freq, q_gamma, k_gamma, static_cast<uint16_t*>(q_out),
+                     const CacheView* cache, const QkMore& more, void* q_out, void* k_out, hipStream_t s) {
+  QkArgs a{q, k, v, positions, seq, more.axis, more.rows, more.axis_stride, freq, q_gamma, k_gamma, static_cast<uint16_t*>(q_out),
            static_cast<uint16_t*>(k_out), d.q_token, d.q_head, d.k_token, d.k_head, d.v_token, d.v_head,
            d.qo_token, d.qo_head, d.ko_token, d.ko_head, d.tokens, d.heads, d.kv_heads, d.rot_dim, d.rot_first,
-           d.prefix_len, d.norm, 0, 0, d.eps, d.mscale, cache ? *cache : CacheView{}, cache != nullptr};
+           d.prefix_len, d.norm, 0, 0, d.eps, d.mscale, cache ? *cache : CacheView{}, cache != nullptr,
+           more.n_axes, more.key_weights, more.k_scale, more.v_scale, 0, 0};
   if (d.head_dim == 64) launch_qk_d<64>(d, a, s);
   else launch_qk_d<128>(d, a, s);
   return hipGetLastError();

@@ -92,6 +92,24 @@ class PagedDesc(ctypes.Structure):
                 + [(n, _i64) for n in ("q_token", "q_head", "o_token", "o_head")])
 
 
+class RopeAxes(ctypes.Structure):
+    """Mirror of ``dsk_rope_axes``."""
+
+    _fields_ = [("axis_stride", _i64), ("n_axes", _i32), ("axis", _vp)]
+
+
+class KVExtra(ctypes.Structure):
+    """Mirror of ``dsk_kv_extra``."""
+
+    _fields_ = [("k_scale", _vp), ("v_scale", _vp), ("key_weights", _vp)]
+
+
+class EvictDesc(ctypes.Structure):
+    """Mirror of ``dsk_evict_desc``."""
+
+    _fields_ = [(n, _i32) for n in ("kv_heads", "head_dim", "keep", "first", "recent")]
+
+
 PDesc = ctypes.POINTER(Desc)
 PCache = ctypes.POINTER(KVCache)
 
@@ -127,6 +145,12 @@ SIGNATURES = {
     "dsk_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "dsk_paged_attention_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache, ctypes.POINTER(_sz)]),
     "dsk_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache] + [_vp] * 8 + [_sz, _vp]),
+    "dsk_qk_norm_rope_axes": (ctypes.c_int, [ctypes.POINTER(QkDesc), ctypes.POINTER(RopeAxes)] + [_vp] * 9),
+    "dsk_kv_append_extra": (ctypes.c_int, [ctypes.POINTER(QkDesc), PCache, ctypes.POINTER(RopeAxes), ctypes.POINTER(KVExtra)] + [_vp] * 15),
+    "dsk_paged_attention_extra_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache, ctypes.POINTER(KVExtra), ctypes.POINTER(_sz)]),
+    "dsk_paged_attention_extra": (ctypes.c_int, [ctypes.POINTER(PagedDesc), PCache, ctypes.POINTER(KVExtra)] + [_vp] * 8 + [_sz, _vp]),
+    "dsk_kv_evict_workspace_size": (ctypes.c_int, [ctypes.POINTER(EvictDesc), PCache, ctypes.POINTER(KVExtra), ctypes.POINTER(_sz)]),
+    "dsk_kv_evict": (ctypes.c_int, [ctypes.POINTER(EvictDesc), PCache, ctypes.POINTER(KVExtra)] + [_vp] * 6 + [_sz, _vp]),
     "dsk_rmsnorm": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, ctypes.c_float, _i32, _vp, _vp, _vp]),
 }
 

@@ -144,7 +144,7 @@ class MoEStack:
         # what the graph reads and writes stays as long as the graph
         self._step = step
         self._places = [(k, v) for k, v in vars(step).items() if isinstance(v, torch.Tensor)] if step is not None else []
-        self._caches = [(a, a.k_cache, a.v_cache) for a in self.attention or ()]
+        self._caches = [(a, a.cache_tensors()) for a in self.attention or ()]
         self._weights = [(a.w_qkv, a.w_o) for a in self.attention or ()]
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
@@ -157,7 +157,7 @@ class MoEStack:
         returns the static output buffer."""
         if self._graph is None:
             raise RuntimeError("capture() the stack first")
-        if any(a.k_cache is not k or a.v_cache is not v for a, k, v in self._caches):
+        if any(x is not y for a, had in self._caches for x, y in zip(a.cache_tensors(), had)):
             raise RuntimeError("an attention layer has another cache than the graph's: capture() the stack again")
         if any(getattr(self._step, k) is not v for k, v in self._places):
             raise RuntimeError("the step has other tensors than the graph's: write into those, or capture() the stack again")
@@ -165,3 +165,16 @@ class MoEStack:
             self._x.copy_(x)
         self._graph.replay()
         return self._out
+
+    def evict(self, step: DecodeStep, keep: int, *, first: int = 0, recent: int = 0) -> None:
+        """``kv_evict`` of every layer's cache (``new_cache(weigh=..)``) after a decode step: of each of ``step``'s sequences with more
+        than ``keep`` keys, every layer's key heads keep ``keep`` of their own.  step.lens and step.rows, which must be given, follow in
+        place; positions go on as they were."""
+        if not isinstance(step, DecodeStep) or step.rows is None:
+            raise ValueError("evict needs a DecodeStep with rows: behind it positions do not give them")
+        if self.attention is None or any(a.key_weights is None for a in self.attention):
+            raise RuntimeError("evict needs attention sublayers whose caches keep weights: new_cache(weigh=..)")
+        for a in self.attention:
+            lens = a.evict(step.table, step.lens, keep, first=first, recent=recent)
+        step.rows -= (step.lens - lens).repeat_interleave(step.q_len, output_size=step.rows.numel())
+        step.lens.copy_(lens)

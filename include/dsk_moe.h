@@ -423,6 +423,92 @@ int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, cons
                         const void* v_cache, const int32_t* table, const int32_t* lens, const int32_t* prefix,
                         void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Positions on several axes (time, height, width of a picture's or video's tokens).
+ * Pair i of the rotated elements turns by positions[axis[i] * axis_stride + t] *
+ * freq[i]; a pair whose axis is none of 0 .. n_axes - 1 does not turn.  A token
+ * that is negative on any axis is left out. */
+typedef struct dsk_rope_axes {
+  int64_t axis_stride;    /* elements between the axes of positions, >= tokens */
+  int32_t n_axes;         /* 1..8 */
+  const int32_t* axis;    /* [rot_dim / 2] i32, device */
+} dsk_rope_axes;
+
+/* What a paged cache holds beside its rows; members that are NULL it does not have.
+ *
+ * k_scale and v_scale (both or none): the cache is held in 8 bits, k_cache and
+ * v_cache [n_pages, kv_heads, page_size, head_dim] OCP e4m3 codes, with a scale
+ * 2^(b - 127) for every 16 rows of a page and head, [n_pages, kv_heads,
+ * page_size / 16] bytes b.  A block's scale is the least that holds its largest
+ * magnitude in 448 of it (b from 27 to 246).  An infinity or NaN is kept as NaN,
+ * without a part in the scale.
+ *
+ * key_weights [n_pages, kv_heads, page_size] f32: the softmax weight that every key
+ * has received. */
+typedef struct dsk_kv_extra {
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  float* key_weights;
+} dsk_kv_extra;
+
+/* dsk_qk_norm_rope with positions on several axes. */
+int dsk_qk_norm_rope_axes(const dsk_qk_desc* d, const dsk_rope_axes* axes, const void* q, const void* k,
+                          const int32_t* positions, const double* freq, const float* q_gamma, const float* k_gamma,
+                          void* q_out, void* k_out, void* stream);
+
+/* dsk_kv_append with positions on several axes (axes, or NULL), with the tokens'
+ * rows given apart (rows [tokens] i32: token t goes to row rows[t] of its sequence,
+ * a negative one is not kept; d->prefix_len is then 0; NULL: positions -
+ * prefix_len, on the first axis), and to what extra names (or NULL): the weight of a
+ * kept key is set to zero, and a cache in 8 bits takes rounded keys and values.
+ *
+ * In 8 bits, the tokens of a call that go to one block of 16 rows stand next to each
+ * other (a prompt's and a verify step's do).  A call that brings a block's first row
+ * starts the block afresh: its scale is that of the call's rows.  Otherwise the larger
+ * of that and the block's own, and the rows that are there are rounded to it. */
+int dsk_kv_append_extra(const dsk_qk_desc* d, const dsk_kv_cache* cache, const dsk_rope_axes* axes, const dsk_kv_extra* extra,
+                        const void* q, const void* k, const void* v, const int32_t* positions, const int32_t* seq,
+                        const int32_t* rows, const double* freq, const float* q_gamma, const float* k_gamma, void* k_cache,
+                        void* v_cache, const int32_t* table, void* q_out, void* k_out, void* stream);
+
+/* dsk_paged_attention over a cache with what extra names: in 8 bits, and adding to
+ * every key's weight the softmax weights that the queries of its head's group give it
+ * (own keys; a prefix takes its part of the weights, which nobody keeps).  NaN
+ * outputs give NaN to the keys that they see; of a sequence whose length is beyond its
+ * table row, and of unused slots, no weight changes. */
+int dsk_paged_attention_extra_workspace_size(const dsk_paged_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra,
+                                             size_t* bytes);
+int dsk_paged_attention_extra(const dsk_paged_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, const void* q,
+                              const void* k_cache, const void* v_cache, const int32_t* table, const int32_t* lens,
+                              const int32_t* prefix, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct dsk_evict_desc {
+  int32_t kv_heads;       /* 1..1024 */
+  int32_t head_dim;       /* 64 or 128 */
+  int32_t keep;           /* rows of a sequence that stay, >= 1 */
+  int32_t first;          /* of them, its first ones */
+  int32_t recent;         /* and its last ones; first + recent <= keep */
+} dsk_evict_desc;
+
+/* Eviction by accumulated weight (extra->key_weights, which is required).  Of every
+ * sequence with lens[s] > keep rows each key head keeps the first `first` rows, the
+ * last `recent`, and of the others the keep - first - recent of largest weight (NaN
+ * above all; of equal ones the earlier rows).  They are then the rows 0 .. keep - 1:
+ * with middle = keep - recent, kept rows in front of middle stay where they are, the
+ * i-th other kept row behind it takes the place of the i-th row in front that is given up,
+ * and the last rows follow in their order.  Weights move with their rows.  In 8
+ * bits a block of 16 rows with a row from elsewhere takes the largest of its rows'
+ * scales.  What lies behind row keep is left as it was.  lens_out[s] = min(lens[s],
+ * keep); lens_out may be lens.  Sequences that are unused or longer than their table row are
+ * left alone, and rows whose page, or whose place's, is outside the cache do not move; such
+ * rows count as those of least weight.  Rows keep the rotation they have, so later
+ * tokens go on at their own positions (dsk_kv_append_extra's rows).  workspace:
+ * dsk_kv_evict_workspace_size bytes, 256-byte aligned, no initialisation; one call
+ * at a time. */
+int dsk_kv_evict_workspace_size(const dsk_evict_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, size_t* bytes);
+int dsk_kv_evict(const dsk_evict_desc* d, const dsk_kv_cache* cache, const dsk_kv_extra* extra, void* k_cache, void* v_cache,
+                 const int32_t* table, const int32_t* lens, int32_t* lens_out, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,7 +36,8 @@ def norm_rope(x, positions, freq=None, *, interleaved=False, rot_first=0, mscale
         r = freq.numel()
         i = torch.arange(r)
         a, b = (rot_first + 2 * i, rot_first + 2 * i + 1) if interleaved else (rot_first + i, rot_first + i + r)
-        t = positions.to(F64)[:, None] * freq.to(F64).cpu()
+        # positions [T], or [T, pairs] where pairs turn by axes of their own
+        t = (positions if positions.dim() == 2 else positions[:, None]).to(F64) * freq.to(F64).cpu()
         c, s = (mscale * torch.cos(t))[:, None], (mscale * torch.sin(t))[:, None]
         ya, yb = y[..., a].clone(), y[..., b].clone()
         y[..., a], y[..., b] = ya * c - yb * s, yb * c + ya * s
@@ -106,3 +107,140 @@ def paged(q, k_cache, v_cache, table, lens, prefix=None, prefix_len=0, scale=Non
         last = prefix_len + torch.clamp(own, min=-1)
         o[b], tol[b] = attention(q[b], k, v, last, scale)
     return o, tol
+
+
+def key_weights(q, k, last, scale):
+    """(w, tol) [Lk, kv heads]: softmax weight that each key receives from q [Lq, heads, D], in all.
+
+    A weight is 2 to a float32 score: its relative error is the score's absolute one, D products and their sums
+    of at most |q| |k| each, with the logarithm of the sum taken off (n terms); one rounding for every addition."""
+    q, k = q.to(F64), k.to(F64)
+    heads, kv = q.shape[1], k.shape[1]
+    w, tol = torch.zeros(k.shape[:2], dtype=F64), torch.zeros(k.shape[:2], dtype=F64)
+    for i in range(q.shape[0]):
+        n = min(int(last[i]) + 1, k.shape[0])
+        if n <= 0:
+            continue
+        for h in range(heads):
+            g = h * kv // heads
+            kh = k[:n, g]
+            p = torch.softmax(scale * (kh @ q[i, h]), 0)
+            size = scale * float((kh.abs() @ q[i, h].abs()).max())
+            w[:n, g] += p
+            tol[:n, g] += p * 4.0 * (n + q.shape[2] * size + 16) * F32_HALF_STEP
+    return w, tol + w * q.shape[0] * heads * F32_HALF_STEP
+
+
+# ------------------------------------------------------------------ the cache in 8 bits
+BLOCK = 16
+LEAST, MOST = 27, 246
+
+_CODES = torch.tensor([[(-1.0) ** (c >> 7) * ((c & 7) / 8 * 2.0 ** -6 if not c >> 3 & 15 else (1 + (c & 7) / 8) * 2.0 ** ((c >> 3 & 15) - 7)),
+                        math.nan][c & 127 == 127] for c in range(256)], dtype=F64)
+
+
+def to_codes(x, byte):
+    """uint8 e4m3 codes of x (float64) in the scale of byte (same shape), nearest, ties to the even code."""
+    y = x / 2.0 ** (byte.to(F64) - 127)
+    size = y.abs().nan_to_num(0.0).clamp(max=448.0)
+    positive = _CODES[:127]
+    hi = torch.searchsorted(positive, size).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    low, high = size - positive[lo], positive[hi] - size
+    code = torch.where((low < high) | ((low == high) & (lo % 2 == 0)), lo, hi)
+    code = torch.where(torch.signbit(y), code + 128, code)
+    return torch.where(torch.isfinite(x), code, torch.full_like(code, 127)).to(torch.uint8)
+
+
+def values(codes, byte):
+    """float64 values of uint8 codes [pages, kv heads, page, D] with scales [pages, kv heads, page / 16]."""
+    return _CODES[codes.long()] * 2.0 ** (byte.to(F64).repeat_interleave(BLOCK, -1)[..., None] - 127)
+
+
+def scale_byte(top):
+    """Least b with top <= 448 * 2^(b - 127) (a float), in range."""
+    if top == 0:
+        return LEAST
+    m, e = math.frexp(top / 448.0)
+    return min(max((e if m > 0.5 else e - 1) + 127, LEAST), MOST)
+
+
+def append_codes(x, codes, byte, slots):
+    """codes and byte (changed in place) after a call whose token t brings the rows x[t] [kv heads, D] to
+    (page, row) = slots[t] (None: not kept)."""
+    blocks = {}
+    for t, at in enumerate(slots):
+        if at is not None:
+            blocks.setdefault((at[0], at[1] // BLOCK), []).append((t, at[1]))
+    for (page, sub), rows in blocks.items():
+        for h in range(x.shape[1]):
+            brought = torch.stack([x[t, h] for t, _ in rows]).to(F64)
+            b = scale_byte(float(torch.where(torch.isfinite(brought), brought.abs(), torch.zeros_like(brought)).max()))
+            if not any(r % BLOCK == 0 for _, r in rows):
+                old = int(byte[page, h, sub])
+                b = max(b, old)
+                if b > old:
+                    block = codes[page, h, sub * BLOCK:(sub + 1) * BLOCK]
+                    block[:] = rescale(block, old, b)
+            byte[page, h, sub] = b
+            for t, r in rows:
+                codes[page, h, r] = to_codes(x[t, h].to(F64), torch.tensor(b))
+
+
+def rescale(codes, old, new):
+    """Codes of the scale of byte old in that of new; a NaN stays one."""
+    got = to_codes(_CODES[codes.long()] * 2.0 ** (old - new), torch.tensor(127))
+    return torch.where((codes & 127) == 127, codes, got)
+
+
+def evict(caches, weights, table, lens, keep, first, recent, page):
+    """New lengths; caches (a list of (rows [pages, kv heads, page, D], scales or None)) and weights are changed in place.
+
+    Row by row from the definition: an item's whole order first, then all of its rows at once."""
+    new = []
+    n_pages = weights.shape[0]
+    for b, n in enumerate(lens):
+        if n <= keep or n > table.shape[1] * page:
+            new.append(n)
+            continue
+        new.append(keep)
+        place = [(int(table[b, j // page]), j % page) for j in range(n)]
+        ok = [0 <= p < n_pages for p, _ in place]
+        for h in range(weights.shape[1]):
+            def order(j):
+                w = float(weights[place[j][0], h, place[j][1]]) if ok[j] else None
+                return (0 if w is None else 2 if math.isnan(w) else 1, 0.0 if w is None or math.isnan(w) else w)
+            free = sorted(range(first, n - recent), key=order, reverse=True)      # (stable: of equal ones the earlier)
+            stay = set(free[:keep - first - recent]) | set(range(first))
+            middle = keep - recent
+            src = list(range(middle)) + [n - recent + i for i in range(recent)]
+            fills = iter(sorted(j for j in stay if j >= middle))
+            for j in range(middle):
+                if j not in stay:
+                    src[j] = next(fills)
+            assert next(fills, None) is None
+            src = [s if ok[s] else j for j, s in enumerate(src)]
+            moved = [j for j in range(keep) if src[j] != j and ok[j]]
+            had = {j: (weights[place[src[j]][0], h, place[src[j]][1]].clone(),
+                       [(r[place[src[j]][0], h, place[src[j]][1]].clone(), None if s is None else int(s[place[src[j]][0], h, place[src[j]][1] // BLOCK]))
+                        for r, s in caches])
+                   for j in range(keep) if ok[j]}
+            # in 8 bits a block is touched as a whole, also where the row that should come is not there
+            want = {j // BLOCK for j in range(middle) if j not in stay} | ({j // BLOCK for j in range(middle, keep)} if recent else set())
+            for j in moved:
+                weights[place[j][0], h, place[j][1]] = had[j][0]
+            for c, (rows, scales) in enumerate(caches):
+                if scales is None:
+                    for j in moved:
+                        rows[place[j][0], h, place[j][1]] = had[j][1][c][0]
+                    continue
+                for block in sorted(want):
+                    js = [j for j in range(block * BLOCK, min((block + 1) * BLOCK, keep)) if ok[j]]
+                    if not js:
+                        continue
+                    top = max(had[j][1][c][1] for j in js)
+                    for j in js:
+                        code, byte = had[j][1][c]
+                        rows[place[j][0], h, place[j][1]] = rescale(code, byte, top) if byte != top else code
+                    scales[place[js[0]][0], h, place[js[0]][1] // BLOCK] = top
+    return new
