@@ -21,7 +21,7 @@
 namespace dsk {
 namespace {
 
-constexpr int kPickThreads = 1024, kMoveThreads = 256;
+constexpr int kMoveThreads = 1024;
 
 // A block with holes (one bit each of mask), which are filled from fills[start ..].
 struct EvictBlock { int32_t block, start; uint32_t mask; int32_t unused; };
@@ -61,110 +61,159 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sums of flags over the workgroup, by wave counts in LDS (two buffers in turn).
-struct Scan {
-  int (*waves)[kPickThreads / 64];
-  int turn = 0;
-  // own: what stands before this thread's flag; returns the number of all
-  __device__ __forceinline__ int operator()(bool flag, int& own) {
-    const uint64_t mask = __ballot(flag);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane == 0) waves[turn][wave] = __popcll(mask);
-    __syncthreads();
-    int all = 0;
-    own = __popcll(mask & ((1ull << lane) - 1));
-    for (int w = 0; w < kPickThreads / 64; ++w) {
-      const int n = waves[turn][w];
-      if (w < wave) own += n;
-      all += n;
-    }
-    turn ^= 1;
-    return all;
-  }
-};
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));   // weights may start anywhere
 
-__global__ __launch_bounds__(kPickThreads) void k_evict_pick(const EvictArgs a) {
-  __shared__ uint32_t counts[256];
-  __shared__ uint32_t chosen[2];                      // digit, rows above it
-  __shared__ int waves[2][kPickThreads / 64];
+// Sum of v over the threads before this one, and over all; `waves`: LDS for a number of each wave.
+template <int kWaves>
+__device__ __forceinline__ uint32_t before_me(uint32_t v, uint32_t& all, uint32_t* waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t up = v;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t x = __shfl_up(up, s, 64);
+    if (lane >= s) up += x;
+  }
+  if (lane == 63) waves[wave] = up;
+  __syncthreads();
+  uint32_t before = up - v;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const uint32_t n = waves[w];
+    if (w < wave) before += n;
+    all += n;
+  }
+  return before;
+}
+
+// A thread takes 16 rows one after the other: they lie in one page, and what becomes of them is a mask (that of
+// the block's holes, in 8 bits); sums over threads are two scans.  Kept in registers, so that a workgroup reads up to 16
+// kThreads rows once.  (A row a thread in rounds, with a ballot and a sum for each: 61 us for 16000 rows and 16 for 1088.)
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void k_evict_pick(const EvictArgs a) {
+  constexpr int kWaves = kThreads / 64, kRows = kScaleRows * kThreads, kCopies = 4;
+  __shared__ uint32_t counts[kCopies][256 + 8];       // of digits: lanes of the same one meet less often in four
+  __shared__ uint32_t chosen[3];                      // digit, rows above it, rows that have it
+  __shared__ uint32_t sums[3][kWaves];
   const int item = blockIdx.x, b = item / a.kv_heads, h = item % a.kv_heads, tid = threadIdx.x;
   const int n = rows_of(a, b);
   if (h == 0 && tid == 0 && a.lens_out != a.lens) a.lens_out[b] = n ? a.keep : a.lens[b];
-  if (n == 0) {
-    return;                          // (the moves do not look either)
-  }
+  if (n == 0) return;                                 // (the moves do not look either)
   const int from = a.first, to = n - a.recent;        // the free rows
   const int want = a.keep - a.first - a.recent;       // how many of them stay: fewer than there are
-  auto key_of = [&](int j) -> uint32_t {
-    const int64_t row = cache_row(a, b, h, j);
-    return row < 0 ? 0 : order_of(ldg<float>(a.weights + row));
+  const int base0 = from / kScaleRows * kScaleRows;
+  uint32_t key[kScaleRows], is_free = 0;              // of the rows from `row0` on; a bit a row
+  int held = -1, row0 = 0;
+  auto hold = [&](int base) {
+    if (held == base) return;
+    held = base;
+    row0 = base + tid * kScaleRows;
+    is_free = 0;
+    if (row0 >= to) return;
+    is_free = 0xffffu;
+    if (row0 < from) is_free &= 0xffffu << (from - row0);
+    if (to - row0 < kScaleRows) is_free &= (1u << (to - row0)) - 1;
+    const int64_t row = cache_row(a, b, h, row0);
+#pragma unroll
+    for (int i = 0; i < kScaleRows; i += 4) {
+      const f32x4 w = row < 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const f32x4_a4*>(a.weights + row + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) key[i + j] = row < 0 ? 0 : order_of(w[j]);
+    }
   };
-  // the want-th largest key: `high` digits known, `left` rows to find among those that share them
+  // the want-th largest key: the digits from `shift` on known, `left` rows to find among those that share them
   uint32_t cut = 0;
   int left = want;
-  if (want > 0)
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) counts[tid] = 0;
-      __syncthreads();
-      for (int j = from + tid; j < to; j += kPickThreads) {
-        const uint32_t k = key_of(j);
-        if (shift == 24 || (k ^ cut) >> (shift + 8) == 0) atomicAdd(&counts[k >> shift & 255], 1u);
-      }
-      __syncthreads();
-      if (tid < 64) {                                 // lane i: digits 255 - 4 i and the three below
-        uint32_t c[4], sum = 0;
-        for (int i = 0; i < 4; ++i) sum += c[i] = counts[255 - 4 * tid - i];
-        uint32_t up = sum;
-        for (int s = 1; s < 64; s <<= 1) {
-          const uint32_t v = __shfl_up(up, s, 64);
-          if (tid >= s) up += v;
-        }
-        uint32_t above = up - sum;                    // rows with larger digits
-        for (int i = 0; i < 4; ++i) {
-          if (above < static_cast<uint32_t>(left) && above + c[i] >= static_cast<uint32_t>(left)) {
-            chosen[0] = 255 - 4 * tid - i;
-            chosen[1] = above;
-          }
-          above += c[i];
-        }
-      }
-      __syncthreads();
-      cut |= chosen[0] << shift;
-      left -= static_cast<int>(chosen[1]);
+  for (int shift = 24; left > 0 && shift >= 0; shift -= 8) {
+    for (int i = tid; i < kCopies * (256 + 8); i += kThreads) (&counts[0][0])[i] = 0;
+    __syncthreads();
+    for (int base = base0; base < to; base += kRows) {
+      hold(base);
+#pragma unroll
+      for (int i = 0; i < kScaleRows; ++i)
+        if ((is_free >> i & 1) && (shift == 24 || (key[i] ^ cut) >> (shift + 8) == 0))
+          atomicAdd(&counts[tid & (kCopies - 1)][key[i] >> shift & 255], 1u);
     }
+    __syncthreads();
+    if (tid < 64) {                                   // lane i: digits 255 - 4 i and the three below
+      uint32_t c[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = 0;
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) c[i] += counts[k][255 - 4 * tid - i];
+        sum += c[i];
+      }
+      uint32_t up = sum;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t v = __shfl_up(up, s, 64);
+        if (tid >= s) up += v;
+      }
+      uint32_t above = up - sum;                      // rows with larger digits
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (above < static_cast<uint32_t>(left) && above + c[i] >= static_cast<uint32_t>(left)) {
+          chosen[0] = 255 - 4 * tid - i;
+          chosen[1] = above;
+          chosen[2] = c[i];
+        }
+        above += c[i];
+      }
+    }
+    __syncthreads();
+    cut |= chosen[0] << shift;
+    left -= static_cast<int>(chosen[1]);
+    if (static_cast<int>(chosen[2]) == left && cut != 0) {   // all rows with these digits stay: no need for the others
+      --cut;
+      left = 0;
+    }
+  }
   // rows above the cut stay, and the first `left` of those at it
-  Scan scan{waves};
   int32_t *holes = a.holes + item * a.most, *fills = a.fills + item * a.most;
   EvictBlock* list = a.blocks + item * a.most;
   const int middle = a.keep - a.recent;
   const int bound = a.k_scale ? (a.keep + kScaleRows - 1) / kScaleRows * kScaleRows : a.keep;   // rows that a move may write
   int equal = 0, hole = 0, fill = 0, near = 0, blocks = 0;
-  for (int j0 = from / kScaleRows * kScaleRows; j0 < to; j0 += kPickThreads) {
-    const int j = j0 + tid;
-    const bool is_free = j >= from && j < to;
-    const uint32_t k = is_free ? key_of(j) : 0;
-    const bool tie = is_free && want > 0 && k == cut;
-    int own;
-    const int ties = scan(tie, own);
-    const bool stays = is_free && want > 0 && (k > cut || (tie && equal + own < left));
-    equal += ties;
-    const bool is_hole = is_free && j < middle && !stays, is_fill = stays && j >= middle;
-    const int new_holes = scan(is_hole, own);
-    if (a.k_scale) {
-      const uint32_t mask = static_cast<uint32_t>(__ballot(is_hole) >> (tid & 48)) & 0xffffu;
-      const bool leads = is_hole && (mask & ((1u << (tid & 15)) - 1)) == 0;
-      int at;
-      const int new_blocks = scan(leads, at);
-      if (leads && blocks + at < a.most) list[blocks + at] = EvictBlock{j / kScaleRows, hole + own, mask, 0};
-      blocks += new_blocks;
-    } else if (is_hole && hole + own < a.most) {
-      holes[hole + own] = j;
+  for (int base = base0; base < to; base += kRows) {
+    hold(base);
+    uint32_t stay = 0, ties = 0;
+    if (is_free) {
+#pragma unroll
+      for (int i = 0; i < kScaleRows; ++i) {
+        stay |= key[i] > cut ? 1u << i : 0;
+        ties |= key[i] == cut ? 1u << i : 0;
+      }
+      stay = want > 0 ? stay & is_free : 0;
+      ties &= is_free;
     }
-    hole += new_holes;
-    const int new_fills = scan(is_fill, own);
-    if (is_fill && fill + own < a.most) fills[fill + own] = j;
-    fill += new_fills;
-    near += scan(is_fill && j < bound, own);
+    if (left > 0) {
+      uint32_t all;
+      int before = equal + static_cast<int>(before_me<kWaves>(__popc(ties), all, sums[0]));
+      equal += static_cast<int>(all);
+      for (; ties && before < left; ++before, ties &= ties - 1) stay |= ties & -ties;
+    }
+    // rows in front of middle, and of `bound`, in this thread's block
+    auto up_to = [&](int end) { return end <= row0 ? 0u : end - row0 >= kScaleRows ? 0xffffu : (1u << (end - row0)) - 1; };
+    const uint32_t front = up_to(middle), gone = is_free & front & ~stay, come = stay & ~front;
+    uint32_t all, others;
+    const uint32_t before = before_me<kWaves>(__popc(gone) | __popc(come) << 16, all, sums[1]);
+    const uint32_t more = before_me<kWaves>((gone ? 1 : 0) | __popc(come & up_to(bound)) << 16, others, sums[2]);
+    int at_hole = hole + static_cast<int>(before & 0xffff), at_fill = fill + static_cast<int>(before >> 16);
+    if (a.k_scale) {
+      const int at = blocks + static_cast<int>(more & 0xffff);
+      if (gone && at < a.most) list[at] = EvictBlock{row0 / kScaleRows, at_hole, gone, 0};
+    } else {
+      for (uint32_t m = gone; m; m &= m - 1, ++at_hole)
+        if (at_hole < a.most) holes[at_hole] = row0 + __ffs(static_cast<int>(m)) - 1;
+    }
+    for (uint32_t m = come; m; m &= m - 1, ++at_fill)
+      if (at_fill < a.most) fills[at_fill] = row0 + __ffs(static_cast<int>(m)) - 1;
+    hole += static_cast<int>(all & 0xffff);
+    fill += static_cast<int>(all >> 16);
+    blocks += static_cast<int>(others & 0xffff);
+    near += static_cast<int>(others >> 16);
+    __syncthreads();                                  // sums have been read
   }
   if (tid == 0) a.counts[item] = EvictCounts{hole, near, blocks, 0};
 }
@@ -212,12 +261,11 @@ __global__ __launch_bounds__(kMoveThreads) void k_evict_move(const EvictArgs a) 
   if (n == 0) return;
   const EvictCounts count = a.counts[item];
   const int32_t *holes = a.holes + item * a.most, *fills = a.fills + item * a.most;
-  // slice 0: what comes from the first rows and the last rows; all: their share of the others
-  const int free = count.holes - count.near;
-  const int i0 = count.near + static_cast<int>(static_cast<int64_t>(free) * slice / a.slices);
-  const int i1 = count.near + static_cast<int>(static_cast<int64_t>(free) * (slice + 1) / a.slices);
-  move_rows<D>(a, b, h, n, holes, fills, i0, i1, false);
-  if (slice == 0) move_rows<D>(a, b, h, n, holes, fills, 0, count.near, true);
+  // slice 0: what comes from the first rows, then the last rows; all: their share of the others
+  const int64_t free = count.holes - count.near;
+  const int i0 = slice ? count.near + static_cast<int>(free * slice / a.slices) : 0;
+  const int i1 = count.near + static_cast<int>(free * (slice + 1) / a.slices);
+  move_rows<D>(a, b, h, n, holes, fills, i0, i1, slice == 0);
 }
 
 // In 8 bits, by blocks: a wave takes a block's 16 rows of K or of V, four lanes a row, so that their largest scale stays
@@ -311,9 +359,8 @@ __global__ __launch_bounds__(kMoveThreads) void k_evict_move_codes(const EvictAr
     }
   };
   const int64_t free = listed - near;
-  some(near + static_cast<int>(free * slice / a.slices), near + static_cast<int>(free * (slice + 1) / a.slices));
+  some(slice ? near + static_cast<int>(free * slice / a.slices) : 0, near + static_cast<int>(free * (slice + 1) / a.slices));
   if (slice) return;
-  some(0, near);
   __syncthreads();                                    // their reads, before the window's writes
   for (int i0 = window; i0 < blocks; i0 += kAhead * kPairs) {
     CodeBlock<D> x[kAhead];
@@ -356,11 +403,13 @@ EvictPlan plan_of(const dsk_evict_desc& d, const dsk_kv_cache& c, bool codes) {
 }
 
 // Workgroups of the moves, at least about.
-constexpr int kMoveBlocks = 1024, kMostSlices = 32;
+constexpr int kMoveBlocks = 512, kMostSlices = 16;
 
 template <int D>
 void launch_evict_d(const EvictArgs& a, int items, hipStream_t s) {
-  launch_kernel(k_evict_pick, items, kPickThreads, 0, s, a);
+  // a table row that 256 threads hold at once needs no more
+  if ((static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) <= 256 * kScaleRows) launch_kernel(k_evict_pick<256>, items, 256, 0, s, a);
+  else launch_kernel(k_evict_pick<1024>, items, 1024, 0, s, a);
   launch_kernel(a.k_scale ? k_evict_move_codes<D> : k_evict_move<D>, items * a.slices, kMoveThreads, 0, s, a);
 }
 
