@@ -26,7 +26,7 @@
 // side by side in the banks) spreads those 16 pieces over all banks.
 #pragma once
 
-#include "attn.h"
+#include "kv8.h"
 
 namespace dsk {
 
@@ -391,6 +391,145 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
   bf16x8 p[2 * KT];
   weights(s, p);
   values(lds + (NS + j % NS) * kTile, p);
+}
+
+// flash for keys and values in 8 bits of which every row sees the first n_keys (a prefix): four waves, 32 rows each.
+// rows(tile, &k, &v, &k_scale, &v_scale) gives the wave's 16 rows of a tile, D codes each and one scale, and returns how many
+// rows after the first may be read.  Codes come to registers a step ahead, and go to LDS as the bf16 that flash
+// reads, so every wave converts a quarter of a tile once for all.  A NaN is seen by all rows, so nothing is kept
+// from any.
+template <int D, class Rows>
+__device__ __forceinline__ void flash_codes(const bf16x8 (&q)[D / 16], int t0, int t1, int n_keys, float c2, char* lds, Rows rows,
+                                            FlashRows<D>& st) {
+  t0 = __builtin_amdgcn_readfirstlane(t0);
+  t1 = __builtin_amdgcn_readfirstlane(t1);
+  if (t0 >= t1) return;
+  constexpr int NW = 4, KS = D / 16, WR = kFlKeys / NW, CH = D / 16, RPI = 64 / CH, NI = WR / RPI, kTile = kFlKeys * D * 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hf = lane >> 5, l16 = lane & 15;
+  struct Raw { u32x4 c[NI]; float scale; };
+  Raw rk, rv;
+  auto load = [&](int t, bool is_v, Raw& raw) {
+    const uint8_t *kp, *vp;
+    float ks, vs;
+    const int last = rows(t, kp, vp, ks, vs);
+    raw.scale = is_v ? vs : ks;
+    const uint8_t* p = uniform_ptr(is_v ? vp : kp);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) raw.c[i] = ldg16(p + min(i * RPI + lane / CH, last) * D + 16 * (lane % CH));
+  };
+  // to tile t's buffer, of K or V
+  auto put = [&](int t, bool is_v, const Raw& raw) {
+    char* tile = lds + ((is_v ? kFlBuffers : 0) + (t - t0) % kFlBuffers) * kTile;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = wave * WR + i * RPI + lane / CH, swz = is_v ? swz_v<D>(r) : swz_k<D>(r);
+      u32x2 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = codes_to_bf16(raw.c[i][j], raw.scale);
+      char* row = tile + r * D * 2;
+      *reinterpret_cast<u32x4*>(row + 16 * ((2 * (lane % CH)) ^ swz)) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+      *reinterpret_cast<u32x4*>(row + 16 * ((2 * (lane % CH) + 1) ^ swz)) = u32x4{w[2][0], w[2][1], w[3][0], w[3][1]};
+    }
+  };
+  auto value_frag = [&](const char* vl, int s4, int dt) {
+    const int r0 = 16 * s4 + 4 * hf + (l16 >> 2);
+    const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    const u32x2 lo = read_tr(vl + r0 * D * 2 + 16 * (c ^ swz_v<D>(r0)) + 8 * (l16 & 1));
+    const u32x2 hi = read_tr(vl + (r0 + 8) * D * 2 + 16 * (c ^ swz_v<D>(r0 + 8)) + 8 * (l16 & 1));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto scores = [&](int t, f32x16 (&s)[2]) {
+    const char* kl = lds + (t - t0) % kFlBuffers * kTile;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = f32x16{};
+      const int row = 32 * kt + n;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[kt] = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(kl + row * D * 2 + 16 * ((2 * ks + hf) ^ swz_k<D>(row)))), q[ks], s[kt]);
+    }
+  };
+  auto top_of = [&](const f32x16 (&s)[2]) {
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+    return max_across32(top) * c2;
+  };
+  // as in flash
+  auto attend = [&](int t, float top, const f32x16 (&s)[2]) {
+    if (__any(top > st.m + 8.0f)) {
+      const float mn = fmaxf(st.m, top);
+      const float f = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
+      st.m = mn;
+      st.l *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= f;
+    }
+    const float mu = st.m == kNegInf ? 0.0f : st.m;
+    const char* vl = lds + (kFlBuffers + (t - t0) % kFlBuffers) * kTile;
+    float even = 0.0f, odd = 0.0f;
+#pragma unroll
+    for (int s4 = 0; s4 < 4; ++s4) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = pack_bf16(__builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i] * c2 - mu),
+                         __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu));
+      even = add_bf16_pair(w[0], even);
+      odd = add_bf16_pair(w[1], odd);
+      even = add_bf16_pair(w[2], even);
+      odd = add_bf16_pair(w[3], odd);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = mfma32(as_bf16x8(value_frag(vl, s4, dt)), as_bf16x8(w), st.o[dt]);
+    }
+    st.l += even + odd;
+  };
+  // LDS writes are done, then the workgroup's barrier; loads to registers may be on their way
+  auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+  load(t0, false, rk);
+  load(t0, true, rv);
+  put(t0, false, rk);
+  put(t0, true, rv);
+  if (t0 + 1 < t1) {
+    load(t0 + 1, false, rk);
+    load(t0 + 1, true, rv);
+    put(t0 + 1, false, rk);
+  }
+  if (t0 + 2 < t1) load(t0 + 2, false, rk);
+  barrier();
+  // Between two barriers: tile t + 1's scores and tile t's values are read; K of t + 2 and V of t + 1, which have come to
+  // registers, are put where those of t and t - 1 were, and the next are asked for.
+  f32x16 s[2];
+  scores(t0, s);
+  float top = top_of(s);
+  for (int t = t0; t + 1 < t1; ++t) {
+    barrier();                       // K of t has been read, V of t - 1 too
+    f32x16 next[2];
+    scores(t + 1, next);
+    attend(t, top, s);
+    put(t + 1, true, rv);
+    if (t + 2 < t1) {
+      put(t + 2, false, rk);
+      load(t + 2, true, rv);
+      if (t + 3 < t1) load(t + 3, false, rk);
+    }
+    top = top_of(next);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) s[kt] = next[kt];
+  }
+  barrier();
+  const int last = t1 - 1;
+  if (last * kFlKeys + kFlKeys > n_keys) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (last * kFlKeys + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) >= n_keys) s[kt][i] = kNegInf;
+    top = top_of(s);
+  }
+  attend(last, top, s);
 }
 
 // The two waves of 32 rows (KH 2) put their keys together: afterwards both have the

@@ -43,7 +43,6 @@
 #include <type_traits>
 
 #include "attn_core.h"
-#include "kv8.h"
 
 namespace dsk {
 namespace {
@@ -52,8 +51,12 @@ constexpr int kPgThreads = 256;
 // Keys of a wave's step: the bytes in flight are the same with codes of half the size.
 template <bool F8>
 constexpr int step_keys() { return F8 ? 64 : 32; }
+// Units, of which shares are made: 128 keys (a step of each of four waves, of two in 8 bits).
+constexpr int kPgUnit = 128;
+// Units that an item counts for beside its keys'.  It has a start and an end of its own, 4 us; of half the bytes
+// a share of short items would take longest (64 sequences of 1 to 8192 keys in 8 bits: TODO).
 template <bool F8>
-constexpr int unit_keys() { return 4 * step_keys<F8>(); }   // keys of a unit: a step of each of four waves
+constexpr uint32_t item_units() { return F8 ? 1 : 0; }
 constexpr int kPgShort = 512;       // keys of a table row that one workgroup takes alone
 constexpr int kPgShortMany = 1024;  // where there are kPgMany items
 constexpr int kPgMany = 512;
@@ -78,7 +81,6 @@ struct PagedArgs {
   int32_t batch, q_len, kv_heads, group, prefix, shares, splits;
   int32_t row_tiles, prefix_blocks; // of the prefix: tiles of all rows, workgroups
   const uint8_t *k_scale, *v_scale; // of a cache in 8 bits
-  uint16_t *pre_k, *pre_v;          // of such a cache, the prefix's pages as bf16
   float* weights;                   // of the cache's rows, to be added to, or null; then also:
   float* scores;                    // [item][key of the table row][M], times c
   float* lse;                       // [item][M]: log2 of the sum of 2^score (infinite: the row sees no key)
@@ -90,10 +92,9 @@ __device__ __forceinline__ int length_of(const PagedArgs& a, int b, bool& bad) {
   bad = n > cap;
   return min(max(n, 0), cap);
 }
-template <int U>
-__device__ __forceinline__ int units_of(const PagedArgs& a, int b) {
-  bool bad;
-  return (length_of(a, b, bad) + U - 1) / U;
+template <bool F8>
+__device__ __forceinline__ uint32_t units_of(int len) {
+  return len > 0 ? (len + kPgUnit - 1) / kPgUnit + item_units<F8>() : 0;
 }
 
 template <int V>
@@ -116,10 +117,11 @@ __device__ __forceinline__ uint32_t sum_up_to_lane(uint32_t v) {
 // Units of one key head, 64 sequences at a time: lane's own, and up to its own.
 // Fewer than 2^31 in all, times the key heads too.
 struct Units { uint32_t own, up_to; };
-template <int U>
+template <bool F8>
 __device__ __forceinline__ Units units_at(const PagedArgs& a, int b0) {
   const int b = b0 + (threadIdx.x & 63);
-  const uint32_t n = b < a.batch ? units_of<U>(a, b) : 0;
+  bool bad;
+  const uint32_t n = b < a.batch ? units_of<F8>(length_of(a, b, bad)) : 0;
   return Units{n, sum_up_to_lane(n)};
 }
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
@@ -177,25 +179,25 @@ struct SegLds {
   float ml[W][16 * RT][2];
 };
 
-// Lane T i + kt: the page of the wave's 16-key tile kt of T in step kk + i (the table row's
-// last one behind its end; the sequence's length need not be known yet).
+// Lane T i + kt: the page of the wave's 16-key tile kt of T in step kk + i of those that begin at
+// tile `tile0` (the table row's last one behind its end; the sequence's length need not be known yet).
 template <int W, int T>
-__device__ __forceinline__ int page_ids(const PagedArgs& a, int b, int kk) {
+__device__ __forceinline__ int page_ids(const PagedArgs& a, int b, int tile0, int kk) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t tile = (static_cast<int64_t>(kk) + lane / T) * (T * W) + T * wave + lane % T;
+  const int64_t tile = tile0 + (static_cast<int64_t>(kk) + lane / T) * (T * W) + T * wave + lane % T;
   const int page = static_cast<int>(min(tile >> (a.c.page_shift - 4), static_cast<int64_t>(a.c.max_pages - 1)));
   return ldg<int32_t>(a.c.table + b * a.c.table_stride + page);
 }
 
-// Units [k0, k1) of the keys of item (b, h), in units of a step of W waves, for the rows from
+// Keys [start, stop) of item (b, h), whole steps of a wave, for the rows from
 // r0 on: to `out` (slot < 0: they are all of the item's) or to the partial rows of `slot`.
-// first_ids: page_ids of k0.
+// first_ids: page_ids of start.
 //
 // F8: a cache in 8 bits.  A lane's piece of a key is D / 4 codes, of which product ks takes 8 (queries
 // are held in the same order), so that K too comes in 16-byte loads; a 16-key tile is a block of one scale, which the
 // conversion to bf16 applies.  kWeigh: scores are kept for k_key_weights.
 template <int D, int RT, int W, bool F8, bool kWeigh>
-__device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int len, bool bad_len, int r0, int k0, int k1,
+__device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int len, bool bad_len, int r0, int start, int stop,
                                         int64_t slot, int first_ids, SegLds<D, RT, W>& lds) {
   using S = Step<D, F8>;
   constexpr int VW = D / 16, KS = D / 32, kKeys = step_keys<F8>(), kUnit = kKeys * W, T = S::kTiles;
@@ -224,16 +226,18 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     }
 
     const int32_t* trow = a.c.table + b * a.c.table_stride;
-    const int last_tile = (len - 1) >> 4;
-    int ids = first_ids, ids0 = k0;   // lane T i + kt: the page of tile kt of step ids0 + i
+    const int last_tile = (len - 1) >> 4, first_tile = start >> 4;
+    stop = min(stop, len);
+    const int k1 = (stop - start + kUnit - 1) / kUnit;   // steps of W waves
+    int ids = first_ids, ids0 = 0;    // lane T i + kt: the page of tile kt of step ids0 + i
     int bad_tile = INT32_MAX;         // the lane's first 16 keys on a page outside the cache
     // F8: scale bytes of the lane's tile, and those of the ids before, which a step may still need
     uint32_t k_byte = 0, v_byte = 0, old_k_byte = 0, old_v_byte = 0;
-    int old0 = k0;
+    int old0 = 0;
     auto check_ids = [&]() {
-      const int step = ids0 + lane / T, tile = step * (T * W) + T * wave + lane % T;
+      const int tile = first_tile + (ids0 + lane / T) * (T * W) + T * wave + lane % T;
       const bool out_of = ids < 0 || ids >= a.c.n_pages;
-      if (out_of && step < k1 && tile <= last_tile) bad_tile = min(bad_tile, tile);
+      if (out_of && tile * 16 < stop) bad_tile = min(bad_tile, tile);
       if (out_of) ids = 0;
       if constexpr (F8) {
         const int64_t at = ((static_cast<int64_t>(ids) * a.kv_heads + h) << (a.c.page_shift - 4)) +
@@ -249,11 +253,11 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
       if (kk - ids0 >= 64 / T) {
         old0 = ids0;
         ids0 = kk;
-        ids = page_ids<W, T>(a, b, kk);
+        ids = page_ids<W, T>(a, b, first_tile, kk);
         check_ids();
       }
-      const int tile0 = kk * (T * W) + T * wave;
-      if (tile0 > last_tile) return;                  // none of the wave's keys in this step
+      const int tile0 = first_tile + kk * (T * W) + T * wave;
+      if (tile0 * 16 >= stop) return;                 // none of the wave's keys in this step
 #pragma unroll
       for (int kt = 0; kt < T; ++kt) {
         const int tile = min(tile0 + kt, last_tile);
@@ -281,7 +285,7 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     // products then leave them out)
     auto add_nonfinite = [&](int kk) {
 #pragma unroll 1
-      for (int key = kk * kUnit + kKeys * wave, end = min(key + kKeys, len); key < end; ++key) {
+      for (int key = start + kk * kUnit + kKeys * wave, end = min(key + kKeys, len); key < end; ++key) {
         int id = ldg<int32_t>(trow + (key >> a.c.page_shift));
         if (id < 0 || id >= a.c.n_pages) id = 0;
         const int in_page = key & ((1 << a.c.page_shift) - 1);
@@ -304,8 +308,8 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
       }
     };
     auto compute = [&](const S& s, int kk) {
-      const int key0 = kk * kUnit + kKeys * wave;
-      if (key0 >= len) return;
+      const int key0 = start + kk * kUnit + kKeys * wave;
+      if (key0 >= stop) return;
       const bool masked = key0 + kKeys - 1 > len - a.q_len;
       float k_scale[T], v_scale[T];
       bool good_scales = true;
@@ -322,107 +326,106 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
           v_scale[kt] = scale_of(byte);
         }
       }
-      bf16x8 p[RT][T / 2], rest[RT][T / 2];   // the weights: bf16, and what that rounds off
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        f32x4 x[T];
-#pragma unroll
-        for (int kt = 0; kt < T; ++kt) {
-          x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            u32x4 key;
-            if constexpr (F8) {
-              const u32x4 c = s.k[kt][ks / 2];
-              const u32x2 lo = codes_to_bf16(c[2 * (ks & 1)], k_scale[kt]), hi = codes_to_bf16(c[2 * (ks & 1) + 1], k_scale[kt]);
-              key = u32x4{lo[0], lo[1], hi[0], hi[1]};
-            } else {
-              key = s.k[kt][ks];
-            }
-            x[kt] = mfma16(as_bf16x8(key), q[rt][ks], x[kt]);
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int kt = 0; kt < T; ++kt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (key0 + 16 * kt + 4 * g + r > lim[rt]) x[kt][r] = kNegInf;
-        }
-        if constexpr (kWeigh) {
-          const int row = r0 + 16 * rt + n16;
-          const int64_t item = static_cast<int64_t>(b) * a.kv_heads + h;
-          float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + key0) * M + row;
-          if (row < M)
-#pragma unroll
-            for (int kt = 0; kt < T; ++kt)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int i = 16 * kt + 4 * g + r;
-                if (key0 + i < len) to[static_cast<int64_t>(i) * M] = x[kt][r] * a.c2;
-              }
-        }
-        float top = kNegInf;
-#pragma unroll
-        for (int kt = 0; kt < T; ++kt) top = fmaxf(top, fmaxf(fmaxf(x[kt][0], x[kt][1]), fmaxf(x[kt][2], x[kt][3])));
-        top = max_across32(max_across16(top)) * a.c2;
-        // the reference point follows the maximum once it lags by more than 2^8
-        if (__any(top > m[rt] + 8.0f)) {
-          const float mn = fmaxf(m[rt], top);
-          const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
-          m[rt] = mn;
-          l[rt] *= f;
-#pragma unroll
-          for (int t = 0; t < VW; ++t) o[rt][t] *= f;
-        }
-        const float mu = m[rt] == kNegInf ? 0.0f : m[rt];
-        float e[4 * T];
-#pragma unroll
-        for (int i = 0; i < 4 * T; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
-          l[rt] += e[i];
-        }
-        // as the sum of two bf16: 2^-16 of each is left, far below the output's own rounding of 2^-8
-#pragma unroll
-        for (int hh = 0; hh < T / 2; ++hh) {
-          u32x4 w, u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e0 = e[8 * hh + 2 * i], e1 = e[8 * hh + 2 * i + 1];
-            w[i] = pack_bf16(e0, e1);
-            u[i] = pack_bf16(e0 - __uint_as_float(w[i] << 16), e1 - __uint_as_float(w[i] & 0xffff0000u));
-          }
-          p[rt][hh] = as_bf16x8(w);
-          rest[rt][hh] = as_bf16x8(u);
-        }
-      }
       // An infinite value times a weight's rest, which may be zero or negative, or the weight zero of a key that a
       // row does not see or of a place behind the last key (that key's values again), would be NaN: are
       // all the values finite?  The largest exponents of the pairs tell (decode_64 0.5 us more than without).
       // Codes have no infinity, and a NaN that every row sees may go through the products: there the question is
       // for the last keys alone.
-      bool finite = true;
-      if constexpr (F8) {
-        if (masked) {
+      auto all_finite = [&]() {
+        if constexpr (F8) {
+          if (!masked) return true;
           uint32_t bits = 0;
 #pragma unroll
           for (int j = 0; j < 4 * T; ++j)
 #pragma unroll
             for (int i = 0; i < S::kPieces; ++i) bits |= nan_codes(s.v[j][i]);
-          finite = good_scales && !__any(bits != 0);
+          return good_scales && !__any(bits != 0);
+        } else {
+          u16x2 largest = {0, 0};
+#pragma unroll
+          for (int j = 0; j < 4 * T; ++j)
+#pragma unroll
+            for (int i = 0; i < VW / 2; ++i)
+              largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, s.v[j][i] & 0x7f807f80u));
+          return !__any(nonfinite_bits(__builtin_bit_cast(uint32_t, largest)) != 0);
         }
-      } else {
-        u16x2 largest = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 4 * T; ++j)
-#pragma unroll
-          for (int i = 0; i < VW / 2; ++i)
-            largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, s.v[j][i] & 0x7f807f80u));
-        finite = !__any(nonfinite_bits(__builtin_bit_cast(uint32_t, largest)) != 0);
-      }
-      if (!finite) add_nonfinite(kk);
+      };
+      // 32 keys at a time
+      bool finite = true;
 #pragma unroll
       for (int hh = 0; hh < T / 2; ++hh) {
+        bf16x8 p[RT], rest[RT];       // the weights: bf16, and what that rounds off
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          f32x4 x[2];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              u32x4 key;
+              if constexpr (F8) {
+                const u32x4 c = s.k[2 * hh + kt][ks / 2];
+                const u32x2 lo = codes_to_bf16(c[2 * (ks & 1)], k_scale[2 * hh + kt]), hi = codes_to_bf16(c[2 * (ks & 1) + 1], k_scale[2 * hh + kt]);
+                key = u32x4{lo[0], lo[1], hi[0], hi[1]};
+              } else {
+                key = s.k[kt][ks];
+              }
+              x[kt] = mfma16(as_bf16x8(key), q[rt][ks], x[kt]);
+            }
+          }
+          if (masked) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (key0 + 32 * hh + 16 * kt + 4 * g + r > lim[rt]) x[kt][r] = kNegInf;
+          }
+          if constexpr (kWeigh) {
+            const int row = r0 + 16 * rt + n16;
+            const int64_t item = static_cast<int64_t>(b) * a.kv_heads + h;
+            const int at = key0 + 32 * hh + 4 * g;
+            float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + at) * M + row;
+            if (row < M)
+#pragma unroll
+              for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (at + 16 * kt + r < len) to[(16 * kt + r) * M] = x[kt][r] * a.c2;
+          }
+          float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                            fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+          top = max_across32(max_across16(top)) * a.c2;
+          // the reference point follows the maximum once it lags by more than 2^8
+          if (__any(top > m[rt] + 8.0f)) {
+            const float mn = fmaxf(m[rt], top);
+            const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
+            m[rt] = mn;
+            l[rt] *= f;
+#pragma unroll
+            for (int t = 0; t < VW; ++t) o[rt][t] *= f;
+          }
+          const float mu = m[rt] == kNegInf ? 0.0f : m[rt];
+          float e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
+            l[rt] += e[i];
+          }
+          // as the sum of two bf16: 2^-16 of each is left, far below the output's own rounding of 2^-8
+          u32x4 w, u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = pack_bf16(e[2 * i], e[2 * i + 1]);
+            u[i] = pack_bf16(e[2 * i] - __uint_as_float(w[i] << 16), e[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+          }
+          p[rt] = as_bf16x8(w);
+          rest[rt] = as_bf16x8(u);
+        }
+        if (hh == 0) {
+          finite = all_finite();
+          if (!finite) add_nonfinite(kk);
+        }
         u32x2 w0[VW], w1[VW];
         if constexpr (F8) {
           values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[8 * hh]), v_scale[2 * hh], w0);
@@ -436,22 +439,20 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
           } else {
             const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = __builtin_amdgcn_perm(s.v[8 * hh + 2 * i + 1][t / 2], s.v[8 * hh + 2 * i][t / 2], sel);
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(s.v[2 * i + 1][t / 2], s.v[2 * i][t / 2], sel);
           }
           if (!finite)
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            o[rt][t] = mfma16(as_bf16x8(w), rest[rt][hh], mfma16(as_bf16x8(w), p[rt][hh], o[rt][t]));
+          for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), rest[rt], mfma16(as_bf16x8(w), p[rt], o[rt][t]));
         }
       }
     };
 
     S s0, s1;
-    load(s0, k0);
-    int kk = k0;
+    load(s0, 0);
+    int kk = 0;
     for (; kk + 1 < k1; kk += 2) {
       load(s1, kk + 1);
       compute(s0, kk);
@@ -529,22 +530,39 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 // Workgroup `share` of a.shares takes its share of all units.
 template <int D, int RT, bool F8, bool kWeigh>
 __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, SegLds<D, RT, 4>& lds) {
-  constexpr int kUnit = unit_keys<F8>(), T = Step<D, F8>::kTiles;
+  constexpr int T = Step<D, F8>::kTiles;
+  constexpr uint32_t kHead = item_units<F8>();
   Units n;
   uint32_t all = 0;                  // units of one key head
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    n = units_at<kUnit>(a, b0);
+    n = units_at<F8>(a, b0);
     all += lane_value(n.up_to, 63);
   }
   const uint32_t total = all * a.kv_heads, quota = (total + a.shares - 1) / a.shares;
-  const uint32_t u0 = share * quota, u1 = min(u0 + quota, total);
-  if (u0 >= u1) return;
+  uint32_t u0, u1;
+  // in 8 bits shares that differ by one unit at most, no more of them than units
+  const uint32_t n_shares = F8 ? min(total, static_cast<uint32_t>(a.shares)) : a.shares;
+  if constexpr (F8) {
+    if (static_cast<uint32_t>(share) >= n_shares) return;
+    const uint32_t each = total / n_shares, rest = total % n_shares;   // rest * share: below 2^18
+    u0 = share * each + share * rest / n_shares;
+    u1 = (share + 1) * each + (share + 1) * rest / n_shares;
+  } else {
+    u0 = share * quota;
+    u1 = min(u0 + quota, total);
+    if (u0 >= u1) return;
+  }
+  // the share that a unit lies in
+  auto share_of = [&](uint32_t u) {
+    if constexpr (F8) return static_cast<int>((static_cast<double>(u + 1) * n_shares - 1.0) / static_cast<double>(total));
+    else return static_cast<int>(u / quota);
+  };
   // the sequence that u0 lies in, and the units of one key head in those before it
   const uint32_t first_unit = u0 / a.kv_heads;
   uint32_t before = 0;
   int b = a.batch;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (a.batch > 64) n = units_at<kUnit>(a, b0);
+    if (a.batch > 64) n = units_at<F8>(a, b0);
     const uint64_t past = __ballot(before + n.up_to > first_unit);
     if (past) {
       const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
@@ -557,7 +575,7 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
   for (uint32_t u = u0; u < u1 && b < a.batch;) {
     bool bad_len;
     const int len = length_of(a, b, bad_len);
-    const uint32_t nb = (len + kUnit - 1) / kUnit, first = before * a.kv_heads;
+    const uint32_t nb = units_of<F8>(len), first = before * a.kv_heads;
     if (nb == 0 || u >= first + nb * a.kv_heads) {
       before += nb;
       ++b;
@@ -565,16 +583,17 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
     }
     // an item's first unit is kv_heads * before + h * its units
     const int h = static_cast<int>((u - first) / nb);
-    const uint32_t item0 = first + h * nb;
-    const int k0 = static_cast<int>(u - item0), k1 = static_cast<int>(min(nb, u1 - item0));
-    const bool whole = k0 == 0 && k1 == static_cast<int>(nb);
+    const uint32_t item0 = first + h * nb, begin = u, end = min(item0 + nb, u1);
+    u = end;
+    const int k0 = static_cast<int>(max(begin, item0 + kHead) - item0 - kHead), k1 = static_cast<int>(end - item0) - static_cast<int>(kHead);
+    if (k0 >= k1) continue;          // none of its keys: the next share begins with them
+    const bool whole = k0 == 0 && end == item0 + nb;
     const int64_t slot = whole ? (a.splits ? 2 * static_cast<int64_t>(a.shares) + static_cast<int64_t>(b) * a.kv_heads + h : -1)
-                               : 2 * static_cast<int64_t>(share) + (u == u0 ? 0 : 1);
+                               : 2 * static_cast<int64_t>(share) + (begin == u0 ? 0 : 1);
     if (k0 == 0 && r0 == 0 && threadIdx.x == 0)
       a.parts[b * a.kv_heads + h] =
-          i32x2{static_cast<int>(slot), whole ? (a.splits ? 1 : 0) : static_cast<int>((item0 + nb - 1) / quota) - share + 1};
-    segment<D, RT, 4, F8, kWeigh>(a, b, h, len, bad_len, r0, k0, k1, slot, page_ids<4, T>(a, b, k0), lds);
-    u = item0 + k1;
+          i32x2{static_cast<int>(slot), whole ? (a.splits ? 1 : 0) : share_of(item0 + nb - 1) - share + 1};
+    segment<D, RT, 4, F8, kWeigh>(a, b, h, len, bad_len, r0, k0 * kPgUnit, k1 * kPgUnit, slot, page_ids<4, T>(a, b, k0 * (kPgUnit / 16), 0), lds);
   }
 }
 
@@ -612,24 +631,38 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
   for (int c0 = t0; c0 < t1; c0 += kPreChunk) {
     const int c1 = min(c0 + kPreChunk, t1), row = wave * (kFlKeys / kPreWaves);
     const int key = min((c0 + lane) * kFlKeys + row, a.prefix - 1);
-    int id = key >> a.c.page_shift;
-    if constexpr (!F8) {
-      id = ldg<int32_t>(a.pages + id);
-      const bool out_of = id < 0 || id >= a.c.n_pages;
-      bad |= __ballot(out_of && c0 + lane < c1);
-      if (out_of) id = 0;
-    }
+    int id = ldg<int32_t>(a.pages + (key >> a.c.page_shift));
+    const bool out_of = id < 0 || id >= a.c.n_pages;
+    bad |= __ballot(out_of && c0 + lane < c1);
+    if (out_of) id = 0;
     const int64_t at = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))) * D;
     const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
-    auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
+    auto base_of = [&](int t) {
       const uint32_t lo = __builtin_amdgcn_readlane(at_lo, t - c0), hi = __builtin_amdgcn_readlane(at_hi, t - c0);
-      const int64_t base = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-      kp = (F8 ? a.pre_k : a.c.k) + base;
-      vp = (F8 ? a.pre_v : a.c.v) + base;
-      last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
+      return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
     };
     if (c0 > t0) __syncthreads();      // the last chunk's reads of LDS are done
-    flash<D, kPreWaves, 1>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
+    if constexpr (F8) {
+      // a wave's 16 rows of a tile are a block of one scale
+      const int k_byte = ldg<uint8_t>(a.k_scale + at / (kScaleRows * D)), v_byte = ldg<uint8_t>(a.v_scale + at / (kScaleRows * D));
+      auto src = [&](int t, const uint8_t*& kp, const uint8_t*& vp, float& ks, float& vs) {
+        const int64_t base = base_of(t);
+        kp = reinterpret_cast<const uint8_t*>(a.c.k) + base;
+        vp = reinterpret_cast<const uint8_t*>(a.c.v) + base;
+        ks = scale_of(static_cast<uint32_t>(__builtin_amdgcn_readlane(k_byte, t - c0)));
+        vs = scale_of(static_cast<uint32_t>(__builtin_amdgcn_readlane(v_byte, t - c0)));
+        return max(a.prefix - 1 - (t * kFlKeys + row), 0);
+      };
+      flash_codes<D>(q, c0, c1, a.prefix, a.c2, lds, src, st);
+    } else {
+      auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
+        const int64_t base = base_of(t);
+        kp = a.c.k + base;
+        vp = a.c.v + base;
+        last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
+      };
+      flash<D, kPreWaves, 1>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
+    }
   }
   // a page outside the cache: the waves load different rows, so all tell
   const bool any_bad = __syncthreads_or(bad != 0);
@@ -679,13 +712,12 @@ __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged_prefix(co
 template <int D, bool F8, bool kWeigh>
 __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const PagedArgs a) {
   __shared__ SegLds<D, 1, kPgShortWaves> lds;
-  constexpr int kUnit = step_keys<F8>() * kPgShortWaves;
   const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, M = a.q_len * a.group, r0 = 16 * blockIdx.y;
-  const int ids = page_ids<kPgShortWaves, Step<D, F8>::kTiles>(a, b, 0);   // on its way beside the length
+  const int ids = page_ids<kPgShortWaves, Step<D, F8>::kTiles>(a, b, 0, 0);   // on its way beside the length
   bool bad_len;
   const int len = length_of(a, b, bad_len);
   if (len > 0) {
-    segment<D, 1, kPgShortWaves, F8, kWeigh>(a, b, h, len, bad_len, r0, 0, (len + kUnit - 1) / kUnit, -1, ids, lds);
+    segment<D, 1, kPgShortWaves, F8, kWeigh>(a, b, h, len, bad_len, r0, 0, len, -1, ids, lds);
     return;
   }
   for (int i = threadIdx.x; i < (min(M, r0 + 16) - r0) * (D / 8); i += 64 * kPgShortWaves) {
@@ -827,41 +859,12 @@ __global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, i
   }
 }
 
-// The prefix's pages of a cache in 8 bits as bf16 (exact), one after the other; NaN for one outside the cache.
-template <int D>
-__global__ __launch_bounds__(kPgThreads) void k_prefix_values(const PagedArgs a) {
-  const int rows = a.kv_heads << a.c.page_shift;     // of a page, with all heads
-  const int64_t all = static_cast<int64_t>((a.prefix + (1 << a.c.page_shift) - 1) >> a.c.page_shift) * rows * (D / 16);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPgThreads + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kPgThreads) {
-    const int64_t at = i / (D / 16);                 // row of all
-    const int page = static_cast<int>(at / rows), row = static_cast<int>(at % rows), e = 16 * static_cast<int>(i % (D / 16));
-    const int id = a.pages[page];
-    const bool bad = id < 0 || id >= a.c.n_pages;
-    const int64_t from = static_cast<int64_t>(bad ? 0 : id) * rows + row, to = at * D + e;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const u32x4 c = ldg16(reinterpret_cast<const uint8_t*>(w ? a.c.v : a.c.k) + from * D + e);
-      const float scale = bad ? __builtin_nanf("") : scale_of(ldg<uint8_t>((w ? a.v_scale : a.k_scale) + from / kScaleRows));
-      u32x4 y[2];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u32x2 t = codes_to_bf16(c[j], scale);
-        y[j / 2][2 * (j & 1)] = bad ? 0x7fc07fc0u : t[0];
-        y[j / 2][2 * (j & 1) + 1] = bad ? 0x7fc07fc0u : t[1];
-      }
-      u32x4* dst = reinterpret_cast<u32x4*>((w ? a.pre_v : a.pre_k) + to);
-      dst[0] = y[0];
-      dst[1] = y[1];
-    }
-  }
-}
-
 // Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's, then
-// scores, and the prefix's pages.
+// scores.
 struct PagedPlan {
   int rt, shares, splits, row_tiles;
   bool alone;                        // k_paged_short
-  size_t po, pml, parts, pre_o, pre_ml, scores, lse, pre_k, pre_v, total;
+  size_t po, pml, parts, pre_o, pre_ml, scores, lse, total;
 };
 
 PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more) {
@@ -886,18 +889,10 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
       p.lse = up(p.scores + static_cast<size_t>(items) * keys * M * 4);
       p.total = up(p.lse + static_cast<size_t>(items) * M * 4);
     }
-    if (more.f8 && d.prefix_len > 0) {
-      const size_t pages = (d.prefix_len + static_cast<size_t>(c.page_size) - 1) / c.page_size;
-      const size_t bytes = pages * d.kv_heads * c.page_size * d.head_dim * 2;
-      p.pre_k = p.total;
-      p.pre_v = up(p.pre_k + bytes);
-      p.total = up(p.pre_v + bytes);
-    }
     return p;
   };
   if (p.alone) return add_more();
-  const int unit = more.f8 ? unit_keys<true>() : unit_keys<false>();
-  const int64_t units = items * ((keys + unit - 1) / unit);
+  const int64_t units = items * ((keys + kPgUnit - 1) / kPgUnit + (more.f8 ? item_units<true>() : item_units<false>()));
   // the workgroups that are resident at once, two a CU (64 sequences of up to 8192 keys, 8 heads
   // of 128: 81 us, 90 with 256 and 86 with 768); one a CU where registers allow no
   // more, or beside a prefix's (36.5 us with 256, 39.4 with 512, 64 sequences behind 16385 keys)
@@ -941,11 +936,6 @@ void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
     return;
   }
   if (p.splits) {
-    if constexpr (F8) {
-      const int64_t rows = static_cast<int64_t>((a.prefix + (1 << a.c.page_shift) - 1) >> a.c.page_shift) * (a.kv_heads << a.c.page_shift);
-      const int64_t blocks = (rows * (D / 16) + kPgThreads - 1) / kPgThreads;
-      launch_kernel(k_prefix_values<D>, static_cast<uint32_t>(std::min<int64_t>(blocks, 4096)), kPgThreads, 0, s, a);
-    }
     constexpr size_t lds = sizeof(SegLds<D, RT, 4>) > flash_lds<D>() ? sizeof(SegLds<D, RT, 4>) : flash_lds<D>();
     launch_kernel(k_paged_prefix<D, RT, F8, kWeigh>, a.prefix_blocks + p.shares * halves, kPgThreads, lds, s, a);
   } else {
@@ -980,8 +970,7 @@ hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const Pa
                     reinterpret_cast<float*>(w + p.pre_o), reinterpret_cast<float*>(w + p.pre_ml), prefix,
                     d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
                     d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits, p.row_tiles,
-                    p.row_tiles * p.splits * d.kv_heads, more.k_scale, more.v_scale, reinterpret_cast<uint16_t*>(w + p.pre_k),
-                    reinterpret_cast<uint16_t*>(w + p.pre_v), more.key_weights, reinterpret_cast<float*>(w + p.scores),
+                    p.row_tiles * p.splits * d.kv_heads, more.k_scale, more.v_scale, more.key_weights, reinterpret_cast<float*>(w + p.scores),
                     reinterpret_cast<float*>(w + p.lse)};
   auto form = [&](auto f8, auto weigh) {
     constexpr bool kF = decltype(f8)::value, kW = decltype(weigh)::value;

@@ -109,8 +109,8 @@ def test_workspaces_hold_what_is_asked_for():
     assert size(plain) == n.value
     # a float32 for each of 4 x 2 items, 4 rows and 2048 places
     assert size(weights) >= size(plain) + 4 * 2 * 4 * 2048 * 4
-    # the prefix's pages in bf16, keys and values
-    assert size(codes, prefix_len=100) >= size(codes) + 2 * 2 * 2 * 64 * 128 * 2
+    # the prefix's partial rows: a float32 row, a maximum and a sum for each of 4 x 8 query rows
+    assert size(codes, prefix_len=100) >= size(codes) + 4 * 8 * (128 + 2) * 4
 
 
 @pytest.mark.parametrize("kw,want", [(dict(kv_heads=0), -1), (dict(kv_heads=1025), -1), (dict(head_dim=80), -3), (dict(keep=0), -1),
