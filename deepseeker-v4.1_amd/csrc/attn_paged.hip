@@ -61,6 +61,7 @@ constexpr int kPgShort = 512;       // keys of a table row that one workgroup ta
 constexpr int kPgShortMany = 1024;  // where there are kPgMany items
 constexpr int kPgMany = 512;
 constexpr int kPgShortWaves = 8;
+constexpr int64_t kPgFewKeys = 512 << 10;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
@@ -82,7 +83,7 @@ struct PagedArgs {
   int32_t row_tiles, prefix_blocks; // of the prefix: tiles of all rows, workgroups
   const uint8_t *k_scale, *v_scale; // of a cache in 8 bits
   float* weights;                   // of the cache's rows, to be added to, or null; then also:
-  float* scores;                    // [item][key of the table row][M], times c
+  float* scores;                    // [item][key of the table row][M rounded up to fours], times c
   float* lse;                       // [item][M]: log2 of the sum of 2^score (infinite: the row sees no key)
 };
 
@@ -385,13 +386,14 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
             const int row = r0 + 16 * rt + n16;
             const int64_t item = static_cast<int64_t>(b) * a.kv_heads + h;
             const int at = key0 + 32 * hh + 4 * g;
-            float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + at) * M + row;
+            const int stride = (M + 3) & ~3;
+            float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + at) * stride + row;
             if (row < M)
 #pragma unroll
               for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                  if (at + 16 * kt + r < len) to[(16 * kt + r) * M] = x[kt][r] * a.c2;
+                  if (at + 16 * kt + r < len) to[(16 * kt + r) * stride] = x[kt][r] * a.c2;
           }
           float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                             fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
@@ -823,38 +825,39 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
       u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
 }
 
-// Adds to every key's weight what the item's rows gave it, in their order: 2^(score - lse) of each.
-// Workgroups of an item take its keys in turn.  M float32 a key and head are written by the scores' kernel and
-// read here, against 4 D bytes of its key and value (2 D in 8 bits).
+// Adds to every key's weight what the item's rows gave it, 2^(score - lse) of each, in a fixed order: kLanes lanes take
+// a key's rows by fours, then a tree over them.  Workgroups of an item take its keys in turn.  M float32 a key and head
+// are written by the scores' kernel and read here, against 4 D bytes of its key and value (2 D in 8 bits).
 constexpr int kKwRows = 64;          // most rows of an item
 
+template <int kLanes>
 __global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, int each) {
-  __shared__ float lse[kKwRows];
+  constexpr int kKeys = kPgThreads / kLanes;
+  __shared__ __align__(16) float lse[kKwRows];
   const int item = blockIdx.x / each, part = blockIdx.x % each, b = item / a.kv_heads, h = item % a.kv_heads, M = a.q_len * a.group;
   bool bad;
   const int len = length_of(a, b, bad);
-  if (bad || len <= part * kPgThreads) return;
-  if (static_cast<int>(threadIdx.x) < M) lse[threadIdx.x] = a.lse[static_cast<int64_t>(item) * M + threadIdx.x];
+  if (bad || len <= part * kKeys) return;
+  // (no score reaches past -infinity in the rows that fill up the fours)
+  if (threadIdx.x < kKwRows)
+    lse[threadIdx.x] = static_cast<int>(threadIdx.x) < M ? a.lse[static_cast<int64_t>(item) * M + threadIdx.x] : -kNegInf;
   __syncthreads();
   const int64_t cap = static_cast<int64_t>(a.c.max_pages) << a.c.page_shift;
-  for (int key = part * kPgThreads + threadIdx.x; key < len; key += each * kPgThreads) {
+  const int lane = threadIdx.x % kLanes, stride = (M + 3) & ~3;
+  for (int key0 = part * kKeys; key0 < len; key0 += each * kKeys) {
+    const int key = min(key0 + static_cast<int>(threadIdx.x) / kLanes, len - 1);   // (all lanes go on to the tree)
     const int id = ldg<int32_t>(a.c.table + b * a.c.table_stride + (key >> a.c.page_shift));
-    const float* x = a.scores + (item * cap + key) * M;
+    const float* x = a.scores + (item * cap + key) * stride;
     float sum = 0.0f;
-    auto add = [&](float score, int r) {
-      // a key that the row does not see, whatever the row is
-      sum += score == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(score - lse[r]);
-    };
-    if (M % 4 == 0) {
-      for (int r = 0; r < M; r += 4) {
-        const f32x4 v = ldg<f32x4>(x + r);
+    for (int r = 4 * lane; r < M; r += 4 * kLanes) {
+      const f32x4 v = ldg<f32x4>(x + r), e = *reinterpret_cast<const f32x4*>(&lse[r]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) add(v[i], r + i);
-      }
-    } else {
-      for (int r = 0; r < M; ++r) add(ldg<float>(x + r), r);
+      for (int i = 0; i < 4; ++i)                     // nothing of a key that the row does not see, whatever the row is
+        if (r + i < M && v[i] != kNegInf) sum += __builtin_amdgcn_exp2f(v[i] - e[i]);
     }
-    if (id >= 0 && id < a.c.n_pages)
+#pragma unroll
+    for (int s = kLanes / 2; s >= 1; s >>= 1) sum += __shfl_xor(sum, s, 64);
+    if (lane == 0 && key0 + static_cast<int>(threadIdx.x) / kLanes < len && id >= 0 && id < a.c.n_pages)
       a.weights[((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))] += sum;
   }
 }
@@ -871,8 +874,12 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   PagedPlan p{};
   auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
   const int64_t M = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
-  p.rt = M <= 16 ? 1 : 2;
   const int64_t items = static_cast<int64_t>(d.batch) * d.kv_heads, keys = static_cast<int64_t>(c.max_pages) * c.page_size;
+  // With scales or weights, up to kPgFewKeys places of more than 16 rows: 16 rows a workgroup, two a CU, read the cache
+  // once more but wait less.  8 key heads of 128, weights in 8 bits: one sequence of 8000 keys and three of 300, 64 rows, 39 us, 44 with 32 rows a
+  // workgroup, 32 rows 36 and 40; four of 8000, 64 rows, 75 and 72; 64 of 4000, 32 rows, 398 and 318.
+  const bool extra = more.f8 || more.weigh, few = extra && items * keys <= kPgFewKeys;
+  p.rt = M <= 16 || few ? 1 : 2;
   // Up to kPgShort keys are two steps of a workgroup of eight waves, whose loads are all in flight at once: one
   // sequence with 8 key heads of 128 takes 7.3 us for 260 keys, with shares and their join
   // 9.3, but 9.9 against 9.3 for 517 and 14.6 against 9.3 for 1000.  Where items fill the
@@ -886,7 +893,7 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   auto add_more = [&]() {
     if (more.weigh) {
       p.scores = p.total;
-      p.lse = up(p.scores + static_cast<size_t>(items) * keys * M * 4);
+      p.lse = up(p.scores + static_cast<size_t>(items) * keys * ((M + 3) & ~int64_t{3}) * 4);
       p.total = up(p.lse + static_cast<size_t>(items) * M * 4);
     }
     return p;
@@ -896,7 +903,10 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   // the workgroups that are resident at once, two a CU (64 sequences of up to 8192 keys, 8 heads
   // of 128: 81 us, 90 with 256 and 86 with 768); one a CU where registers allow no
   // more, or beside a prefix's (36.5 us with 256, 39.4 with 512, 64 sequences behind 16385 keys)
-  const int64_t most = p.rt == 1 && d.prefix_len == 0 ? 512 : 256;
+  // (with scales or weights, workgroups for all rows of a share are resident at once: 4 sequences of up to 8000 keys with 64
+  // rows 63 us with 256 shares of two workgroups, 49 with 128)
+  const int64_t each = extra && (M > 32 || few) ? (M + 16 * p.rt - 1) / (16 * p.rt) : 1;
+  const int64_t most = (p.rt == 1 && d.prefix_len == 0 ? 512 : 256) / each;
   p.shares = static_cast<int>(units < most ? units : most);
   const int64_t rows = static_cast<int64_t>(d.batch) * M;
   if (d.prefix_len > 0) {
@@ -922,7 +932,8 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   return add_more();
 }
 
-// Workgroups of k_key_weights, at least about.
+// Workgroups of k_key_weights, at least about, for a lane a key (of 16 lanes a key four times as many: 11.1 -> 9.3 us for 64 rows
+// of four sequences of up to 8000 keys).
 constexpr int kKwBlocks = 2048;
 
 template <int D, int RT, bool F8, bool kWeigh>
@@ -951,9 +962,10 @@ void launch_paged_d(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
   if (p.rt == 1) launch_paged_rt<D, 1, F8, kWeigh>(p, a, s);
   else launch_paged_rt<D, 2, F8, kWeigh>(p, a, s);
   if constexpr (kWeigh) {
-    const int items = a.batch * a.kv_heads, keys = a.c.max_pages << a.c.page_shift;
-    const int each = std::min((kKwBlocks + items - 1) / items, (keys + kPgThreads - 1) / kPgThreads);
-    launch_kernel(k_key_weights, items * each, kPgThreads, 0, s, a, each);
+    const int items = a.batch * a.kv_heads, M = a.q_len * a.group, lanes = M <= 4 ? 1 : M <= 16 ? 4 : 16;
+    const int keys = kPgThreads / lanes, of_row = ((a.c.max_pages << a.c.page_shift) + keys - 1) / keys;
+    const int each = std::min((kKwBlocks * (lanes == 16 ? 4 : lanes == 4 ? 2 : 1) + items - 1) / items, of_row);
+    launch_kernel(lanes == 1 ? k_key_weights<1> : lanes == 4 ? k_key_weights<4> : k_key_weights<16>, items * each, kPgThreads, 0, s, a, each);
   }
 }
 
