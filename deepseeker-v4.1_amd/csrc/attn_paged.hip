@@ -542,8 +542,8 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
   }
   const uint32_t total = all * a.kv_heads, quota = (total + a.shares - 1) / a.shares;
   uint32_t u0, u1;
-  // in 8 bits shares that differ by one unit at most, no more of them than units
-  const uint32_t n_shares = F8 ? min(total, static_cast<uint32_t>(a.shares)) : a.shares;
+  // in 8 bits shares that differ by one unit at most, of two units at least
+  const uint32_t n_shares = F8 ? max(min(total / 2, static_cast<uint32_t>(a.shares)), min(total, 1u)) : a.shares;
   if constexpr (F8) {
     if (static_cast<uint32_t>(share) >= n_shares) return;
     const uint32_t each = total / n_shares, rest = total % n_shares;   // rest * share: below 2^18
@@ -886,7 +886,7 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   // machine without shares, the join is all that they would add (64 such sequences of 600 / 1000 keys: 30.2 / 44.5 us, 31.6 / 45.9
   // with shares).
   // (a launch counts its threads in 32 bits)
-  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany ? kPgShortMany : kPgShort) &&
+  p.alone = d.prefix_len == 0 && keys <= (more.f8 ? 2 : 1) * (items >= kPgMany ? kPgShortMany : kPgShort) &&
             items * (64 * kPgShortWaves) < (int64_t{1} << 32);
   p.total = 256;
   // behind what the call needs otherwise

@@ -27,19 +27,18 @@ __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_floa
 // 2^(127 - b) for a byte that is given out.
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float(static_cast<uint32_t>(254 - byte) << 23); }
 
-__device__ __forceinline__ float finite_or(float x, float otherwise) {
-  return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? otherwise : x;
-}
-
-// Eight values times inv (a power of two) as codes, to nearest even; an infinity or NaN as NaN
-// (the type has no infinity), beyond 448 as 448.
-__device__ __forceinline__ u32x2 to_codes(const float (&x)[8], float inv) {
+// Eight values times inv (a power of two) as codes, to nearest even.  check: some may be no finite number, an
+// infinity or NaN, which are NaN then (the type has no infinity), or beyond 448, which are 448.
+__device__ __forceinline__ u32x2 to_codes(const float (&x)[8], float inv, bool check) {
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float z = fminf(fmaxf(x[i] * inv, -kMostCode), kMostCode);
-    y[i] = (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u ? __builtin_nanf("") : z;
-  }
+  for (int i = 0; i < 8; ++i) y[i] = x[i] * inv;
+  if (check)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = fminf(fmaxf(y[i], -kMostCode), kMostCode);
+      if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) y[i] = __builtin_nanf("");
+    }
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);

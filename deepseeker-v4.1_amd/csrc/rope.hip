@@ -180,6 +180,7 @@ struct CodeLds {
   int lead[kSlots];                  // first token of the block; kSkip, or kCopy: for k_out alone
   uint32_t rows[kSlots];             // of the block that begins here: its rows that the call brings
   uint32_t top[3][2][kSlots];        // largest magnitudes, of three heads in turn
+  int begin, end;                    // the slots from the first to the last that have something to do
 };
 constexpr int kSkip = -1, kCopy = -2;
 
@@ -203,64 +204,110 @@ __device__ __forceinline__ void append_codes(const QkArgs& a, int block) {
     const uint64_t starts = __ballot(tid > 0 && (key < 0 || key != before));
     const uint64_t mine = starts & ((2ull << tid) - 1);
     const int first = mine ? 62 - __clzll(static_cast<long long>(mine)) : -1;
+    const int lead = i < 0 || i >= kSlots ? kSkip : key >= 0 ? (first >= 0 && first < kWindow ? first : kSkip) : live && i < kWindow ? kCopy : kSkip;
+    const uint64_t busy = __ballot(lead != kSkip);    // bit 1 + i
     if (i >= 0 && i < kSlots) {
       s.slot[i] = slot;
       s.rows[i] = 0;
-      s.lead[i] = key >= 0 ? (first >= 0 && first < kWindow ? first : kSkip) : (live && i < kWindow ? kCopy : kSkip);
+      s.lead[i] = lead;
+    }
+    if (tid == 0) {
+      s.begin = busy ? __ffsll(static_cast<long long>(busy)) - 2 : 0;
+      s.end = busy ? 63 - __clzll(static_cast<long long>(busy)) : 0;
     }
   } else {
     for (int i = tid - 64; i < 3 * 2 * kSlots; i += 64 * (kQkWaves - 1)) (&s.top[0][0][0])[i] = 0;
   }
   __syncthreads();
   if (tid < kSlots && s.lead[tid] >= 0) atomicOr(&s.rows[s.lead[tid]], 1u << (s.slot[tid] & (kScaleRows - 1)));
-  const int half = a.rot_dim / 2;
-  for (int i = tid; i < kSlots * half; i += 64 * kQkWaves) {
-    const int64_t t = t0 + i / half;
-    if (s.lead[i / half] != kSkip) s.turn[i / half][i % half] = turn_of(a, t, a.positions[t], i % half);
+  // (a prompt's blocks begin anywhere in its windows, and are 16 slots from there: one pass of rows)
+  const int half = a.rot_dim / 2, begin = s.begin, end = s.end;
+  if (begin >= end) return;
+  for (int i = tid; i < (end - begin) * half; i += 64 * kQkWaves) {
+    const int slot = begin + i / half;
+    if (s.lead[slot] != kSkip) s.turn[slot][i % half] = turn_of(a, t0 + slot, a.positions[t0 + slot], i % half);
   }
   __syncthreads();
   const Pairs<kInter> pairs(a, lane);
-  int lead[kPasses];
-  int64_t slot[kPasses];
-  float own[kPasses][8], pair[kPasses][8];
+  const int passes = end - begin > kRows ? kPasses : 1;
+  struct Row {
+    int lead, own;                   // slots of the block's first row and of this one
+    int64_t row;                     // of the cache, of the head in work
+    const char *k, *v;               // the head's rows
+    uint16_t* k_out;
+    float own_f[8], pair_f[8];
+  } rows[kPasses];
+  const int size = kBF16 ? 2 : 4;
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int i = p * kRows + tid / kLanes;
-    lead[p] = s.lead[i];
-    slot[p] = s.slot[i];
-    if (lead[p] != kSkip) pairs.factors(a.k_gamma, s.turn[i], own[p], pair[p]);
+    const int i = begin + p * kRows + tid / kLanes;
+    Row& r = rows[p];
+    r.own = i;
+    r.lead = i < end ? s.lead[i] : kSkip;
+    if (r.lead == kSkip) continue;
+    const int64_t t = t0 + i;
+    r.row = s.slot[i] + (static_cast<int64_t>(part) << a.cache.page_shift);
+    r.k = static_cast<const char*>(a.k) + (t * a.k_token + part * a.k_head) * size;
+    r.v = static_cast<const char*>(a.v) + (t * a.v_token + part * a.v_head) * size;
+    r.k_out = a.k_out ? a.k_out + t * a.ko_token + part * a.ko_head : nullptr;
+    pairs.factors(a.k_gamma, s.turn[i], r.own_f, r.pair_f);
   }
+  // a head's rows, on their way beside the work on the head before
+  struct Loaded { Raw8<kBF16> x, y, v; int byte[2]; } raw[kPasses];
+  auto load = [&](int p, const Row& r) {
+    raw[p].x.load(r.k, pairs.e);
+    if (!kInter) raw[p].y.load(r.k, pairs.ep);
+    if (r.lead >= 0) {
+      raw[p].v.load(r.v, pairs.e);
+      raw[p].byte[0] = a.k_scale[r.row / kScaleRows];
+      raw[p].byte[1] = a.v_scale[r.row / kScaleRows];
+    }
+  };
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p)
+    if (p < passes && rows[p].lead != kSkip) load(p, rows[p]);
   int buffer = 0;
   for (int h = part; h < a.kv_heads; h += a.code_parts, buffer = buffer == 2 ? 0 : buffer + 1) {
     float z[kPasses][2][8];          // keys, values
     int old[kPasses][2];
+    bool odd[kPasses];               // of this lane's elements one is not finite
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      const int i = p * kRows + tid / kLanes;
-      const int64_t t = t0 + i;
-      if (lead[p] == kSkip) continue;                 // (all lanes of a row alike)
-      Raw8<kBF16> x, y, v;
-      x.load(a.k, t * a.k_token + h * a.k_head + pairs.e);
-      if (!kInter) y.load(a.k, t * a.k_token + h * a.k_head + pairs.ep);
-      if (lead[p] >= 0) {
-        v.load(a.v, t * a.v_token + h * a.v_head + pairs.e);
-        const int64_t at = (slot[p] + (static_cast<int64_t>(h) << a.cache.page_shift)) / kScaleRows;
-        old[p][0] = min(static_cast<int>(a.k_scale[at]), 254);
-        old[p][1] = min(static_cast<int>(a.v_scale[at]), 254);
+      Row& r = rows[p];
+      if (p >= passes || r.lead == kSkip) continue;   // (all lanes of a row alike)
+      norm_turn<D, kBF16, kInter>(a.norm, a.eps, pairs.rotated, raw[p].x, raw[p].y, r.own_f, r.pair_f, z[p][0]);
+      if (r.k_out) *reinterpret_cast<u32x4*>(r.k_out + pairs.e) = pack8(z[p][0]);
+      if (r.lead >= 0) {
+        odd[p] = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[p][1][j] = raw[p].v[j];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          // magnitudes as whole numbers: their order, with what is not finite above
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(z[p][w][j]) & 0x7fffffffu);
+          if (top >= 0x7f800000u) {                   // rarely: without those
+            odd[p] = true;
+            top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t u = __float_as_uint(z[p][w][j]) & 0x7fffffffu;
+              if (u < 0x7f800000u) top = max(top, u);
+            }
+          }
+#pragma unroll
+          for (int m = kLanes / 2; m >= 1; m >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m, 64)));
+          if (lane == 0) atomicMax(&s.top[buffer][w][r.lead], top);
+          old[p][w] = min(raw[p].byte[w], 254);
+        }
       }
-      norm_turn<D, kBF16, kInter>(a.norm, a.eps, pairs.rotated, x, y, own[p], pair[p], z[p][0]);
-      if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + pairs.e) = pack8(z[p][0]);
-      if (lead[p] < 0) continue;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z[p][1][j] = v[j];
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        float top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_or(fabsf(z[p][w][j]), 0.0f));
-#pragma unroll
-        for (int m = kLanes / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-        if (lane == 0) atomicMax(&s.top[buffer][w][lead[p]], __float_as_uint(top));
+      if (h + a.code_parts < a.kv_heads) {            // the next head
+        r.k += a.code_parts * a.k_head * size;
+        r.v += a.code_parts * a.v_head * size;
+        if (r.k_out) r.k_out += a.code_parts * a.ko_head;
+        r.row += static_cast<int64_t>(a.code_parts) << a.cache.page_shift;
+        load(p, r);
       }
     }
     __syncthreads();
@@ -268,26 +315,26 @@ __device__ __forceinline__ void append_codes(const QkArgs& a, int block) {
     if (tid < 2 * kSlots) (&s.top[buffer == 0 ? 2 : buffer - 1][0][0])[tid] = 0;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      if (lead[p] < 0) continue;
-      const int i = p * kRows + tid / kLanes;
-      const int64_t row = slot[p] + (static_cast<int64_t>(h) << a.cache.page_shift);
-      const uint32_t here = s.rows[lead[p]];
+      const Row& r = rows[p];
+      if (p >= passes || r.lead < 0) continue;
+      const int64_t row = s.slot[r.own] + (static_cast<int64_t>(h) << a.cache.page_shift);
+      const uint32_t here = s.rows[r.lead];
       const bool fresh = here & 1;
       if (a.key_weights && lane == 0) a.key_weights[row] = 0.0f;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         uint8_t* codes = reinterpret_cast<uint8_t*>(w ? a.cache.v : a.cache.k);
-        const int want = scale_byte(__uint_as_float(s.top[buffer][w][lead[p]])), b = fresh ? want : max(want, old[p][w]);
-        *reinterpret_cast<u32x2*>(codes + row * D + pairs.e) = to_codes(z[p][w], inverse_scale(b));
-        if (i != lead[p]) continue;
+        const int want = scale_byte(__uint_as_float(s.top[buffer][w][r.lead])), b = fresh ? want : max(want, old[p][w]);
+        *reinterpret_cast<u32x2*>(codes + row * D + pairs.e) = to_codes(z[p][w], inverse_scale(b), odd[p] || b >= kMostScale);
+        if (r.own != r.lead) continue;
         if (lane == 0) (w ? a.v_scale : a.k_scale)[row / kScaleRows] = static_cast<uint8_t>(b);
         if (fresh || b <= old[p][w]) continue;
         // the block's other rows, in the larger scale
         const float f = scale_step(old[p][w], b);
-        uint8_t* rows = codes + row / kScaleRows * kScaleRows * D + pairs.e;
-        for (int r = 0; r < kScaleRows; ++r) {
-          if (here >> r & 1) continue;
-          u32x2* c = reinterpret_cast<u32x2*>(rows + r * D);
+        uint8_t* block = codes + row / kScaleRows * kScaleRows * D + pairs.e;
+        for (int i = 0; i < kScaleRows; ++i) {
+          if (here >> i & 1) continue;
+          u32x2* c = reinterpret_cast<u32x2*>(block + i * D);
           *c = u32x2{rescale4((*c)[0], f), rescale4((*c)[1], f)};
         }
       }
