@@ -738,32 +738,51 @@ __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const Pag
 // the loads after each other: length and place, maxima and sums beside the first parts.
 constexpr int kPgWaveRows = 1024;
 
+// Where the parts of the rows of item (b, h), whose sequence has len keys, lie among the partial rows.
+struct Parts {
+  int own, all, slot0;               // of its own keys; with the prefix's; the first of them
+  int64_t pre, pre_step;             // rows of the prefix's first part, and from one to the next
+  int M;
+  bool done;                         // finished where it was computed: no parts
+  __device__ __forceinline__ Parts(const PagedArgs& a, const i32x2& of_item, int b, int h, int len) {
+    M = a.q_len * a.group;
+    done = len > 0 && of_item.y == 0;
+    // (kept inside the partial rows, also where a length has changed since the shares ran)
+    slot0 = min(max(of_item.x, 0), 2 * a.shares + (a.splits ? a.batch * a.kv_heads : 0) - 1);
+    own = len > 0 ? min(max(of_item.y, 1), max(a.shares - (slot0 >> 1), 1)) : 0;
+    all = done ? 0 : own + a.splits;
+    pre_step = static_cast<int64_t>(a.kv_heads) * a.batch * M;
+    pre = static_cast<int64_t>(h) * a.batch * M + static_cast<int64_t>(b) * M;
+  }
+  // row r in part i: of a share its first (2 share) or last (2 share + 1) item, the
+  // later parts are the first of theirs; parts >= own are the prefix's
+  __device__ __forceinline__ int64_t row(int i, int r) const {
+    if (i >= own) return (i - own) * pre_step + pre + r;
+    return static_cast<int64_t>(i == 0 ? slot0 : (slot0 | 1) - 1 + 2 * i) * M + r;
+  }
+  __device__ __forceinline__ f32x2 ml(const PagedArgs& a, int i, int r) const {
+    return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row(i, r) * 2);
+  }
+};
+
 template <int D, int WPR, bool kWeigh>
-__global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
+__device__ __forceinline__ void join_rows(const PagedArgs& a, int block) {
   constexpr int kLanes = D / 4, kThreads = 64 * WPR, kWays = kThreads / kLanes, kRows = kPgThreads / kThreads;
   __shared__ float red[kRows][WPR];
   __shared__ f32x4 sums[kRows][kWays][kLanes];
   const int M = a.q_len * a.group, tid = threadIdx.x % kThreads, lane = threadIdx.x & 63, wave = tid >> 6;
-  const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), row = blockIdx.x * kRows + mine;
+  const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), row = block * kRows + mine;
   const bool live = row < a.batch * a.kv_heads * M;
   const int r = row % M, item = row / M, h = item % a.kv_heads, b = live ? item / a.kv_heads : 0;
   const i32x2 of_item = ldg<i32x2>(a.parts + b * a.kv_heads + h);   // beside the length; nothing where there are no keys
   bool bad;
   const int len = length_of(a, b, bad);
-  const bool done = len > 0 && of_item.y == 0;        // finished where it was computed
+  const Parts of(a, of_item, b, h, len);
+  const bool done = of.done;
   if (WPR > 1 && done) return;
-  // (kept inside the partial rows, also where a length has changed since the shares ran)
-  const int slot0 = min(max(of_item.x, 0), 2 * a.shares + (a.splits ? a.batch * a.kv_heads : 0) - 1);
-  const int own = len > 0 ? min(max(of_item.y, 1), max(a.shares - (slot0 >> 1), 1)) : 0;
-  const int parts = !live || done ? 0 : own + a.splits;
-  // row of part i among the partial rows: of a share its first (2 share) or last (2 share + 1) item, the
-  // later parts are the first of theirs; parts >= own are the prefix's
-  auto row_of = [&](int i) -> int64_t {
-    if (i >= own)
-      return (static_cast<int64_t>(i - own) * a.kv_heads + h) * (static_cast<int64_t>(a.batch) * M) + static_cast<int64_t>(b) * M + r;
-    return static_cast<int64_t>(i == 0 ? slot0 : (slot0 | 1) - 1 + 2 * i) * M + r;
-  };
-  auto ml_of = [&](int i) { return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row_of(i) * 2); };
+  const int own = of.own, parts = live ? of.all : 0;
+  auto row_of = [&](int i) { return of.row(i, r); };
+  auto ml_of = [&](int i) { return of.ml(a, i, r); };
   // the first parts of every group of lanes, on their way beside the maxima and sums
   const int way = tid / kLanes, d0 = 4 * (tid % kLanes);
   auto part_of = [&](int i) { return ldg<f32x4>((i < own ? a.po : a.pre_o) + row_of(i) * D + d0); };
@@ -830,15 +849,44 @@ __global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
 // are written by the scores' kernel and read here, against 4 D bytes of its key and value (2 D in 8 bits).
 constexpr int kKwRows = 64;          // most rows of an item
 
-template <int kLanes>
-__global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, int each) {
+// log2 of a row's sum of 2^score, by its parts: 16 lanes a row, for 16 rows.
+constexpr int kKwPartRows = kPgThreads / 16;
+__device__ __forceinline__ float lse_of_parts(const PagedArgs& a, const Parts& of, int b, int len) {
+  const int r = threadIdx.x / 16, lane = threadIdx.x % 16;
+  float top = kNegInf, l = 0.0f;
+  if (r < of.M)
+    for (int i = lane; i < of.all; i += 16) top = fmaxf(top, of.ml(a, i, r)[0]);
+#pragma unroll
+  for (int s = 8; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+  const float mu = top == kNegInf ? 0.0f : top;
+  if (r < of.M)
+    for (int i = lane; i < of.all; i += 16) {
+      const f32x2 ml = of.ml(a, i, r);
+      l += ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
+    }
+#pragma unroll
+  for (int s = 8; s >= 1; s >>= 1) l += __shfl_xor(l, s, 64);
+  const bool sees = a.lens[b] >= 0 && (a.prefix > 0 || len - a.q_len + r / a.group >= 0 || l != l);
+  return sees ? top + log2f(l) : -kNegInf;
+}
+
+// kParts: rows in parts have no lse yet (the join is in the same launch), so it is made from the parts.
+template <int kLanes, bool kParts>
+__device__ __forceinline__ void weigh_keys(const PagedArgs& a, int block, int each) {
   constexpr int kKeys = kPgThreads / kLanes;
   __shared__ __align__(16) float lse[kKwRows];
-  const int item = blockIdx.x / each, part = blockIdx.x % each, b = item / a.kv_heads, h = item % a.kv_heads, M = a.q_len * a.group;
+  const int item = block / each, part = block % each, b = item / a.kv_heads, h = item % a.kv_heads, M = a.q_len * a.group;
+  i32x2 of_item{};
+  if constexpr (kParts) of_item = ldg<i32x2>(a.parts + item);
   bool bad;
   const int len = length_of(a, b, bad);
   if (bad || len <= part * kKeys) return;
-  // (no score reaches past -infinity in the rows that fill up the fours)
+  const Parts of(a, of_item, b, h, len);
+  if (kParts && !of.done) {
+    const float x = lse_of_parts(a, of, b, len);
+    if (threadIdx.x % 16 == 0) lse[threadIdx.x / 16] = x;
+    if (static_cast<int>(threadIdx.x) >= kKwPartRows && threadIdx.x < kKwRows) lse[threadIdx.x] = -kNegInf;
+  } else
   if (threadIdx.x < kKwRows)
     lse[threadIdx.x] = static_cast<int>(threadIdx.x) < M ? a.lse[static_cast<int64_t>(item) * M + threadIdx.x] : -kNegInf;
   __syncthreads();
@@ -860,6 +908,22 @@ __global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, i
     if (lane == 0 && key0 + static_cast<int>(threadIdx.x) / kLanes < len && id >= 0 && id < a.c.n_pages)
       a.weights[((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))] += sum;
   }
+}
+
+template <int D, int WPR, bool kWeigh>
+__global__ __launch_bounds__(kPgThreads) void k_paged_join(const PagedArgs a) {
+  join_rows<D, WPR, kWeigh>(a, blockIdx.x);
+}
+template <int kLanes>
+__global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, int each) {
+  weigh_keys<kLanes, false>(a, blockIdx.x, each);
+}
+// Both in one launch, for up to kKwPartRows rows an item (48 sequences of up to 2100 keys, 4 rows: TODO).
+template <int D, int WPR, int kLanes>
+__global__ __launch_bounds__(kPgThreads) void k_join_weights(const PagedArgs a, int each, int join_blocks) {
+  const int block = blockIdx.x - join_blocks;
+  if (block < 0) join_rows<D, WPR, false>(a, blockIdx.x);
+  else weigh_keys<kLanes, true>(a, block, each);
 }
 
 // Workspace: partial rows of the shares (and, beside a prefix, of whole items), then the prefix's, then
@@ -932,9 +996,16 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   return add_more();
 }
 
-// Workgroups of k_key_weights, at least about, for a lane a key (of 16 lanes a key four times as many: 11.1 -> 9.3 us for 64 rows
-// of four sequences of up to 8000 keys).
+// Weights: lanes a key, workgroups an item, and whether they go with the join.  At least about kKwBlocks workgroups for a lane a key
+// (of 16 lanes a key four times as many: 11.1 -> 9.3 us for 64 rows of four sequences of up to 8000 keys).
 constexpr int kKwBlocks = 2048;
+int weigh_lanes(int M) { return M <= 4 ? 1 : M <= 16 ? 4 : 16; }
+int weigh_each(const PagedArgs& a, int M) {
+  const int lanes = weigh_lanes(M), items = a.batch * a.kv_heads, keys = kPgThreads / lanes;
+  const int of_row = ((a.c.max_pages << a.c.page_shift) + keys - 1) / keys;
+  return std::min((kKwBlocks * (lanes == 16 ? 4 : lanes == 4 ? 2 : 1) + items - 1) / items, of_row);
+}
+bool weigh_beside_join(const PagedPlan& p, int M) { return !p.alone && M <= kKwPartRows; }
 
 template <int D, int RT, bool F8, bool kWeigh>
 void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
@@ -953,8 +1024,16 @@ void launch_paged_rt(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
     launch_kernel(k_paged<D, RT, F8, kWeigh>, dim3(p.shares, halves), kPgThreads, 0, s, a);
   }
   const int rows = a.batch * a.kv_heads * M;
-  if (rows >= kPgWaveRows) launch_kernel(k_paged_join<D, 1, kWeigh>, (rows + 3) / 4, kPgThreads, 0, s, a);
-  else launch_kernel(k_paged_join<D, 4, kWeigh>, rows, kPgThreads, 0, s, a);
+  const bool waves = rows >= kPgWaveRows;
+  const int blocks = waves ? (rows + 3) / 4 : rows;
+  if constexpr (kWeigh)
+    if (weigh_beside_join(p, M)) {
+      const int lanes = weigh_lanes(M), each = weigh_each(a, M);
+      auto kernel = lanes == 1 ? (waves ? k_join_weights<D, 1, 1> : k_join_weights<D, 4, 1>) : (waves ? k_join_weights<D, 1, 4> : k_join_weights<D, 4, 4>);
+      launch_kernel(kernel, blocks + a.batch * a.kv_heads * each, kPgThreads, 0, s, a, each, blocks);
+      return;
+    }
+  launch_kernel(waves ? k_paged_join<D, 1, kWeigh> : k_paged_join<D, 4, kWeigh>, blocks, kPgThreads, 0, s, a);
 }
 
 template <int D, bool F8, bool kWeigh>
@@ -962,10 +1041,10 @@ void launch_paged_d(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
   if (p.rt == 1) launch_paged_rt<D, 1, F8, kWeigh>(p, a, s);
   else launch_paged_rt<D, 2, F8, kWeigh>(p, a, s);
   if constexpr (kWeigh) {
-    const int items = a.batch * a.kv_heads, M = a.q_len * a.group, lanes = M <= 4 ? 1 : M <= 16 ? 4 : 16;
-    const int keys = kPgThreads / lanes, of_row = ((a.c.max_pages << a.c.page_shift) + keys - 1) / keys;
-    const int each = std::min((kKwBlocks * (lanes == 16 ? 4 : lanes == 4 ? 2 : 1) + items - 1) / items, of_row);
-    launch_kernel(lanes == 1 ? k_key_weights<1> : lanes == 4 ? k_key_weights<4> : k_key_weights<16>, items * each, kPgThreads, 0, s, a, each);
+    const int M = a.q_len * a.group, lanes = weigh_lanes(M), each = weigh_each(a, M);
+    if (!weigh_beside_join(p, M))
+      launch_kernel(lanes == 1 ? k_key_weights<1> : lanes == 4 ? k_key_weights<4> : k_key_weights<16>, a.batch * a.kv_heads * each, kPgThreads,
+                    0, s, a, each);
   }
 }
 
