@@ -502,6 +502,32 @@ def test_key_weights(codes, heads, kv, dim, page, q_len, prefix, spare):
     assert torch.equal(wd.cpu()[untouched], w[untouched])
 
 
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,q_len", [(4, 1, 5), (8, 1, 4), (8, 1, 8), (4, 1, 16)])
+def test_many_rows_in_wide_tables(codes, dim, heads, kv, q_len):
+    """More than 16 rows an item where the tables have many places (the other cases have few)."""
+    g = gen(heads + q_len + dim)
+    lens = [900, 40, 0]
+    _, table, kc, ks, vc, vs = paged8_setup(g, lens, kv, 256, dim)
+    wide = torch.full((3, 700), -1, dtype=I32)                   # 537600 places
+    wide[:, :table.shape[1]] = table
+    k64, v64 = O.values(kc, ks), O.values(vc, vs)
+    q = normal(g, 3, q_len, heads, dim)
+    w = torch.rand(kc.shape[:3], generator=g)
+    wd = w.to(DEV)
+    if codes:
+        got = run_paged8(q, wide, lens, kc, ks, vc, vs, key_weights=wd)
+        assert torch.equal(got, run_paged8(q, wide, lens, kc, ks, vc, vs))
+    else:
+        k64, v64 = k64.to(BF16).double(), v64.to(BF16).double()
+        got = dsk_moe.paged_attention(q.to(DEV), k64.to(BF16).to(DEV), v64.to(BF16).to(DEV), wide.to(DEV), ints(lens), key_weights=wd)
+    want, tol = O.paged(q, k64, v64, wide, lens)
+    assert_within(got, want, tol)
+    want, tol = weights_want(w, q, k64, wide, lens, 256, dim ** -0.5)
+    assert_within(wd, want, tol + 1e-38, "weights")
+
+
 def test_key_weights_add_up_and_repeat():
     """The same call twice gives twice the weight, bit for bit the same each time; outputs are those without weights."""
     g = gen(41)
@@ -577,10 +603,16 @@ def test_evict(codes, dim, page, kv, keep, first, recent):
 
 @pytest.mark.parametrize("codes", [False, True])
 @pytest.mark.parametrize("lens,keep,first,recent", [([5000], 1000, 4, 200), ([2500, 1500], 1400, 0, 700), ([3000], 2999, 0, 0), ([1030, 1090], 1024, 4, 128),
-                                                    ([4200], 30, 0, 10)])
+                                                    ([4200], 30, 0, 10), ([40000, 17000], 16500, 3, 100)])
 def test_evict_of_long_sequences(codes, lens, keep, first, recent):
     g = gen(sum(lens) + keep)
-    evict_case(g, lens, keep, first, recent, 2, 64, 64, codes)
+    evict_case(g, lens, keep, first, recent, 1 if lens[0] > 10000 else 2, 64, 64, codes)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+def test_evict_of_sequences_in_wide_tables(codes):
+    """Short sequences whose tables have room for many more rows."""
+    evict_case(gen(50), [300, 41, 100, 40, 0], 40, 2, 9, 2, 32, 64, codes, spare=200)
 
 
 @pytest.mark.parametrize("codes", [False, True])
@@ -654,6 +686,35 @@ def test_evict_again_and_again_in_place(codes):
         w += more
         wd += more.to(DEV)
         assert torch.equal(wd.cpu(), w)
+
+
+def test_calls_on_two_streams():
+    """Appends, attention with weights and evictions of two caches at once, on streams of their own: as one after the other."""
+    runs = []
+    for streams in ((None, None), (torch.cuda.Stream(), torch.cuda.Stream())):
+        outs = []
+        states = []
+        for i in range(2):
+            g = gen(80 + i)
+            lens = [700 - 300 * i, 90, 33]
+            _, table, kc, ks, vc, vs = paged8_setup(g, [n + 16 for n in lens], 2, 32, 128, 1 + 100 * i)
+            kd, vd = dev8(kc, vc)
+            states.append((table.to(DEV), kd, vd, ks.to(DEV), vs.to(DEV), torch.zeros(kc.shape[:3], device=DEV),
+                           [(normal(g, 3, 8, 128).to(DEV), normal(g, 3, 2, 128).to(DEV)) for _ in range(4)], lens))
+        torch.cuda.synchronize()
+        for t in range(4):
+            for st, (table, kd, vd, ks, vs, w, qk, lens) in zip(streams, states):
+                with torch.cuda.stream(st) if st is not None else torch.cuda.stream(torch.cuda.current_stream()):
+                    rows = ints([n + t for n in lens])
+                    extra = dict(k_scale=ks, v_scale=vs, key_weights=w)
+                    q = dsk_moe.kv_append(qk[t][0], qk[t][1], qk[t][1], rows, ints([0, 1, 2]), table, kd, vd, dsk_moe.rope_frequencies(128)[0], **extra)
+                    outs.append(dsk_moe.paged_attention(q, kd, vd, table, rows + 1, **extra))
+                    if t == 2:
+                        dsk_moe.kv_evict(kd, vd, w, table, rows + 1, 95, first=1, recent=20, k_scale=ks, v_scale=vs)
+        torch.cuda.synchronize()
+        runs.append(outs + [x.view(U8) if x.dtype == F8 else x for s in states for x in s[1:6]])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
 
 
 # ------------------------------------------------------------------ together
