@@ -145,23 +145,46 @@ def _out_strides(out: torch.Tensor | None, shape: tuple, dev: torch.device, what
 
 # A call's checks depend on its tensors' sizes, strides, types and devices and on its numbers alone, so what they
 # found -- a plan: the device, the entry point and its descriptors; no tensor, no address -- serves later calls of the
-# same kind.  A number given as something else (a tensor, say, which may change) is read at every call.  A decode step's
-# host work is then a third of that of checking each time (18 us a call).
-_plans: dict[str, dict[tuple, tuple]] = {"qk": {}, "append": {}, "prompt": {}, "paged": {}, "evict": {}}
-_MOST_PLANS = 1024
+# same kind.  A number given as something else (a tensor, say, which may change) is read at every call.  Whether a call is of a kind
+# that was met before is asked of torch's own record of a list of tensors' properties, one call for all of them; where that says
+# no, or is not there, of a dictionary.  Host work of an append in 8 bits: TODO us, TODO with the dictionary alone.
+_MOST_PLANS, _MOST_RECENT = 1024, 8
 _CONTIGUOUS = torch.contiguous_format
+_Properties = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "TensorGuards", None)
 
 
 def _sig(t: torch.Tensor | None):
     return (t.shape, t.stride(), t.dtype, t.get_device()) if t is not None else None
 
 
-def _plan(kind: str, key: tuple, make, *args) -> tuple:
-    plan = make(*args)
-    if len(_plans[kind]) >= _MOST_PLANS:
-        _plans[kind].clear()
-    _plans[kind][key] = plan
-    return plan
+class _Plans:
+    """Plans of one function's calls, which ``make`` makes of a call's arguments."""
+
+    def __init__(self, make):
+        self._make, self._by_key, self._recent = make, {}, []
+
+    def find(self, numbers: tuple, tensors: tuple, args: tuple) -> tuple:
+        """The plan of a call with these numbers (which optional tensors it has among them) and tensors (None: not given)."""
+        given = [t for t in tensors if t is not None]
+        for had, properties, plan in self._recent:
+            if had == numbers and properties.check(*given):
+                return plan
+        key = (numbers, tuple(map(_sig, tensors)))
+        entry = self._by_key.get(key)
+        if entry is None:
+            if len(self._by_key) >= _MOST_PLANS:
+                self._by_key.clear()
+                self._recent.clear()
+            entry = self._by_key[key] = [self._make(*args), 0]
+        plan, misses = entry
+        entry[1] += 1
+        # (again after 1, 2, 4, .. calls that were not found among the recent ones)
+        if _Properties is not None and misses & (misses - 1) == 0:
+            properties = _Properties(*given, dynamic_dims_sizes=[list(t.shape) for t in given],
+                                     dynamic_dims_strides=[list(t.stride()) for t in given])
+            self._recent.insert(0, (numbers, properties, plan))
+            del self._recent[_MOST_RECENT:]
+        return plan
 
 
 def _call(name: str, fn, dev: torch.device, *args) -> None:
@@ -270,6 +293,9 @@ def _extra(k_scale, v_scale, key_weights):
     return ctypes.byref(_lib.KVExtra(_p(k_scale), _p(v_scale), _p(key_weights)))
 
 
+_qk_plans, _append_plans = _Plans(_qk_plan), _Plans(_qk_plan)
+
+
 def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor | None = None, *,
                  axis: torch.Tensor | None = None, interleaved: bool = False, rot_first: int = 0, mscale: float = 1.0,
                  q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, norm: bool = True,
@@ -284,12 +310,11 @@ def qk_norm_rope(q: torch.Tensor | None, k: torch.Tensor, positions: torch.Tenso
     (``rope_axes``; one of no axis does not turn), and a token that is negative on any axis is left out."""
     if not (type(mscale) is type(eps) is float and type(interleaved) is type(norm) is bool and type(rot_first) is int):
         interleaved, rot_first, mscale, norm, eps = bool(interleaved), int(rot_first), float(mscale), bool(norm), float(eps)
-    key = (_sig(q), _sig(k), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out), _sig(axis),
-           interleaved, rot_first, mscale, norm, eps)
-    plan = _plans["qk"].get(key)
-    if plan is None:
-        plan = _plan("qk", key, _qk_plan, q, k, None, positions, freq, q_gamma, k_gamma, q_out, k_out, None, None, None, None,
-                     interleaved, rot_first, mscale, norm, eps, 0, axis)
+    plan = _qk_plans.find(
+        (q is None, freq is None, q_gamma is None, k_gamma is None, q_out is None, k_out is None, axis is None,
+         interleaved, rot_first, mscale, norm, eps),
+        (q, k, positions, freq, q_gamma, k_gamma, q_out, k_out, axis),
+        (q, k, None, positions, freq, q_gamma, k_gamma, q_out, k_out, None, None, None, None, interleaved, rot_first, mscale, norm, eps, 0, axis))
     fn, dev, desc, _ = plan
     if q_out is None and q is not None:
         q_out = torch.empty_like(q, dtype=_BF16, memory_format=_CONTIGUOUS)
@@ -324,15 +349,13 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, position
         interleaved, rot_first, mscale, norm, eps = bool(interleaved), int(rot_first), float(mscale), bool(norm), float(eps)
     if type(prefix_len) is not int:
         prefix_len = int(prefix_len)
-    key = (_sig(q), _sig(k), _sig(v), _sig(positions), _sig(freq), _sig(q_gamma), _sig(k_gamma), _sig(q_out), _sig(k_out),
-           _sig(seq), _sig(table), _sig(k_cache), _sig(v_cache), interleaved, rot_first, mscale, norm, eps, prefix_len)
     plain = axis is None and rows is None and k_scale is None and v_scale is None and key_weights is None
-    if not plain:
-        key += (_sig(axis), _sig(rows), _sig(k_scale), _sig(v_scale), _sig(key_weights))
-    plan = _plans["append"].get(key)
-    if plan is None:
-        plan = _plan("append", key, _qk_plan, q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache,
-                     interleaved, rot_first, mscale, norm, eps, prefix_len, axis, rows, k_scale, v_scale, key_weights)
+    plan = _append_plans.find(
+        (q is None, freq is None, q_gamma is None, k_gamma is None, q_out is None, k_out is None, plain or
+         (axis is None, rows is None, k_scale is None, v_scale is None, key_weights is None), interleaved, rot_first, mscale, norm, eps, prefix_len),
+        (q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache, axis, rows, k_scale, v_scale, key_weights),
+        (q, k, v, positions, freq, q_gamma, k_gamma, q_out, k_out, seq, table, k_cache, v_cache, interleaved, rot_first, mscale, norm, eps,
+         prefix_len, axis, rows, k_scale, v_scale, key_weights))
     fn, dev, desc, cache = plan
     if q_out is None and q is not None:
         q_out = torch.empty_like(q, dtype=_BF16, memory_format=_CONTIGUOUS)
@@ -363,6 +386,9 @@ def _prompt_plan(q, k, v, cu_q, cu_k, out, causal, scale):
     return _lib.load().dsk_prompt_attention, dev, ctypes.byref(desc)
 
 
+_prompt_plans = _Plans(_prompt_plan)
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
                      cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:
@@ -373,10 +399,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         cu_k = cu_q
     if type(causal) is not bool or not (scale is None or type(scale) is float):
         causal, scale = bool(causal), float(scale) if scale is not None else None
-    key = (_sig(q), _sig(k), _sig(v), _sig(cu_q), _sig(cu_k), _sig(out), causal, scale)
-    plan = _plans["prompt"].get(key)
-    if plan is None:
-        plan = _plan("prompt", key, _prompt_plan, q, k, v, cu_q, cu_k, out, causal, scale)
+    # (cu_k may be cu_q itself: then it is not looked at twice)
+    plan = _prompt_plans.find((cu_k is cu_q, out is None, causal, scale), (q, k, v, cu_q, None if cu_k is cu_q else cu_k, out),
+                              (q, k, v, cu_q, cu_k, out, causal, scale))
     fn, dev, desc = plan
     if out is None:
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)
@@ -424,6 +449,9 @@ def _paged_plan(q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale
     return _lib.load().dsk_paged_attention, dev, ctypes.byref(desc), cache, n.value
 
 
+_paged_plans = _Plans(_paged_plan)
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
                     lens: torch.Tensor, *, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                     key_weights: torch.Tensor | None = None, prefix: torch.Tensor | None = None, prefix_len: int = 0,
@@ -440,14 +468,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (``dsk_paged_attention_extra_workspace_size``) then holds a float32 for every query row and place of the table."""
     if type(prefix_len) is not int or not (scale is None or type(scale) is float):
         prefix_len, scale = int(prefix_len), float(scale) if scale is not None else None
-    key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(table), _sig(lens), _sig(prefix), _sig(out), prefix_len, scale)
     plain = k_scale is None and v_scale is None and key_weights is None
-    if not plain:
-        key += (_sig(k_scale), _sig(v_scale), _sig(key_weights))
-    plan = _plans["paged"].get(key)
-    if plan is None:
-        plan = _plan("paged", key, _paged_plan, q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale, k_scale, v_scale,
-                     key_weights)
+    plan = _paged_plans.find(
+        (prefix is None, out is None, plain or (k_scale is None, v_scale is None, key_weights is None), prefix_len, scale),
+        (q, k_cache, v_cache, table, lens, prefix, out, k_scale, v_scale, key_weights),
+        (q, k_cache, v_cache, table, lens, prefix, out, prefix_len, scale, k_scale, v_scale, key_weights))
     fn, dev, desc, cache, nbytes = plan
     if out is None:
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)
@@ -484,6 +509,9 @@ def _evict_plan(k_cache, v_cache, key_weights, table, lens, keep, first, recent,
     return dev, desc, cache, n.value
 
 
+_evict_plans = _Plans(_evict_plan)
+
+
 def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
              keep: int, *, first: int = 0, recent: int = 0, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
              lens_out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -493,11 +521,10 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch.Te
     (``lens_out``, which may be ``lens``).  Rows behind are left as they were, and the pages that they fill are free.  The next
     token of a sequence goes on at its own position, in row ``keep`` (``kv_append``'s ``rows``)."""
     keep, first, recent = int(keep), int(first), int(recent)
-    key = (_sig(k_cache), _sig(v_cache), _sig(key_weights), _sig(table), _sig(lens), _sig(k_scale), _sig(v_scale), _sig(lens_out),
-           keep, first, recent)
-    plan = _plans["evict"].get(key)
-    if plan is None:
-        plan = _plan("evict", key, _evict_plan, k_cache, v_cache, key_weights, table, lens, keep, first, recent, k_scale, v_scale, lens_out)
+    plan = _evict_plans.find(
+        (key_weights is None, k_scale is None, v_scale is None, lens_out is None or (lens_out is lens,), keep, first, recent),
+        (k_cache, v_cache, key_weights, table, lens, k_scale, v_scale, None if lens_out is lens else lens_out),
+        (k_cache, v_cache, key_weights, table, lens, keep, first, recent, k_scale, v_scale, lens_out))
     dev, desc, cache, nbytes = plan
     if lens_out is None:
         lens_out = torch.empty_like(lens)
