@@ -48,13 +48,13 @@ namespace dsk {
 namespace {
 
 constexpr int kPgThreads = 256;
-// Keys of a wave's step: the bytes in flight are the same with codes of half the size.
-template <bool F8>
-constexpr int step_keys() { return F8 ? 64 : 32; }
-// Units, of which shares are made: 128 keys (a step of each of four waves, of two in 8 bits).
-constexpr int kPgUnit = 128;
-// Units that an item counts for beside its keys'.  It has a start and an end of its own, 4 us; of half the bytes
-// a share of short items would take longest (64 sequences of 1 to 8192 keys in 8 bits: TODO).
+// Keys of a wave's step, in tiles of 16.  Also of codes, which are half the bytes: with 64 their conversions spill (64
+// sequences of up to 8192 keys of 128 37.8 us, 29.9 with 32; 8 of up to 32768 keys of 64 21.2 and 19.4).
+constexpr int kPgStep = 32, kPgTiles = kPgStep / 16;
+constexpr int kPgUnit = 4 * kPgStep; // of which shares are made: a step of each of four waves
+// Units that an item counts for beside its keys'.  It has a start and an end of its own, about 4 us, beside which codes are
+// little: 64 sequences of 1 to 8192 keys of 128 take 29.9 us with 1, 30.4 with 2, 33.6 with 4 (and with steps of 64
+// keys 37.8 with 1, 52.8 with none); 8 of up to 32768 of 64 19.4, 18.8, 18.7.
 template <bool F8>
 constexpr uint32_t item_units() { return F8 ? 1 : 0; }
 constexpr int kPgShort = 512;       // keys of a table row that one workgroup takes alone
@@ -138,9 +138,9 @@ __device__ __forceinline__ void wave_fence() {
 
 template <int D, bool F8>
 struct Step {                       // one wave's keys, in tiles of 16
-  static constexpr int kTiles = step_keys<F8>() / 16, kPieces = D / (F8 ? 64 : 32);
-  u32x4 k[kTiles][kPieces];
-  uint32_t v[4 * kTiles][kPieces];  // VW = D / 16 elements of 4 keys of each
+  static constexpr int kPieces = D / (F8 ? 64 : 32);
+  u32x4 k[kPgTiles][kPieces];
+  uint32_t v[4 * kPgTiles][kPieces]; // VW = D / 16 elements of 4 keys of each
 };
 
 template <int N>
@@ -180,12 +180,12 @@ struct SegLds {
   float ml[W][16 * RT][2];
 };
 
-// Lane T i + kt: the page of the wave's 16-key tile kt of T in step kk + i of those that begin at
+// Lane 2 i + kt: the page of the wave's 16-key tile kt in step kk + i of those that begin at
 // tile `tile0` (the table row's last one behind its end; the sequence's length need not be known yet).
-template <int W, int T>
+template <int W>
 __device__ __forceinline__ int page_ids(const PagedArgs& a, int b, int tile0, int kk) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t tile = tile0 + (static_cast<int64_t>(kk) + lane / T) * (T * W) + T * wave + lane % T;
+  const int64_t tile = tile0 + (static_cast<int64_t>(kk) + (lane >> 1)) * (2 * W) + 2 * wave + (lane & 1);
   const int page = static_cast<int>(min(tile >> (a.c.page_shift - 4), static_cast<int64_t>(a.c.max_pages - 1)));
   return ldg<int32_t>(a.c.table + b * a.c.table_stride + page);
 }
@@ -201,7 +201,7 @@ template <int D, int RT, int W, bool F8, bool kWeigh>
 __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int len, bool bad_len, int r0, int start, int stop,
                                         int64_t slot, int first_ids, SegLds<D, RT, W>& lds) {
   using S = Step<D, F8>;
-  constexpr int VW = D / 16, KS = D / 32, kKeys = step_keys<F8>(), kUnit = kKeys * W, T = S::kTiles;
+  constexpr int VW = D / 16, KS = D / 32, kUnit = kPgStep * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
   const int M = a.q_len * a.group;
@@ -230,13 +230,13 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     const int last_tile = (len - 1) >> 4, first_tile = start >> 4;
     stop = min(stop, len);
     const int k1 = (stop - start + kUnit - 1) / kUnit;   // steps of W waves
-    int ids = first_ids, ids0 = 0;    // lane T i + kt: the page of tile kt of step ids0 + i
+    int ids = first_ids, ids0 = 0;    // lane 2 i + kt: the page of tile kt of step ids0 + i
     int bad_tile = INT32_MAX;         // the lane's first 16 keys on a page outside the cache
     // F8: scale bytes of the lane's tile, and those of the ids before, which a step may still need
     uint32_t k_byte = 0, v_byte = 0, old_k_byte = 0, old_v_byte = 0;
     int old0 = 0;
     auto check_ids = [&]() {
-      const int tile = first_tile + (ids0 + lane / T) * (T * W) + T * wave + lane % T;
+      const int tile = first_tile + (ids0 + (lane >> 1)) * (2 * W) + 2 * wave + (lane & 1);
       const bool out_of = ids < 0 || ids >= a.c.n_pages;
       if (out_of && tile * 16 < stop) bad_tile = min(bad_tile, tile);
       if (out_of) ids = 0;
@@ -251,18 +251,18 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     };
     check_ids();
     auto load = [&](S& s, int kk) {
-      if (kk - ids0 >= 64 / T) {
+      if (kk - ids0 >= 32) {
         old0 = ids0;
         ids0 = kk;
-        ids = page_ids<W, T>(a, b, first_tile, kk);
+        ids = page_ids<W>(a, b, first_tile, kk);
         check_ids();
       }
-      const int tile0 = first_tile + kk * (T * W) + T * wave;
+      const int tile0 = first_tile + kk * (2 * W) + 2 * wave;
       if (tile0 * 16 >= stop) return;                 // none of the wave's keys in this step
 #pragma unroll
-      for (int kt = 0; kt < T; ++kt) {
+      for (int kt = 0; kt < kPgTiles; ++kt) {
         const int tile = min(tile0 + kt, last_tile);
-        const int id = __builtin_amdgcn_readlane(ids, T * (kk - ids0) + tile - tile0);
+        const int id = __builtin_amdgcn_readlane(ids, 2 * (kk - ids0) + tile - tile0);
         const int last_row = len - 1 - tile * 16;     // rows past the length: the last one again
         const int row0 = (tile * 16) & ((1 << a.c.page_shift) - 1);
         const int64_t base = (((static_cast<int64_t>(id) * a.kv_heads + h) << a.c.page_shift) + row0) * D;
@@ -286,7 +286,7 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
     // products then leave them out)
     auto add_nonfinite = [&](int kk) {
 #pragma unroll 1
-      for (int key = start + kk * kUnit + kKeys * wave, end = min(key + kKeys, len); key < end; ++key) {
+      for (int key = start + kk * kUnit + kPgStep * wave, end = min(key + kPgStep, len); key < end; ++key) {
         int id = ldg<int32_t>(trow + (key >> a.c.page_shift));
         if (id < 0 || id >= a.c.n_pages) id = 0;
         const int in_page = key & ((1 << a.c.page_shift) - 1);
@@ -309,18 +309,18 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
       }
     };
     auto compute = [&](const S& s, int kk) {
-      const int key0 = start + kk * kUnit + kKeys * wave;
+      const int key0 = start + kk * kUnit + kPgStep * wave;
       if (key0 >= stop) return;
-      const bool masked = key0 + kKeys - 1 > len - a.q_len;
-      float k_scale[T], v_scale[T];
+      const bool masked = key0 + kPgStep - 1 > len - a.q_len;
+      float k_scale[kPgTiles], v_scale[kPgTiles];
       bool good_scales = true;
       if constexpr (F8) {
         const bool old = kk < ids0;
         const uint32_t kb = old ? old_k_byte : k_byte, vb = old ? old_v_byte : v_byte;
         const int tile0 = key0 >> 4;
 #pragma unroll
-        for (int kt = 0; kt < T; ++kt) {
-          const int at = T * (kk - (old ? old0 : ids0)) + min(tile0 + kt, last_tile) - tile0;
+        for (int kt = 0; kt < kPgTiles; ++kt) {
+          const int at = 2 * (kk - (old ? old0 : ids0)) + min(tile0 + kt, last_tile) - tile0;
           k_scale[kt] = scale_of(lane_value(kb, at));
           const uint32_t byte = lane_value(vb, at);
           good_scales = good_scales && byte <= kMostScale;
@@ -337,118 +337,111 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
           if (!masked) return true;
           uint32_t bits = 0;
 #pragma unroll
-          for (int j = 0; j < 4 * T; ++j)
+          for (int j = 0; j < 4 * kPgTiles; ++j)
 #pragma unroll
             for (int i = 0; i < S::kPieces; ++i) bits |= nan_codes(s.v[j][i]);
           return good_scales && !__any(bits != 0);
         } else {
           u16x2 largest = {0, 0};
 #pragma unroll
-          for (int j = 0; j < 4 * T; ++j)
+          for (int j = 0; j < 4 * kPgTiles; ++j)
 #pragma unroll
             for (int i = 0; i < VW / 2; ++i)
               largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, s.v[j][i] & 0x7f807f80u));
           return !__any(nonfinite_bits(__builtin_bit_cast(uint32_t, largest)) != 0);
         }
       };
-      // 32 keys at a time
-      bool finite = true;
+      bf16x8 p[RT], rest[RT];       // the weights: bf16, and what that rounds off
 #pragma unroll
-      for (int hh = 0; hh < T / 2; ++hh) {
-        bf16x8 p[RT], rest[RT];       // the weights: bf16, and what that rounds off
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 x[2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          f32x4 x[2];
+        for (int kt = 0; kt < 2; ++kt) {
+          x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-              u32x4 key;
-              if constexpr (F8) {
-                const u32x4 c = s.k[2 * hh + kt][ks / 2];
-                const u32x2 lo = codes_to_bf16(c[2 * (ks & 1)], k_scale[2 * hh + kt]), hi = codes_to_bf16(c[2 * (ks & 1) + 1], k_scale[2 * hh + kt]);
-                key = u32x4{lo[0], lo[1], hi[0], hi[1]};
-              } else {
-                key = s.k[kt][ks];
-              }
-              x[kt] = mfma16(as_bf16x8(key), q[rt][ks], x[kt]);
+          for (int ks = 0; ks < KS; ++ks) {
+            u32x4 key;
+            if constexpr (F8) {
+              const u32x4 c = s.k[kt][ks / 2];
+              const u32x2 lo = codes_to_bf16(c[2 * (ks & 1)], k_scale[kt]), hi = codes_to_bf16(c[2 * (ks & 1) + 1], k_scale[kt]);
+              key = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+              key = s.k[kt][ks];
             }
+            x[kt] = mfma16(as_bf16x8(key), q[rt][ks], x[kt]);
           }
-          if (masked) {
+        }
+        if (masked) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (key0 + 16 * kt + 4 * g + r > lim[rt]) x[kt][r] = kNegInf;
+        }
+        if constexpr (kWeigh) {
+          const int row = r0 + 16 * rt + n16;
+          const int64_t item = static_cast<int64_t>(b) * a.kv_heads + h;
+          const int at = key0 + 4 * g;
+          const int stride = (M + 3) & ~3;
+          float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + at) * stride + row;
+          if (row < M)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
               for (int r = 0; r < 4; ++r)
-                if (key0 + 32 * hh + 16 * kt + 4 * g + r > lim[rt]) x[kt][r] = kNegInf;
-          }
-          if constexpr (kWeigh) {
-            const int row = r0 + 16 * rt + n16;
-            const int64_t item = static_cast<int64_t>(b) * a.kv_heads + h;
-            const int at = key0 + 32 * hh + 4 * g;
-            const int stride = (M + 3) & ~3;
-            float* to = a.scores + (item * (static_cast<int64_t>(a.c.max_pages) << a.c.page_shift) + at) * stride + row;
-            if (row < M)
-#pragma unroll
-              for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (at + 16 * kt + r < len) to[(16 * kt + r) * stride] = x[kt][r] * a.c2;
-          }
-          float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                            fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-          top = max_across32(max_across16(top)) * a.c2;
-          // the reference point follows the maximum once it lags by more than 2^8
-          if (__any(top > m[rt] + 8.0f)) {
-            const float mn = fmaxf(m[rt], top);
-            const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
-            m[rt] = mn;
-            l[rt] *= f;
-#pragma unroll
-            for (int t = 0; t < VW; ++t) o[rt][t] *= f;
-          }
-          const float mu = m[rt] == kNegInf ? 0.0f : m[rt];
-          float e[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
-            l[rt] += e[i];
-          }
-          // as the sum of two bf16: 2^-16 of each is left, far below the output's own rounding of 2^-8
-          u32x4 w, u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[i] = pack_bf16(e[2 * i], e[2 * i + 1]);
-            u[i] = pack_bf16(e[2 * i] - __uint_as_float(w[i] << 16), e[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
-          }
-          p[rt] = as_bf16x8(w);
-          rest[rt] = as_bf16x8(u);
+                if (at + 16 * kt + r < len) to[(16 * kt + r) * stride] = x[kt][r] * a.c2;
         }
-        if (hh == 0) {
-          finite = all_finite();
-          if (!finite) add_nonfinite(kk);
+        float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                          fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        top = max_across32(max_across16(top)) * a.c2;
+        // the reference point follows the maximum once it lags by more than 2^8
+        if (__any(top > m[rt] + 8.0f)) {
+          const float mn = fmaxf(m[rt], top);
+          const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
+          m[rt] = mn;
+          l[rt] *= f;
+#pragma unroll
+          for (int t = 0; t < VW; ++t) o[rt][t] *= f;
         }
-        u32x2 w0[VW], w1[VW];
+        const float mu = m[rt] == kNegInf ? 0.0f : m[rt];
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] * a.c2 - mu);
+          l[rt] += e[i];
+        }
+        // as the sum of two bf16: 2^-16 of each is left, far below the output's own rounding of 2^-8
+        u32x4 w, u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = pack_bf16(e[2 * i], e[2 * i + 1]);
+          u[i] = pack_bf16(e[2 * i] - __uint_as_float(w[i] << 16), e[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+        }
+        p[rt] = as_bf16x8(w);
+        rest[rt] = as_bf16x8(u);
+      }
+      const bool finite = all_finite();
+      if (!finite) add_nonfinite(kk);
+      u32x2 w0[VW], w1[VW];
+      if constexpr (F8) {
+        values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[0]), v_scale[0], w0);
+        values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[4]), v_scale[1], w1);
+      }
+#pragma unroll
+      for (int t = 0; t < VW; ++t) {
+        u32x4 w;
         if constexpr (F8) {
-          values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[8 * hh]), v_scale[2 * hh], w0);
-          values_of<VW>(*reinterpret_cast<const uint32_t(*)[4][VW / 4]>(&s.v[8 * hh + 4]), v_scale[2 * hh + 1], w1);
+          w = u32x4{w0[t][0], w0[t][1], w1[t][0], w1[t][1]};
+        } else {
+          const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(s.v[2 * i + 1][t / 2], s.v[2 * i][t / 2], sel);
         }
+        if (!finite)
 #pragma unroll
-        for (int t = 0; t < VW; ++t) {
-          u32x4 w;
-          if constexpr (F8) {
-            w = u32x4{w0[t][0], w0[t][1], w1[t][0], w1[t][1]};
-          } else {
-            const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
+          for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(s.v[2 * i + 1][t / 2], s.v[2 * i][t / 2], sel);
-          }
-          if (!finite)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = finite_only(w[i]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), rest[rt], mfma16(as_bf16x8(w), p[rt], o[rt][t]));
-        }
+        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma16(as_bf16x8(w), rest[rt], mfma16(as_bf16x8(w), p[rt], o[rt][t]));
       }
     };
 
@@ -532,7 +525,6 @@ __device__ __forceinline__ void segment(const PagedArgs& a, int b, int h, int le
 // Workgroup `share` of a.shares takes its share of all units.
 template <int D, int RT, bool F8, bool kWeigh>
 __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, SegLds<D, RT, 4>& lds) {
-  constexpr int T = Step<D, F8>::kTiles;
   constexpr uint32_t kHead = item_units<F8>();
   Units n;
   uint32_t all = 0;                  // units of one key head
@@ -595,7 +587,7 @@ __device__ __forceinline__ void shares(const PagedArgs& a, int share, int r0, Se
     if (k0 == 0 && r0 == 0 && threadIdx.x == 0)
       a.parts[b * a.kv_heads + h] =
           i32x2{static_cast<int>(slot), whole ? (a.splits ? 1 : 0) : share_of(item0 + nb - 1) - share + 1};
-    segment<D, RT, 4, F8, kWeigh>(a, b, h, len, bad_len, r0, k0 * kPgUnit, k1 * kPgUnit, slot, page_ids<4, T>(a, b, k0 * (kPgUnit / 16), 0), lds);
+    segment<D, RT, 4, F8, kWeigh>(a, b, h, len, bad_len, r0, k0 * kPgUnit, k1 * kPgUnit, slot, page_ids<4>(a, b, k0 * (kPgUnit / 16), 0), lds);
   }
 }
 
@@ -715,7 +707,7 @@ template <int D, bool F8, bool kWeigh>
 __global__ __launch_bounds__(64 * kPgShortWaves, 2) void k_paged_short(const PagedArgs a) {
   __shared__ SegLds<D, 1, kPgShortWaves> lds;
   const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, M = a.q_len * a.group, r0 = 16 * blockIdx.y;
-  const int ids = page_ids<kPgShortWaves, Step<D, F8>::kTiles>(a, b, 0, 0);   // on its way beside the length
+  const int ids = page_ids<kPgShortWaves>(a, b, 0, 0);   // on its way beside the length
   bool bad_len;
   const int len = length_of(a, b, bad_len);
   if (len > 0) {
