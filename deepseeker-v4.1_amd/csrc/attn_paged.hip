@@ -37,6 +37,15 @@
 // for 16385 keys and 64 sequences).  There the kernel takes 29 us: 9 us from the launch to the
 // first tile's end and for 16.8 MB of partial rows, 1 us for each of 16 tiles, the rest the
 // shares' loads beside them; the join of 16 parts and the own keys' takes 6.6 us.
+//
+// A cache in 8 bits (kv8.h) is the same kernel with codes made to bf16 in registers, exactly.  64 sequences of 1
+// to 8192 keys: 26 us for 101 MB, of which the bytes are 17 at the 6 TB/s that long sequences reach, a workgroup's start and
+// end most of the rest, and 4.8 us for the join.  The prefix of 16385 keys: 33 us beside 29 in bf16, since its products,
+// not its bytes, bound it and the conversions come to them.
+//
+// Weights of the keys need every row's final sum, so scores wait in float32 for a pass of their own beside (or behind) the
+// join: 8 M bytes a key and head more, against 4 D (2 D) for the key and value.  With few rows that is little: 48
+// sequences of up to 2100 keys, four rows, 16 us and 5.8 for the join and weights; with 64 rows the weights take as long as all else.
 #include <math.h>
 
 #include <algorithm>
@@ -58,7 +67,7 @@ constexpr int kPgUnit = 4 * kPgStep; // of which shares are made: a step of each
 template <bool F8>
 constexpr uint32_t item_units() { return F8 ? 1 : 0; }
 constexpr int kPgShort = 512;       // keys of a table row that one workgroup takes alone
-constexpr int kPgShortMany = 1024;  // where there are kPgMany items
+constexpr int kPgShortMany = 1024;  // where there are kPgMany items, or codes to read
 constexpr int kPgMany = 512;
 constexpr int kPgShortWaves = 8;
 constexpr int64_t kPgFewKeys = 512 << 10;
@@ -910,7 +919,7 @@ template <int kLanes>
 __global__ __launch_bounds__(kPgThreads) void k_key_weights(const PagedArgs a, int each) {
   weigh_keys<kLanes, false>(a, blockIdx.x, each);
 }
-// Both in one launch, for up to kKwPartRows rows an item (48 sequences of up to 2100 keys, 4 rows: TODO).
+// Both in one launch, for up to kKwPartRows rows an item (48 sequences of up to 2100 keys, 4 rows: 21.7 us, 24.7 with two).
 template <int D, int WPR, int kLanes>
 __global__ __launch_bounds__(kPgThreads) void k_join_weights(const PagedArgs a, int each, int join_blocks) {
   const int block = blockIdx.x - join_blocks;
@@ -932,8 +941,8 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   const int64_t M = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
   const int64_t items = static_cast<int64_t>(d.batch) * d.kv_heads, keys = static_cast<int64_t>(c.max_pages) * c.page_size;
   // With scales or weights, up to kPgFewKeys places of more than 16 rows: 16 rows a workgroup, two a CU, read the cache
-  // once more but wait less.  8 key heads of 128, weights in 8 bits: one sequence of 8000 keys and three of 300, 64 rows, 39 us, 44 with 32 rows a
-  // workgroup, 32 rows 36 and 40; four of 8000, 64 rows, 75 and 72; 64 of 4000, 32 rows, 398 and 318.
+  // once more but wait less.  8 key heads of 128, weights in 8 bits: one sequence of 8000 keys and three of 300, 64 rows, 35.1 us, 38.7 with 32 rows
+  // a workgroup, 32 rows 32.5 and 35.4; four of 8000, 64 rows, 74.0 and 74.4; 64 of 4000, 32 rows, 335 and 315 (bf16: 602 and 412).
   const bool extra = more.f8 || more.weigh, few = extra && items * keys <= kPgFewKeys;
   p.rt = M <= 16 || few ? 1 : 2;
   // Up to kPgShort keys are two steps of a workgroup of eight waves, whose loads are all in flight at once: one
@@ -941,8 +950,10 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   // 9.3, but 9.9 against 9.3 for 517 and 14.6 against 9.3 for 1000.  Where items fill the
   // machine without shares, the join is all that they would add (64 such sequences of 600 / 1000 keys: 30.2 / 44.5 us, 31.6 / 45.9
   // with shares).
+  // Codes take half the time: one sequence of 517 keys in 8 bits, with 640 places, 9.6 us, 12.2 with shares; with weights, whose kernel
+  // waits for it, 13.8 and 12.5.
   // (a launch counts its threads in 32 bits)
-  p.alone = d.prefix_len == 0 && keys <= (more.f8 ? 2 : 1) * (items >= kPgMany ? kPgShortMany : kPgShort) &&
+  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany || (more.f8 && !more.weigh) ? kPgShortMany : kPgShort) &&
             items * (64 * kPgShortWaves) < (int64_t{1} << 32);
   p.total = 256;
   // behind what the call needs otherwise
@@ -959,8 +970,8 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   // the workgroups that are resident at once, two a CU (64 sequences of up to 8192 keys, 8 heads
   // of 128: 81 us, 90 with 256 and 86 with 768); one a CU where registers allow no
   // more, or beside a prefix's (36.5 us with 256, 39.4 with 512, 64 sequences behind 16385 keys)
-  // (with scales or weights, workgroups for all rows of a share are resident at once: 4 sequences of up to 8000 keys with 64
-  // rows 63 us with 256 shares of two workgroups, 49 with 128)
+  // (with scales or weights, workgroups for all rows of a share are resident at once: that sequence of 8000 keys with 64
+  // rows takes 45.9 us with shares for one workgroup each, 35.1 with a quarter as many)
   const int64_t each = extra && (M > 32 || few) ? (M + 16 * p.rt - 1) / (16 * p.rt) : 1;
   const int64_t most = (p.rt == 1 && d.prefix_len == 0 ? 512 : 256) / each;
   p.shares = static_cast<int>(units < most ? units : most);

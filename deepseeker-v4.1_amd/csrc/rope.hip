@@ -24,7 +24,7 @@
 //
 // Keys and values for a cache in 8 bits: a block's scale needs the largest element of all its rows, so
 // a workgroup takes the tokens of whole blocks (append_codes), beside those of the
-// queries in one launch.
+// queries in one launch: 8192 tokens of 32 + 8 + 8 heads of 128 take 43 us (4.2 TB/s), 64 of them 6.6.
 #include <type_traits>
 
 #include "kv8.h"
@@ -464,7 +464,8 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
 // reads for every row tile, always stay: past L2 they cost it up to 16 % (3000 tokens of 12 + 12 + 12: 43.9 -> 50.5).
 constexpr int64_t kPastL2 = 4 << 20;
 
-// Workgroups for the keys and values of a cache in 8 bits, at least about: a head's, until there are these.
+// Workgroups for the keys and values of a cache in 8 bits, at least about: heads of a token apart until there are these, though
+// each makes the angles anew (8192 tokens 43.4 us, 46.9 with 1024, 54 with 2048).
 constexpr int kCodeBlocks = 512;
 
 template <int D>
