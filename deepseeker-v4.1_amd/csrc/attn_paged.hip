@@ -950,10 +950,10 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   // 9.3, but 9.9 against 9.3 for 517 and 14.6 against 9.3 for 1000.  Where items fill the
   // machine without shares, the join is all that they would add (64 such sequences of 600 / 1000 keys: 30.2 / 44.5 us, 31.6 / 45.9
   // with shares).
-  // Codes take half the time: one sequence of 517 keys in 8 bits, with 640 places, 9.6 us, 12.2 with shares; with weights, whose kernel
-  // waits for it, 13.8 and 12.5.
+  // Codes take half the time: one sequence of 517 keys in 8 bits, with 640 places, 9.6 us, 12.2 with shares (with weights, whose kernel
+  // waits for it, 13.8 and 12.5, but a decode step then has the same bits with and without them).
   // (a launch counts its threads in 32 bits)
-  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany || (more.f8 && !more.weigh) ? kPgShortMany : kPgShort) &&
+  p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany || more.f8 ? kPgShortMany : kPgShort) &&
             items * (64 * kPgShortWaves) < (int64_t{1} << 32);
   p.total = 256;
   // behind what the call needs otherwise

@@ -341,10 +341,11 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, position
     are also written to ``k_out`` if given.  Tokens outside the table or with a page outside the cache are not kept; two
     tokens of one call must not share a row.
 
-    ``rows`` (int32): the tokens' rows in their sequences, where positions do not give them (several axes, a cache that was
-    evicted from; prefix_len is then 0).  ``k_scale``, ``v_scale``: a cache in 8 bits.  There the tokens that go to one block of
+    ``rows`` (int32): the tokens' rows in their sequences, where positions (of several axes: the first) do not give them, as
+    those of pictures and behind an eviction; prefix_len is then 0.  ``k_scale``, ``v_scale``: a cache in 8 bits.  There the tokens that go to one block of
     16 rows stand next to each other in the call; a call that brings a block's first row starts the block afresh, otherwise the
-    rows that are there are rounded to the larger of the block's scale and the call's.  ``key_weights``: zero for the kept keys."""
+    rows that are there are rounded to the larger of the block's scale and the call's.  ``key_weights``: zero for the kept keys.
+    With scales or weights no page belongs to two sequences."""
     if not (type(mscale) is type(eps) is float and type(interleaved) is type(norm) is bool and type(rot_first) is int):
         interleaved, rot_first, mscale, norm, eps = bool(interleaved), int(rot_first), float(mscale), bool(norm), float(eps)
     if type(prefix_len) is not int:
@@ -597,6 +598,10 @@ class DecodeStep:
     prefix: torch.Tensor | None = None
     prefix_len: int = 0
     rows: torch.Tensor | None = None
+
+    def __post_init__(self):
+        if self.rows is None and isinstance(self.positions, torch.Tensor) and self.positions.dim() > 1:
+            raise ValueError("positions on several axes do not say which rows the tokens take: give rows")
 
     def idle(self) -> DecodeStep:
         """A step of the same sizes whose slots are all unused: it keeps nothing."""

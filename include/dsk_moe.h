@@ -428,7 +428,7 @@ int dsk_paged_attention(const dsk_paged_desc* d, const dsk_kv_cache* cache, cons
  * freq[i]; a pair whose axis is none of 0 .. n_axes - 1 does not turn.  A token
  * that is negative on any axis is left out. */
 typedef struct dsk_rope_axes {
-  int64_t axis_stride;    /* elements between the axes of positions, >= tokens */
+  int64_t axis_stride;    /* elements between the axes of positions, >= 0 (0: all axes have the same) */
   int32_t n_axes;         /* 1..8 */
   const int32_t* axis;    /* [rot_dim / 2] i32, device */
 } dsk_rope_axes;
@@ -443,7 +443,10 @@ typedef struct dsk_rope_axes {
  * without a part in the scale.
  *
  * key_weights [n_pages, kv_heads, page_size] f32: the softmax weight that every key
- * has received. */
+ * has received.
+ *
+ * Scales and weights belong to a page, so with them a page is written, weighed and
+ * evicted from for one sequence alone; pages that sequences share are a prefix. */
 typedef struct dsk_kv_extra {
   uint8_t* k_scale;
   uint8_t* v_scale;

@@ -71,8 +71,9 @@ def test_equal_axes_are_one_axis():
     pos = torch.randint(0, 1 << 30, (50,), generator=g, dtype=I32).to(DEV)
     freq, axis = dsk_moe.rope_axes([16, 24, 24], base=1e6)
     one = dsk_moe.qk_norm_rope(q, k, pos, freq)
-    for got, want in zip(dsk_moe.qk_norm_rope(q, k, pos.expand(3, 50).contiguous(), freq, axis=axis), one):
-        assert torch.equal(got, want)
+    for same in (pos.expand(3, 50).contiguous(), pos.expand(3, 50)):
+        for got, want in zip(dsk_moe.qk_norm_rope(q, k, same, freq, axis=axis), one):
+            assert torch.equal(got, want)
     for got, want in zip(dsk_moe.qk_norm_rope(q, k, pos[None], freq, axis=torch.zeros_like(axis)), one):
         assert torch.equal(got, want)
 

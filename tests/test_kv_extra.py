@@ -62,7 +62,7 @@ def test_structs_have_the_header_s_sizes():
 
 
 @pytest.mark.parametrize("kw,want", [(dict(n_axes=0), -1), (dict(n_axes=9), -1), (dict(axis=None), -1), (dict(axis=ODD), -2),
-                                     (dict(axis_stride=3), -1), (dict(axis_stride=-4), -1), (dict(axis_stride=1 << 41), -1)])
+                                     (dict(axis_stride=-4), -1), (dict(axis_stride=(1 << 40) + 1), -1)])
 def test_axes_refused(kw, want):
     assert code("dsk_qk_norm_rope_axes", ctypes.byref(qk_desc()), axes(**kw), *[P] * 8, None) == want
     assert code("dsk_kv_append_extra", ctypes.byref(qk_desc()), ctypes.byref(cache()), axes(**kw), extra(), *[P] * 14, None) == want
@@ -164,6 +164,14 @@ def test_steps_on_several_axes_name_their_rows():
     for rows in ([0, 1, 3, 2], [4, 5, 6, 7], [0, 1, 2, -1]):
         with pytest.raises(ValueError, match="whole prompts"):
             dsk_moe.PromptStep(pos, ints([0] * 4), ints([[0]]), ints([0, 4]), rows=ints(rows))
+
+
+def test_decode_steps_on_several_axes_name_their_rows():
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match="give rows"):
+        dsk_moe.DecodeStep(ints([[5], [6]]), ints([0]), ints([[0]]), ints([6]))
+    step = dsk_moe.DecodeStep(ints([[5], [6]]), ints([0]), ints([[0]]), ints([6]), rows=ints([5]))
+    assert (step.idle().positions == -1).all() and step.idle().lens.tolist() == [-1]
 
 
 def test_caches_and_stacks_refuse_what_they_cannot_keep():
