@@ -206,6 +206,47 @@ def test_append_codes(dtype, dim, page, kv, turned):
     check_append(g, k, v, table, seq, rows, kc, ks, vc, vs, pos, freq, weights=True, norm=turned)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,rot,first,inter", [(128, 128, 0, True), (128, 64, 32, False), (64, 32, 16, True), (64, 64, 0, False)])
+def test_append_codes_turned(dtype, dim, rot, first, inter):
+    """Both kinds of pairs, a part of the head turned, gammas, three axes: the values within their one rounding, as k_out's."""
+    g = gen(dim + rot + first)
+    kv, page, t = 3, 32, 90
+    table = torch.randperm(8, generator=g)[:6].view(2, 3).to(I32)
+    rows = torch.cat([torch.arange(5, 60), torch.arange(35)]).to(I32)
+    seq = torch.tensor([0] * 55 + [1] * 35, dtype=I32)
+    q, k, v = (normal(g, t, n, dim, dtype=dtype) for n in (5, kv, kv))
+    pos = torch.randint(0, 9000, (3, t), generator=g, dtype=I32)
+    freq, axis = dsk_moe.rope_axes([rot // 2 - 2 * (rot // 8), rot // 8, rot // 8], in_turn=inter, device="cpu")
+    gq, gk = torch.rand(dim, generator=g) + 0.5, torch.randn(dim, generator=g)
+    more = dict(interleaved=inter, rot_first=first, mscale=1.1)
+    kd, vd = dev8(torch.zeros(8, kv, page, dim, dtype=U8), torch.zeros(8, kv, page, dim, dtype=U8))
+    ks, vs = (torch.zeros(8, kv, page // 16, dtype=U8, device=DEV) for _ in range(2))
+    ko = torch.empty((t, kv, dim), dtype=BF16, device=DEV)
+    got = dsk_moe.kv_append(q.to(DEV), k.to(DEV), v.to(DEV), pos.to(DEV), seq.to(DEV), table.to(DEV), kd, vd, freq.to(DEV), axis=axis.to(DEV),
+                            rows=rows.to(DEV), k_scale=ks, v_scale=vs, q_gamma=gq.to(DEV), k_gamma=gk.to(DEV), k_out=ko, **more)
+    at = pos[axis.long()].t()
+    assert_within(got, *O.norm_rope(q, at, freq, gamma=gq, **more), "q")
+    want, tol = O.norm_rope(k, at, freq, gamma=gk, **more)
+    assert_within(ko, want, tol, "k")
+    real, byte = O.values(kd.cpu().view(U8), ks.cpu()), ks.cpu()
+    p, r = table[seq.long(), rows.long() // page].long(), rows.long() % page
+    size = 2.0 ** (byte[p, :, r // 16].double()[..., None] - 127)
+    arithmetic = tol - O.BF16_HALF_STEP * want.abs()
+    # (each block comes in one call: one rounding, of a scale that is at most twice the least)
+    bound = torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * size) + arithmetic * (1 + 2.0 ** -4)
+    assert ((real[p, :, r] - want).abs() <= bound).all()
+    # both sequences' blocks: the least scale for their largest, up to float32's roundings at a border
+    for b, lo, hi in ((0, 5, 60), (1, 0, 35)):
+        for block in range(lo // 16, -(-hi // 16)):
+            mine = (seq == b) & (rows // 16 == block)
+            if bool((rows[mine] % 16 == 0).any()):
+                top = want[mine].abs().amax((0, 2))
+                have = byte[int(table[b, block * 16 // page]), :, block * 16 % page // 16]
+                for h in range(kv):
+                    assert int(have[h]) in {O.scale_byte(float(top[h]) * f) for f in (1 - 1e-6, 1.0, 1 + 1e-6)}
+
+
 @pytest.mark.parametrize("tokens,batch", [(1, 1), (64, 64), (130, 65), (2060, 2)])
 def test_append_codes_of_few_and_many(tokens, batch):
     """Decode steps, verify steps and prompts: as many workgroups for a token as for 16."""
@@ -506,11 +547,13 @@ def test_key_weights(codes, heads, kv, dim, page, q_len, prefix, spare):
 @pytest.mark.parametrize("codes", [False, True])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv,q_len", [(4, 1, 5), (8, 1, 4), (8, 1, 8), (4, 1, 16)])
-def test_many_rows_in_wide_tables(codes, dim, heads, kv, q_len):
+@pytest.mark.parametrize("prefix", [0, 300])
+def test_many_rows_in_wide_tables(codes, dim, heads, kv, q_len, prefix):
     """More than 16 rows an item where the tables have many places (the other cases have few)."""
     g = gen(heads + q_len + dim)
     lens = [900, 40, 0]
-    _, table, kc, ks, vc, vs = paged8_setup(g, lens, kv, 256, dim)
+    pre, table, kc, ks, vc, vs = paged8_setup(g, lens, kv, 256, dim, 1, prefix)
+    more = dict(prefix=pre.to(DEV), prefix_len=prefix) if prefix else {}
     wide = torch.full((3, 700), -1, dtype=I32)                   # 537600 places
     wide[:, :table.shape[1]] = table
     k64, v64 = O.values(kc, ks), O.values(vc, vs)
@@ -518,14 +561,14 @@ def test_many_rows_in_wide_tables(codes, dim, heads, kv, q_len):
     w = torch.rand(kc.shape[:3], generator=g)
     wd = w.to(DEV)
     if codes:
-        got = run_paged8(q, wide, lens, kc, ks, vc, vs, key_weights=wd)
-        assert torch.equal(got, run_paged8(q, wide, lens, kc, ks, vc, vs))
+        got = run_paged8(q, wide, lens, kc, ks, vc, vs, key_weights=wd, **more)
+        assert torch.equal(got, run_paged8(q, wide, lens, kc, ks, vc, vs, **more))
     else:
         k64, v64 = k64.to(BF16).double(), v64.to(BF16).double()
-        got = dsk_moe.paged_attention(q.to(DEV), k64.to(BF16).to(DEV), v64.to(BF16).to(DEV), wide.to(DEV), ints(lens), key_weights=wd)
-    want, tol = O.paged(q, k64, v64, wide, lens)
+        got = dsk_moe.paged_attention(q.to(DEV), k64.to(BF16).to(DEV), v64.to(BF16).to(DEV), wide.to(DEV), ints(lens), key_weights=wd, **more)
+    want, tol = O.paged(q, k64, v64, wide, lens, pre, prefix)
     assert_within(got, want, tol)
-    want, tol = weights_want(w, q, k64, wide, lens, 256, dim ** -0.5)
+    want, tol = weights_want(w, q, k64, wide, lens, 256, dim ** -0.5, pre, prefix)
     assert_within(wd, want, tol + 1e-38, "weights")
 
 
@@ -859,6 +902,41 @@ def test_decoder_on_several_axes_in_8_bits(dtype):
         outs.append(got)
     for a, b in zip(*outs):
         assert torch.equal(a, b) and torch.isfinite(a.float()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F8])
+def test_captured_prompts_that_weigh(dtype):
+    """A captured step of whole prompts on three axes follows its bounds, places and positions: outputs, caches and weights as
+    the eager step's, every replay."""
+    g, stack = decoder_with(76, dtype, 5, True)
+    tokens = 60
+    table = torch.randperm(60, generator=g)[:36].view(3, 12).to(I32).to(DEV)
+
+    def fill(step, lens):
+        rows = torch.full((tokens,), -1, dtype=I32)
+        rows[:sum(lens)] = torch.tensor([i for n in lens for i in range(n)], dtype=I32)
+        step.rows.copy_(rows)
+        step.positions.copy_(torch.where(rows >= 0, torch.randint(0, 50, (3, tokens), generator=g, dtype=I32), -1))
+        step.seq.copy_(torch.tensor([b for b, n in enumerate(lens) for _ in range(n)] + [0] * (tokens - sum(lens)), dtype=I32))
+        step.cu.copy_(torch.tensor(cumulative(lens), dtype=I32))
+
+    rows = torch.arange(tokens, dtype=I32, device=DEV)
+    step = dsk_moe.PromptStep(rows.repeat(3, 1), torch.zeros_like(rows), table, ints([0, tokens, tokens, tokens]), rows=rows)
+    stack.capture(tokens, step=step)
+    caches = [c for a in stack.attention for c in a.cache_tensors() if c is not None]
+    raw = [c.view(U8) if c.dtype == F8 else c for c in caches]
+    for lens in ([20, 1, 30], [60, 0, 0], [3, 4, 2], [20, 20, 20]):
+        fill(step, lens)
+        x = normal(g, tokens, 1024).to(DEV)
+        for c in raw:
+            c.zero_()
+        got = stack.replay(x).clone()
+        held = [c.clone() for c in raw]
+        assert any(a.key_weights.any() for a in stack.attention)
+        for c in raw:
+            c.zero_()
+        want = stack(x, step=step)
+        assert torch.equal(got[:sum(lens)], want[:sum(lens)]) and all(torch.equal(c, h) for c, h in zip(raw, held))
 
 
 def test_8_bit_decoder_is_near_the_bf16_one():
