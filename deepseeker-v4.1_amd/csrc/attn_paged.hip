@@ -73,6 +73,7 @@ constexpr int kPgShortWaves = 8;
 constexpr int64_t kPgFewKeys = 512 << 10;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct PagedArgs {
@@ -876,6 +877,7 @@ template <int kLanes, bool kParts>
 __device__ __forceinline__ void weigh_keys(const PagedArgs& a, int block, int each) {
   constexpr int kKeys = kPgThreads / kLanes;
   __shared__ __align__(16) float lse[kKwRows];
+  __shared__ __align__(16) int last[kKwRows];          // key that the row sees (-1: there is no such row)
   const int item = block / each, part = block % each, b = item / a.kv_heads, h = item % a.kv_heads, M = a.q_len * a.group;
   i32x2 of_item{};
   if constexpr (kParts) of_item = ldg<i32x2>(a.parts + item);
@@ -883,6 +885,8 @@ __device__ __forceinline__ void weigh_keys(const PagedArgs& a, int block, int ea
   const int len = length_of(a, b, bad);
   if (bad || len <= part * kKeys) return;
   const Parts of(a, of_item, b, h, len);
+  if (threadIdx.x < kKwRows)
+    last[threadIdx.x] = static_cast<int>(threadIdx.x) < M ? len - a.q_len + static_cast<int>(threadIdx.x) / a.group : -1;
   if (kParts && !of.done) {
     const float x = lse_of_parts(a, of, b, len);
     if (threadIdx.x % 16 == 0) lse[threadIdx.x / 16] = x;
@@ -900,9 +904,10 @@ __device__ __forceinline__ void weigh_keys(const PagedArgs& a, int block, int ea
     float sum = 0.0f;
     for (int r = 4 * lane; r < M; r += 4 * kLanes) {
       const f32x4 v = ldg<f32x4>(x + r), e = *reinterpret_cast<const f32x4*>(&lse[r]);
+      const i32x4 n = *reinterpret_cast<const i32x4*>(&last[r]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)                     // nothing of a key that the row does not see, whatever the row is
-        if (r + i < M && v[i] != kNegInf) sum += __builtin_amdgcn_exp2f(v[i] - e[i]);
+        if (key <= n[i]) sum += __builtin_amdgcn_exp2f(v[i] - e[i]);
     }
 #pragma unroll
     for (int s = kLanes / 2; s >= 1; s >>= 1) sum += __shfl_xor(sum, s, 64);

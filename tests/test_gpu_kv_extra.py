@@ -609,6 +609,55 @@ def test_key_weights_of_bad_sequences(spare):
         assert at(3, r) == w[int(table[3, r // 16]), 0, r % 16] if r < 48 else True
 
 
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("heads,q_len", [(2, 2), (8, 2), (8, 8)])
+@pytest.mark.parametrize("spare", [1, 200])
+def test_key_weights_of_endless_scores(codes, heads, q_len, spare):
+    """Scores of minus infinity: a row of nothing else is NaN, as its output is, to all keys that it sees and to no others; among
+    others such a key gets nothing; beside a NaN score it is NaN as well."""
+    g = gen(heads + q_len)
+    lens = [37, 37, 37]
+    _, table, kc, ks, vc, vs = paged8_setup(g, lens, 1, 16, 64, spare)
+    k64 = O.values(kc, ks) if codes else normal(g, *kc.shape).double()
+    v64 = O.values(vc, vs) if codes else normal(g, *vc.shape).double()
+    q = normal(g, 3, q_len, heads, 64)
+    row = lambda b, r: (int(table[b, r // 16]), 0, r % 16)  # noqa: E731
+    minus = 0xb8                                           # the code of -1
+
+    def put(b, r, code, value):
+        if codes:
+            kc[row(b, r)][0] = code
+        k64[row(b, r)][0] = value
+
+    q[0, 0, 1, 0] = q[1, 0, 1, 0] = INF
+    for r in range(37):
+        for b in (0, 1):
+            put(b, r, minus, -1.0)
+    put(1, 3, 0x7f, NAN)
+    if codes:
+        k64 = O.values(kc, ks)
+    else:
+        k64[row(2, 5)][0] = -INF
+        q[2, :, :, 0] = q[2, :, :, 0].abs() + 1
+    w = torch.zeros(kc.shape[:3], dtype=F32)
+    wd = w.to(DEV)
+    if codes:
+        out = run_paged8(q, table, lens, kc, ks, vc, vs, key_weights=wd)
+    else:
+        out = dsk_moe.paged_attention(q.to(DEV), k64.to(BF16).to(DEV), v64.to(BF16).to(DEV), table.to(DEV), ints(lens), key_weights=wd)
+    got = wd.cpu()
+    assert out[0, 0, 1].isnan().all() and out[1, 0, 1].isnan().all()
+    seen = 37 - q_len + 1                                  # by the first token
+    for r in range(37):
+        assert bool(got[row(0, r)].isnan()) == (r < seen), r
+        assert bool(got[row(1, r)].isnan()), r             # the other heads and tokens meet the NaN itself
+    assert not got[table[2, :3].long()].isnan().any() and torch.isfinite(out[2]).all()
+    total = q_len * heads                                  # (the first tokens see fewer keys, but some)
+    assert abs(float(got[table[2, :3].long()].double().sum()) - total) < total * 2.0 ** -15
+    if not codes:
+        assert got[row(2, 5)] == 0
+
+
 # ------------------------------------------------------------------ eviction
 def evict_case(g, lens, keep, first, recent, kv, page, dim, codes, weights=None, spoil=None, spare=1, **kw):
     used = [-(-max(0, n) // page) for n in lens]
