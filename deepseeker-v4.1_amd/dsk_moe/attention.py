@@ -496,6 +496,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 # ------------------------------------------------------------------ eviction
 def _evict_plan(k_cache, v_cache, key_weights, table, lens, keep, first, recent, k_scale, v_scale, lens_out):
     """(device, descriptor, cache, bytes of workspace)."""
+    if max(map(abs, (keep, first, recent))) >= 1 << 31:     # (the entry point's are 32 bits)
+        raise ValueError(f"keep={keep}, first={first} and recent={recent} must fit 32 bits")
     dev = _hip(k_cache)
     if k_cache.dim() != 4:
         raise ValueError(f"k_cache must be [pages, kv_heads, page_size, head_dim], got {tuple(k_cache.shape)}")

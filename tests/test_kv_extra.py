@@ -141,6 +141,10 @@ def test_functions_refuse_cpu_tensors_and_other_caches():
     b, i = torch.zeros(4, 2, 64, 128, dtype=torch.bfloat16), torch.zeros(1, 4, dtype=torch.int32)
     with pytest.raises(ValueError, match="HIP device"):
         dsk_moe.kv_evict(b, b, torch.zeros(4, 2, 64), i, i[0, :1], 2)
+    # numbers that 32 bits would make others of
+    for bad in (dict(keep=(1 << 32) + 2), dict(keep=1 << 31), dict(keep=8, first=1 << 32), dict(keep=8, recent=-(1 << 32))):
+        with pytest.raises(ValueError, match="keep"):
+            dsk_moe.kv_evict(b, b, torch.zeros(4, 2, 64), i, i[0, :1], **bad)
     check = lambda k=b.to(torch.float8_e4m3fn), s=torch.zeros(4, 2, 4, dtype=torch.uint8), v=None, w=None: A._check_cache(  # noqa: E731
         k, k, i, 2, 128, torch.device("cpu"), s, s if v is None else v, w)
     check()
