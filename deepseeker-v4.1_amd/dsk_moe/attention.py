@@ -549,11 +549,12 @@ class PromptStep:
     pages are table[seq[t]] (all int32 on the device).  A prompt's tokens attend over its own keys alone, so its
     positions are 0, 1, ..; rows of no prompt have position -1.  A step with other positions (a prompt's later part,
     which would not see the keys kept before, or a prompt behind a shared prefix) is refused when it is made, by
-    one look at the device's values (40 us, 65 for 8192 tokens); inside a graph capture, and of values written
+    one look at the device's values (40 us, 65 for 8192 tokens; with rows at both); inside a graph capture, and of values written
     later, nothing is looked at.
 
     rows: the tokens' rows of the cache where positions do not give them, as with positions [axes, tokens] on several axes;
-    then they are 0, 1, .. in the rows cu[i] .. cu[i+1] and -1 in others."""
+    then they are 0, 1, .. in the rows cu[i] .. cu[i+1] and -1 in others, and no position of a prompt's token is negative
+    (such a token would be left out, and others of its prompt would attend over a key that nobody wrote)."""
 
     positions: torch.Tensor
     seq: torch.Tensor
@@ -576,6 +577,8 @@ class PromptStep:
         if not (whole and (at[:cu[0]] < 0).all() and (at[cu[-1]:] < 0).all()
                 and (at[cu[0]:cu[-1]] == np.arange(cu[0], cu[-1]) - np.repeat(cu[:-1], n)).all()):
             raise ValueError("a PromptStep takes whole prompts: positions (rows) 0, 1, .. in the rows cu[i] .. cu[i+1], and -1 in others")
+        if self.rows is not None and (self.positions.shape[-1:] != (t,) or (self.positions[..., cu[0]:cu[-1]].cpu().numpy() < 0).any()):
+            raise ValueError(f"positions of a PromptStep with rows must be those of {t} tokens, not negative in the rows cu[i] .. cu[i+1]")
 
     def idle(self) -> PromptStep:
         """A step of the same sizes that has no sequences and keeps nothing."""

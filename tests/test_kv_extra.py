@@ -170,6 +170,28 @@ def test_steps_on_several_axes_name_their_rows():
             dsk_moe.PromptStep(pos, ints([0] * 4), ints([[0]]), ints([0, 4]), rows=ints(rows))
 
 
+@pytest.mark.parametrize("axes", [None, 1, 3])
+def test_prompt_steps_with_rows_refuse_tokens_that_would_be_left_out(axes):
+    """A negative position of a prompt's token on any axis: its key would not be written, and its prompt would read it."""
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    rows, cu = ints([-1, 0, 1, 2, 0, 1, -1]), ints([1, 4, 4, 6])
+
+    def step(pos):
+        return dsk_moe.PromptStep(pos, ints([0, 0, 0, 0, 1, 1, 0]), ints([[0], [1]]), cu, rows=rows)
+
+    good = torch.where(rows >= 0, 5 + rows, -1)
+    good = good if axes is None else good.repeat(axes, 1)
+    step(good)
+    step(torch.full_like(good, 9))                                  # tokens of no prompt are not kept wherever they are
+    for t in (1, 2, 5):
+        bad = good.clone()
+        bad[(-1, t) if axes else t] = -1
+        with pytest.raises(ValueError, match="not negative"):
+            step(bad)
+    with pytest.raises(ValueError, match="7 tokens"):
+        step(good[..., :6])
+
+
 def test_decode_steps_on_several_axes_name_their_rows():
     ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     with pytest.raises(ValueError, match="give rows"):
