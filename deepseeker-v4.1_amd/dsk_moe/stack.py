@@ -59,6 +59,14 @@ def rmsnorm(x: torch.Tensor, eps: float = 1e-6, gamma: torch.Tensor | None = Non
     return out if want else None
 
 
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from a's first to its last element meets that of b."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a.device == b.device and a0 < b1 and b0 < a1
+
+
 class MoEStack:
     """``len(layers)`` MoE layers on an RMSNorm residual stream (eps, gamma per layer or none), each after an attention
     sublayer of its own if ``attention`` (one for each layer; ``attention_gammas`` likewise) is given."""
@@ -169,11 +177,15 @@ class MoEStack:
     def evict(self, step: DecodeStep, keep: int, *, first: int = 0, recent: int = 0) -> None:
         """``kv_evict`` of every layer's cache (``new_cache(weigh=..)``) after a decode step: of each of ``step``'s sequences with more
         than ``keep`` keys, every layer's key heads keep ``keep`` of their own.  step.lens and step.rows, which must be given, follow in
-        place; positions go on as they were."""
+        place, so neither may share memory with another of step's tensors; positions go on as they were."""
         if not isinstance(step, DecodeStep) or step.rows is None:
             raise ValueError("evict needs a DecodeStep with rows: behind it positions do not give them")
         if self.attention is None or any(a.key_weights is None for a in self.attention):
             raise RuntimeError("evict needs attention sublayers whose caches keep weights: new_cache(weigh=..)")
+        for name, t in vars(step).items():
+            for other in ("lens", "rows"):
+                if name != other and isinstance(t, torch.Tensor) and _share(t, getattr(step, other)):
+                    raise ValueError(f"step.{other} is changed in place and shares memory with step.{name}: give it its own")
         for a in self.attention:
             lens = a.evict(step.table, step.lens, keep, first=first, recent=recent)
         step.rows -= (step.lens - lens).repeat_interleave(step.q_len, output_size=step.rows.numel())

@@ -215,6 +215,34 @@ def test_caches_and_stacks_refuse_what_they_cannot_keep():
         att.evict(None, None, 4)
 
 
+class FakeAttention:
+    """What ``MoEStack.evict`` asks of an attention sublayer: every sequence is cut down to 4 keys."""
+
+    key_weights = torch.zeros(1)
+
+    def evict(self, table, lens, keep, *, first, recent):
+        return lens.clamp(max=keep)
+
+
+def test_stack_evict_refuses_rows_and_lengths_that_are_other_tensors_too():
+    """Before the first eviction positions and rows count the same, but rows are taken back and positions are not."""
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    stack = dsk_moe.MoEStack([object()], attention=[FakeAttention()])
+    pos, seq, table = ints([9, 3]), ints([0, 1]), ints([[0], [1]])
+    step = dsk_moe.DecodeStep(pos, seq, table, pos + 1, rows=pos.clone())
+    stack.evict(step, 4)
+    assert step.lens.tolist() == [4, 4] and step.rows.tolist() == [3, 3] and pos.tolist() == [9, 3]
+    three, buffer = pos.repeat(3, 1), ints([9, 3, 10, 4])
+    for bad in (dict(positions=pos, rows=pos), dict(positions=three, rows=three[2]), dict(positions=pos, rows=pos.view(2)),
+                dict(positions=pos.clone(), rows=buffer[:2], lens=buffer[1:3]), dict(positions=buffer[2:], rows=pos, lens=buffer[2:])):
+        held = [t.clone() for t in bad.values()]
+        with pytest.raises(ValueError, match="shares memory"):
+            stack.evict(dsk_moe.DecodeStep(**{**dict(seq=seq, table=table, lens=ints([10, 4])), **bad}), 4)
+        assert all(torch.equal(t, h) for t, h in zip(bad.values(), held))
+    stack.evict(dsk_moe.DecodeStep(pos, seq, table, buffer[2:], rows=buffer[:2]), 4)     # next to each other
+    assert buffer.tolist() == [3, 3, 4, 4]
+
+
 # ------------------------------------------------------------------ axes
 def test_rope_axes():
     f, a = dsk_moe.rope_axes([16, 24, 24], device="cpu")
