@@ -157,6 +157,19 @@ def _sig(t: torch.Tensor | None):
     return (t.shape, t.stride(), t.dtype, t.get_device()) if t is not None else None
 
 
+def _properties_of(given: list[torch.Tensor]):
+    """torch's record of these tensors' properties, or None: it never finds a tensor that is given twice, and is no public class,
+    so that one which does not find the tensors that it is made of is not used."""
+    if _Properties is None or len(set(map(id, given))) < len(given):
+        return None
+    try:
+        properties = _Properties(*given, dynamic_dims_sizes=[list(t.shape) for t in given],
+                                 dynamic_dims_strides=[list(t.stride()) for t in given])
+        return properties if properties.check(*given) else None
+    except Exception:
+        return None
+
+
 class _Plans:
     """Plans of one function's calls, which ``make`` makes of a call's arguments."""
 
@@ -179,11 +192,11 @@ class _Plans:
         plan, misses = entry
         entry[1] += 1
         # (again after 1, 2, 4, .. calls that were not found among the recent ones)
-        if _Properties is not None and misses & (misses - 1) == 0:
-            properties = _Properties(*given, dynamic_dims_sizes=[list(t.shape) for t in given],
-                                     dynamic_dims_strides=[list(t.stride()) for t in given])
-            self._recent.insert(0, (numbers, properties, plan))
-            del self._recent[_MOST_RECENT:]
+        if misses & (misses - 1) == 0:
+            properties = _properties_of(given)
+            if properties is not None:
+                self._recent.insert(0, (numbers, properties, plan))
+                del self._recent[_MOST_RECENT:]
         return plan
 
 

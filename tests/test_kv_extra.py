@@ -243,6 +243,78 @@ def test_stack_evict_refuses_rows_and_lengths_that_are_other_tensors_too():
     assert buffer.tolist() == [3, 3, 4, 4]
 
 
+# ------------------------------------------------------------------ plans
+class Records:
+    """Stands in for torch's record of tensors' properties, and counts."""
+
+    def __init__(self, fault=None):
+        self.fault, self.made, self.asked = fault, 0, 0
+
+    def __call__(self, *tensors, **kw):
+        self.made += 1
+        if self.fault == "raises":
+            raise TypeError("other arguments")
+        kinds = [(t.shape, t.dtype) for t in tensors]
+        records = self
+
+        class Record:
+            def check(self, *given):
+                records.asked += 1
+                return records.fault is None and [(t.shape, t.dtype) for t in given] == kinds
+        return Record()
+
+
+def find(plans, *tensors):
+    return plans.find((1, 0.5), tensors, tensors)
+
+
+def test_plans_of_a_kind_are_made_once():
+    made = []
+    plans = A._Plans(lambda *tensors: made.append(tensors) or tuple(t.shape for t in tensors))
+    a, b = torch.zeros(3, 4), torch.zeros(5)
+    for _ in range(4):
+        assert find(plans, a, b) == (a.shape, b.shape) and find(plans, b, a) == (b.shape, a.shape)
+    assert find(plans, a.double(), b) == (a.shape, b.shape)         # another kind
+    assert find(plans, torch.zeros(4, 3).t(), b) == (a.shape, b.shape)
+    assert len(made) == 4
+
+
+@pytest.mark.parametrize("real", [False, True])
+def test_plans_record_no_call_that_a_record_cannot_find(monkeypatch, real):
+    """A tensor given twice is never found by torch's record: such calls ask the dictionary alone, and leave the records of others in place."""
+    if real and A._Properties is None:
+        pytest.skip("this torch has no record of tensors' properties")
+    records = Records()
+    if not real:
+        monkeypatch.setattr(A, "_Properties", records)
+    plans = A._Plans(lambda *tensors: object())
+    one, two = torch.zeros(3, 4), torch.zeros(3, 4)
+    apart = find(plans, one, two)
+    assert find(plans, one, two) is apart and len(plans._recent) == 1
+    for _ in range(600):
+        assert find(plans, one, one) is apart                       # (of the same kind: what is checked is the same)
+    assert len(plans._recent) == 1
+    plans = A._Plans(lambda *tensors: object())
+    both = find(plans, one, one)
+    for _ in range(600):
+        assert find(plans, one, one) is both
+    assert not plans._recent
+
+
+@pytest.mark.parametrize("fault", ["raises", "never finds"])
+def test_plans_do_without_a_record_that_does_not_work(monkeypatch, fault):
+    records = Records(fault)
+    monkeypatch.setattr(A, "_Properties", records)
+    plans = A._Plans(lambda *tensors: object())
+    a, b = torch.zeros(3, 4), torch.zeros(5)
+    plan = find(plans, a, b)
+    for _ in range(100):
+        assert find(plans, a, b) is plan
+    assert not plans._recent and 0 < records.made < 10
+    monkeypatch.setattr(A, "_Properties", None)
+    assert find(plans, a, b) is plan
+
+
 # ------------------------------------------------------------------ axes
 def test_rope_axes():
     f, a = dsk_moe.rope_axes([16, 24, 24], device="cpu")
