@@ -191,8 +191,8 @@ class _Plans:
             entry = self._by_key[key] = [self._make(*args), 0]
         plan, misses = entry
         entry[1] += 1
-        # (again after 1, 2, 4, .. calls that were not found among the recent ones)
-        if misses & (misses - 1) == 0:
+        # (once a kind was met again, and after 2, 4, .. calls that were not found among the recent ones)
+        if misses and misses & (misses - 1) == 0:
             properties = _properties_of(given)
             if properties is not None:
                 self._recent.insert(0, (numbers, properties, plan))

@@ -301,6 +301,18 @@ def test_plans_record_no_call_that_a_record_cannot_find(monkeypatch, real):
     assert not plans._recent
 
 
+def test_plans_record_no_kind_that_comes_once(monkeypatch):
+    """Prompts of ever new lengths: a record of each would cost more than it finds."""
+    records = Records()
+    monkeypatch.setattr(A, "_Properties", records)
+    plans = A._Plans(lambda *tensors: object())
+    for n in range(1, 50):
+        find(plans, torch.zeros(n), torch.zeros(n, 1))
+    assert not plans._recent and records.made == 0
+    find(plans, torch.zeros(7), torch.zeros(7, 1))
+    assert len(plans._recent) == 1
+
+
 @pytest.mark.parametrize("fault", ["raises", "never finds"])
 def test_plans_do_without_a_record_that_does_not_work(monkeypatch, fault):
     records = Records(fault)
