@@ -81,11 +81,12 @@ __device__ __forceinline__ u32x2 read_tr(const char* p) {
 }
 
 // State of a wave's 32 rows: lane l holds row l & 31; register 4 a + b of o[dt]
-// is element 32 dt + 8 a + 4 (l >> 5) + b; l is this lane half's part of the sum.
+// is element 32 dt + 8 a + 4 (l >> 5) + b; l is this lane half's part of the sum of the weights as the product uses
+// them, exact (kExact alone) of the weights themselves, for those who divide other weights by it.
 template <int D>
 struct FlashRows {
   f32x16 o[D / 32];
-  float m, l;
+  float m, l, exact;
 };
 
 constexpr int kFlBuffers = 2;        // tiles of K and of V in LDS
@@ -102,7 +103,7 @@ constexpr int flash_lds() { return 2 * kFlBuffers * kFlKeys * D * 2 + 16; }   //
 //
 // KH 2: two waves for 32 rows, with the lower and the upper 32 keys of every tile
 // (half = wave / (NW / 2); add_halves joins them).
-template <int D, int NW, int KH, class Rows>
+template <int D, int NW, int KH, bool kExact = false, class Rows>
 __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1, int lim, int w_min, int b_min,
                                       float c2, char* lds, int64_t kstride, int64_t vstride, Rows rows, FlashRows<D>& st) {
   // wave-uniform by their meaning: in scalar registers
@@ -185,6 +186,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       const float f = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
       st.m = mn;
       st.l *= f;
+      if constexpr (kExact) st.exact *= f;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= f;
     }
@@ -198,9 +200,12 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
       // rounding of 2^-8.  As the sum of two bf16, with two products each, 8192 tokens of 32 heads of 128
       // take 695 instead of 488 us, 16 prompts of 5375 tokens together 37 instead of 25.5.
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[s4][i] = pack_bf16(__builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i] * c2 - mu),
-                             __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu));
+      for (int i = 0; i < 4; ++i) {
+        const float lo = __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i] * c2 - mu);
+        const float hi = __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu);
+        if constexpr (kExact) st.exact += lo + hi;
+        w[s4][i] = pack_bf16(lo, hi);
+      }
       p[s4] = as_bf16x8(w[s4]);
     }
     // The sum is that of the rounded weights, which the product uses: a row whose visible values are all the
@@ -398,7 +403,7 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
 // rows after the first may be read.  Codes come to registers a step ahead, and go to LDS as the bf16 that flash
 // reads, so every wave converts a quarter of a tile once for all.  A NaN is seen by all rows, so nothing is kept
 // from any.
-template <int D, class Rows>
+template <int D, bool kExact, class Rows>
 __device__ __forceinline__ void flash_codes(const bf16x8 (&q)[D / 16], int t0, int t1, int n_keys, float c2, char* lds, Rows rows,
                                             FlashRows<D>& st) {
   t0 = __builtin_amdgcn_readfirstlane(t0);
@@ -463,6 +468,7 @@ __device__ __forceinline__ void flash_codes(const bf16x8 (&q)[D / 16], int t0, i
       const float f = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
       st.m = mn;
       st.l *= f;
+      if constexpr (kExact) st.exact *= f;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= f;
     }
@@ -473,9 +479,12 @@ __device__ __forceinline__ void flash_codes(const bf16x8 (&q)[D / 16], int t0, i
     for (int s4 = 0; s4 < 4; ++s4) {
       u32x4 w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = pack_bf16(__builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i] * c2 - mu),
-                         __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu));
+      for (int i = 0; i < 4; ++i) {
+        const float lo = __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i] * c2 - mu);
+        const float hi = __builtin_amdgcn_exp2f(s[s4 >> 1][8 * (s4 & 1) + 2 * i + 1] * c2 - mu);
+        if constexpr (kExact) st.exact += lo + hi;
+        w[i] = pack_bf16(lo, hi);
+      }
       even = add_bf16_pair(w[0], even);
       odd = add_bf16_pair(w[1], odd);
       even = add_bf16_pair(w[2], even);

@@ -95,6 +95,7 @@ struct PagedArgs {
   float* weights;                   // of the cache's rows, to be added to, or null; then also:
   float* scores;                    // [item][key of the table row][M rounded up to fours], times c
   float* lse;                       // [item][M]: log2 of the sum of 2^score (infinite: the row sees no key)
+  float* pre_l;                     // the prefix partials' sums of the weights before their rounding to bf16
 };
 
 // Keys of sequence b that the cache can hold; `bad` if lens[b] claims more.
@@ -609,7 +610,7 @@ constexpr int kPreBlocks = 256;      // workgroups of the prefix, at most about:
                                      // sequences: 40 us, 45 with 128, 47 with 384, 50 with 512)
 constexpr int kPreChunk = 64;        // tiles whose places in the cache a wave holds at once
 
-template <int D, bool F8>
+template <int D, bool F8, bool kWeigh>
 __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
@@ -626,7 +627,7 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
   for (int ks = 0; ks < D / 16; ++ks) q[ks] = as_bf16x8(ldg16(qp + 16 * ks));
   FlashRows<D> st;
   st.m = kNegInf;
-  st.l = 0.0f;
+  st.l = st.exact = 0.0f;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
   uint64_t bad = 0;
@@ -657,7 +658,7 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
         vs = scale_of(static_cast<uint32_t>(__builtin_amdgcn_readlane(v_byte, t - c0)));
         return max(a.prefix - 1 - (t * kFlKeys + row), 0);
       };
-      flash_codes<D>(q, c0, c1, a.prefix, a.c2, lds, src, st);
+      flash_codes<D, kWeigh>(q, c0, c1, a.prefix, a.c2, lds, src, st);
     } else {
       auto src = [&](int t, int row, const uint16_t*& kp, const uint16_t*& vp, int& last) {
         const int64_t base = base_of(t);
@@ -665,12 +666,16 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
         vp = a.c.v + base;
         last = max(a.prefix - 1 - (t * kFlKeys + row), 0);
       };
-      flash<D, kPreWaves, 1>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
+      flash<D, kPreWaves, 1, kWeigh>(q, c0, c1, a.prefix - 1, a.prefix - 1, a.prefix - 1, a.c2, lds, D, D, src, st);
     }
   }
   // a page outside the cache: the waves load different rows, so all tell
   const bool any_bad = __syncthreads_or(bad != 0);
   const float l = any_bad ? __builtin_nanf("") : sum_across32(st.l);
+  // own keys' weights are 2^score over a sum: of the prefix's weights as they are, since a rounding to bf16 that many
+  // of them share is one of the sum (up to 2^-8 of it)
+  float exact = 0.0f;
+  if constexpr (kWeigh) exact = any_bad ? __builtin_nanf("") : sum_across32(st.exact);
   // the rows' partial sums by way of LDS (32 rows a wave, 16-byte chunk c of row n at c ^ n), so that a
   // store writes whole lines (16.8 MB of them: 0.8 us less than from the registers, 32 bytes
   // of a row at a time)
@@ -692,7 +697,10 @@ __device__ __forceinline__ void prefix_part(const PagedArgs& a, int block, char*
       *reinterpret_cast<f32x4*>(a.pre_o + (at0 + row) * D + 4 * c) =
           *reinterpret_cast<const f32x4*>(wl + row * D * 4 + 16 * (c ^ (row & (kChunks - 1))));
   }
-  if (hf == 0 && wr0 + n < rows) *reinterpret_cast<float2*>(a.pre_ml + (at0 + n) * 2) = float2{st.m, l};
+  if (hf == 0 && wr0 + n < rows) {
+    *reinterpret_cast<float2*>(a.pre_ml + (at0 + n) * 2) = float2{st.m, l};
+    if constexpr (kWeigh) a.pre_l[at0 + n] = exact;
+  }
 }
 
 template <int D, int RT, bool F8, bool kWeigh>
@@ -706,7 +714,7 @@ template <int D, int RT, bool F8, bool kWeigh>
 __global__ __launch_bounds__(kPgThreads, RT == 1 ? 2 : 1) void k_paged_prefix(const PagedArgs a) {
   extern __shared__ __align__(16) char lds[];
   const int block = blockIdx.x - a.prefix_blocks;
-  if (block < 0) prefix_part<D, F8>(a, blockIdx.x, lds);
+  if (block < 0) prefix_part<D, F8, kWeigh>(a, blockIdx.x, lds);
   else shares<D, RT, F8, kWeigh>(a, block % a.shares, 16 * RT * (block / a.shares), *reinterpret_cast<SegLds<D, RT, 4>*>(lds));
 }
 
@@ -765,12 +773,16 @@ struct Parts {
   __device__ __forceinline__ f32x2 ml(const PagedArgs& a, int i, int r) const {
     return ldg<f32x2>((i < own ? a.pml : a.pre_ml) + row(i, r) * 2);
   }
+  // the sum of part i's weights before any rounding, its ml being `had`
+  __device__ __forceinline__ float exact(const PagedArgs& a, int i, int r, const f32x2& had) const {
+    return i < own ? had[1] : ldg<float>(a.pre_l + row(i, r));
+  }
 };
 
 template <int D, int WPR, bool kWeigh>
 __device__ __forceinline__ void join_rows(const PagedArgs& a, int block) {
   constexpr int kLanes = D / 4, kThreads = 64 * WPR, kWays = kThreads / kLanes, kRows = kPgThreads / kThreads;
-  __shared__ float red[kRows][WPR];
+  __shared__ float red[kRows][WPR], red_exact[kRows][WPR];
   __shared__ f32x4 sums[kRows][kWays][kLanes];
   const int M = a.q_len * a.group, tid = threadIdx.x % kThreads, lane = threadIdx.x & 63, wave = tid >> 6;
   const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), row = block * kRows + mine;
@@ -798,7 +810,7 @@ __device__ __forceinline__ void join_rows(const PagedArgs& a, int block) {
     first_m[i] = is ? ml_of(way + i * kWays)[0] : kNegInf;
   }
 
-  float top = kNegInf, ll = 0.0f;
+  float top = kNegInf, ll = 0.0f, exact = 0.0f;
   for (int i = tid; i < parts; i += kThreads) top = fmaxf(top, ml_of(i)[0]);
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
@@ -814,15 +826,27 @@ __device__ __forceinline__ void join_rows(const PagedArgs& a, int block) {
   for (int i = tid; i < parts; i += kThreads) {
     const f32x2 ml = ml_of(i);
     ll += ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
+    if constexpr (kWeigh) exact += of.exact(a, i, r, ml) * __builtin_amdgcn_exp2f(ml[0] - mu);
   }
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) ll += __shfl_xor(ll, s, 64);
+  for (int s = 32; s >= 1; s >>= 1) {
+    ll += __shfl_xor(ll, s, 64);
+    if constexpr (kWeigh) exact += __shfl_xor(exact, s, 64);
+  }
   if constexpr (WPR > 1) {
-    if (lane == 0) red[mine][wave] = ll;
+    if (lane == 0) {
+      red[mine][wave] = ll;
+      if constexpr (kWeigh) red_exact[mine][wave] = exact;
+    }
     __syncthreads();
     ll = red[mine][0];
 #pragma unroll
     for (int w = 1; w < WPR; ++w) ll += red[mine][w];
+    if constexpr (kWeigh) {
+      exact = red_exact[mine][0];
+#pragma unroll
+      for (int w = 1; w < WPR; ++w) exact += red_exact[mine][w];
+    }
   }
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -840,7 +864,7 @@ __device__ __forceinline__ void join_rows(const PagedArgs& a, int block) {
   // no key, or an unused slot (its q may hold anything): zeros
   const bool sees = a.lens[b] >= 0 && (a.prefix > 0 || len - a.q_len + tok >= 0 || ll != ll);
   if constexpr (kWeigh)
-    if (d0 == 0) a.lse[static_cast<int64_t>(item) * M + r] = sees ? top + log2f(ll) : -kNegInf;
+    if (d0 == 0) a.lse[static_cast<int64_t>(item) * M + r] = sees ? top + log2f(exact) : -kNegInf;
   y = sees ? y * (1.0f / ll) : f32x4{0.f, 0.f, 0.f, 0.f};
   *reinterpret_cast<u32x2*>(a.out + (static_cast<int64_t>(b) * a.q_len + tok) * a.o_token + hd * a.o_head + d0) =
       u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
@@ -855,7 +879,7 @@ constexpr int kKwRows = 64;          // most rows of an item
 constexpr int kKwPartRows = kPgThreads / 16;
 __device__ __forceinline__ float lse_of_parts(const PagedArgs& a, const Parts& of, int b, int len) {
   const int r = threadIdx.x / 16, lane = threadIdx.x % 16;
-  float top = kNegInf, l = 0.0f;
+  float top = kNegInf, l = 0.0f;     // l: of the weights before any rounding
   if (r < of.M)
     for (int i = lane; i < of.all; i += 16) top = fmaxf(top, of.ml(a, i, r)[0]);
 #pragma unroll
@@ -864,7 +888,7 @@ __device__ __forceinline__ float lse_of_parts(const PagedArgs& a, const Parts& o
   if (r < of.M)
     for (int i = lane; i < of.all; i += 16) {
       const f32x2 ml = of.ml(a, i, r);
-      l += ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
+      l += of.exact(a, i, r, ml) * __builtin_amdgcn_exp2f(ml[0] - mu);
     }
 #pragma unroll
   for (int s = 8; s >= 1; s >>= 1) l += __shfl_xor(l, s, 64);
@@ -937,7 +961,7 @@ __global__ __launch_bounds__(kPgThreads) void k_join_weights(const PagedArgs a, 
 struct PagedPlan {
   int rt, shares, splits, row_tiles;
   bool alone;                        // k_paged_short
-  size_t po, pml, parts, pre_o, pre_ml, scores, lse, total;
+  size_t po, pml, parts, pre_o, pre_ml, scores, lse, pre_l, total;
 };
 
 PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMore& more) {
@@ -966,7 +990,8 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
     if (more.weigh) {
       p.scores = p.total;
       p.lse = up(p.scores + static_cast<size_t>(items) * keys * ((M + 3) & ~int64_t{3}) * 4);
-      p.total = up(p.lse + static_cast<size_t>(items) * M * 4);
+      p.pre_l = up(p.lse + static_cast<size_t>(items) * M * 4);
+      p.total = up(p.pre_l + static_cast<size_t>(p.splits) * items * M * 4);
     }
     return p;
   };
@@ -1070,7 +1095,7 @@ hipError_t launch_paged(const dsk_paged_desc& d, const dsk_kv_cache& c, const Pa
                     d.q_token, d.q_head, d.o_token, d.o_head, d.scale * kLog2e, d.batch, d.q_len, d.kv_heads,
                     d.heads / d.kv_heads, d.prefix_len, p.shares, p.splits, p.row_tiles,
                     p.row_tiles * p.splits * d.kv_heads, more.k_scale, more.v_scale, more.key_weights, reinterpret_cast<float*>(w + p.scores),
-                    reinterpret_cast<float*>(w + p.lse)};
+                    reinterpret_cast<float*>(w + p.lse), reinterpret_cast<float*>(w + p.pre_l)};
   auto form = [&](auto f8, auto weigh) {
     constexpr bool kF = decltype(f8)::value, kW = decltype(weigh)::value;
     if (d.head_dim == 64) launch_paged_d<64, kF, kW>(p, a, s);
