@@ -81,6 +81,24 @@ def attention(q, k, v, last, scale):
     return o, tol + 1e-38
 
 
+def attention_of_many(q, k, v, last, scale):
+    """``attention`` with the rows of a key head at once, for long sequences."""
+    heads, kv, n = q.shape[1], k.shape[1], k.shape[0]
+    o, tol = torch.zeros(q.shape, dtype=F64), torch.zeros(q.shape, dtype=F64)
+    hidden = torch.arange(n)[:, None] > last.repeat_interleave(heads // kv)[None]
+    seen = (last + 1).clamp(0, n).repeat_interleave(heads // kv)[:, None]
+    for g in range(kv):
+        mine = slice(g * heads // kv, (g + 1) * heads // kv)
+        rows, kh, vh = q[:, mine].to(F64).flatten(0, 1), k[:, g].to(F64).contiguous(), v[:, g].to(F64).contiguous()
+        w = torch.softmax((kh @ rows.t()).mul_(scale).masked_fill_(hidden, -math.inf), 0).nan_to_num_(0.0).t()
+        size = scale * (kh.abs() @ rows.abs().t()).masked_fill_(hidden, 0.0).amax(0)[:, None]
+        y = w @ vh
+        slack = 4.0 * (seen + q.shape[2] * size + 16) * F32_HALF_STEP
+        bound = (w @ vh.abs()) * (BF16_HALF_STEP + slack) + y.abs() * BF16_HALF_STEP * (1 + 2.0 ** -6)
+        o[:, mine], tol[:, mine] = y.view(q.shape[0], -1, q.shape[2]), bound.view(q.shape[0], -1, q.shape[2])
+    return o, tol + 1e-38
+
+
 def prompt(q, k, v, cu_q, cu_k, causal=True, scale=None):
     """(o, tol) over packed sequences; rows of no sequence are NaN in o."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[2])

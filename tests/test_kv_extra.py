@@ -385,6 +385,14 @@ def test_oracle_weights_are_the_softmax():
     assert torch.allclose(w, want, atol=1e-12) and math.isclose(float(w.sum()), 12.0)
 
 
+def test_oracle_rows_of_a_head_at_once():
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(n, h, 16, generator=g) for n, h in ((3, 6), (11, 2), (11, 2)))
+    for last in ([8, 9, 10], [-2, 0, 10], [10, 10, 12]):
+        for got, want in zip(O.attention_of_many(q, k, v, torch.tensor(last), 0.3), O.attention(q, k, v, torch.tensor(last), 0.3)):
+            assert torch.allclose(got, want, rtol=1e-11, atol=1e-14)
+
+
 def test_oracle_eviction_by_hand():
     """Eight keys, five kept, one first and two recent: of the middle five those of weight 9 and 5."""
     page = 16
