@@ -56,19 +56,23 @@ struct QkArgs {
   int32_t windows, code_parts;       // workgroups for it: of kWindow tokens, times parts of the heads
 };
 
+// kMore: the call may have several axes, rows of its own or weights.
+
 // Whether token t, at pos on the first axis, is one of padding.
+template <bool kMore>
 __device__ __forceinline__ bool left_out(const QkArgs& a, int64_t t, int pos) {
   bool out = pos < 0;
-  for (int x = 1; x < a.n_axes; ++x) out |= a.positions[x * a.axis_stride + t] < 0;
+  if constexpr (kMore)
+    for (int x = 1; x < a.n_axes; ++x) out |= a.positions[x * a.axis_stride + t] < 0;
   return out;
 }
 // Cosine and sine of pair i's angle, times mscale; a pair of no axis does not turn.  kFine: quarter turns are taken off in
 // float64 too, so that the rest is at most an eighth and loses up to two bits less.  For codes, which are
 // off by a whole step where the key's own error crosses a border (16 times 8192 tokens: 187 such codes, 342 without, 43.4 us
 // either way).
-template <bool kFine>
+template <bool kFine, bool kMore>
 __device__ __forceinline__ float2 turn_of(const QkArgs& a, int64_t t, int pos, int i) {
-  if (a.axis) {
+  if (kMore && a.axis) {
     const int x = a.axis[i];
     pos = x >= 0 && x < a.n_axes ? a.positions[x * a.axis_stride + t] : 0;
   }
@@ -89,9 +93,10 @@ __device__ __forceinline__ float2 turn_of(const QkArgs& a, int64_t t, int pos, i
   return float2{cs * a.mscale, sn * a.mscale};
 }
 // Row of token t among all rows of the cache with one head, or -1.
+template <bool kMore>
 __device__ __forceinline__ int64_t slot_of(const QkArgs& a, int64_t t, int pos) {
   const int sq = a.seq[t];
-  const int64_t at = a.rows ? a.rows[t] : static_cast<int64_t>(pos) - a.prefix_len, page = at >> a.cache.page_shift;
+  const int64_t at = kMore && a.rows ? a.rows[t] : static_cast<int64_t>(pos) - a.prefix_len, page = at >> a.cache.page_shift;
   if (sq < 0 || sq >= a.cache.n_seqs || at < 0 || page >= a.cache.max_pages) return -1;
   const int id = a.cache.table[sq * a.cache.table_stride + page];
   if (id < 0 || id >= a.cache.n_pages) return -1;
@@ -211,8 +216,8 @@ __device__ __forceinline__ void append_codes(const QkArgs& a, int block) {
     bool live = false;
     if (i < kSlots && t >= 0 && t < a.tokens) {
       const int pos = a.positions[t];
-      live = !left_out(a, t, pos);
-      if (live) slot = slot_of(a, t, pos);
+      live = !left_out<true>(a, t, pos);
+      if (live) slot = slot_of<true>(a, t, pos);
     }
     const int64_t key = slot < 0 ? -1 : slot / kScaleRows, before = __shfl_up(key, 1, 64);
     const uint64_t starts = __ballot(tid > 0 && (key < 0 || key != before));
@@ -239,7 +244,7 @@ __device__ __forceinline__ void append_codes(const QkArgs& a, int block) {
   if (begin >= end) return;
   for (int i = tid; i < (end - begin) * half; i += 64 * kQkWaves) {
     const int slot = begin + i / half;
-    if (s.lead[slot] != kSkip) s.turn[slot][i % half] = turn_of<true>(a, t0 + slot, a.positions[t0 + slot], i % half);
+    if (s.lead[slot] != kSkip) s.turn[slot][i % half] = turn_of<true, true>(a, t0 + slot, a.positions[t0 + slot], i % half);
   }
   __syncthreads();
   const Pairs<kInter> pairs(a, lane);
@@ -358,8 +363,9 @@ __device__ __forceinline__ void append_codes(const QkArgs& a, int block) {
 
 // A lane's part of a head row: elements e .. e + 7 of 8 lanes (D 64) or 16 (D 128).  kAll: a
 // wave takes all heads of its token.  kPast: queries and rows of the cache are written past L2.
-// kCodes: a cache in 8 bits, whose workgroups come first; then the queries'.
-template <int D, bool kBF16, bool kInter, bool kAll, bool kPast, bool kCodes>
+// kCodes: a cache in 8 bits, whose workgroups come first; then the queries'.  Plain calls have a form without kMore, which
+// asks nothing about what they do not have (8192 tokens 43.3 -> 43.1 us).
+template <int D, bool kBF16, bool kInter, bool kAll, bool kPast, bool kCodes, bool kMore>
 __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a head row, rows of a wave
   __shared__ float2 turns[kQkWaves][D / 2];
@@ -378,8 +384,8 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   if (t >= a.tokens) return;
   const int lane = wl % kLanes;
   const Pairs<kInter> pairs(a, lane);
-  const int e = pairs.e, ep = pairs.ep, half = pairs.half;
-  const bool rotated = pairs.rotated;
+  const int e = pairs.e, ep = pairs.ep, er = pairs.er, half = pairs.half;
+  const bool rotated = pairs.rotated, low = pairs.low;
   // this lane's heads: row0, row0 + step, ..
   const bool is_q = kAll || kCodes || by < a.q_parts;
   const int part = is_q ? by : by - a.q_parts;
@@ -404,12 +410,38 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
   }
 
   const int pos = a.positions[t];
-  if (left_out(a, t, pos)) return;
+  if (left_out<kMore>(a, t, pos)) return;
   float2* turn = turns[wave];
-  if (wl < half) turn[wl] = turn_of<false>(a, t, pos, wl);
-  const int64_t slot = !kCodes && a.append ? slot_of(a, t, pos) : -1;   // the token's row of the cache, or none
+  if (wl < half) turn[wl] = turn_of<false, kMore>(a, t, pos, wl);
+  const int64_t slot = !kCodes && a.append ? slot_of<kMore>(a, t, pos) : -1;   // the token's row of the cache, or none
 
-  auto factors = [&](const float* gamma, float (&own)[8], float (&pair)[8]) { pairs.factors(gamma, turn, own, pair); };
+  // as pairs.factors, written out with a branch around the reads of the angles, which is faster for a cache in bf16 (8192 tokens 42.4
+  // us, 43.2 with pairs.factors, 44.1 with that and the branch; in 8 bits 43.8, 43.3 with pairs.factors)
+  auto factors = [&](const float* gamma, float (&own)[8], float (&pair)[8]) {
+    if constexpr (kCodes) {
+      pairs.factors(gamma, turn, own, pair);
+      return;
+    }
+    float g[8], gp[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = gp[j] = 1.0f;
+    if (gamma) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const f32x4 u = *reinterpret_cast<const f32x4_a4*>(gamma + e + j), v = *reinterpret_cast<const f32x4_a4*>(gamma + ep + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { g[j + i] = u[i]; gp[j + i] = v[i]; }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int pr = kInter ? er / 2 + j / 2 : (low ? er : er - half) + j;
+      const float2 cs = rotated ? turn[pr] : float2{1.0f, 0.0f};
+      own[j] = g[j] * cs.x;
+      if constexpr (kInter) pair[j] = j & 1 ? g[j - 1] * cs.y : -(g[j + 1] * cs.y);
+      else pair[j] = (low ? -cs.y : cs.y) * gp[j];
+    }
+  };
   auto normed = [&](const Raw8<kBF16>& x, const Raw8<kBF16>& y, const float (&own)[8], const float (&pair)[8]) {
     float z[8];
     norm_turn<D, kBF16, kInter>(a.norm, a.eps, rotated, x, y, own, pair, z);
@@ -459,7 +491,7 @@ __global__ __launch_bounds__(64 * kQkWaves) void k_qk(const QkArgs a) {
       if (a.k_out) *reinterpret_cast<u32x4*>(a.k_out + t * a.ko_token + h * a.ko_head + e) = out[i];   // read many times next
       if (slot >= 0) {
         const int64_t to = (slot + (static_cast<int64_t>(h) << a.cache.page_shift)) * D + e;
-        if (a.key_weights && lane == 0) a.key_weights[to / D] = 0.0f;
+        if (kMore && a.key_weights && lane == 0) a.key_weights[to / D] = 0.0f;
         store(a.cache.k + to, out[i]);
         const Raw8<kBF16>& x = v.x[i];
         store(a.cache.v + to, u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])});
@@ -504,8 +536,13 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
   auto form = [&](auto bf16, auto inter) {
     constexpr bool kB = decltype(bf16)::value, kI = decltype(inter)::value;
     if (!a.k_scale) {
-      launch(k_qk<D, kB, kI, true, false, false>, k_qk<D, kB, kI, false, false, false>, k_qk<D, kB, kI, true, true, false>,
-             k_qk<D, kB, kI, false, true, false>);
+      auto rows = [&](auto more) {
+        constexpr bool kM = decltype(more)::value;
+        launch(k_qk<D, kB, kI, true, false, false, kM>, k_qk<D, kB, kI, false, false, false, kM>, k_qk<D, kB, kI, true, true, false, kM>,
+               k_qk<D, kB, kI, false, true, false, kM>);
+      };
+      if (a.axis || a.rows || a.key_weights) rows(std::true_type{});
+      else rows(std::false_type{});
       return;
     }
     a.windows = (d.tokens + kWindow - 1) / kWindow;
@@ -513,7 +550,7 @@ void launch_qk_d(const dsk_qk_desc& d, const QkArgs& args, hipStream_t s) {
     a.code_parts = want < d.kv_heads ? want : d.kv_heads;
     if (!split) a.q_parts = d.heads > 0 ? 1 : 0;
     const int64_t blocks = static_cast<int64_t>(a.windows) * a.code_parts + static_cast<int64_t>(grid.x) * a.q_parts;
-    launch_kernel(past ? k_qk<D, kB, kI, false, true, true> : k_qk<D, kB, kI, false, false, true>, dim3(static_cast<uint32_t>(blocks)),
+    launch_kernel(past ? k_qk<D, kB, kI, false, true, true, true> : k_qk<D, kB, kI, false, false, true, true>, dim3(static_cast<uint32_t>(blocks)),
                   64 * kQkWaves, 0, s, a);
   };
   if (d.dtype == DSK_DTYPE_BF16) {
