@@ -14,7 +14,8 @@
 // read whole before it is written.  24.4 us for 98 MB read and written (4.0 TB/s; a large copy 4.9).
 //
 // In 8 bits a block of 16 rows has one scale: a block with a row from elsewhere takes the largest of its rows'
-// scales, and its rows move to it, so blocks are made whole.
+// scales, and its rows move to it, so blocks are made whole.  Rows behind the kept ones in the last block do not: they are none of the
+// sequence's any more, and a smaller scale might not hold them.
 #include <algorithm>
 
 #include "kv8.h"

@@ -534,7 +534,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch.Te
     """``dsk_kv_evict``: of every sequence with lens[s] (int32) > ``keep`` rows, each key head keeps the first ``first``, the
     last ``recent`` and, of the others, those of most ``key_weights`` (of equal ones the earlier), in the rows 0 .. keep - 1; the
     last rows stay the last, in their order, of the others as few as can change place.  Returns the new lengths, min(lens, keep)
-    (``lens_out``, which may be ``lens``).  Rows behind are left as they were, and the pages that they fill are free.  The next
+    (``lens_out``, which may be ``lens``).  Rows behind are left as they were (in 8 bits but those of the last kept row's block, whose
+    scale may be another one now), and the pages that they fill are free.  The next
     token of a sequence goes on at its own position, in row ``keep`` (``kv_append``'s ``rows``)."""
     keep, first, recent = int(keep), int(first), int(recent)
     plan = _evict_plans.find(

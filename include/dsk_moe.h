@@ -500,7 +500,8 @@ typedef struct dsk_evict_desc {
  * i-th other kept row behind it takes the place of the i-th row in front that is given up,
  * and the last rows follow in their order.  Weights move with their rows.  In 8
  * bits a block of 16 rows with a row from elsewhere takes the largest of its rows'
- * scales.  What lies behind row keep is left as it was.  lens_out[s] = min(lens[s],
+ * scales, and the codes of its rows behind keep - 1, if it has any, are then under a
+ * scale that is not theirs; nothing else behind row keep - 1 changes.  lens_out[s] = min(lens[s],
  * keep); lens_out may be lens.  Sequences that are unused or longer than their table row are
  * left alone, and rows whose page, or whose place's, is outside the cache do not move; such
  * rows count as those of least weight.  Rows keep the rotation they have, so later
