@@ -188,7 +188,8 @@ __device__ __forceinline__ u32x4 pack8(const float (&z)[8]) {
 
 // Keys and values of a cache in 8 bits.  The tokens of a call that go to one block of 16 rows stand
 // next to each other; the workgroup of the first one's window of 16 tokens takes them all (kSlots: up to
-// 15 behind its window).  A row lies in D / 8 lanes as elsewhere, its largest magnitude goes to the
+// 15 behind its window).  (With another token between them, also one that is left out, two take the block at once, and its
+// scale and codes may be of either.)  A row lies in D / 8 lanes as elsewhere, its largest magnitude goes to the
 // block's by way of LDS, and with that the block's scale is known before a code is made.
 constexpr int kWindow = 16, kSlots = 2 * kWindow;
 

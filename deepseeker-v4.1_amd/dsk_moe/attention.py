@@ -356,7 +356,8 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, position
 
     ``rows`` (int32): the tokens' rows in their sequences, where positions (of several axes: the first) do not give them, as
     those of pictures and behind an eviction; prefix_len is then 0.  ``k_scale``, ``v_scale``: a cache in 8 bits.  There the tokens that go to one block of
-    16 rows stand next to each other in the call; a call that brings a block's first row starts the block afresh, otherwise the
+    16 rows stand next to each other in the call, none between them, be it one that is left out (nothing checks this; otherwise the
+    block's keys and values are undefined); a call that brings a block's first row starts the block afresh, otherwise the
     rows that are there are rounded to the larger of the block's scale and the call's.  ``key_weights``: zero for the kept keys.
     With scales or weights no page belongs to two sequences."""
     if not (type(mscale) is type(eps) is float and type(interleaved) is type(norm) is bool and type(rot_first) is int):

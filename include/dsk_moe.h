@@ -465,7 +465,9 @@ int dsk_qk_norm_rope_axes(const dsk_qk_desc* d, const dsk_rope_axes* axes, const
  * kept key is set to zero, and a cache in 8 bits takes rounded keys and values.
  *
  * In 8 bits, the tokens of a call that go to one block of 16 rows stand next to each
- * other (a prompt's and a verify step's do).  A call that brings a block's first row
+ * other, in any order, with no other token between them, be it one that is left out (a
+ * prompt's and a verify step's do); nothing checks this, and where they do not, the
+ * block's scale and codes are undefined (nothing else is touched).  A call that brings a block's first row
  * starts the block afresh: its scale is that of the call's rows.  Otherwise the larger
  * of that and the block's own, and the rows that are there are rounded to it. */
 int dsk_kv_append_extra(const dsk_qk_desc* d, const dsk_kv_cache* cache, const dsk_rope_axes* axes, const dsk_kv_extra* extra,
