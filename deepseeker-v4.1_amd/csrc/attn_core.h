@@ -402,7 +402,9 @@ __device__ __forceinline__ void flash(const bf16x8 (&q)[D / 16], int t0, int t1,
 // rows(tile, &k, &v, &k_scale, &v_scale) gives the wave's 16 rows of a tile, D codes each and one scale, and returns how many
 // rows after the first may be read.  Codes come to registers a step ahead, and go to LDS as the bf16 that flash
 // reads, so every wave converts a quarter of a tile once for all.  A NaN is seen by all rows, so nothing is kept
-// from any.
+// from any.  Weights are one bf16 each in the second product, as in flash: as the sum of two, with two products each, 64 sequences
+// behind 16385 keys take 41.1 us instead of 35.5, and their outputs are 0.00167 of their size from the definition in 64 bits
+// instead of 0.00176 (outputs of float32 operations, rounded to bf16 once: 0.00167).
 template <int D, bool kExact, class Rows>
 __device__ __forceinline__ void flash_codes(const bf16x8 (&q)[D / 16], int t0, int t1, int n_keys, float c2, char* lds, Rows rows,
                                             FlashRows<D>& st) {

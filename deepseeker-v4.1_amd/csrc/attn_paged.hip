@@ -985,8 +985,10 @@ PagedPlan plan_of(const dsk_paged_desc& d, const dsk_kv_cache& c, const PagedMor
   // 9.3, but 9.9 against 9.3 for 517 and 14.6 against 9.3 for 1000.  Where items fill the
   // machine without shares, the join is all that they would add (64 such sequences of 600 / 1000 keys: 30.2 / 44.5 us, 31.6 / 45.9
   // with shares).
-  // Codes take half the time: one sequence of 517 keys in 8 bits, with 640 places, 9.6 us, 12.2 with shares (with weights, whose kernel
-  // waits for it, 13.8 and 12.5, but a decode step then has the same bits with and without them).
+  // Codes take half the time, so up to 1024 places whatever the items.  Calls alone / with shares, us: 8 key heads of 128, one sequence of
+  // 517 keys 10.1 / 12.2, 800 11.5 / 12.4, 1000 12.9 / 12.4; 16 of 1000 13.5 / 17.6; 48 of 800 23.3 / 23.1, of 1000 28.9 / 28.1; 4 key heads
+  // of 64, one of 1000 9.7 / 12.3, 48 10.8 / 16.7.  With weights too, whose kernel waits for it, though few items then take longer (one
+  // of 517 14.5 / 13.4, of 1000 17.5 / 13.4; 16 of 1000 19.4 / 21.2), since in 8 bits outputs are the same bits with and without weights.
   // (a launch counts its threads in 32 bits)
   p.alone = d.prefix_len == 0 && keys <= (items >= kPgMany || more.f8 ? kPgShortMany : kPgShort) &&
             items * (64 * kPgShortWaves) < (int64_t{1} << 32);
